@@ -56,7 +56,11 @@ KERNEL_SYMBOLS = (
     "l2c_matmul_bf16", "l2c_matmul_mxfp6", "l2c_mxfp6_bytes",
     "l2c_matmul_qs", "l2c_quantize_mxfp8", "l2c_mxfp8_workspace_bytes", "l2c_matmul_qs_static",
     "l2c_copy_to_host",
+    "l2c_residual_rmsnorm", "l2c_quantize_mxfp4_bf16", "l2c_matmul_mxfp4",
+    "l2c_decoder_beam_select", "l2c_decoder_beam_reorder", "l2c_decoder_beam_workspace_bytes",
 )
+MAX_BEAMS = 32  # L2C_MAX_BEAMS
+F32, BF16 = 0, 1  # enum l2c_type
 QS_STATIC_SCRATCH_BYTES = 24 << 20  # L2C_QS_STATIC_SCRATCH_BYTES
 NVFP4_PARTIALS = 1024  # L2C_NVFP4_PARTIALS
 HOST_SYMBOLS = ("l2c_harness_main", "l2c_compare_dumps", "l2c_decoder_main", "l2c_decoder_run",
@@ -121,6 +125,11 @@ def load() -> ctypes.CDLL:
         "l2c_quantize_mxfp8": [p, sz, p, i, i, p],
         "l2c_matmul_qs_static": [p, p, p, p, i, i, i, i, p],
         "l2c_copy_to_host": [p, p, sz, p],
+        "l2c_residual_rmsnorm": [p, i, p, p, i, p, i, p, p, i, p, i, i, f, f, p],
+        "l2c_quantize_mxfp4_bf16": [p, p, p, i, i, p],
+        "l2c_matmul_mxfp4": [p, p, p, p, p, i, i, i, p],
+        "l2c_decoder_beam_select": [p, p, p, p, p, p, p, i, i, i, i, i, i, p, sz, p],
+        "l2c_decoder_beam_reorder": [p, p, p, i, i, i, i, *[ctypes.c_longlong] * 4, p],
     }
     for name, args in sigs.items():
         fn = getattr(lib, name)
@@ -128,6 +137,8 @@ def load() -> ctypes.CDLL:
         fn.restype = ctypes.c_int
     lib.l2c_mxfp8_workspace_bytes.argtypes = [i, i]
     lib.l2c_mxfp8_workspace_bytes.restype = sz
+    lib.l2c_decoder_beam_workspace_bytes.argtypes = [i, i, i]
+    lib.l2c_decoder_beam_workspace_bytes.restype = sz
     lib.l2c_mxfp6_bytes.argtypes = [i, i, ctypes.POINTER(sz), ctypes.POINTER(sz)]
     lib.l2c_mxfp6_bytes.restype = ctypes.c_int
     lib.l2c_strerror.argtypes = [ctypes.c_int]
@@ -163,7 +174,8 @@ def _load_native() -> None:
 _ENTRIES = ("rmsnorm", "softmax", "matvec", "fused", "matmul", "matmul_q", "matmul_qs", "matmul_qs_static",
             "quantize_mxfp8", "quantize_mxfp4", "quantize_fp8", "to_bf16", "decoder_init_model", "decoder_rmsnorm",
             "decoder_rmsnorm_absmax", "decoder_softmax_argmax", "quantize_mxfp6", "nvfp4_tensor_scales",
-            "nvfp4_tensor_scales_absmax", "quantize_nvfp4", "to_bf16_x4", "matmul_bf16", "matmul_mxfp6")
+            "nvfp4_tensor_scales_absmax", "quantize_nvfp4", "to_bf16_x4", "matmul_bf16", "matmul_mxfp6",
+            "residual_rmsnorm", "quantize_mxfp4_bf16", "matmul_mxfp4", "decoder_beam_select", "decoder_beam_reorder")
 _native = {}
 
 
@@ -255,6 +267,27 @@ def rmsnorm(out, inp, weight, size, batch, eps=RMS_EPSILON, stream=None):
     code = _c_rmsnorm(out, inp, weight, size, batch, eps, stream)
     if code:
         _check(code, "l2c_rmsnorm")
+
+
+def _type(t):
+    """The enum l2c_type of a tensor: 32-bit values or bf16 (any two-byte type)."""
+    size = t.element_size()
+    if size not in (2, 4):
+        raise ValueError("l2c.residual_rmsnorm takes fp32 and bf16 tensors")
+    return F32 if size == 4 else BF16
+
+
+def residual_rmsnorm(normalized, residual_out, residual, block, weight, size, batch, block_weight=None, gate=None,
+                     rows_per_gate=1, residual_scale=1.0, eps=RMS_EPSILON, stream=None):
+    """The types are the tensors'; residual_out, block_weight and gate may be None."""
+    kind = _type(residual)
+    if residual_out is not None and _type(residual_out) != kind:
+        raise ValueError("residual_out has another type than residual")
+    code = _c_residual_rmsnorm(normalized, _type(normalized), residual_out, residual, kind, block, _type(block),
+                               block_weight, gate, rows_per_gate, weight, size, batch, float(residual_scale), float(eps),
+                               stream)
+    if code:
+        _check(code, "l2c_residual_rmsnorm")
 
 
 def softmax(out, logits, size, batch, stream=None):
@@ -362,6 +395,27 @@ def decoder_softmax_argmax(probabilities, logits, tokens, generated, vocab, batc
     code = _c_decoder_softmax_argmax(probabilities, logits, tokens, generated, vocab, batch, steps, step, stream)
     if code:
         _check(code, "l2c_decoder_softmax_argmax")
+
+
+def decoder_beam_workspace_bytes(vocab, beams, batch):
+    return load().l2c_decoder_beam_workspace_bytes(vocab, beams, batch)
+
+
+def decoder_beam_select(scores_out, tokens_out, parents, generated, logits, scores, tokens, eos, vocab, beams, batch,
+                        steps, step, workspace, stream=None):
+    code = _c_decoder_beam_select(scores_out, tokens_out, parents, generated, logits, scores, tokens, eos, vocab, beams,
+                                  batch, steps, step, workspace, workspace.numel() * workspace.element_size(), stream)
+    if code:
+        _check(code, "l2c_decoder_beam_select")
+
+
+def decoder_beam_reorder(out, inp, parents, beams, batch, piece_bytes, row_stride=None, pieces=1, piece_stride=0,
+                         groups=1, group_stride=0, stream=None):
+    """Strides and sizes in bytes; rows of one piece follow each other unless row_stride says otherwise."""
+    code = _c_decoder_beam_reorder(out, inp, parents, beams, batch, groups, pieces, group_stride,
+                                   piece_bytes if row_stride is None else row_stride, piece_stride, piece_bytes, stream)
+    if code:
+        _check(code, "l2c_decoder_beam_reorder")
 
 
 def launch_shape(op, batch, cols, rows, variant=0):
@@ -570,3 +624,15 @@ def matmul_mxfp6(out, X, Xscales, W, Wscales, batch, cols, rows, stream=None):
     code = _c_matmul_mxfp6(out, X, Xscales, W, Wscales, batch, cols, rows, stream)
     if code:
         _check(code, "l2c_matmul_mxfp6")
+
+
+def quantize_mxfp4_bf16(codes, scales, xbf16, rows, cols, stream=None):
+    code = _c_quantize_mxfp4_bf16(codes, scales, xbf16, rows, cols, stream)
+    if code:
+        _check(code, "l2c_quantize_mxfp4_bf16")
+
+
+def matmul_mxfp4(out, X, Xscales, W, Wscales, batch, cols, rows, stream=None):
+    code = _c_matmul_mxfp4(out, X, Xscales, W, Wscales, batch, cols, rows, stream)
+    if code:
+        _check(code, "l2c_matmul_mxfp4")

@@ -33,6 +33,11 @@
  *   l2c_decoder_rmsnorm         rmsnorm_kernel         applications/loom_private/decoder/decoder.cu:45-77
  *   l2c_decoder_softmax_argmax  softmax_argmax_kernel  applications/loom_private/decoder/decoder.cu:127-198
  *   (the decoder's classifier_kernel, decoder.cu:79-125, is l2c_matmul)
+ *   l2c_residual_rmsnorm, l2c_quantize_mxfp4_bf16, l2c_matmul_mxfp4,
+ *   l2c_decoder_beam_select, l2c_decoder_beam_reorder
+ *                 no kernels in the reference: the norms around a block with its
+ *                 residual, the product of 4-bit operands and the beam-search form
+ *                 of the decoder's step
  */
 #ifndef L2C_H
 #define L2C_H
@@ -59,6 +64,12 @@ enum l2c_qformat {
                       fp32 scale per row: scales[r] */
 };
 
+/* Element types of l2c_residual_rmsnorm's tensors. */
+enum l2c_type {
+  L2C_F32 = 0,
+  L2C_BF16 = 1 /* uint16 bit patterns */
+};
+
 /*
  * out[b][j] = in[b][j] * (1 / sqrt(sum_j in[b][j]^2 / size + eps)) * weight[j]
  * for b < batch, j < size; rows are `size` floats apart.
@@ -66,6 +77,30 @@ enum l2c_qformat {
  */
 int l2c_rmsnorm(float *out, const float *in, const float *weight, int size, int batch,
                 float eps, hipStream_t stream);
+
+/*
+ * The sum after a block and the norm before the next, in one launch. For b < batch,
+ * j < size, rows `size` values apart:
+ *   z = block[b][j] * (1 / sqrt(mean_j block[b]^2 + eps)) * block_weight[j]
+ *   h = residual_scale * residual[b][j] + gate[b / rows_per_gate][j] * z
+ *   normalized[b][j] = h * (1 / sqrt(mean_j h[b]^2 + eps)) * weight[j]
+ *   residual_out[b][j] = h
+ * block_weight NULL: the block's output is not normalized (z = block). gate NULL: no
+ * gate (1); rows_per_gate >= batch: one gate vector for all rows; 1: one for each.
+ * residual_out NULL: h is not kept (after the last block).
+ * residual and residual_out are of residual_type, block of block_type, normalized of
+ * normalized_type (enum l2c_type); weights and gates are fp32. All arithmetic is fp32;
+ * h and normalized are rounded once, to nearest even (bf16 overflows to infinity), and
+ * normalized is computed from h before that rounding.
+ * An output may be an input (residual_out == residual or block, normalized == block or
+ * residual, of the same type), but the outputs are not each other and overlap nothing
+ * in part. Pointers need their elements' alignment (4 or 2 bytes).
+ */
+int l2c_residual_rmsnorm(void *normalized, int normalized_type, void *residual_out,
+                         const void *residual, int residual_type, const void *block, int block_type,
+                         const float *block_weight, const float *gate, int rows_per_gate,
+                         const float *weight, int size, int batch, float residual_scale, float eps,
+                         hipStream_t stream);
 
 /*
  * out[b][j] = exp(logits[b][j] - max_b) / sum_j exp(logits[b][j] - max_b).
@@ -246,6 +281,27 @@ int l2c_matmul_mxfp6(float *out, const uint8_t *X, const uint8_t *Xscales, const
                      const uint8_t *Wscales, int batch, int cols, int rows, hipStream_t stream);
 
 /*
+ * Products of 4-bit operands on the scaled matrix cores, which take them at twice the
+ * rate of l2c_matmul_qs's 8-bit activations:
+ * l2c_quantize_mxfp4_bf16: bf16 activations [rows][cols] (cols % 32 == 0, Xbf16 and
+ *   codes 16-byte aligned) to MXFP4 in l2c_quantize_mxfp4's layout: codes [rows][cols / 2],
+ *   scales [rows][cols / 32]. Per 32 consecutive values the shared exponent is X =
+ *   floor(log2(block max)) - 2, at least -127 (a zero block gets -127), scale code X + 127,
+ *   codes e2m1(x * 2^-X), nearest, ties to the even code, saturating at 6, -0 encoded as
+ *   +0. A block with an Inf or a NaN gets scale code 0xff (NaN) and zero codes, so every
+ *   output of its row becomes NaN.
+ * l2c_matmul_mxfp4: out[b][r] = sum_k deq(X, Xscales)[b][k] * deq(W, Wscales)[r][k], X
+ *   batch x cols, W rows x cols, both as l2c_quantize_mxfp4 or l2c_quantize_mxfp4_bf16
+ *   writes them (cols % 32 == 0, X and W 16-byte aligned; scales at any address), out
+ *   batch x rows, row-major. Products of the dequantized operands are exact, sums fp32.
+ * Operands stay addressable in 31 bits for a tile's rows: cols below 2^24.
+ */
+int l2c_quantize_mxfp4_bf16(uint8_t *codes, uint8_t *scales, const uint16_t *Xbf16, int rows, int cols,
+                            hipStream_t stream);
+int l2c_matmul_mxfp4(float *out, const uint8_t *X, const uint8_t *Xscales, const uint8_t *W,
+                     const uint8_t *Wscales, int batch, int cols, int rows, hipStream_t stream);
+
+/*
  * Batched greedy decoder (applications/loom_private/decoder): one step is
  *   l2c_decoder_rmsnorm -> l2c_matmul(logits, normalized, classifier) ->
  *   l2c_decoder_softmax_argmax
@@ -277,6 +333,52 @@ int l2c_decoder_rmsnorm_absmax(float *normalized, const int *tokens, const float
 int l2c_decoder_softmax_argmax(float *probabilities, const float *logits, int *tokens,
                                int *generated, int vocab, int batch, int steps, int step,
                                hipStream_t stream);
+
+/*
+ * Beam search for the batched decoder: `batch` requests of `beams` beams (1 to
+ * L2C_MAX_BEAMS), beam k of request b in row b * beams + k. One step is
+ *   l2c_decoder_rmsnorm -> l2c_matmul(logits, ...) over the batch * beams rows ->
+ *   l2c_decoder_beam_select -> l2c_decoder_beam_reorder of whatever state the rows have.
+ *
+ * l2c_decoder_beam_select: the `beams` best continuations of every request among
+ *   scores[row k] + logits[row k][v] - log(sum_u exp(logits[row k][u]))
+ *   over its beams k and tokens v < vocab, the largest first, equal scores in the order of
+ *   (k, v). They become the request's next beams: scores_out, tokens_out (v) and parents
+ *   (k) in rows b * beams + 0, 1, ...; and generated[row * steps + step] = v, unless
+ *   generated is NULL (the earlier columns follow by l2c_decoder_beam_reorder).
+ *   A beam whose token tokens[row k] is eos (eos >= 0) has ended: its one continuation is
+ *   eos at its own score, and its logits are not read. A beam has no continuation if its
+ *   score is not finite (start a request with scores 0, -Inf, -Inf, ...), or its row holds a
+ *   NaN or a +Inf or nothing but -Inf; nor has a token whose logit is -Inf. Where fewer than
+ *   `beams` are left, the other rows get score -Inf, token -1 and parent -1.
+ *   Scores are computed in 64 bits (the exponentials in 32) and rounded once.
+ *   scores_out may be scores and tokens_out may be tokens. workspace: 16-byte aligned, at
+ *   least l2c_decoder_beam_workspace_bytes (0 for sizes that are not supported), which is
+ *   at most batch * beams * ceil(vocab / 1024) * (8 * beams + 16); its contents need not be
+ *   kept between calls, and calls that share one must be ordered.
+ *
+ * l2c_decoder_beam_reorder: lets state follow the beams, for g < groups, b < batch, k <
+ *   beams and every byte of the row's pieces:
+ *     out[g][b][k] = in[g][b][parents[b * beams + k]]
+ *   A row is `pieces` pieces of piece_bytes, piece_stride apart; rows are row_stride apart
+ *   and groups (layers, say) group_stride apart, all in bytes, the same in `in` and `out`;
+ *   each stride is at least the extent of what it separates. Bytes between the pieces are
+ *   left as they are, and so is a row whose parent lies outside [0, beams). A cache
+ *   [layers][batch * beams][heads][positions][width] of which the first `live` positions
+ *   are in use has pieces = heads and piece_bytes = live * width * element size.
+ *   out == in moves the rows in place; otherwise the two do not overlap. Any alignment
+ *   (16-byte addresses and strides are fastest). A row has at most 2^31 - 1 units of 16
+ *   bytes and odd bytes.
+ */
+#define L2C_MAX_BEAMS 32
+size_t l2c_decoder_beam_workspace_bytes(int vocab, int beams, int batch);
+int l2c_decoder_beam_select(float *scores_out, int *tokens_out, int *parents, int *generated,
+                            const float *logits, const float *scores, const int *tokens, int eos,
+                            int vocab, int beams, int batch, int steps, int step, void *workspace,
+                            size_t workspace_bytes, hipStream_t stream);
+int l2c_decoder_beam_reorder(void *out, const void *in, const int *parents, int beams, int batch,
+                             int groups, int pieces, long long group_stride, long long row_stride,
+                             long long piece_stride, long long piece_bytes, hipStream_t stream);
 
 /*
  * bytes from device memory `src` to pinned host memory `host_dst`

@@ -12,6 +12,7 @@
 #include <climits>
 
 #include "l2c_common.h"
+#include "l2c_mx4gemm.h"
 #include "../../include/l2c.h"
 
 namespace {
@@ -138,6 +139,10 @@ extern "C" int l2c_matmul_mxfp4(float *out, const uint8_t *X, const uint8_t *Xsc
   if (batch == 0 || rows == 0) return hipSuccess;
   if (!out || !X || !Xscales || !W || !Wscales || !l2c_aligned16(X) || !l2c_aligned16(W)) return hipErrorInvalidValue;
   if (256LL * (cols / 2) > INT_MAX) return hipErrorInvalidValue;
+  if (batch > 128 && l2c_mx4_tiles(out, X, Xscales, W, Wscales, batch, cols / 32, rows, stream)) {
+    L2C_LAUNCH_CHECK();
+    return hipSuccess;
+  }
   const long long tiles = ((batch + 15LL) / 16) * ((rows + 15LL) / 16);
   if (!l2c::launchable(tiles, kWaves * L2C_WAVE)) return hipErrorInvalidValue;
   hipLaunchKernelGGL(mxfp4_gemm_kernel, dim3(static_cast<unsigned>(tiles)), dim3(kWaves * L2C_WAVE), 0, stream, out, X,

@@ -177,3 +177,5 @@ bool l2c_scgemm_ksplit(float *out, const uint8_t *X, const uint8_t *Xs, const ui
                        int fmt, int batch, int cols, int rows, hipStream_t stream);
 bool l2c_scgemm_ksplit_launch_shape(int fmt, int batch, int cols, int rows, int *grid, int *block, const void **fn);
 void (*l2c_qgemm_mid_kernel(int fmt))(float *, const uint16_t *, const uint8_t *, const void *, int, int, int);
+// Launch shape of l2c_matmul_mxfp4 (l2c_mx4gemm.hip); false for shapes it does not launch.
+bool l2c_mx4_launch_shape(int batch, int cols, int rows, int *grid, int *block, const void **fn);

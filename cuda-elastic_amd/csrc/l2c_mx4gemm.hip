@@ -17,11 +17,7 @@
 
 namespace {
 
-using l2c::f32x4;
-typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-
-constexpr int kE2M1 = 4;  // MFMA operand format
 
 // ---------------------------------------------------------------------------
 // bf16 activations to MXFP4. A block's shared exponent is floor(log2(maximum)) - 2, at
@@ -71,50 +67,30 @@ __global__ __launch_bounds__(kQuantThreads) void quantize_mxfp4_bf16_kernel(uint
 }
 
 // ---------------------------------------------------------------------------
-// The contraction: a workgroup computes 16 x 16 outputs, its waves every kWaves-th
-// 128-deep step each, operands straight from memory into registers.
-//
-// v_mfma_scale_f32_16x16x128_f8f6f4 in format E2M1: lane (r, q) = (l % 16, l / 16)
-// supplies row r's block q (k 32 q .. 32 q + 31), 16 bytes, and its scale byte; value v
-// of lane l of the result is C[4 (l / 16) + v][l % 16].
+// Choice of the contraction's tile: the one of least estimated time. Fitted to the times of
+// these and 18 other tiles on 132 shapes of 1 to 1024 x 288 to 16384 x 600 to 11008: what a
+// CU takes for its tiles in turn is linear in their number and in K to about 12%, and
+// the choice among these eight is 3% slower than the best of the 26 in the mean. Measured
+// on either side of a border, us: 33 x 5024 x 8004 12.5 on 32 x 32 tiles, 11.2 on 64 x
+// 64; 128 x 4096 x 11008 13.1 on 64 x 64, 11.2 on 64 x 128; 400 x 4096 x 11008 27.2 on
+// 128 x 128, 21.1 on 256 x 128.
 
-constexpr int kWaves = 4;
+long long tiles_of(const l2c::Mx4Tile &t, int batch, int rows) {
+  return ((batch + static_cast<long long>(t.bm) - 1) / t.bm) * ((rows + static_cast<long long>(t.bn) - 1) / t.bn);
+}
 
-__global__ __launch_bounds__(kWaves *L2C_WAVE) void mxfp4_gemm_kernel(float *__restrict__ out,
-                                                                      const uint8_t *__restrict__ X,
-                                                                      const uint8_t *__restrict__ Xs,
-                                                                      const uint8_t *__restrict__ W,
-                                                                      const uint8_t *__restrict__ Ws, int M, int N,
-                                                                      int blocks) {
-  __shared__ float partial[kWaves][256];
-  const int tile = l2c::xcd_tile(blockIdx.x, gridDim.x);
-  const int mtiles = (M + 15) / 16;
-  const int m0 = tile % mtiles * 16, n0 = tile / mtiles * 16;
-  const int lane = threadIdx.x % L2C_WAVE, wave = threadIdx.x / L2C_WAVE;
-  const int r = lane % 16, q = lane / 16;
-  const size_t xrow = static_cast<size_t>(min(m0 + r, M - 1)) * blocks;
-  const size_t wrow = static_cast<size_t>(min(n0 + r, N - 1)) * blocks;
-  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int s = wave; 4 * s < blocks; s += kWaves) {
-    const int block = min(4 * s + q, blocks - 1);
-    u32x4 x = *reinterpret_cast<const u32x4 *>(X + 16 * (xrow + block));
-    const u32x4 w = *reinterpret_cast<const u32x4 *>(W + 16 * (wrow + block));
-    const int xs = Xs[xrow + block], ws = Ws[wrow + block];
-    if (4 * s + q >= blocks) x = u32x4{0u, 0u, 0u, 0u};
-    i32x8 a = {0, 0, 0, 0, 0, 0, 0, 0}, b = a;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) a[e] = static_cast<int>(x[e]), b[e] = static_cast<int>(w[e]);
-    acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, kE2M1, kE2M1, 0, xs, 0, ws);
-  }
-#pragma unroll
-  for (int v = 0; v < 4; ++v) partial[wave][v * L2C_WAVE + lane] = acc[v];
-  __syncthreads();
-  const int v = wave;  // value v of the waves' lanes
-  float sum = partial[0][threadIdx.x];
-#pragma unroll
-  for (int w = 1; w < kWaves; ++w) sum += partial[w][threadIdx.x];
-  const int m = m0 + 4 * q + v, n = n0 + r;
-  if (m < M && n < N) out[static_cast<size_t>(m) * N + n] = sum;
+const l2c::Mx4Tile *choose(int batch, int blocks, int rows) {
+  const l2c::Mx4Tile *best = nullptr;
+  double least = 0.0;
+  auto consider = [&](const l2c::Mx4Tile &t) {
+    const long long tiles = tiles_of(t, batch, rows);
+    if (blocks < t.min_blocks || !l2c::launchable(tiles, t.threads)) return;
+    const double cost = t.launch + static_cast<double>((tiles + 255) / 256) * (t.tile + t.k * 32.0 * blocks);
+    if (!best || cost < least) best = &t, least = cost;
+  };
+  for (const l2c::Mx4Tile &t : l2c::mx4_row_tiles) consider(t);
+  for (const l2c::Mx4Tile &t : l2c::mx4_lds_tiles) consider(t);
+  return best;
 }
 
 }  // namespace
@@ -139,14 +115,19 @@ extern "C" int l2c_matmul_mxfp4(float *out, const uint8_t *X, const uint8_t *Xsc
   if (batch == 0 || rows == 0) return hipSuccess;
   if (!out || !X || !Xscales || !W || !Wscales || !l2c_aligned16(X) || !l2c_aligned16(W)) return hipErrorInvalidValue;
   if (256LL * (cols / 2) > INT_MAX) return hipErrorInvalidValue;
-  if (batch > 128 && l2c_mx4_tiles(out, X, Xscales, W, Wscales, batch, cols / 32, rows, stream)) {
-    L2C_LAUNCH_CHECK();
-    return hipSuccess;
-  }
-  const long long tiles = ((batch + 15LL) / 16) * ((rows + 15LL) / 16);
-  if (!l2c::launchable(tiles, kWaves * L2C_WAVE)) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(mxfp4_gemm_kernel, dim3(static_cast<unsigned>(tiles)), dim3(kWaves * L2C_WAVE), 0, stream, out, X,
+  const l2c::Mx4Tile *t = choose(batch, cols / 32, rows);
+  if (!t) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(t->fn, dim3(static_cast<unsigned>(tiles_of(*t, batch, rows))), dim3(t->threads), 0, stream, out, X,
                      Xscales, W, Wscales, batch, rows, cols / 32);
   L2C_LAUNCH_CHECK();
   return hipSuccess;
+}
+
+bool l2c_mx4_launch_shape(int batch, int cols, int rows, int *grid, int *block, const void **fn) {
+  const l2c::Mx4Tile *t = batch > 0 && rows > 0 && cols % 32 == 0 ? choose(batch, cols / 32, rows) : nullptr;
+  if (!t) return false;
+  *grid = static_cast<int>(tiles_of(*t, batch, rows));
+  *block = t->threads;
+  *fn = reinterpret_cast<const void *>(t->fn);
+  return true;
 }

@@ -11,7 +11,7 @@
 //    wave's sub-tile is twice as large as with eight, which saves a quarter of the LDS
 //    reads (256 x 128: 96 KB in 1024 cycles of MFMA a step).
 //  * A step is 256 k: 128 bytes a row, a whole cache line. LDS DMA (16 B a lane) fills
-//    three stages; step t + 2 is under way while step t is multiplied. The 16-byte
+//    STAGES stages, all but one under way while a step is multiplied. The 16-byte
 //    blocks of a row are stored XOR-swizzled by the row.
 //  * Which block of a step a lane multiplies when is free, as long as X and W agree:
 //    half h of group g takes blocks 4 h + 2 g and 4 h + 2 g + 1, whose scale bytes are
@@ -40,7 +40,6 @@ typedef __attribute__((address_space(3))) void lds_ptr;
 
 constexpr int kE2M1 = 4;
 constexpr int kThreads = 512;
-constexpr int kStages = 3;
 constexpr int kRow = 128;  // code bytes of a row and step
 constexpr int kQueue = 4;  // pairs of steps whose scales a lane loads at once
 
@@ -63,8 +62,9 @@ __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t rsrc, unsigned char
   __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr *)dst, 16, voffset, soffset, 0, 0);
 }
 
-template <int MI, int NI>
+template <int MI, int NI, int STAGES>
 struct Tile {
+  static constexpr int kStages = STAGES;
   static constexpr int kBM = 64 * MI, kBN = 64 * NI;
   static constexpr int kStage = (kBM + kBN) * kRow;
   static constexpr int kDma = (kBM + kBN) / 64;  // a wave's DMAs of 8 rows a step
@@ -74,12 +74,13 @@ struct Tile {
   static_assert(kBM + kBN <= kThreads, "a lane loads the scales of one row");
 };
 
-template <int MI, int NI>
+template <int MI, int NI, int STAGES>
 __global__ __launch_bounds__(kThreads) void mxfp4_tile_kernel(float *__restrict__ out, const uint8_t *__restrict__ X,
                                                               const uint8_t *__restrict__ Xs,
                                                               const uint8_t *__restrict__ W,
                                                               const uint8_t *__restrict__ Ws, int M, int N, int blocks) {
-  using T = Tile<MI, NI>;
+  using T = Tile<MI, NI, STAGES>;
+  constexpr int kStages = STAGES;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[T::kLds];
   const int tile = l2c::xcd_tile(blockIdx.x, gridDim.x);
   const int mtiles = (M + T::kBM - 1) / T::kBM;
@@ -139,12 +140,12 @@ __global__ __launch_bounds__(kThreads) void mxfp4_tile_kernel(float *__restrict_
 #pragma unroll
     for (int i = 0; i < T::kDma; ++i) dma(stage, t, i);
   };
-  // All but this wave's newest loads, a step's DMAs, have landed and its LDS accesses are
-  // done; then the workgroup's barrier. Nothing is scheduled across it. (The loads of scales
+  // All but the DMAs of this wave's newest steps have landed and its LDS accesses are done;
+  // then the workgroup's barrier. Nothing is scheduled across it. (The loads of scales
   // come ahead of the DMAs; wherever they are, they make the wait stricter.)
   auto sync = [&]() __attribute__((always_inline)) {
     __builtin_amdgcn_sched_barrier(0);
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(T::kDma) : "memory");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((kStages - 2) * T::kDma) : "memory");
     __builtin_amdgcn_sched_barrier(0);
   };
 
@@ -171,7 +172,7 @@ __global__ __launch_bounds__(kThreads) void mxfp4_tile_kernel(float *__restrict_
   };
   // Step t, in stage `at`: the products of its first half, among them the reads of its
   // second half's fragments; then, with all waves past their reads of the stage, the
-  // second half's, among them step t + 3's DMAs into the stage and the reads of step t + 1's
+  // second half's, among them step t + STAGES's DMAs into the stage and the reads of step t + 1's
   // first half. One of each a product: a wave issues in order, and six DMAs in a row hold
   // up what follows them. Steps go in pairs: the second of pair u stores the scales of pair
   // u + 2 once all waves have read those of u + 1, as they do in its first.
@@ -196,7 +197,7 @@ __global__ __launch_bounds__(kThreads) void mxfp4_tile_kernel(float *__restrict_
 #pragma unroll
     for (int k = 0; k < kRounds; ++k) {
       if (k < kProducts) multiply(Second{}, parity, k, now);
-      if (k < T::kDma) dma(at, min(t + 3, last), k);
+      if (k < T::kDma) dma(at, min(t + kStages, last), k);
       if (k < kReads) read(after, 0, k);
       if (!kOdd && k < kReads) read_scales(next, k);
       __builtin_amdgcn_sched_barrier(0);
@@ -213,13 +214,14 @@ __global__ __launch_bounds__(kThreads) void mxfp4_tile_kernel(float *__restrict_
     }
   };
   load_scales(0);
-  dma_step(0, 0);
-  dma_step(1, min(1, last));
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int s = 0; s < kStages; ++s) dma_step(s, min(s, last));
+  __builtin_amdgcn_sched_barrier(0);
   store_scales(queue[0]);
 #pragma unroll
-  for (int k = 0; k < kQueue; ++k) asm volatile("" : "+v"(queue[k]));  // not sunk behind the DMAs
-  dma_step(2, min(2, last));
-  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * T::kDma) : "memory");
+  for (int k = 0; k < kQueue; ++k) asm volatile("" : "+v"(queue[k]));  // loaded here, not where they are used
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((kStages - 1) * T::kDma) : "memory");
 #pragma unroll
   for (int k = 0; k < kReads; ++k) {
     read(0, 0, k);
@@ -310,15 +312,13 @@ __global__ __launch_bounds__(kThreads) void mxfp4_tile_kernel(float *__restrict_
   else finish(Second{});
 }
 
+template <int MI, int NI, int STAGES>
+constexpr l2c::Mx4Tile tile(double launch, double per_tile, double per_k) {
+  using T = Tile<MI, NI, STAGES>;
+  return {mxfp4_tile_kernel<MI, NI, STAGES>, T::kBM, T::kBN, kThreads, 16, launch, per_tile, per_k};
+}
+
 }  // namespace
 
-bool l2c_mx4_tiles(float *out, const uint8_t *X, const uint8_t *Xs, const uint8_t *W, const uint8_t *Ws, int batch,
-                   int blocks, int rows, hipStream_t stream) {
-  if (blocks < 16) return false;
-  const int mi = 4, ni = 2;
-  const long long tiles = static_cast<long long>((batch + 64 * mi - 1) / (64 * mi)) * ((rows + 64 * ni - 1) / (64 * ni));
-  if (!l2c::launchable(tiles, kThreads)) return false;
-  hipLaunchKernelGGL((mxfp4_tile_kernel<4, 2>), dim3(static_cast<unsigned>(tiles)), dim3(kThreads), 0, stream, out, X, Xs, W,
-                     Ws, batch, rows, blocks);
-  return true;
-}
+const l2c::Mx4Tile l2c::mx4_lds_tiles[kMx4LdsTiles] = {tile<1, 1, 4>(2400, 1210, 1.08), tile<1, 2, 4>(700, 3500, 1.60),
+                                                       tile<2, 2, 4>(0, 5600, 1.97), tile<4, 2, 3>(1100, 6600, 2.76)};

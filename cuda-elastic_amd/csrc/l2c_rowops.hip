@@ -480,6 +480,9 @@ extern "C" int l2c_launch_shape(int op, int batch, int cols, int rows, int varia
       *block = 512;
       return l2c_scgemm_occupancy(variant, wide, blocks_per_cu);
     }
+    case L2C_OP_MATMUL_MXFP4:
+      if (!l2c_mx4_launch_shape(batch, cols, rows, grid, block, &fn)) return hipErrorInvalidValue;
+      break;
     default:
       return hipErrorInvalidValue;
   }

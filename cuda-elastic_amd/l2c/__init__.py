@@ -43,7 +43,7 @@ MATVEC_NAIVE = 0
 MATVEC_COALESCED = 1
 Q_MXFP4 = 0
 Q_FP8 = 1
-OP_RMSNORM, OP_SOFTMAX, OP_MATVEC, OP_FUSED, OP_MATMUL, OP_MATMUL_Q, OP_MATMUL_QS = range(7)
+OP_RMSNORM, OP_SOFTMAX, OP_MATVEC, OP_FUSED, OP_MATMUL, OP_MATMUL_Q, OP_MATMUL_QS, OP_MATMUL_MXFP4 = range(8)
 
 # Symbols declared in include/l2c.h and include/l2c_harness.h.
 KERNEL_SYMBOLS = (

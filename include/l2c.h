@@ -400,7 +400,8 @@ enum l2c_op {
   L2C_OP_FUSED = 3,
   L2C_OP_MATMUL = 4,
   L2C_OP_MATMUL_Q = 5,
-  L2C_OP_MATMUL_QS = 6  /* the contraction kernel of l2c_matmul_qs */
+  L2C_OP_MATMUL_QS = 6, /* the contraction kernel of l2c_matmul_qs */
+  L2C_OP_MATMUL_MXFP4 = 7
 };
 
 /*

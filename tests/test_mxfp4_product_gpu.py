@@ -133,6 +133,28 @@ def test_product_shapes(torch_gpu, l2c, batch, cols, rows):
     check_product(torch_gpu, l2c, batch, cols, rows)
 
 
+# Every kernel: lanes, batch rows and weight rows of its tile, and shapes that run on it, with
+# ragged edges, one step to many, odd and even steps and a part of one at the end.
+KERNELS = [((512, 16, 16), [(7, 544, 1003), (1, 11008, 500), (16, 4128, 900)]),
+           ((512, 16, 32), [(13, 512, 8004), (5, 4096, 8190), (128, 8192, 1003)]),
+           ((256, 32, 32), [(61, 288, 5003), (40, 800, 8001), (300, 480, 1009)]),
+           ((512, 32, 32), [(63, 8192, 3001), (100, 10016, 1403), (256, 8192, 1000)]),
+           ((512, 64, 64), [(200, 544, 3800), (64, 4064, 11001), (1021, 2016, 1003), (1000, 8224, 1001)]),
+           ((512, 64, 128), [(120, 3904, 10003), (505, 1312, 3003), (1000, 16384, 2001)]),
+           ((512, 128, 128), [(240, 4096, 10001), (513, 2080, 4003), (1010, 11008, 4001)]),
+           ((512, 256, 128), [(1011, 768, 8001), (400, 4192, 11002)])]
+
+
+@pytest.mark.parametrize("kernel,shapes", KERNELS, ids=str)
+def test_every_kernel(torch_gpu, l2c, kernel, shapes):
+    lanes, bm, bn = kernel
+    for batch, cols, rows in shapes:
+        grid, block, per_cu = l2c.launch_shape(l2c.OP_MATMUL_MXFP4, batch, cols, rows)
+        assert (grid, block) == (-(-batch // bm) * -(-rows // bn), lanes), (batch, cols, rows)
+        assert per_cu >= 1
+        check_product(torch_gpu, l2c, batch, cols, rows, shift=1)
+
+
 @pytest.mark.parametrize("batch,cols,rows", [(2, 160, 40), (300, 608, 520), (1024, 1056, 1100)])
 def test_nan_scales(torch_gpu, l2c, batch, cols, rows):
     """A row with a NaN scale in its last block gives NaN in all its outputs and no others."""

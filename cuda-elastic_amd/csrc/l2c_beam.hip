@@ -6,15 +6,16 @@
 // over all beams k and tokens v; the `beams` largest are the next beams. Two kernels:
 //
 //  * beam_chunks_kernel, a workgroup per chunk of a row of logits: one pass over the
-//    data, which the lanes hold in registers. It leaves the chunk's maximum, its sum of
-//    exponentials and its `beams` largest logits in order. Nothing is sorted: the K-th
-//    largest of a wave's 64 lane maxima is a bound that at least K values of the chunk
-//    reach, and few more do. It is found bit by bit, a ballot a bit. The values that
-//    reach the largest of the waves' bounds go to a list in LDS, where each finds its
-//    rank by comparison with the others. A wave has at most K lanes whose maximum
-//    reaches the bound, so the list's length has a bound too.
+//    data, 1024 V logits at a time, which the lanes hold in registers. It leaves the
+//    chunk's maximum, its sum of exponentials and its `beams` largest logits in order.
+//    Nothing is sorted: the K-th largest of the maxima of a wave's groups of 8 to 32 values
+//    is a bound that at least K values reach, and few more do. It is found bit by bit, by
+//    ballots. The values that reach the largest of the waves' bounds (and the K-th so far)
+//    go to a list in LDS, where each finds its rank by comparison with the others. A wave
+//    has at most K groups that reach the bound, so the list's length has a bound too.
 //  * beam_join_kernel, a workgroup per request: the rows' sums, and the same choice
-//    among the chunks' lists by their 64-bit scores.
+//    among the chunks' lists by their 64-bit scores. Rows are cut into no more chunks than
+//    leave it kJoinCandidates candidates.
 //
 // The order is total: larger first, then the lower beam, then the lower token; within
 // a row by the logits themselves. Results do not depend on the order of the list's
@@ -34,7 +35,8 @@ constexpr int kMaxBeams = L2C_MAX_BEAMS;
 
 typedef unsigned long long u64;
 
-// What a chunk leaves in the workspace, followed by `beams` candidates.
+// The workspace: what every chunk of every row leaves, [row][chunk]; then the candidates,
+// [request][rank][beam][chunk]: the join's lanes read the chunks' best side by side.
 struct ChunkStat {
   double sum;  // of exp(x - maximum); NaN if the chunk holds a NaN or +Inf
   float maximum;
@@ -44,9 +46,6 @@ struct Candidate {
   float logit;
   int token;  // -1: none
 };
-__host__ __device__ __forceinline__ size_t chunk_bytes(int beams) {
-  return sizeof(ChunkStat) + sizeof(Candidate) * static_cast<size_t>(beams);
-}
 
 // Unsigned keys in the order of the numbers; 0 is below every number's key and NaN's.
 __device__ __forceinline__ unsigned key_of(float v) {
@@ -64,15 +63,17 @@ __device__ __forceinline__ double number_of(u64 key) {
   return __longlong_as_double((key >> 63) ? key & ~(1ULL << 63) : ~key);
 }
 
-// The largest T that at least k of the wave's 64 values reach: the k-th largest.
-template <typename T>
-__device__ __forceinline__ T wave_kth(T v, int k) {
-  T bound = 0;
-  for (int bit = 8 * sizeof(T) - 1; bit >= 0; --bit) {
-    const T next = bound | (static_cast<T>(1) << bit);
-    if (__popcll(__ballot(v >= next)) >= k) bound = next;
-  }
-  return bound;
+// exp(t) for t <= 0: the hardware's exp2 of t log2(e) rounded, times 1 + ln(2) times what
+// the rounding left, to about 1.2 ulp; NaN stays NaN, results below 2^-126 may be 0.
+__device__ __forceinline__ float exp_nonpositive(float t) {
+  constexpr float kLog2e = 1.44269504088896340736f;
+  constexpr float kLog2eLow = 1.925963033500011e-08f;  // log2(e) - kLog2e
+  constexpr float kLn2 = 0.693147180559945309417f;
+  t = t < -150.0f ? -150.0f : t;
+  const float high = t * kLog2e;
+  const float low = fmaf(t, kLog2eLow, fmaf(t, kLog2e, -high));
+  const float e = __builtin_amdgcn_exp2f(high);
+  return fmaf(e, low * kLn2, e);
 }
 
 // 64-bit order of a chunk's values: the logit, then the lower place first.
@@ -80,116 +81,298 @@ __device__ __forceinline__ u64 ordered(unsigned key, unsigned place) {
   return (static_cast<u64>(key) << 32) | (UINT_MAX - place);
 }
 
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-  for (int offset = 32; offset > 0; offset >>= 1) v += __shfl_xor(v, offset, L2C_WAVE);
-  return v;
+// Values of other lanes through the adders' operand paths (DPP), which take a tenth of a
+// trip through LDS: from 1, 2, 4 or 8 lanes before in rows of 16, from the row before's
+// last lane, from the lower half's last lane; or rotated in rows of 16.
+enum Dpp { kBefore1 = 0x111, kBefore2 = 0x112, kBefore4 = 0x114, kBefore8 = 0x118, kRowBefore = 0x142, kHalfBefore = 0x143,
+           kRotate1 = 0x121, kRotate2 = 0x122, kRotate4 = 0x124, kRotate8 = 0x128 };
+
+// `none` where there is no such lane.
+template <int FROM>
+__device__ __forceinline__ int other(int v, int none = 0) {
+  constexpr int kRows = FROM == kRowBefore ? 0xa : FROM == kHalfBefore ? 0xc : 0xf;
+  return __builtin_amdgcn_update_dpp(none, v, FROM, kRows, 0xf, false);
+}
+template <int FROM>
+__device__ __forceinline__ float other(float v, float none) {
+  return __int_as_float(other<FROM>(__float_as_int(v), __float_as_int(none)));
+}
+template <int FROM>
+__device__ __forceinline__ double other(double v) {  // none: 0
+  const long long bits = __double_as_longlong(v);
+  const unsigned low = other<FROM>(static_cast<int>(bits)), high = other<FROM>(static_cast<int>(bits >> 32));
+  return __longlong_as_double(static_cast<long long>(high) << 32 | low);
 }
 
-// V float4 a lane; `chunks` chunks of kThreads * 4 V logits a row.
-template <int V>
+// The sum of v over this lane and those before it; lane 63 has the wave's.
+template <typename T>
+__device__ __forceinline__ T wave_scan(T v) {
+  v += other<kBefore1>(v);
+  v += other<kBefore2>(v);
+  v += other<kBefore4>(v);
+  v += other<kBefore8>(v);
+  v += other<kRowBefore>(v);
+  v += other<kHalfBefore>(v);
+  return v;
+}
+// Lane 63 has the wave's maximum.
+__device__ __forceinline__ float wave_top(float v) {
+  v = fmaxf(v, other<kBefore1>(v, v));
+  v = fmaxf(v, other<kBefore2>(v, v));
+  v = fmaxf(v, other<kBefore4>(v, v));
+  v = fmaxf(v, other<kBefore8>(v, v));
+  v = fmaxf(v, other<kRowBefore>(v, v));
+  return fmaxf(v, other<kHalfBefore>(v, v));
+}
+// Every lane has its 16 lanes' maximum, or sum.
+__device__ __forceinline__ float row_max(float v) {
+  v = fmaxf(v, other<kRotate8>(v, v));
+  v = fmaxf(v, other<kRotate4>(v, v));
+  v = fmaxf(v, other<kRotate2>(v, v));
+  return fmaxf(v, other<kRotate1>(v, v));
+}
+__device__ __forceinline__ double row_sum(double v) {
+  v += other<kRotate8>(v);
+  v += other<kRotate4>(v);
+  v += other<kRotate2>(v);
+  return v + other<kRotate1>(v);
+}
+
+// A bound that at least k of the wave's 64 G values reach: exactly k of them, or, where the
+// k-th largest ties with the next, all that are as large, and the bound is that value. 0 if
+// fewer than k are not 0. A bit at a time, to where just k are left: the steps wait for
+// each other, but are scalar instructions for the most part, which other waves leave idle
+// (starting at the first bit in which the values differ, or two bits a step, measured 20%
+// slower for 256 x 4 x 32003).
+template <typename T, int G>
+__device__ __forceinline__ int wave_reach(const T (&v)[G], T bound) {
+  int reach = 0;
+#pragma unroll
+  for (int g = 0; g < G; ++g) reach += __popcll(__ballot(v[g] >= bound));
+  return reach;
+}
+template <int G>
+__device__ __forceinline__ unsigned wave_bound(const unsigned (&v)[G], int k) {
+  unsigned bound = 0;
+  for (int bit = 31; bit >= 0; --bit) {
+    const unsigned next = bound | 1u << bit;
+    const int reach = wave_reach(v, next);
+    if (reach >= k) bound = next;
+    if (reach == k) break;
+  }
+  return bound;
+}
+// Of one 64-bit value a lane, two bits a step, whose ballots do not wait for each other: one
+// wave's time counts where nothing else runs.
+__device__ __forceinline__ u64 wave_bound(u64 value, int k) {
+  const u64 v[1] = {value};
+  u64 bound = 0;
+  if (wave_reach(v, static_cast<u64>(1)) < k) return bound;
+  for (int bit = 62; bit >= 0; bit -= 2) {
+    const u64 one = bound | 1ULL << bit, two = bound | 2ULL << bit, three = one | two;
+    const int reach1 = wave_reach(v, one), reach2 = wave_reach(v, two), reach3 = wave_reach(v, three);
+    bound = reach3 >= k ? three : reach2 >= k ? two : reach1 >= k ? one : bound;
+    if (reach3 == k || reach2 == k || reach1 == k) break;
+  }
+  return bound;
+}
+
+// How many of n values are larger, and how many equal. Reads in eights, up to seven past
+// the end: one after the other they would wait for LDS each time.
+struct Order {
+  int larger, equal;
+};
+__device__ __forceinline__ Order order(const u64 *values, int n, u64 than) {
+  Order count = {0, 0};
+  for (int o = 0; o < n; o += 8) {
+    u64 v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = values[o + u];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      count.larger += o + u < n && v[u] > than;
+      count.equal += o + u < n && v[u] == than;
+    }
+  }
+  return count;
+}
+
+// V float4 a lane, in GROUPS groups. A row is `chunks` chunks of `parts` parts of kThreads * 4 V
+// logits (the last ones shorter); MANY: of more than one part.
+template <int V, int GROUPS, bool MANY>
 __global__ __launch_bounds__(kThreads) void beam_chunks_kernel(unsigned char *__restrict__ workspace,
                                                                const float *__restrict__ logits,
                                                                const int *__restrict__ tokens, int eos, int vocab,
-                                                               int beams, int chunks) {
-  extern __shared__ u64 list[];  // at most kWaves * beams lanes' 4 V values
+                                                               int beams, int chunks, int parts) {
+  constexpr int kPart = kThreads * 4 * V;
+  constexpr int kEach = 4 * V / GROUPS;  // values of a group
+  extern __shared__ u64 list[];  // `beams` groups of each wave at most, and eight that order() may read
+  __shared__ u64 kept[2][kMaxBeams + 8];  // the largest so far, in order
   __shared__ u64 bounds[kWaves];
-  __shared__ unsigned tops[kWaves];
+  __shared__ float tops[kWaves];
   __shared__ double sums[kWaves];
   __shared__ int length;
   const int row = blockIdx.x / chunks, chunk = blockIdx.x - row * chunks;
   if (eos >= 0 && tokens[row] == eos) return;  // ended: its logits do not count
   const int t = threadIdx.x, lane = t % L2C_WAVE, wave = t / L2C_WAVE;
-  const int first = chunk * (kThreads * 4 * V);
-  const int n = min(kThreads * 4 * V, vocab - first);
-  const float *x = logits + static_cast<size_t>(row) * vocab + first;
-  float4 q[V];
+  const long long size = static_cast<long long>(parts) * kPart;
+  const int first = static_cast<int>(chunk * size);  // below vocab: no chunk is empty
+  const int whole = static_cast<int>(min(size, static_cast<long long>(vocab - first)));
+  const float *const x = logits + static_cast<size_t>(row) * vocab + first;
+  auto load = [&](float4 (&q)[V], int start) __attribute__((always_inline)) {
+    const int n = min(kPart, whole - start);
 #pragma unroll
-  for (int c = 0; c < V; ++c) {
-    const int j = 4 * (t + c * kThreads);
-    if (j < n) q[c] = l2c::ld_chunk(x, j, n);
-  }
-  if (t == 0) length = 0;
-  float v[4 * V];
-#pragma unroll
-  for (int c = 0; c < V; ++c) {
-    const int j = 4 * (t + c * kThreads);
-    const float4 w = j < n ? l2c::whole_chunk(q[c], j, n, -INFINITY) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-    v[4 * c] = w.x, v[4 * c + 1] = w.y, v[4 * c + 2] = w.z, v[4 * c + 3] = w.w;
-  }
-  // The lane's first maximum.
-  auto place = [&](int i) __attribute__((always_inline)) { return 4 * (t + i / 4 * kThreads) + i % 4; };
-  auto key = [&](int i) __attribute__((always_inline)) { return place(i) < n ? key_of(v[i]) : 0u; };
-  unsigned best = 0, best_place = UINT_MAX;
-#pragma unroll
-  for (int i = 0; i < 4 * V; ++i) {
-    const unsigned k = key(i);
-    if (k > best) best = k, best_place = place(i);
-  }
-  const unsigned bound = wave_kth(best, beams);
-  unsigned bound_place = UINT_MAX;
-  const u64 tied = __ballot(best == bound && bound != 0);
-  const int wanted = beams - __popcll(__ballot(best > bound));
-  if (__popcll(tied) > wanted) {  // of the lanes whose maxima tie, those with the lowest places
-    bound_place = UINT_MAX - wave_kth(best == bound ? UINT_MAX - best_place : 0u, wanted);
-  }
-  unsigned top = best;
-#pragma unroll
-  for (int offset = 32; offset > 0; offset >>= 1) top = max(top, static_cast<unsigned>(__shfl_xor(static_cast<int>(top), offset, L2C_WAVE)));
-  if (lane == 0) {
-    bounds[wave] = ordered(bound, bound_place);
-    tops[wave] = top;
-  }
-  __syncthreads();
-  u64 least = bounds[0];
-  unsigned most = tops[0];
-#pragma unroll
-  for (int w = 1; w < kWaves; ++w) {
-    least = max(least, bounds[w]);
-    most = max(most, tops[w]);
-  }
-  // All -Inf or NaN: no finite maximum to subtract.
-  const float maximum = most ? number_of(most) : -INFINITY;
-  const float shift = maximum == -INFINITY ? 0.0f : maximum;
-  float sum = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 4 * V; ++i) sum += expf(v[i] - shift);
-  const double total = wave_sum(static_cast<double>(sum));
-  if (lane == 0) sums[wave] = total;
-  if (ordered(best, best_place) >= least) {
-#pragma unroll
-    for (int i = 0; i < 4 * V; ++i) {
-      const unsigned k = key(i);
-      if (k != 0 && ordered(k, place(i)) >= least) list[atomicAdd(&length, 1)] = ordered(k, place(i));
+    for (int c = 0; c < V; ++c) {
+      const int j = 4 * (t + c * kThreads);
+      if (j < n) q[c] = l2c::ld_chunk(x + start, j, n);
     }
-  }
-  __syncthreads();
-  unsigned char *entry = workspace + (static_cast<size_t>(row) * chunks + chunk) * chunk_bytes(beams);
-  Candidate *out = reinterpret_cast<Candidate *>(entry + sizeof(ChunkStat));
-  const int m = length;
-  for (int e = t; e < m; e += kThreads) {
-    const u64 mine = list[e];
-    int rank = 0;
-    for (int o = 0; o < m; ++o) rank += list[o] > mine;
-    if (rank < beams)
-      out[rank] = {number_of(static_cast<unsigned>(mine >> 32)), first + static_cast<int>(UINT_MAX - static_cast<unsigned>(mine))};
-  }
-  for (int e = m + t; e < beams; e += kThreads) out[e] = {-INFINITY, -1};
-  if (t == 0) {
-    double all = sums[0];
+  };
+  float4 q[V];
+  load(q, 0);
+  if (t == 0) length = 0;
+  double total = 0.0;          // the lane's sum of exp(x - shift)
+  float shift = -INFINITY;     // the largest so far
+  int count = 0;               // of `kept`
+  int turn = 0;
+  for (int start = 0;;) {
+    const int n = min(kPart, whole - start);
+    const bool more = MANY && whole - start > kPart;
+    float v[4 * V];
+    if (n < kPart) {  // -Inf past the end
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) all += sums[w];
-    *reinterpret_cast<ChunkStat *>(entry) = {all, maximum, 0};
+      for (int c = 0; c < V; ++c) {
+        const int j = 4 * (t + c * kThreads);
+        q[c] = j < n ? l2c::whole_chunk(q[c], j, n, -INFINITY) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < V; ++c) v[4 * c] = q[c].x, v[4 * c + 1] = q[c].y, v[4 * c + 2] = q[c].z, v[4 * c + 3] = q[c].w;
+    if (more) load(q, start + kPart);
+    auto place = [&](int i) __attribute__((always_inline)) { return 4 * (t + i / 4 * kThreads) + i % 4; };
+    auto key = [&](int i) __attribute__((always_inline)) { return place(i) < n ? key_of(v[i]) : 0u; };
+    // NaN does not count: a group of NaN has the key of -Inf here and
+    // emits nothing; one past the row has none.
+    float top = -INFINITY;
+    unsigned best[GROUPS];
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) {
+      float m = -INFINITY;
+#pragma unroll
+      for (int i = kEach * g; i < kEach * (g + 1); ++i) m = fmaxf(m, v[i]);
+      best[g] = place(kEach * g) < n ? key_of(m) : 0u;
+      top = fmaxf(top, m);
+    }
+    const unsigned bound = wave_bound(best, beams);
+    unsigned bound_place = UINT_MAX;
+    if (bound != 0 && wave_reach(best, bound) > beams) {
+      // Of the groups whose maxima tie, those with the lowest first places.
+      unsigned before[GROUPS];  // UINT_MAX - place
+      int larger = 0;
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g) {
+        before[g] = 0;
+        larger += __popcll(__ballot(best[g] > bound));
+        if (best[g] != bound) continue;
+#pragma unroll
+        for (int i = kEach * (g + 1) - 1; i >= kEach * g; --i)
+          if (key(i) == bound) before[g] = UINT_MAX - (static_cast<unsigned>(start) + place(i));
+      }
+      const unsigned least_before = wave_bound(before, beams - larger);
+      bound_place = least_before == 0 ? UINT_MAX : UINT_MAX - least_before;
+    }
+    const float largest = wave_top(top);
+    if (lane == L2C_WAVE - 1) {
+      bounds[wave] = ordered(bound, bound_place);
+      tops[wave] = largest;
+    }
+    __syncthreads();
+    u64 least = MANY && count == beams ? kept[turn][beams - 1] : 0;
+    float maximum = shift;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      least = max(least, bounds[w]);
+      maximum = fmaxf(maximum, tops[w]);
+    }
+    if (maximum > shift) {  // the lane's sum so far is of exp(x - the old maximum)
+      if (MANY && start > 0) total *= exp(static_cast<double>(shift) - static_cast<double>(maximum));
+      shift = maximum;
+    }
+    const float subtract = shift == -INFINITY ? 0.0f : shift;  // nothing but -Inf and NaN: no maximum
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4 * V; ++i) sum += exp_nonpositive(v[i] - subtract);
+    total += static_cast<double>(sum);
+    // The values that reach the bound into the list, a wave's after each other's.
+    unsigned reach = 0;
+    const unsigned least_key = static_cast<unsigned>(least >> 32);
+    if (least_key > key_of(-INFINITY) && static_cast<unsigned>(least) == 0) {  // no ties to break, and none past the end
+      const float limit = number_of(least_key);
+#pragma unroll
+      for (int i = 0; i < 4 * V; ++i) reach |= v[i] >= limit ? 1u << i : 0u;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4 * V; ++i)
+        if (key(i) != 0 && ordered(key(i), static_cast<unsigned>(start) + place(i)) >= least) reach |= 1u << i;
+    }
+    if (__ballot(reach != 0)) {
+      const int count_here = __popc(reach), upto = wave_scan(count_here);
+      int base = 0;
+      if (lane == L2C_WAVE - 1) base = atomicAdd(&length, upto);
+      int to = __builtin_amdgcn_readlane(base, L2C_WAVE - 1) + upto - count_here;
+#pragma unroll
+      for (int c = 0; c < V; ++c) {
+        if (__ballot(reach >> 4 * c & 15u) == 0) continue;
+#pragma unroll
+        for (int i = 4 * c; i < 4 * c + 4; ++i)
+          if (reach >> i & 1) list[to++] = ordered(key_of(v[i]), static_cast<unsigned>(start) + place(i));
+      }
+    }
+    __syncthreads();
+    const int m = length, all = count + m;
+    for (int e = t; e < all; e += kThreads) {
+      const u64 mine = MANY && e < count ? kept[turn][e] : list[e - count];
+      const int rank = (MANY ? order(kept[turn], count, mine).larger : 0) + order(list, m, mine).larger;
+      if (rank < beams) kept[turn ^ 1][rank] = mine;
+    }
+    count = min(all, beams);
+    turn ^= 1;
+    __syncthreads();
+    if (!more) break;
+    if (t == 0) length = 0;  // before the next barrier, after which it is counted again
+    start += kPart;
+  }
+  ChunkStat *const stats = reinterpret_cast<ChunkStat *>(workspace);
+  if (t < beams) {
+    const int request = row / beams;
+    Candidate *const out = reinterpret_cast<Candidate *>(stats + gridDim.x) +
+                           ((static_cast<size_t>(request) * beams + t) * beams + (row - request * beams)) * chunks + chunk;
+    const u64 mine = t < count ? kept[turn][t] : 0;
+    *out = t < count ? Candidate{number_of(static_cast<unsigned>(mine >> 32)),
+                                 first + static_cast<int>(UINT_MAX - static_cast<unsigned>(mine))}
+                     : Candidate{-INFINITY, -1};
+  }
+  total = wave_scan(total);
+  if (lane == L2C_WAVE - 1) sums[wave] = total;
+  __syncthreads();
+  if (t == 0) {
+    total = sums[0];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) total += sums[w];
+    stats[blockIdx.x] = {total, shift, 0};  // [row][chunk]
   }
 }
 
-constexpr int kJoinList = 2048;
+constexpr int kJoinCandidates = 16 * kThreads;
 
-// A candidate's place in the request: beam, then token.
-__device__ __forceinline__ u64 place_of(int beam, int token) {
-  return (static_cast<u64>(beam) << 32) | static_cast<unsigned>(token);
-}
+// Quotients of values below 2^16 by one of 1 to 2^16, without a division each.
+struct Quotient {
+  unsigned by;
+  __device__ explicit Quotient(int divisor) : by(divisor > 1 ? UINT_MAX / divisor + 1 : 0) {}
+  __device__ __forceinline__ int operator()(int v) const { return by ? __umulhi(v, by) : v; }
+};
 
+// The lanes hold HELD candidates each in registers.
+template <int HELD>
 __global__ __launch_bounds__(kThreads) void beam_join_kernel(float *scores_out, int *tokens_out, int *parents,
                                                              int *generated, const unsigned char *workspace,
                                                              const float *scores, const int *tokens, int eos,
@@ -199,57 +382,66 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(float *scores_out, 
   __shared__ double base[kMaxBeams];
   __shared__ float tops[kMaxBeams];
   __shared__ bool ended[kMaxBeams];
-  __shared__ u64 list_key[kJoinList], list_place[kJoinList];
-  __shared__ u64 slots[kWaves], place_slots[kWaves];
+  __shared__ u64 list_key[HELD * kThreads + 8], list_place[HELD * kThreads + 8];
+  __shared__ u64 slots[kWaves];
   __shared__ int length;
+  constexpr int kGroup = 16;  // lanes a beam for its chunks' sums
   const int t = threadIdx.x, lane = t % L2C_WAVE, wave = t / L2C_WAVE;
   const int first = blockIdx.x * beams;
-  const size_t bytes = chunk_bytes(beams);
+  const ChunkStat *const stats = reinterpret_cast<const ChunkStat *>(workspace);
   auto stat = [&](int beam, int chunk) __attribute__((always_inline)) {
-    return reinterpret_cast<const ChunkStat *>(workspace + (static_cast<size_t>(first + beam) * chunks + chunk) * bytes);
+    return stats + static_cast<size_t>(first + beam) * chunks + chunk;
   };
+  // Candidate i: rank i / lists of list i % lists, a list a chunk, beam after beam: the first
+  // lanes have the lists' best, and their maxima are a good bound.
+  const int lists = beams * chunks, candidates = lists * beams;
+  const Quotient by_lists(lists), by_chunks(chunks);
+  auto beam_of = [&](int i) __attribute__((always_inline)) { return by_chunks(i - by_lists(i) * lists); };
+  const Candidate *const all = reinterpret_cast<const Candidate *>(stats + static_cast<size_t>(gridDim.x) * lists) +
+                               static_cast<size_t>(blockIdx.x) * candidates;
+  Candidate held[HELD];
+#pragma unroll
+  for (int r = 0; r < HELD; ++r) held[r] = all[min(t + r * kThreads, candidates - 1)];  // together, without a branch
   if (t == 0) length = 0;
-  for (int k = wave; k < beams; k += kWaves) {
+  for (int k = t / kGroup; k < beams; k += kThreads / kGroup) {  // whole groups stay together
+    const int member = t % kGroup;
+    // Of an ended row the workspace holds nothing; what is read there is not used.
+    ChunkStat s = {0.0, -INFINITY, 0};
+    if (member < chunks) s = *stat(k, member);
     const float score = scores[first + k];
     const bool end = eos >= 0 && tokens[first + k] == eos;
-    const bool live = score >= -FLT_MAX && score <= FLT_MAX;
-    double b = score;
-    float m = 0.0f;
-    if (!end && live) {
-      m = -INFINITY;
-      for (int c = lane; c < chunks; c += L2C_WAVE) m = fmaxf(m, stat(k, c)->maximum);
-      m = l2c::wave_max(m);
-      double sum = 0.0;
-      for (int c = lane; c < chunks; c += L2C_WAVE) {
-        const ChunkStat s = *stat(k, c);
-        // A chunk of -Inf has sum 0; NaN stays NaN.
-        sum += s.maximum == -INFINITY ? s.sum * 0.0 : s.sum * exp(static_cast<double>(s.maximum) - static_cast<double>(m));
-      }
-      sum = wave_sum(sum);
-      b -= log(sum);
+    float m = s.maximum;
+    for (int c = member + kGroup; c < chunks; c += kGroup) m = fmaxf(m, stat(k, c)->maximum);
+    m = row_max(m);
+    double sum = 0.0;
+    for (int c = member; c < chunks; c += kGroup) {
+      if (c != member) s = *stat(k, c);
+      // A chunk of -Inf has sum 0; NaN stays NaN.
+      sum += s.maximum == m ? s.sum
+             : s.maximum == -INFINITY ? s.sum * 0.0
+                                      : s.sum * exp(static_cast<double>(s.maximum) - static_cast<double>(m));
     }
-    // Of a row of -Inf the sum is 0 and b +Inf, of one with NaN or +Inf it is NaN.
-    if (lane == 0) {
+    sum = row_sum(sum);
+    if (member == 0) {
+      // Of a row of -Inf the sum is 0 and b +Inf, of one with NaN or +Inf it is NaN.
+      const double b = end ? static_cast<double>(score) : static_cast<double>(score) - log(sum);
+      base[k] = b >= -DBL_MAX && b <= DBL_MAX ? b : __longlong_as_double(0x7ff8000000000000LL);
       tops[k] = m;
-      base[k] = live && b >= -DBL_MAX && b <= DBL_MAX ? b : __longlong_as_double(0x7ff8000000000000LL);
       ended[k] = end;
     }
   }
   __syncthreads();
-  const int lists = beams * chunks;
-  // Score key and place of candidate e of list l; key 0 where there is none.
-  auto candidate = [&](int l, int e, u64 *place) __attribute__((always_inline)) -> u64 {
-    const int beam = l / chunks, chunk = l - beam * chunks;
-    if (ended[beam]) {
-      *place = place_of(beam, eos);
-      return chunk == 0 && e == 0 ? key_of(base[beam]) : 0ULL;
-    }
-    const Candidate c = reinterpret_cast<const Candidate *>(stat(beam, chunk) + 1)[e];
-    *place = place_of(beam, c.token);
-    return c.token >= 0 && c.logit > -INFINITY ? key_of(base[beam] + (static_cast<double>(c.logit) - tops[beam])) : 0ULL;
+  // A candidate's key, 0 where it is none, and place.
+  auto key_at = [&](int i, Candidate c) __attribute__((always_inline)) -> u64 {
+    const int beam = beam_of(i);
+    const bool end = ended[beam];
+    const double score = base[beam] + (end ? 0.0 : static_cast<double>(c.logit) - static_cast<double>(tops[beam]));
+    const bool is = end ? i == beam * chunks : c.token >= 0 && c.logit > -INFINITY;
+    return is && i < candidates ? key_of(score) : 0ULL;
   };
-  auto before = [](u64 key, u64 place, u64 other, u64 other_place) __attribute__((always_inline)) {
-    return key > other || (key == other && place < other_place);
+  auto place_at = [&](int i, Candidate c) __attribute__((always_inline)) {
+    const int beam = beam_of(i);
+    return static_cast<u64>(beam) << 32 | static_cast<unsigned>(ended[beam] ? eos : c.token);
   };
   auto write = [&](int rank, u64 key, u64 place) __attribute__((always_inline)) {
     const int to = first + rank;
@@ -260,91 +452,89 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(float *scores_out, 
     if (generated) generated[static_cast<size_t>(to) * steps + step] = token;
   };
 
-  // The lists' heads are their largest: the k-th largest of the lanes' best heads is a
-  // bound that at least `beams` candidates reach. Equal keys all pass.
-  u64 best = 0;
-  for (int l = t; l < lists; l += kThreads) {
-    u64 place;
-    best = max(best, candidate(l, 0, &place));
+  // A bound that at least `beams` candidates reach, from the lanes' best; equal keys all pass.
+  u64 best = 0, held_key[HELD];
+#pragma unroll
+  for (int r = 0; r < HELD; ++r) {
+    held_key[r] = key_at(t + r * kThreads, held[r]);
+    best = max(best, held_key[r]);
   }
-  const u64 bound = wave_kth(best, beams);
+  const u64 bound = wave_bound(best, beams);
   if (lane == 0) slots[wave] = bound;
   __syncthreads();
   u64 least = slots[0];
 #pragma unroll
   for (int w = 1; w < kWaves; ++w) least = max(least, slots[w]);
   least = max(least, static_cast<u64>(1));
-  if (best >= least) {
-    for (int l = t; l < lists; l += kThreads) {
-      for (int e = 0; e < beams; ++e) {
-        u64 place;
-        const u64 key = candidate(l, e, &place);
-        if (key < least) break;  // so are the rest of the list
-        const int at = atomicAdd(&length, 1);
-        if (at < kJoinList) list_key[at] = key, list_place[at] = place;
+  unsigned reach = 0;
+#pragma unroll
+  for (int r = 0; r < HELD; ++r) reach |= held_key[r] >= least ? 1u << r : 0u;
+  if (__ballot(reach != 0)) {
+    const int count_here = __popc(reach), upto = wave_scan(count_here);
+    int from = 0;
+    if (lane == L2C_WAVE - 1) from = atomicAdd(&length, upto);
+    int to = __builtin_amdgcn_readlane(from, L2C_WAVE - 1) + upto - count_here;
+#pragma unroll
+    for (int r = 0; r < HELD; ++r) {
+      if (reach >> r & 1) {
+        list_key[to] = held_key[r], list_place[to] = place_at(t + r * kThreads, held[r]);
+        ++to;
       }
     }
   }
   __syncthreads();
   const int m = length;
-  if (m <= kJoinList) {
-    for (int e = t; e < m; e += kThreads) {
-      const u64 key = list_key[e], place = list_place[e];
-      int rank = 0;
-      for (int o = 0; o < m; ++o) rank += before(list_key[o], list_place[o], key, place);
-      if (rank < beams) write(rank, key, place);
-    }
-    for (int e = m + t; e < beams; e += kThreads) write(e, 0, 0);
-    return;
+  for (int e = t; e < m; e += kThreads) {
+    const u64 key = list_key[e], place = list_place[e];
+    const Order among = order(list_key, m, key);
+    int rank = among.larger;
+    if (among.equal > 1)  // it and others: the lower place first
+      for (int o = 0; o < m; ++o) rank += list_key[o] == key && list_place[o] < place;
+    if (rank < beams) write(rank, key, place);
   }
-  // More than the list holds: one beam after another, each the best after the last.
-  u64 last = ~0ULL, last_place = 0;
-  bool any = false;
-  for (int r = 0; r < beams; ++r) {
-    u64 top = 0, top_place = ~0ULL;
-    for (int l = t; l < lists; l += kThreads) {
-      for (int e = 0; e < beams; ++e) {
-        u64 place;
-        const u64 key = candidate(l, e, &place);
-        if (key == 0) break;
-        if (any && !before(last, last_place, key, place)) continue;
-        if (before(key, place, top, top_place)) top = key, top_place = place;
-      }
-    }
-#pragma unroll
-    for (int offset = 32; offset > 0; offset >>= 1) {
-      const u64 k = __shfl_xor(top, offset, L2C_WAVE), p = __shfl_xor(top_place, offset, L2C_WAVE);
-      if (before(k, p, top, top_place)) top = k, top_place = p;
-    }
-    __syncthreads();  // the slots of the round before are read
-    if (lane == 0) slots[wave] = top, place_slots[wave] = top_place;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w)
-      if (before(slots[w], place_slots[w], top, top_place)) top = slots[w], top_place = place_slots[w];
-    if (t == 0) write(r, top, top_place);
-    last = top, last_place = top_place, any = true;
-  }
+  for (int e = m + t; e < beams; e += kThreads) write(e, 0, 0);
 }
 
-using ChunkKernel = void (*)(unsigned char *, const float *, const int *, int, int, int, int);
+using ChunkKernel = void (*)(unsigned char *, const float *, const int *, int, int, int, int, int);
 
 struct ChunkConfig {
   ChunkKernel fn;
-  int values, chunks;  // values a lane, chunks a row
+  int values;         // of a group
+  int chunks, parts;  // chunks a row, parts a chunk
 };
 
+template <int V, int GROUPS>
+ChunkConfig config(int vocab, int most_chunks) {
+  const int parts = (vocab - 1) / (kThreads * 4 * V) + 1;
+  const int each = (parts - 1) / most_chunks + 1;
+  return {each > 1 ? beam_chunks_kernel<V, GROUPS, true> : beam_chunks_kernel<V, GROUPS, false>, 4 * V / GROUPS,
+          (parts - 1) / each + 1, each};
+}
+
+// 2048 logits a chunk as long as that makes at most 4096 chunks, and then 4096 logits: small
+// chunks have the least latency (1 x 4 x 32000: 8.1 us in chunks of 2048, 9.3 of 4096, 10.9
+// of 8192). Else 8192, which cost the least instructions a logit (256 x 4 x 32003: 42.6, 35.4,
+// 33.8). With many beams a lane's values go in groups of eight: the bound is
+// closer, and the list four times shorter (32 x 32 x 32000 54 us, 66 in one group; 256 x 4 x
+// 32003 35.4, 33.8 in one).
 ChunkConfig chunk_config(int vocab, int beams, int batch) {
-  (void)beams, (void)batch;
-  const int values = 8;
-  return {beam_chunks_kernel<2>, values, (vocab - 1) / (kThreads * values) + 1};
+  const int most = kJoinCandidates / (beams * beams);
+  const double rows = static_cast<double>(batch) * beams;
+  auto fits = [&](int part) {
+    const int parts = (vocab - 1) / part + 1;
+    return parts <= most && rows * parts <= 4096;
+  };
+  if (fits(2048)) return config<2, 1>(vocab, most);
+  if (fits(4096)) return beams > 8 ? config<4, 2>(vocab, most) : config<4, 1>(vocab, most);
+  return beams > 8 ? config<8, 4>(vocab, most) : config<8, 1>(vocab, most);
 }
 
 }  // namespace
 
 extern "C" size_t l2c_decoder_beam_workspace_bytes(int vocab, int beams, int batch) {
   if (vocab <= 0 || beams <= 0 || beams > kMaxBeams || batch <= 0) return 0;
-  return static_cast<size_t>(batch) * beams * chunk_config(vocab, beams, batch).chunks * chunk_bytes(beams);
+  return static_cast<size_t>(batch) * beams * chunk_config(vocab, beams, batch).chunks *
+         (sizeof(ChunkStat) + sizeof(Candidate) * static_cast<size_t>(beams));
 }
 
 extern "C" int l2c_decoder_beam_select(float *scores_out, int *tokens_out, int *parents, int *generated,
@@ -363,11 +553,13 @@ extern "C" int l2c_decoder_beam_select(float *scores_out, int *tokens_out, int *
   if (static_cast<long long>(batch) * beams > INT_MAX || grid > INT_MAX || !l2c::launchable(grid, kThreads))
     return hipErrorInvalidValue;
   unsigned char *w = static_cast<unsigned char *>(workspace);
-  const size_t list = sizeof(u64) * kWaves * static_cast<size_t>(beams) * c.values;
+  const size_t list = sizeof(u64) * (kWaves * static_cast<size_t>(beams) * c.values + 8);
   hipLaunchKernelGGL(c.fn, dim3(static_cast<unsigned>(grid)), dim3(kThreads), list, stream, w, logits, tokens, eos,
-                     vocab, beams, c.chunks);
+                     vocab, beams, c.chunks, c.parts);
   L2C_LAUNCH_CHECK();
-  hipLaunchKernelGGL(beam_join_kernel, dim3(static_cast<unsigned>(batch)), dim3(kThreads), 0, stream, scores_out,
+  const int candidates = beams * beams * c.chunks;
+  hipLaunchKernelGGL(candidates <= kThreads ? beam_join_kernel<1>
+                     : candidates <= 4 * kThreads ? beam_join_kernel<4> : beam_join_kernel<16>, dim3(static_cast<unsigned>(batch)), dim3(kThreads), 0, stream, scores_out,
                      tokens_out, parents, generated, w, scores, tokens, eos, beams, c.chunks, steps, step);
   L2C_LAUNCH_CHECK();
   return hipSuccess;

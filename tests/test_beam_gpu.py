@@ -169,8 +169,8 @@ def test_ended_beams(torch_gpu, l2c):
 
 
 def test_many_candidates_over_the_bound(torch_gpu, l2c):
-    """More candidates reach the join's bound than its list holds: the beams that win have many
-    good tokens in few chunks, every fourth row of lists decides the bound."""
+    """Rows whose best values crowd: in few lists of the join; in few lanes of a chunk, where more
+    reach the bound than its list holds; and rows of one value."""
     rng = np.random.default_rng(6)
     beams, vocab = 32, 131072
     logits = rng.standard_normal((beams, vocab)).astype(np.float32) * 0.01 - 30
@@ -182,6 +182,11 @@ def test_many_candidates_over_the_bound(torch_gpu, l2c):
             else:
                 logits[k, first + 5] = 9.0 + rng.random() * 0.1
     check_select(torch_gpu, l2c, logits, np.full(beams, -2.0), np.zeros(beams, int), -1, beams)
+    for beams, vocab in ((4, 20000), (32, 100000), (32, 1500), (9, 65536)):
+        crowd = np.arange(vocab) // 4 % 64 < beams - 1  # the first lanes of every wave, four values each time
+        logits = np.where(crowd, 10 + rng.random((beams, vocab)), rng.random((beams, vocab))).astype(np.float32)
+        check_select(torch_gpu, l2c, logits, -rng.random(beams), np.zeros(beams, int), -1, beams)
+    beams = 32
     same = np.zeros((beams, 40000), np.float32)  # every continuation has the same score
     _, to, pa = check_select(torch_gpu, l2c, same, np.zeros(beams), np.ones(beams, int), -1, beams)
     np.testing.assert_array_equal(to, np.arange(beams))

@@ -300,6 +300,30 @@ def test_reorder_long_state(torch_gpu, l2c):
         assert int(state[k * row + 1000:k * row + 2000].sum()) == 0
 
 
+def test_reorder_long_state_out_of_place(torch_gpu, l2c):
+    torch = torch_gpu
+    beams, row = 2, (1 << 32) + 48
+    state = torch.empty(beams * row, dtype=torch.uint8, device="cuda")
+    out = torch.zeros_like(state)
+    for k in range(beams):
+        state[k * row:(k + 1) * row] = k + 1
+    p = torch.tensor([1, 0], dtype=torch.int32, device="cuda")
+    l2c.decoder_beam_reorder(out, state, p, beams, 1, row)
+    for k in range(beams):
+        assert int(out[k * row:(k + 1) * row].min()) == int(out[k * row:(k + 1) * row].max()) == 2 - k
+
+
+@pytest.mark.parametrize("groups,width", [(65536, 16), (70001, 20), (131075, 1)])
+def test_reorder_many_groups(torch_gpu, l2c, groups, width):
+    check_reorder(torch_gpu, l2c, (groups, 2, 3, 1, 2, width), 1)
+
+
+@pytest.mark.parametrize("length", [126 * 16 + 3, 127 * 16 + 1, 128 * 16, 128 * 16 + 1, 255 * 16, 257 * 16 + 5])
+def test_reorder_short_and_long_rows(torch_gpu, l2c, length):
+    check_reorder(torch_gpu, l2c, (2, 5, 3, 1, 1, length), 1)
+    check_reorder(torch_gpu, l2c, (1, 37, 7, 1, 1, length), 1)
+
+
 # ---------------------------------------------------------------------------
 
 def bf16(x):

@@ -18,9 +18,8 @@ struct Mx4Tile {
   double launch, tile, k;
 };
 
-// l2c_mx4gemm_rows.hip and l2c_mx4gemm_tiles.hip.
-constexpr int kMx4RowTiles = 4, kMx4LdsTiles = 4;
-extern const Mx4Tile mx4_row_tiles[kMx4RowTiles];
-extern const Mx4Tile mx4_lds_tiles[kMx4LdsTiles];
+// l2c_mx4gemm_rows.hip, l2c_mx4gemm_slices.hip and l2c_mx4gemm_tiles.hip.
+constexpr int kMx4SliceTiles = 2, kMx4LdsTiles = 4;
+extern const Mx4Tile mx4_row_tile, mx4_slice_tiles[kMx4SliceTiles], mx4_lds_tiles[kMx4LdsTiles];
 
 }  // namespace l2c

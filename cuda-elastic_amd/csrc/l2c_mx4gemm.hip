@@ -68,12 +68,12 @@ __global__ __launch_bounds__(kQuantThreads) void quantize_mxfp4_bf16_kernel(uint
 
 // ---------------------------------------------------------------------------
 // Choice of the contraction's tile: the one of least estimated time. Fitted to the times of
-// these and 18 other tiles on 132 shapes of 1 to 1024 x 288 to 16384 x 600 to 11008: what a
+// these and 9 other tiles on 132 shapes of 1 to 1024 x 288 to 16384 x 600 to 11008: what a
 // CU takes for its tiles in turn is linear in their number and in K to about 12%, and
-// the choice among these eight is 3% slower than the best of the 26 in the mean. Measured
-// on either side of a border, us: 33 x 5024 x 8004 12.5 on 32 x 32 tiles, 11.2 on 64 x
-// 64; 128 x 4096 x 11008 13.1 on 64 x 64, 11.2 on 64 x 128; 400 x 4096 x 11008 27.2 on
-// 128 x 128, 21.1 on 256 x 128.
+// the choice among these seven is 3% slower than the best of the 16 in the mean. Measured
+// on either side of a border, us: 1 x 4096 x 11008 6.8 on 16 x 16 tiles, 6.0 on 32 x 64,
+// 8.1 on 64 x 64; 64 x 4096 x 11008 11.9 on 32 x 64, 8.9 on 64 x 64; 128 x 4096 x 11008
+// 13.1 on 64 x 64, 11.2 on 64 x 128; 400 x 4096 x 11008 27.2 on 128 x 128, 21.1 on 256 x 128.
 
 long long tiles_of(const l2c::Mx4Tile &t, int batch, int rows) {
   return ((batch + static_cast<long long>(t.bm) - 1) / t.bm) * ((rows + static_cast<long long>(t.bn) - 1) / t.bn);
@@ -88,7 +88,8 @@ const l2c::Mx4Tile *choose(int batch, int blocks, int rows) {
     const double cost = t.launch + static_cast<double>((tiles + 255) / 256) * (t.tile + t.k * 32.0 * blocks);
     if (!best || cost < least) best = &t, least = cost;
   };
-  for (const l2c::Mx4Tile &t : l2c::mx4_row_tiles) consider(t);
+  consider(l2c::mx4_row_tile);
+  for (const l2c::Mx4Tile &t : l2c::mx4_slice_tiles) consider(t);
   for (const l2c::Mx4Tile &t : l2c::mx4_lds_tiles) consider(t);
   return best;
 }

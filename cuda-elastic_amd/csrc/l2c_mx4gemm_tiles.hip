@@ -213,6 +213,17 @@ __global__ __launch_bounds__(kThreads) void mxfp4_tile_kernel(float *__restrict_
       for (int j = 0; j < NI; ++j) now.w[j][p] = next.w[j][p] >> (16 * g);
     }
   };
+  // The scales of the blocks past the last whole step, of which some are the last again.
+  unsigned tail[kReads] = {};
+  if (rest) {
+    const int b0 = 8 * full + min(sblock, rest - 1), b1 = 8 * full + min(sblock + 1, rest - 1);
+#pragma unroll
+    for (int k = 0; k < kReads; ++k) {
+      const uint8_t *s = k < MI ? Xs + static_cast<size_t>(m0 + min(32 * (MI * wm + k) + r, mrows - 1)) * blocks
+                                : Ws + static_cast<size_t>(n0 + min(32 * (NI * wn + k - MI) + r, nrows - 1)) * blocks;
+      tail[k] = s[b0] | s[b1] << 8;
+    }
+  }
   load_scales(0);
   __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -221,6 +232,8 @@ __global__ __launch_bounds__(kThreads) void mxfp4_tile_kernel(float *__restrict_
   store_scales(queue[0]);
 #pragma unroll
   for (int k = 0; k < kQueue; ++k) asm volatile("" : "+v"(queue[k]));  // loaded here, not where they are used
+#pragma unroll
+  for (int k = 0; k < kReads; ++k) asm volatile("" : "+v"(tail[k]));
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((kStages - 1) * T::kDma) : "memory");
 #pragma unroll
   for (int k = 0; k < kReads; ++k) {
@@ -254,17 +267,10 @@ __global__ __launch_bounds__(kThreads) void mxfp4_tile_kernel(float *__restrict_
   if (rest) {  // the first half's fragments are read or on their way
 #pragma unroll
     for (int k = 0; k < kReads; ++k) read(at, 1, k);
-    const int b0 = 8 * full + min(sblock, rest - 1), b1 = 8 * full + min(sblock + 1, rest - 1);
 #pragma unroll
-    for (int i = 0; i < MI; ++i) {
-      const uint8_t *s = Xs + static_cast<size_t>(m0 + min(32 * (MI * wm + i) + r, mrows - 1)) * blocks;
-      now.x[i][0] = s[b0] | s[b1] << 8;
-    }
+    for (int i = 0; i < MI; ++i) now.x[i][0] = tail[i];
 #pragma unroll
-    for (int j = 0; j < NI; ++j) {
-      const uint8_t *s = Ws + static_cast<size_t>(n0 + min(32 * (NI * wn + j) + r, nrows - 1)) * blocks;
-      now.w[j][0] = s[b0] | s[b1] << 8;
-    }
+    for (int j = 0; j < NI; ++j) now.w[j][0] = tail[MI + j];
 #pragma unroll
     for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -320,5 +326,5 @@ constexpr l2c::Mx4Tile tile(double launch, double per_tile, double per_k) {
 
 }  // namespace
 
-const l2c::Mx4Tile l2c::mx4_lds_tiles[kMx4LdsTiles] = {tile<1, 1, 4>(2400, 1210, 1.08), tile<1, 2, 4>(700, 3500, 1.60),
-                                                       tile<2, 2, 4>(0, 5600, 1.97), tile<4, 2, 3>(1100, 6600, 2.76)};
+const l2c::Mx4Tile l2c::mx4_lds_tiles[kMx4LdsTiles] = {tile<1, 1, 4>(2515, 1150, 1.166), tile<1, 2, 4>(498, 3560, 1.731),
+                                                       tile<2, 2, 4>(0, 5454, 2.199), tile<4, 2, 3>(1317, 7368, 2.907)};

@@ -135,11 +135,10 @@ def test_product_shapes(torch_gpu, l2c, batch, cols, rows):
 
 # Every kernel: lanes, batch rows and weight rows of its tile, and shapes that run on it, with
 # ragged edges, one step to many, odd and even steps and a part of one at the end.
-KERNELS = [((512, 16, 16), [(7, 544, 1003), (1, 11008, 500), (16, 4128, 900)]),
-           ((512, 16, 32), [(13, 512, 8004), (5, 4096, 8190), (128, 8192, 1003)]),
-           ((256, 32, 32), [(61, 288, 5003), (40, 800, 8001), (300, 480, 1009)]),
-           ((512, 32, 32), [(63, 8192, 3001), (100, 10016, 1403), (256, 8192, 1000)]),
-           ((512, 64, 64), [(200, 544, 3800), (64, 4064, 11001), (1021, 2016, 1003), (1000, 8224, 1001)]),
+KERNELS = [((256, 16, 16), [(7, 544, 1003), (1, 11008, 500), (16, 4128, 900), (100, 192, 1009), (33, 4128, 1003)]),
+           ((512, 32, 32), [(33, 288, 4001), (61, 1056, 3005), (128, 2080, 1003), (250, 14016, 300), (5, 4096, 8190)]),
+           ((512, 32, 64), [(40, 5024, 8004), (100, 10016, 3003), (20, 736, 13001)]),
+           ((512, 64, 64), [(200, 544, 3800), (64, 4064, 11001), (1021, 2016, 1003), (63, 11008, 9003)]),
            ((512, 64, 128), [(120, 3904, 10003), (505, 1312, 3003), (1000, 16384, 2001)]),
            ((512, 128, 128), [(240, 4096, 10001), (513, 2080, 4003), (1010, 11008, 4001)]),
            ((512, 256, 128), [(1011, 768, 8001), (400, 4192, 11002)])]

@@ -327,4 +327,5 @@ constexpr l2c::Mx4Tile tile(double launch, double per_tile, double per_k) {
 }  // namespace
 
 const l2c::Mx4Tile l2c::mx4_lds_tiles[kMx4LdsTiles] = {tile<1, 1, 4>(2515, 1150, 1.166), tile<1, 2, 4>(498, 3560, 1.731),
-                                                       tile<2, 2, 4>(0, 5454, 2.199), tile<4, 2, 3>(1317, 7368, 2.907)};
+                                                       tile<2, 2, 4>(0, 5454, 2.199), tile<2, 3, 3>(0, 6769, 2.769),
+                                                       tile<4, 2, 3>(1317, 7368, 2.907)};

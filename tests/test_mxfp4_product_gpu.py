@@ -141,7 +141,8 @@ KERNELS = [((256, 16, 16), [(7, 544, 1003), (1, 11008, 500), (16, 4128, 900), (1
            ((512, 64, 64), [(200, 544, 3800), (64, 4064, 11001), (1021, 2016, 1003), (63, 11008, 9003)]),
            ((512, 64, 128), [(120, 3904, 10003), (505, 1312, 3003), (1000, 16384, 2001)]),
            ((512, 128, 128), [(240, 4096, 10001), (513, 2080, 4003), (1010, 11008, 4001)]),
-           ((512, 256, 128), [(1011, 768, 8001), (400, 4192, 11002)])]
+           ((512, 128, 192), [(500, 1120, 10801), (400, 4192, 11002), (384, 608, 10901)]),
+           ((512, 256, 128), [(1011, 768, 8001), (1000, 4192, 8190)])]
 
 
 @pytest.mark.parametrize("kernel,shapes", KERNELS, ids=str)

@@ -8,20 +8,18 @@
 //  * beam_chunks_kernel, a workgroup per chunk of a row of logits: one pass over the
 //    data, 1024 V logits at a time, which the lanes hold in registers. It leaves the
 //    chunk's maximum, its sum of exponentials and its `beams` largest logits in order.
-//    Nothing is sorted: the K-th largest of the maxima of a wave's groups of 8 to 32 values
-//    is a bound that at least K values reach, and few more do. It is found bit by bit, by
-//    ballots. The values that reach the largest of the waves' bounds (and the K-th so far)
-//    go to a list in LDS, where each finds its rank by comparison with the others. A wave
-//    has at most K groups that reach the bound, so the list's length has a bound too.
+//    Nothing is sorted: each of the four waves finds the K/4-th largest of its lanes' maxima,
+//    bit by bit, by ballots (for K <= 4 its maximum); the least of the four is a bound that at
+//    least K values reach, and few more do. Those go to a list in LDS, where each finds its
+//    rank by comparison with the others. So that the list has a length, a wave of which more
+//    than K lanes reach the bound goes by the K-th largest of its own.
 //  * beam_join_kernel, a workgroup per request: the rows' sums, and the same choice
-//    among the chunks' lists by their 64-bit scores. Rows are cut into no more chunks than
-//    leave it kJoinCandidates candidates.
+//    among the chunks' lists by their 64-bit scores. The lists are found by their firsts.
 //
-// The order is total: larger first, then the lower beam, then the lower token; within
-// a row by the logits themselves. Results do not depend on the order of the list's
-// atomics. Sums of exponentials are fp32 within a lane and 64-bit across lanes, scores
-// 64-bit until they are stored: beams' scores lie close together, and a rounding
-// there would change which tokens are chosen.
+// The order is total: larger first, then the lower beam, its larger logit, the lower
+// token. Results do not depend on the order of the list's atomics. Sums of exponentials are
+// fp32 within a lane and 64-bit across lanes, scores 64-bit until they are stored: beams'
+// scores lie close together, and a rounding there would change which tokens are chosen.
 #include <climits>
 
 #include "l2c_common.h"
@@ -138,21 +136,17 @@ __device__ __forceinline__ double row_sum(double v) {
   return v + other<kRotate1>(v);
 }
 
-// A bound that at least k of the wave's 64 G values reach: exactly k of them, or, where the
+// A bound that at least k of the wave's 64 values reach: exactly k of them, or, where the
 // k-th largest ties with the next, all that are as large, and the bound is that value. 0 if
 // fewer than k are not 0. A bit at a time, to where just k are left: the steps wait for
 // each other, but are scalar instructions for the most part, which other waves leave idle
 // (starting at the first bit in which the values differ, or two bits a step, measured 20%
 // slower for 256 x 4 x 32003).
-template <typename T, int G>
-__device__ __forceinline__ int wave_reach(const T (&v)[G], T bound) {
-  int reach = 0;
-#pragma unroll
-  for (int g = 0; g < G; ++g) reach += __popcll(__ballot(v[g] >= bound));
-  return reach;
+template <typename T>
+__device__ __forceinline__ int wave_reach(T v, T bound) {
+  return __popcll(__ballot(v >= bound));
 }
-template <int G>
-__device__ __forceinline__ unsigned wave_bound(const unsigned (&v)[G], int k) {
+__device__ __forceinline__ unsigned wave_bound(unsigned v, int k) {
   unsigned bound = 0;
   for (int bit = 31; bit >= 0; --bit) {
     const unsigned next = bound | 1u << bit;
@@ -162,10 +156,9 @@ __device__ __forceinline__ unsigned wave_bound(const unsigned (&v)[G], int k) {
   }
   return bound;
 }
-// Of one 64-bit value a lane, two bits a step, whose ballots do not wait for each other: one
-// wave's time counts where nothing else runs.
-__device__ __forceinline__ u64 wave_bound(u64 value, int k) {
-  const u64 v[1] = {value};
+// Of 64-bit values two bits a step, whose ballots do not wait for each other: one wave's
+// time counts where nothing else runs.
+__device__ __forceinline__ u64 wave_bound(u64 v, int k) {
   u64 bound = 0;
   if (wave_reach(v, static_cast<u64>(1)) < k) return bound;
   for (int bit = 62; bit >= 0; bit -= 2) {
@@ -197,18 +190,17 @@ __device__ __forceinline__ Order order(const u64 *values, int n, u64 than) {
   return count;
 }
 
-// V float4 a lane, in GROUPS groups. A row is `chunks` chunks of `parts` parts of kThreads * 4 V
-// logits (the last ones shorter); MANY: of more than one part.
-template <int V, int GROUPS, bool MANY>
+// V float4 a lane. A row is `chunks` chunks of `parts` parts of kThreads * 4 V logits (the
+// last ones shorter); MANY: of more than one part.
+template <int V, bool MANY>
 __global__ __launch_bounds__(kThreads) void beam_chunks_kernel(unsigned char *__restrict__ workspace,
                                                                const float *__restrict__ logits,
                                                                const int *__restrict__ tokens, int eos, int vocab,
                                                                int beams, int chunks, int parts) {
   constexpr int kPart = kThreads * 4 * V;
-  constexpr int kEach = 4 * V / GROUPS;  // values of a group
-  extern __shared__ u64 list[];  // `beams` groups of each wave at most, and eight that order() may read
+  extern __shared__ u64 list[];  // `beams` lanes' values of each wave at most, and eight that order() may read
   __shared__ u64 kept[2][kMaxBeams + 8];  // the largest so far, in order
-  __shared__ u64 bounds[kWaves];
+  __shared__ unsigned bounds[kWaves];
   __shared__ float tops[kWaves];
   __shared__ double sums[kWaves];
   __shared__ int length;
@@ -234,6 +226,7 @@ __global__ __launch_bounds__(kThreads) void beam_chunks_kernel(unsigned char *__
   float shift = -INFINITY;     // the largest so far
   int count = 0;               // of `kept`
   int turn = 0;
+  const int quarter = (beams + kWaves - 1) / kWaves;
   for (int start = 0;;) {
     const int n = min(kPart, whole - start);
     const bool more = MANY && whole - start > kPart;
@@ -250,49 +243,26 @@ __global__ __launch_bounds__(kThreads) void beam_chunks_kernel(unsigned char *__
     if (more) load(q, start + kPart);
     auto place = [&](int i) __attribute__((always_inline)) { return 4 * (t + i / 4 * kThreads) + i % 4; };
     auto key = [&](int i) __attribute__((always_inline)) { return place(i) < n ? key_of(v[i]) : 0u; };
-    // NaN does not count: a group of NaN has the key of -Inf here and
-    // emits nothing; one past the row has none.
+    // The lane's largest, -Inf where all are NaN; 0 past the row.
     float top = -INFINITY;
-    unsigned best[GROUPS];
 #pragma unroll
-    for (int g = 0; g < GROUPS; ++g) {
-      float m = -INFINITY;
-#pragma unroll
-      for (int i = kEach * g; i < kEach * (g + 1); ++i) m = fmaxf(m, v[i]);
-      best[g] = place(kEach * g) < n ? key_of(m) : 0u;
-      top = fmaxf(top, m);
-    }
-    const unsigned bound = wave_bound(best, beams);
-    unsigned bound_place = UINT_MAX;
-    if (bound != 0 && wave_reach(best, bound) > beams) {
-      // Of the groups whose maxima tie, those with the lowest first places.
-      unsigned before[GROUPS];  // UINT_MAX - place
-      int larger = 0;
-#pragma unroll
-      for (int g = 0; g < GROUPS; ++g) {
-        before[g] = 0;
-        larger += __popcll(__ballot(best[g] > bound));
-        if (best[g] != bound) continue;
-#pragma unroll
-        for (int i = kEach * (g + 1) - 1; i >= kEach * g; --i)
-          if (key(i) == bound) before[g] = UINT_MAX - (static_cast<unsigned>(start) + place(i));
-      }
-      const unsigned least_before = wave_bound(before, beams - larger);
-      bound_place = least_before == 0 ? UINT_MAX : UINT_MAX - least_before;
-    }
-    const float largest = wave_top(top);
+    for (int i = 0; i < 4 * V; ++i) top = fmaxf(top, v[i]);
+    const unsigned best = place(0) < n ? key_of(top) : 0u;
+    const float largest = wave_top(top);  // of the last lane
+    const unsigned bound = quarter == 1 ? key_of(largest) : wave_bound(best, quarter);
     if (lane == L2C_WAVE - 1) {
-      bounds[wave] = ordered(bound, bound_place);
+      bounds[wave] = bound;
       tops[wave] = largest;
     }
     __syncthreads();
-    u64 least = MANY && count == beams ? kept[turn][beams - 1] : 0;
+    unsigned least = bounds[0];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) least = min(least, bounds[w]);
+    if (MANY && count == beams) least = max(least, static_cast<unsigned>(kept[turn][beams - 1] >> 32));
+    least = max(least, 1u);
     float maximum = shift;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      least = max(least, bounds[w]);
-      maximum = fmaxf(maximum, tops[w]);
-    }
+    for (int w = 0; w < kWaves; ++w) maximum = fmaxf(maximum, tops[w]);
     if (maximum > shift) {  // the lane's sum so far is of exp(x - the old maximum)
       if (MANY && start > 0) total *= exp(static_cast<double>(shift) - static_cast<double>(maximum));
       shift = maximum;
@@ -302,17 +272,30 @@ __global__ __launch_bounds__(kThreads) void beam_chunks_kernel(unsigned char *__
 #pragma unroll
     for (int i = 0; i < 4 * V; ++i) sum += exp_nonpositive(v[i] - subtract);
     total += static_cast<double>(sum);
-    // The values that reach the bound into the list, a wave's after each other's.
+    // The values that reach the bound into the list, a wave's after each other's. If more than
+    // `beams` of its lanes have such, only those of the `beams` lanes with the largest, and
+    // of lanes that tie, with the lowest places of it: no other value can be among the chosen.
+    u64 own = 0;
+    if (wave_reach(best, least) > beams) {
+      const unsigned lanes_bound = wave_bound(best, beams);
+      const int larger = __popcll(__ballot(best > lanes_bound));
+      unsigned before = 0;  // UINT_MAX - place
+      if (best == lanes_bound) {
+#pragma unroll
+        for (int i = 4 * V - 1; i >= 0; --i)
+          if (key(i) == lanes_bound) before = UINT_MAX - (static_cast<unsigned>(start) + place(i));
+      }
+      own = static_cast<u64>(lanes_bound) << 32 | wave_bound(before, beams - larger);
+    }
     unsigned reach = 0;
-    const unsigned least_key = static_cast<unsigned>(least >> 32);
-    if (least_key > key_of(-INFINITY) && static_cast<unsigned>(least) == 0) {  // no ties to break, and none past the end
-      const float limit = number_of(least_key);
+    if (own == 0 && least > key_of(-INFINITY)) {  // neither NaN nor what is past the end reaches it
+      const float limit = number_of(least);
 #pragma unroll
       for (int i = 0; i < 4 * V; ++i) reach |= v[i] >= limit ? 1u << i : 0u;
     } else {
 #pragma unroll
       for (int i = 0; i < 4 * V; ++i)
-        if (key(i) != 0 && ordered(key(i), static_cast<unsigned>(start) + place(i)) >= least) reach |= 1u << i;
+        if (key(i) >= least && ordered(key(i), static_cast<unsigned>(start) + place(i)) >= own) reach |= 1u << i;
     }
     if (__ballot(reach != 0)) {
       const int count_here = __popc(reach), upto = wave_scan(count_here);
@@ -362,8 +345,6 @@ __global__ __launch_bounds__(kThreads) void beam_chunks_kernel(unsigned char *__
   }
 }
 
-constexpr int kJoinCandidates = 16 * kThreads;
-
 // Quotients of values below 2^16 by one of 1 to 2^16, without a division each.
 struct Quotient {
   unsigned by;
@@ -371,20 +352,28 @@ struct Quotient {
   __device__ __forceinline__ int operator()(int v) const { return by ? __umulhi(v, by) : v; }
 };
 
-// The lanes hold HELD candidates each in registers.
-template <int HELD>
+constexpr int kJoinLists = 4 * kThreads;  // at most
+constexpr int kChosenCandidates = kMaxBeams * (kMaxBeams + 1) / 2;
+
+// DIRECT: the lanes hold all candidates, one each. Else they hold the lists' firsts, HELD
+// each. The `beams` lists with the largest firsts have all that can be chosen, of the one
+// in place p (from 0) the first beams - p, and these follow from memory.
+template <int HELD, bool DIRECT>
 __global__ __launch_bounds__(kThreads) void beam_join_kernel(float *scores_out, int *tokens_out, int *parents,
                                                              int *generated, const unsigned char *workspace,
                                                              const float *scores, const int *tokens, int eos,
                                                              int beams, int chunks, int steps, int step) {
+  constexpr int kEntries = (DIRECT || HELD * kThreads > kChosenCandidates ? HELD * kThreads : kChosenCandidates) + 8;
   // A beam's scores are base + (logit - top), in this order: logits of the lowest value
   // would take the rest of the sum with them. NaN: no candidates.
   __shared__ double base[kMaxBeams];
   __shared__ float tops[kMaxBeams];
   __shared__ bool ended[kMaxBeams];
-  __shared__ u64 list_key[HELD * kThreads + 8], list_place[HELD * kThreads + 8];
-  __shared__ u64 slots[kWaves];
-  __shared__ int length;
+  __shared__ u64 list_key[kEntries], list_logit[kEntries];
+  __shared__ int list_at[kEntries];
+  __shared__ int chosen[kMaxBeams];
+  __shared__ u64 slots[kWaves], last_first;
+  __shared__ int lengths[2];
   constexpr int kGroup = 16;  // lanes a beam for its chunks' sums
   const int t = threadIdx.x, lane = t % L2C_WAVE, wave = t / L2C_WAVE;
   const int first = blockIdx.x * beams;
@@ -393,16 +382,15 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(float *scores_out, 
     return stats + static_cast<size_t>(first + beam) * chunks + chunk;
   };
   // Candidate i: rank i / lists of list i % lists, a list a chunk, beam after beam: the first
-  // lanes have the lists' best, and their maxima are a good bound.
-  const int lists = beams * chunks, candidates = lists * beams;
-  const Quotient by_lists(lists), by_chunks(chunks);
-  auto beam_of = [&](int i) __attribute__((always_inline)) { return by_chunks(i - by_lists(i) * lists); };
+  // lanes have the lists' firsts, and their maxima are a good bound.
+  const int lists = beams * chunks, candidates = lists * beams, entries = DIRECT ? candidates : lists;
+  const Quotient by_lists(lists), by_chunks(chunks), by_beams(beams);
   const Candidate *const all = reinterpret_cast<const Candidate *>(stats + static_cast<size_t>(gridDim.x) * lists) +
                                static_cast<size_t>(blockIdx.x) * candidates;
   Candidate held[HELD];
 #pragma unroll
-  for (int r = 0; r < HELD; ++r) held[r] = all[min(t + r * kThreads, candidates - 1)];  // together, without a branch
-  if (t == 0) length = 0;
+  for (int r = 0; r < HELD; ++r) held[r] = all[min(t + r * kThreads, entries - 1)];  // together, without a branch
+  if (t < 2) lengths[t] = 0;
   for (int k = t / kGroup; k < beams; k += kThreads / kGroup) {  // whole groups stay together
     const int member = t % kGroup;
     // Of an ended row the workspace holds nothing; what is read there is not used.
@@ -431,32 +419,40 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(float *scores_out, 
     }
   }
   __syncthreads();
-  // A candidate's key, 0 where it is none, and place.
-  auto key_at = [&](int i, Candidate c) __attribute__((always_inline)) -> u64 {
-    const int beam = beam_of(i);
+  // The key of candidate `rank` of `list`, 0 where it is none.
+  auto key_at = [&](int list, int rank, Candidate c) __attribute__((always_inline)) -> u64 {
+    const int beam = by_chunks(list);
     const bool end = ended[beam];
     const double score = base[beam] + (end ? 0.0 : static_cast<double>(c.logit) - static_cast<double>(tops[beam]));
-    const bool is = end ? i == beam * chunks : c.token >= 0 && c.logit > -INFINITY;
-    return is && i < candidates ? key_of(score) : 0ULL;
+    const bool is = end ? rank == 0 && list == beam * chunks : c.token >= 0 && c.logit > -INFINITY;
+    return is ? key_of(score) : 0ULL;
   };
-  auto place_at = [&](int i, Candidate c) __attribute__((always_inline)) {
-    const int beam = beam_of(i);
-    return static_cast<u64>(beam) << 32 | static_cast<unsigned>(ended[beam] ? eos : c.token);
+  // Entry `to`. What decides between equal keys: the lower beam and its larger logit, then
+  // the lower `at`.
+  auto enter = [&](int to, u64 key, int list, Candidate c, int at) __attribute__((always_inline)) {
+    const int beam = by_chunks(list);
+    list_key[to] = key;
+    list_logit[to] = static_cast<u64>(beam) << 32 | (ended[beam] ? 0u : UINT_MAX - key_of(c.logit));
+    list_at[to] = at;
   };
-  auto write = [&](int rank, u64 key, u64 place) __attribute__((always_inline)) {
-    const int to = first + rank;
-    const int token = key ? static_cast<int>(place) : -1;
-    scores_out[to] = key ? static_cast<float>(number_of(key)) : -INFINITY;
-    tokens_out[to] = token;
-    parents[to] = key ? static_cast<int>(place >> 32) : -1;
-    if (generated) generated[static_cast<size_t>(to) * steps + step] = token;
+  auto token_of = [&](int list, Candidate c) __attribute__((always_inline)) { return ended[by_chunks(list)] ? eos : c.token; };
+  auto rank_of = [&](int e, int m) __attribute__((always_inline)) {
+    const u64 key = list_key[e], logit = list_logit[e];
+    const int at = list_at[e];
+    const Order among = order(list_key, m, key);
+    int rank = among.larger;
+    if (among.equal > 1)
+      for (int o = 0; o < m; ++o)
+        rank += list_key[o] == key && (list_logit[o] < logit || (list_logit[o] == logit && list_at[o] < at));
+    return rank;
   };
 
-  // A bound that at least `beams` candidates reach, from the lanes' best; equal keys all pass.
+  // A bound that at least `beams` entries reach, from the lanes' best; equal keys all pass.
   u64 best = 0, held_key[HELD];
 #pragma unroll
   for (int r = 0; r < HELD; ++r) {
-    held_key[r] = key_at(t + r * kThreads, held[r]);
+    const int i = t + r * kThreads, rank = DIRECT ? by_lists(i) : 0, list = DIRECT ? i - rank * lists : min(i, lists - 1);
+    held_key[r] = i < entries ? key_at(list, rank, held[r]) : 0ULL;
     best = max(best, held_key[r]);
   }
   const u64 bound = wave_bound(best, beams);
@@ -472,61 +468,91 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(float *scores_out, 
   if (__ballot(reach != 0)) {
     const int count_here = __popc(reach), upto = wave_scan(count_here);
     int from = 0;
-    if (lane == L2C_WAVE - 1) from = atomicAdd(&length, upto);
+    if (lane == L2C_WAVE - 1) from = atomicAdd(&lengths[0], upto);
     int to = __builtin_amdgcn_readlane(from, L2C_WAVE - 1) + upto - count_here;
 #pragma unroll
     for (int r = 0; r < HELD; ++r) {
       if (reach >> r & 1) {
-        list_key[to] = held_key[r], list_place[to] = place_at(t + r * kThreads, held[r]);
-        ++to;
+        const int i = t + r * kThreads, list = DIRECT ? i - by_lists(i) * lists : i;
+        enter(to++, held_key[r], list, held[r], DIRECT ? token_of(list, held[r]) : list);
       }
     }
   }
   __syncthreads();
-  const int m = length;
-  for (int e = t; e < m; e += kThreads) {
-    const u64 key = list_key[e], place = list_place[e];
-    const Order among = order(list_key, m, key);
-    int rank = among.larger;
-    if (among.equal > 1)  // it and others: the lower place first
-      for (int o = 0; o < m; ++o) rank += list_key[o] == key && list_place[o] < place;
-    if (rank < beams) write(rank, key, place);
+  int m = lengths[0];
+  if (!DIRECT) {
+    for (int e = t; e < m; e += kThreads) {
+      const int rank = rank_of(e, m);
+      if (rank < beams) chosen[rank] = list_at[e];
+      if (rank == beams - 1) last_first = list_key[e];
+    }
+    if (m < beams && t == 0) last_first = 1;
+    __syncthreads();
+    constexpr int kEach = kMaxBeams * kMaxBeams / kThreads;
+    const int count = min(m, beams);
+    least = last_first;
+    Candidate c[kEach];
+    int list[kEach], rank[kEach];
+#pragma unroll
+    for (int u = 0; u < kEach; ++u) {
+      const int i = t + u * kThreads, place = by_beams(i);
+      rank[u] = i - place * beams;
+      list[u] = place < count && place + rank[u] < beams ? chosen[place] : -1;
+      c[u] = all[list[u] >= 0 ? rank[u] * lists + list[u] : 0];
+    }
+#pragma unroll
+    for (int u = 0; u < kEach; ++u) {
+      if (list[u] < 0) continue;
+      const u64 key = key_at(list[u], rank[u], c[u]);
+      if (key >= least) enter(atomicAdd(&lengths[1], 1), key, list[u], c[u], token_of(list[u], c[u]));
+    }
+    __syncthreads();
+    m = lengths[1];
   }
-  for (int e = m + t; e < beams; e += kThreads) write(e, 0, 0);
+  auto write = [&](int rank, u64 key, int parent, int token) __attribute__((always_inline)) {
+    const int to = first + rank;
+    scores_out[to] = key ? static_cast<float>(number_of(key)) : -INFINITY;
+    tokens_out[to] = token;
+    parents[to] = parent;
+    if (generated) generated[static_cast<size_t>(to) * steps + step] = token;
+  };
+  for (int e = t; e < m; e += kThreads) {
+    const int rank = rank_of(e, m);
+    if (rank < beams) write(rank, list_key[e], static_cast<int>(list_logit[e] >> 32), list_at[e]);
+  }
+  for (int e = m + t; e < beams; e += kThreads) write(e, 0, -1, -1);
 }
 
 using ChunkKernel = void (*)(unsigned char *, const float *, const int *, int, int, int, int, int);
 
 struct ChunkConfig {
   ChunkKernel fn;
-  int values;         // of a group
+  int values;         // of a lane
   int chunks, parts;  // chunks a row, parts a chunk
 };
 
-template <int V, int GROUPS>
+template <int V>
 ChunkConfig config(int vocab, int most_chunks) {
   const int parts = (vocab - 1) / (kThreads * 4 * V) + 1;
   const int each = (parts - 1) / most_chunks + 1;
-  return {each > 1 ? beam_chunks_kernel<V, GROUPS, true> : beam_chunks_kernel<V, GROUPS, false>, 4 * V / GROUPS,
+  return {each > 1 ? beam_chunks_kernel<V, true> : beam_chunks_kernel<V, false>, 4 * V,
           (parts - 1) / each + 1, each};
 }
 
 // 2048 logits a chunk as long as that makes at most 4096 chunks, and then 4096 logits: small
 // chunks have the least latency (1 x 4 x 32000: 8.1 us in chunks of 2048, 9.3 of 4096, 10.9
 // of 8192). Else 8192, which cost the least instructions a logit (256 x 4 x 32003: 42.6, 35.4,
-// 33.8). With many beams a lane's values go in groups of eight: the bound is
-// closer, and the list four times shorter (32 x 32 x 32000 54 us, 66 in one group; 256 x 4 x
-// 32003 35.4, 33.8 in one).
+// 33.8).
 ChunkConfig chunk_config(int vocab, int beams, int batch) {
-  const int most = kJoinCandidates / (beams * beams);
+  const int most = kJoinLists / beams;
   const double rows = static_cast<double>(batch) * beams;
   auto fits = [&](int part) {
     const int parts = (vocab - 1) / part + 1;
     return parts <= most && rows * parts <= 4096;
   };
-  if (fits(2048)) return config<2, 1>(vocab, most);
-  if (fits(4096)) return beams > 8 ? config<4, 2>(vocab, most) : config<4, 1>(vocab, most);
-  return beams > 8 ? config<8, 4>(vocab, most) : config<8, 1>(vocab, most);
+  if (fits(2048)) return config<2>(vocab, most);
+  if (fits(4096)) return config<4>(vocab, most);
+  return config<8>(vocab, most);
 }
 
 }  // namespace
@@ -557,10 +583,12 @@ extern "C" int l2c_decoder_beam_select(float *scores_out, int *tokens_out, int *
   hipLaunchKernelGGL(c.fn, dim3(static_cast<unsigned>(grid)), dim3(kThreads), list, stream, w, logits, tokens, eos,
                      vocab, beams, c.chunks, c.parts);
   L2C_LAUNCH_CHECK();
-  const int candidates = beams * beams * c.chunks;
-  hipLaunchKernelGGL(candidates <= kThreads ? beam_join_kernel<1>
-                     : candidates <= 4 * kThreads ? beam_join_kernel<4> : beam_join_kernel<16>, dim3(static_cast<unsigned>(batch)), dim3(kThreads), 0, stream, scores_out,
-                     tokens_out, parents, generated, w, scores, tokens, eos, beams, c.chunks, steps, step);
+  const int lists = beams * c.chunks;
+  auto join = beams * lists <= kThreads ? beam_join_kernel<1, true>
+              : lists <= kThreads       ? beam_join_kernel<1, false>
+                                        : beam_join_kernel<4, false>;
+  hipLaunchKernelGGL(join, dim3(static_cast<unsigned>(batch)), dim3(kThreads), 0, stream, scores_out, tokens_out, parents,
+                     generated, w, scores, tokens, eos, beams, c.chunks, steps, step);
   L2C_LAUNCH_CHECK();
   return hipSuccess;
 }

@@ -342,8 +342,8 @@ int l2c_decoder_softmax_argmax(float *probabilities, const float *logits, int *t
  *
  * l2c_decoder_beam_select: the `beams` best continuations of every request among
  *   scores[row k] + logits[row k][v] - log(sum_u exp(logits[row k][u]))
- *   over its beams k and tokens v < vocab, the largest first, equal scores in the order of
- *   (k, v). They become the request's next beams: scores_out, tokens_out (v) and parents
+ *   over its beams k and tokens v < vocab, the largest first, equal scores in the order of k
+ *   and, of one beam, of the logits, equal logits in the order of v. They become the request's next beams: scores_out, tokens_out (v) and parents
  *   (k) in rows b * beams + 0, 1, ...; and generated[row * steps + step] = v, unless
  *   generated is NULL (the earlier columns follow by l2c_decoder_beam_reorder).
  *   A beam whose token tokens[row k] is eos (eos >= 0) has ended: its one continuation is

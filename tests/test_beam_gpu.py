@@ -131,6 +131,39 @@ def test_ties(torch_gpu, l2c):
         assert (pa == 0).all()
 
 
+@pytest.mark.parametrize("vocab", [300, 5000, 65540, 200001])
+@pytest.mark.parametrize("beams", [1, 4, 16, 32])
+def test_equal_scores_of_many_lists(torch_gpu, l2c, vocab, beams):
+    """All continuations equal: beam 0's first tokens, in every chunk alike."""
+    rows = beams
+    s, t, p = check_select(torch_gpu, l2c, np.zeros((rows, vocab), np.float32), np.full(rows, -3.0),
+                           np.zeros(rows, int), -1, beams)
+    np.testing.assert_array_equal(t, np.arange(beams))
+    np.testing.assert_array_equal(p, 0)
+
+
+@pytest.mark.parametrize("vocab", [300, 5000, 65540, 200001])
+@pytest.mark.parametrize("beams", [2, 4, 16, 32])
+def test_scores_equal_where_logits_are_not(torch_gpu, l2c, vocab, beams):
+    """Logits whose difference from the largest is the same in 64 bits: a beam's continuations
+    follow its logits, equal scores of several beams the beam."""
+    torch = torch_gpu
+    rng = np.random.default_rng(vocab + beams)
+    logits = np.zeros((beams, vocab), np.float32)
+    logits[:] = 1e-30 * rng.permutation(vocab)
+    logits[:, 7] = 10.0
+    for live in {1, 2}:
+        scores = np.where(np.arange(beams) < live, -1.0, -np.inf)
+        x = torch.from_numpy(logits.reshape(-1)).cuda()
+        dev = {n: torch.zeros(beams, dtype=torch.float32 if n == "s" else torch.int32, device="cuda") for n in "stp"}
+        s0, t0 = torch.from_numpy(scores.astype(np.float32)).cuda(), torch.zeros(beams, dtype=torch.int32, device="cuda")
+        ws = torch.empty(l2c.decoder_beam_workspace_bytes(vocab, beams, 1), dtype=torch.uint8, device="cuda")
+        l2c.decoder_beam_select(dev["s"], dev["t"], dev["p"], None, x, s0, t0, -1, vocab, beams, 1, 1, 0, ws)
+        rest = np.argsort(-logits[0], kind="stable")[1:beams - live + 1]
+        np.testing.assert_array_equal(dev["t"].cpu().numpy(), [7] * live + list(rest))
+        np.testing.assert_array_equal(dev["p"].cpu().numpy(), list(range(live)) + [0] * (beams - live))
+
+
 def test_masks(torch_gpu, l2c):
     """Rows masked in part, but for less than the beams, wholly; with the lowest value instead;
     NaN and +Inf; dead beams; and requests that have fewer continuations than beams or none."""

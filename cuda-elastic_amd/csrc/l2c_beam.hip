@@ -82,8 +82,8 @@ __device__ __forceinline__ u64 ordered(unsigned key, unsigned place) {
 // Values of other lanes through the adders' operand paths (DPP), which take a tenth of a
 // trip through LDS: from 1, 2, 4 or 8 lanes before in rows of 16, from the row before's
 // last lane, from the lower half's last lane; or rotated in rows of 16.
-enum Dpp { kBefore1 = 0x111, kBefore2 = 0x112, kBefore4 = 0x114, kBefore8 = 0x118, kRowBefore = 0x142, kHalfBefore = 0x143,
-           kRotate1 = 0x121, kRotate2 = 0x122, kRotate4 = 0x124, kRotate8 = 0x128 };
+enum Dpp { kBefore1 = 0x111, kBefore2 = 0x112, kBefore4 = 0x114, kBefore8 = 0x118, kRowBefore = 0x142,
+           kHalfBefore = 0x143, kRotate1 = 0x121, kRotate2 = 0x122, kRotate4 = 0x124, kRotate8 = 0x128 };
 
 // `none` where there is no such lane.
 template <int FROM>
@@ -235,7 +235,8 @@ __global__ __launch_bounds__(kThreads) void beam_chunks_kernel(unsigned char *__
 #pragma unroll
       for (int c = 0; c < V; ++c) {
         const int j = 4 * (t + c * kThreads);
-        q[c] = j < n ? l2c::whole_chunk(q[c], j, n, -INFINITY) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        q[c] = j < n ? l2c::whole_chunk(q[c], j, n, -INFINITY)
+                     : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
       }
     }
 #pragma unroll
@@ -327,8 +328,8 @@ __global__ __launch_bounds__(kThreads) void beam_chunks_kernel(unsigned char *__
   ChunkStat *const stats = reinterpret_cast<ChunkStat *>(workspace);
   if (t < beams) {
     const int request = row / beams;
-    Candidate *const out = reinterpret_cast<Candidate *>(stats + gridDim.x) +
-                           ((static_cast<size_t>(request) * beams + t) * beams + (row - request * beams)) * chunks + chunk;
+    const size_t place = (static_cast<size_t>(request) * beams + t) * beams + (row - request * beams);
+    Candidate *const out = reinterpret_cast<Candidate *>(stats + gridDim.x) + place * chunks + chunk;
     const u64 mine = t < count ? kept[turn][t] : 0;
     *out = t < count ? Candidate{number_of(static_cast<unsigned>(mine >> 32)),
                                  first + static_cast<int>(UINT_MAX - static_cast<unsigned>(mine))}
@@ -435,7 +436,9 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(float *scores_out, 
     list_logit[to] = static_cast<u64>(beam) << 32 | (ended[beam] ? 0u : UINT_MAX - key_of(c.logit));
     list_at[to] = at;
   };
-  auto token_of = [&](int list, Candidate c) __attribute__((always_inline)) { return ended[by_chunks(list)] ? eos : c.token; };
+  auto token_of = [&](int list, Candidate c) __attribute__((always_inline)) {
+    return ended[by_chunks(list)] ? eos : c.token;
+  };
   auto rank_of = [&](int e, int m) __attribute__((always_inline)) {
     const u64 key = list_key[e], logit = list_logit[e];
     const int at = list_at[e];
@@ -451,7 +454,8 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(float *scores_out, 
   u64 best = 0, held_key[HELD];
 #pragma unroll
   for (int r = 0; r < HELD; ++r) {
-    const int i = t + r * kThreads, rank = DIRECT ? by_lists(i) : 0, list = DIRECT ? i - rank * lists : min(i, lists - 1);
+    const int i = t + r * kThreads, rank = DIRECT ? by_lists(i) : 0;
+    const int list = DIRECT ? i - rank * lists : min(i, lists - 1);
     held_key[r] = i < entries ? key_at(list, rank, held[r]) : 0ULL;
     best = max(best, held_key[r]);
   }
@@ -587,8 +591,8 @@ extern "C" int l2c_decoder_beam_select(float *scores_out, int *tokens_out, int *
   auto join = beams * lists <= kThreads ? beam_join_kernel<1, true>
               : lists <= kThreads       ? beam_join_kernel<1, false>
                                         : beam_join_kernel<4, false>;
-  hipLaunchKernelGGL(join, dim3(static_cast<unsigned>(batch)), dim3(kThreads), 0, stream, scores_out, tokens_out, parents,
-                     generated, w, scores, tokens, eos, beams, c.chunks, steps, step);
+  hipLaunchKernelGGL(join, dim3(static_cast<unsigned>(batch)), dim3(kThreads), 0, stream, scores_out, tokens_out,
+                     parents, generated, w, scores, tokens, eos, beams, c.chunks, steps, step);
   L2C_LAUNCH_CHECK();
   return hipSuccess;
 }

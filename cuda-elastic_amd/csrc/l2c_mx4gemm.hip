@@ -76,6 +76,8 @@ __global__ __launch_bounds__(kQuantThreads) void quantize_mxfp4_bf16_kernel(uint
 // 12.9 on 64 x 64, 11.3 on 64 x 128; 512 x 4096 x 11008 32.3 on 128 x 128, 21.4 on 128 x
 // 192, 24.4 on 256 x 128; 400 x 4096 x 11008 27.2 on 128 x 128, 21.1 on 256 x 128.
 
+constexpr int kMaxCols = (1 << 24) - 32;  // a tile's 256 rows of codes stay within 31 bits
+
 long long tiles_of(const l2c::Mx4Tile &t, int batch, int rows) {
   return ((batch + static_cast<long long>(t.bm) - 1) / t.bm) * ((rows + static_cast<long long>(t.bn) - 1) / t.bn);
 }
@@ -116,7 +118,7 @@ extern "C" int l2c_matmul_mxfp4(float *out, const uint8_t *X, const uint8_t *Xsc
   if (batch < 0 || cols <= 0 || rows < 0 || cols % 32 != 0) return hipErrorInvalidValue;
   if (batch == 0 || rows == 0) return hipSuccess;
   if (!out || !X || !Xscales || !W || !Wscales || !l2c_aligned16(X) || !l2c_aligned16(W)) return hipErrorInvalidValue;
-  if (256LL * (cols / 2) > INT_MAX) return hipErrorInvalidValue;
+  if (cols > kMaxCols) return hipErrorInvalidValue;
   const l2c::Mx4Tile *t = choose(batch, cols / 32, rows);
   if (!t) return hipErrorInvalidValue;
   hipLaunchKernelGGL(t->fn, dim3(static_cast<unsigned>(tiles_of(*t, batch, rows))), dim3(t->threads), 0, stream, out, X,
@@ -126,7 +128,8 @@ extern "C" int l2c_matmul_mxfp4(float *out, const uint8_t *X, const uint8_t *Xsc
 }
 
 bool l2c_mx4_launch_shape(int batch, int cols, int rows, int *grid, int *block, const void **fn) {
-  const l2c::Mx4Tile *t = batch > 0 && rows > 0 && cols % 32 == 0 ? choose(batch, cols / 32, rows) : nullptr;
+  const bool known = batch > 0 && rows > 0 && cols > 0 && cols % 32 == 0 && cols <= kMaxCols;
+  const l2c::Mx4Tile *t = known ? choose(batch, cols / 32, rows) : nullptr;
   if (!t) return false;
   *grid = static_cast<int>(tiles_of(*t, batch, rows));
   *block = t->threads;

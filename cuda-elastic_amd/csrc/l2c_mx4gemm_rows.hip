@@ -87,8 +87,8 @@ __global__ __launch_bounds__(kThreads) void mxfp4_rows_kernel(float *__restrict_
   auto multiply = [&](const Group &g) __attribute__((always_inline)) {
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-      acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(g.x.codes[k]), wide(g.w.codes[k]), acc, kE2M1, kE2M1, 0,
-                                                             static_cast<int>(g.x.scales[k] >> (8 * q)), 0,
+      acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(g.x.codes[k]), wide(g.w.codes[k]), acc, kE2M1,
+                                                             kE2M1, 0, static_cast<int>(g.x.scales[k] >> (8 * q)), 0,
                                                              static_cast<int>(g.w.scales[k] >> (8 * q)));
   };
   const int groups = (blocks + kGroup - 1) / kGroup;

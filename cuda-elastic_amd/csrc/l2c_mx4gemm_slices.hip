@@ -93,8 +93,8 @@ __global__ __launch_bounds__(kThreads) void mxfp4_slice_kernel(float *__restrict
     for (int f = 0; f < kF; ++f) next[f] = *reinterpret_cast<const u64_any *>(scales[f] + min(8 * t, blocks - 8));
 #pragma unroll
     for (int i = 0; i < 4 * kF; ++i) {
-      const int block = dblock ^ (i % 2 * 4);
-      dma16(i < 4 * MI ? rx : rw, stage + 1024 * i, source[i] + 16 * (t < full ? block : min(block, rest - 1)), kRow * t);
+      const int block = dblock ^ (i % 2 * 4), inside = t < full ? block : min(block, rest - 1);
+      dma16(i < 4 * MI ? rx : rw, stage + 1024 * i, source[i] + 16 * inside, kRow * t);
     }
   };
   f32x16 acc[MI][NI];
@@ -134,8 +134,9 @@ __global__ __launch_bounds__(kThreads) void mxfp4_slice_kernel(float *__restrict
       for (int i = 0; i < MI; ++i)
 #pragma unroll
         for (int j = 0; j < NI; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(codes[i][c]), wide(codes[MI + j][c]), acc[i][j],
-                                                                       kE2M1, kE2M1, c, scale[i], c, scale[MI + j]);
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(codes[i][c]), wide(codes[MI + j][c]),
+                                                                       acc[i][j], kE2M1, kE2M1, c, scale[i], c,
+                                                                       scale[MI + j]);
     };
     multiply(std::integral_constant<int, 0>{});
     multiply(std::integral_constant<int, 1>{});

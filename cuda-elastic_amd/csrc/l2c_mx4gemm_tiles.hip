@@ -78,7 +78,8 @@ template <int MI, int NI, int STAGES>
 __global__ __launch_bounds__(kThreads) void mxfp4_tile_kernel(float *__restrict__ out, const uint8_t *__restrict__ X,
                                                               const uint8_t *__restrict__ Xs,
                                                               const uint8_t *__restrict__ W,
-                                                              const uint8_t *__restrict__ Ws, int M, int N, int blocks) {
+                                                              const uint8_t *__restrict__ Ws, int M, int N,
+                                                              int blocks) {
   using T = Tile<MI, NI, STAGES>;
   constexpr int kStages = STAGES;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[T::kLds];
@@ -167,8 +168,8 @@ __global__ __launch_bounds__(kThreads) void mxfp4_tile_kernel(float *__restrict_
   auto multiply = [&](auto half, auto parity, int k, const Scales &s) __attribute__((always_inline)) {
     constexpr int c = decltype(half)::value, p = decltype(parity)::value;
     const int i = k / NI, j = k % NI;
-    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(fa[c][i]), wide(fb[c][j]), acc[i][j], kE2M1, kE2M1, c,
-                                                                 s.x[i][p], c, s.w[j][p]);
+    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(fa[c][i]), wide(fb[c][j]), acc[i][j], kE2M1,
+                                                                 kE2M1, c, s.x[i][p], c, s.w[j][p]);
   };
   // Step t, in stage `at`: the products of its first half, among them the reads of its
   // second half's fragments; then, with all waves past their reads of the stage, the
@@ -326,6 +327,6 @@ constexpr l2c::Mx4Tile tile(double launch, double per_tile, double per_k) {
 
 }  // namespace
 
-const l2c::Mx4Tile l2c::mx4_lds_tiles[kMx4LdsTiles] = {tile<1, 1, 4>(2515, 1150, 1.166), tile<1, 2, 4>(498, 3560, 1.731),
-                                                       tile<2, 2, 4>(0, 5454, 2.199), tile<2, 3, 3>(0, 6769, 2.769),
-                                                       tile<4, 2, 3>(1317, 7368, 2.907)};
+const l2c::Mx4Tile l2c::mx4_lds_tiles[kMx4LdsTiles] = {
+    tile<1, 1, 4>(2515, 1150, 1.166), tile<1, 2, 4>(498, 3560, 1.731), tile<2, 2, 4>(0, 5454, 2.199),
+    tile<2, 3, 3>(0, 6769, 2.769), tile<4, 2, 3>(1317, 7368, 2.907)};

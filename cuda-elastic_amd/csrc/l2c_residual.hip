@@ -12,7 +12,8 @@
 // values, which its lanes hold in registers from the first load to the last store: eight
 // values a lane and chunk, whole 16-byte loads and stores at any address the types
 // allow. 1024 x 16384, fp32 to fp32 and bf16: 50 us, 4.7 TB/s (74 us with nontemporal
-// loads, which pass the MALL by); 1024 x 16384 bf16 28 us; 1 x 4096 3.0 us. Longer rows are read three times (from HBM once: the later passes hit the caches).
+// loads, which pass the MALL by); 1024 x 16384 bf16 28 us; 1 x 4096 3.0 us. Longer rows are
+// read three times (from HBM once: the later passes hit the caches).
 #include <type_traits>
 
 #include "l2c_common.h"

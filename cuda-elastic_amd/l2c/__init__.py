@@ -269,12 +269,19 @@ def rmsnorm(out, inp, weight, size, batch, eps=RMS_EPSILON, stream=None):
         _check(code, "l2c_rmsnorm")
 
 
+_types = {}  # of torch's
+
+
 def _type(t):
-    """The enum l2c_type of a tensor: 32-bit values or bf16 (any two-byte type)."""
-    size = t.element_size()
-    if size not in (2, 4):
-        raise ValueError("l2c.residual_rmsnorm takes fp32 and bf16 tensors")
-    return F32 if size == 4 else BF16
+    """The enum l2c_type of a tensor: fp32, or bf16, which two-byte integers may hold, too."""
+    kind = _types.get(t.dtype)
+    if kind is None:
+        known = {"torch.float32": F32, "torch.bfloat16": BF16, "torch.int16": BF16, "torch.uint16": BF16}
+        kind = known.get(str(t.dtype))
+        if kind is None:
+            raise ValueError(f"l2c.residual_rmsnorm takes fp32 and bf16 tensors, not {t.dtype}")
+        _types[t.dtype] = kind
+    return kind
 
 
 def residual_rmsnorm(normalized, residual_out, residual, block, weight, size, batch, block_weight=None, gate=None,
@@ -284,8 +291,8 @@ def residual_rmsnorm(normalized, residual_out, residual, block, weight, size, ba
     if residual_out is not None and _type(residual_out) != kind:
         raise ValueError("residual_out has another type than residual")
     code = _c_residual_rmsnorm(normalized, _type(normalized), residual_out, residual, kind, block, _type(block),
-                               block_weight, gate, rows_per_gate, weight, size, batch, float(residual_scale), float(eps),
-                               stream)
+                               block_weight, gate, rows_per_gate, weight, size, batch, float(residual_scale),
+                               float(eps), stream)
     if code:
         _check(code, "l2c_residual_rmsnorm")
 

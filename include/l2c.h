@@ -343,9 +343,10 @@ int l2c_decoder_softmax_argmax(float *probabilities, const float *logits, int *t
  * l2c_decoder_beam_select: the `beams` best continuations of every request among
  *   scores[row k] + logits[row k][v] - log(sum_u exp(logits[row k][u]))
  *   over its beams k and tokens v < vocab, the largest first, equal scores in the order of k
- *   and, of one beam, of the logits, equal logits in the order of v. They become the request's next beams: scores_out, tokens_out (v) and parents
- *   (k) in rows b * beams + 0, 1, ...; and generated[row * steps + step] = v, unless
- *   generated is NULL (the earlier columns follow by l2c_decoder_beam_reorder).
+ *   and, of one beam, of the logits, equal logits in the order of v. They become the request's
+ *   next beams: scores_out, tokens_out (v) and parents (k) in rows b * beams + 0, 1, ...; and
+ *   generated[row * steps + step] = v, unless generated is NULL (the earlier columns follow
+ *   by l2c_decoder_beam_reorder).
  *   A beam whose token tokens[row k] is eos (eos >= 0) has ended: its one continuation is
  *   eos at its own score, and its logits are not read. A beam has no continuation if its
  *   score is not finite (start a request with scores 0, -Inf, -Inf, ...), or its row holds a
@@ -366,7 +367,8 @@ int l2c_decoder_softmax_argmax(float *probabilities, const float *logits, int *t
  *   left as they are, and so is a row whose parent lies outside [0, beams). A cache
  *   [layers][batch * beams][heads][positions][width] of which the first `live` positions
  *   are in use has pieces = heads and piece_bytes = live * width * element size.
- *   out == in moves the rows in place; otherwise the two do not overlap. Any alignment
+ *   out == in moves the rows in place; otherwise the extents of the two, from their first
+ *   to their last byte, do not overlap (hipErrorInvalidValue). Any alignment
  *   (16-byte addresses and strides are fastest). A row has at most 2^31 - 1 units of 16
  *   bytes and odd bytes.
  */

@@ -61,6 +61,14 @@ def test_matmul_mxfp4_refuses(bad):
     assert product(**bad) == INVALID
 
 
+@pytest.mark.parametrize("batch,cols,rows", [(1, 48, 10), (1, 1 << 24, 10), (0, 64, 10), (3, 0, 10), (3, -64, 10),
+                                             (3, 64, 0)])
+def test_no_launch_shape_of_refused_products(batch, cols, rows):
+    import l2c
+    with pytest.raises(l2c.L2CError):
+        l2c.launch_shape(l2c.OP_MATMUL_MXFP4, batch, cols, rows)
+
+
 def test_products_of_nothing():
     assert quantize(rows=0, x=None) == 0
     assert product(batch=0, out=None) == 0 and product(rows=0, out=None) == 0
@@ -109,7 +117,7 @@ def reorder(out=P, inp=1 << 40, parents=P, beams=4, batch=2, groups=1, pieces=1,
     dict(out=P, inp=P + 256), dict(out=P + 2047, inp=P),            # the two overlap
     dict(row_stride=1 << 62, batch=1 << 20),                        # past 63 bits
     dict(piece_bytes=1 << 36, row_stride=1 << 36),                  # more than 2^31 - 1 units a row
-    dict(batch=1 << 20, groups=1 << 10, group_stride=1 << 40),      # more workgroups than one launch has
+    dict(batch=1 << 26, piece_bytes=4096, row_stride=4096, inp=1 << 50),  # more workgroups than one launch has
 ], ids=str)
 def test_beam_reorder_refuses(bad):
     assert reorder(**bad) == INVALID
@@ -130,6 +138,10 @@ def test_wrappers_check_types_and_devices():
         l2c.residual_rmsnorm(f, h, f, f, f, 64, 4)  # residual_out of another type than residual
     with pytest.raises(ValueError):
         l2c.residual_rmsnorm(f, f, f.double(), f, f, 64, 4)
+    for bad in (f.half(), f.int(), torch.zeros(4, 64, dtype=torch.uint8)):
+        for args in ((bad, f, f, f), (f, bad, bad, f), (f, f, f, bad)):
+            with pytest.raises(ValueError, match="fp32 and bf16"):
+                l2c.residual_rmsnorm(*args, f, 64, 4)
     with pytest.raises(ValueError):
         l2c.residual_rmsnorm(f, None, f, f, f, 64, 4)  # not on the GPU
     with pytest.raises(ValueError):

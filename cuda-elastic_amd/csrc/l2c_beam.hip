@@ -122,6 +122,15 @@ __device__ __forceinline__ float wave_top(float v) {
   v = fmaxf(v, other<kRowBefore>(v, v));
   return fmaxf(v, other<kHalfBefore>(v, v));
 }
+__device__ __forceinline__ unsigned wave_top(unsigned v) {  // in every lane
+  v = max(v, static_cast<unsigned>(other<kBefore1>(static_cast<int>(v))));
+  v = max(v, static_cast<unsigned>(other<kBefore2>(static_cast<int>(v))));
+  v = max(v, static_cast<unsigned>(other<kBefore4>(static_cast<int>(v))));
+  v = max(v, static_cast<unsigned>(other<kBefore8>(static_cast<int>(v))));
+  v = max(v, static_cast<unsigned>(other<kRowBefore>(static_cast<int>(v))));
+  v = max(v, static_cast<unsigned>(other<kHalfBefore>(static_cast<int>(v))));
+  return __builtin_amdgcn_readlane(v, L2C_WAVE - 1);
+}
 // Every lane has its 16 lanes' maximum, or sum.
 __device__ __forceinline__ float row_max(float v) {
   v = fmaxf(v, other<kRotate8>(v, v));
@@ -142,10 +151,7 @@ __device__ __forceinline__ double row_sum(double v) {
 // each other, but are scalar instructions for the most part, which other waves leave idle
 // (starting at the first bit in which the values differ, or two bits a step, measured 20%
 // slower for 256 x 4 x 32003).
-template <typename T>
-__device__ __forceinline__ int wave_reach(T v, T bound) {
-  return __popcll(__ballot(v >= bound));
-}
+__device__ __forceinline__ int wave_reach(unsigned v, unsigned bound) { return __popcll(__ballot(v >= bound)); }
 __device__ __forceinline__ unsigned wave_bound(unsigned v, int k) {
   unsigned bound = 0;
   for (int bit = 31; bit >= 0; --bit) {
@@ -156,13 +162,22 @@ __device__ __forceinline__ unsigned wave_bound(unsigned v, int k) {
   }
   return bound;
 }
-// Of 64-bit values two bits a step, whose ballots do not wait for each other: one wave's
-// time counts where nothing else runs.
-__device__ __forceinline__ u64 wave_bound(u64 v, int k) {
-  u64 bound = 0;
-  if (wave_reach(v, static_cast<u64>(1)) < k) return bound;
-  for (int bit = 62; bit >= 0; bit -= 2) {
-    const u64 one = bound | 1ULL << bit, two = bound | 2ULL << bit, three = one | two;
+// The same where one wave's time counts, because nothing else runs: a maximum at a time, and for
+// larger k two bits a step, whose ballots do not wait for each other.
+__device__ __forceinline__ unsigned lone_wave_bound(unsigned v, int k) {
+  if (wave_reach(v, 1) < k) return 0;
+  unsigned bound = 0;
+  if (k <= 8) {
+    for (int reached = 0; reached < k;) {
+      bound = wave_top(v);
+      const u64 lanes = __ballot(v == bound);
+      reached += __popcll(lanes);
+      v = v == bound ? 0u : v;
+    }
+    return bound;
+  }
+  for (int bit = 30; bit >= 0; bit -= 2) {
+    const unsigned one = bound | 1u << bit, two = bound | 2u << bit, three = one | two;
     const int reach1 = wave_reach(v, one), reach2 = wave_reach(v, two), reach3 = wave_reach(v, three);
     bound = reach3 >= k ? three : reach2 >= k ? two : reach1 >= k ? one : bound;
     if (reach3 == k || reach2 == k || reach1 == k) break;
@@ -170,23 +185,56 @@ __device__ __forceinline__ u64 wave_bound(u64 v, int k) {
   return bound;
 }
 
-// How many of n values are larger, and how many equal. Reads in eights, up to seven past
-// the end: one after the other they would wait for LDS each time.
+// How many of n values (16-byte aligned) are larger, and how many equal. Reads in eights, up to
+// seven past the end: one after the other they would wait for LDS each time.
 struct Order {
   int larger, equal;
 };
-__device__ __forceinline__ Order order(const u64 *values, int n, u64 than) {
+__device__ __forceinline__ Order order(const unsigned *values, int n, unsigned than) {
   Order count = {0, 0};
-  for (int o = 0; o < n; o += 8) {
-    u64 v[8];
-#pragma unroll
-    for (int u = 0; u < 8; ++u) v[u] = values[o + u];
+  auto eight = [&](int o, int inside) __attribute__((always_inline)) {
+    const uint4 a = *reinterpret_cast<const uint4 *>(values + o), b = *reinterpret_cast<const uint4 *>(values + o + 4);
+    const unsigned v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
-      count.larger += o + u < n && v[u] > than;
-      count.equal += o + u < n && v[u] == than;
+      count.larger += u < inside && v[u] > than;
+      count.equal += u < inside && v[u] == than;
+    }
+  };
+  int o = 0;
+  for (; o + 8 <= n; o += 8) eight(o, 8);
+  if (o < n) eight(o, n - o);
+  return count;
+}
+// The same for the values from `first` on themselves, 64 for the workgroup's four waves: lane l of
+// wave l / 16 gets those of value first + l. The lanes hold the values that a wave's
+// sixteen are compared with, one ballot for 64 comparisons: the chain of a lane that goes
+// through them by itself is four to five times as long.
+__device__ __forceinline__ Order order_of_64(const unsigned *values, int n, int first) {
+  constexpr int kEach = L2C_WAVE / kWaves;
+  const int lane = threadIdx.x % L2C_WAVE;
+  const int from = kEach * __builtin_amdgcn_readfirstlane(threadIdx.x / L2C_WAVE);
+  Order count = {0, 0};
+  if (first + from >= n) return count;
+  const unsigned mine = first + lane < n ? values[first + lane] : 0u;
+  for (int o = 0; o < n; o += L2C_WAVE) {
+    const unsigned v = o == first ? mine : o + lane < n ? values[o + lane] : 0u;
+#pragma unroll
+    for (int u = 0; u < kEach; ++u) {
+      const unsigned than = __builtin_amdgcn_readlane(mine, from + u);
+      const int larger = __popcll(__ballot(v > than)), equal = __popcll(__ballot(v == than));
+      count.larger += lane == from + u ? larger : 0;
+      count.equal += lane == from + u ? equal : 0;
     }
   }
+  return count;
+}
+// How many of n entries have the key and come before `before` (a larger number).
+__device__ __forceinline__ int earlier(const unsigned *keys, const unsigned *befores, int n, unsigned key,
+                                       unsigned before) {
+  int count = 0;
+#pragma unroll 8
+  for (int o = 0; o < n; ++o) count += static_cast<int>(keys[o] == key) & static_cast<int>(befores[o] > before);
   return count;
 }
 
@@ -198,8 +246,13 @@ __global__ __launch_bounds__(kThreads) void beam_chunks_kernel(unsigned char *__
                                                                const int *__restrict__ tokens, int eos, int vocab,
                                                                int beams, int chunks, int parts) {
   constexpr int kPart = kThreads * 4 * V;
-  extern __shared__ u64 list[];  // `beams` lanes' values of each wave at most, and eight that order() may read
-  __shared__ u64 kept[2][kMaxBeams + 8];  // the largest so far, in order
+  // Keys and UINT_MAX - place of the list: `beams` lanes' values of each wave at most, and what
+  // order() may read.
+  extern __shared__ uint4 lists[];
+  unsigned *const list_key = reinterpret_cast<unsigned *>(lists);
+  unsigned *const list_before = list_key + kWaves * 4 * V * beams + 8;
+  __shared__ __attribute__((aligned(16))) unsigned kept_key[2][kMaxBeams + 8];  // the largest so far, in order
+  __shared__ unsigned kept_before[2][kMaxBeams + 8];
   __shared__ unsigned bounds[kWaves];
   __shared__ float tops[kWaves];
   __shared__ double sums[kWaves];
@@ -259,7 +312,7 @@ __global__ __launch_bounds__(kThreads) void beam_chunks_kernel(unsigned char *__
     unsigned least = bounds[0];
 #pragma unroll
     for (int w = 1; w < kWaves; ++w) least = min(least, bounds[w]);
-    if (MANY && count == beams) least = max(least, static_cast<unsigned>(kept[turn][beams - 1] >> 32));
+    if (MANY && count == beams) least = max(least, kept_key[turn][beams - 1]);
     least = max(least, 1u);
     float maximum = shift;
 #pragma unroll
@@ -308,15 +361,28 @@ __global__ __launch_bounds__(kThreads) void beam_chunks_kernel(unsigned char *__
         if (__ballot(reach >> 4 * c & 15u) == 0) continue;
 #pragma unroll
         for (int i = 4 * c; i < 4 * c + 4; ++i)
-          if (reach >> i & 1) list[to++] = ordered(key_of(v[i]), static_cast<unsigned>(start) + place(i));
+          if (reach >> i & 1) {
+            list_key[to] = key_of(v[i]);
+            list_before[to++] = UINT_MAX - (static_cast<unsigned>(start) + place(i));
+          }
       }
     }
     __syncthreads();
-    const int m = length, all = count + m;
+    const int m = __builtin_amdgcn_readfirstlane(length), all = count + m;
     for (int e = t; e < all; e += kThreads) {
-      const u64 mine = MANY && e < count ? kept[turn][e] : list[e - count];
-      const int rank = (MANY ? order(kept[turn], count, mine).larger : 0) + order(list, m, mine).larger;
-      if (rank < beams) kept[turn ^ 1][rank] = mine;
+      const bool old = MANY && e < count;
+      const unsigned mine = old ? kept_key[turn][e] : list_key[e - count];
+      const unsigned before = old ? kept_before[turn][e] : list_before[e - count];
+      Order among = order(list_key, m, mine);
+      if (MANY) {
+        const Order among_kept = order(kept_key[turn], count, mine);
+        among.larger += among_kept.larger, among.equal += among_kept.equal;
+      }
+      if (among.equal > 1) {  // it and others
+        among.larger += earlier(list_key, list_before, m, mine, before);
+        if (MANY) among.larger += earlier(kept_key[turn], kept_before[turn], count, mine, before);
+      }
+      if (among.larger < beams) kept_key[turn ^ 1][among.larger] = mine, kept_before[turn ^ 1][among.larger] = before;
     }
     count = min(all, beams);
     turn ^= 1;
@@ -330,9 +396,7 @@ __global__ __launch_bounds__(kThreads) void beam_chunks_kernel(unsigned char *__
     const int request = row / beams;
     const size_t place = (static_cast<size_t>(request) * beams + t) * beams + (row - request * beams);
     Candidate *const out = reinterpret_cast<Candidate *>(stats + gridDim.x) + place * chunks + chunk;
-    const u64 mine = t < count ? kept[turn][t] : 0;
-    *out = t < count ? Candidate{number_of(static_cast<unsigned>(mine >> 32)),
-                                 first + static_cast<int>(UINT_MAX - static_cast<unsigned>(mine))}
+    *out = t < count ? Candidate{number_of(kept_key[turn][t]), first + static_cast<int>(UINT_MAX - kept_before[turn][t])}
                      : Candidate{-INFINITY, -1};
   }
   total = wave_scan(total);
@@ -364,16 +428,19 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(float *scores_out, 
                                                              int *generated, const unsigned char *workspace,
                                                              const float *scores, const int *tokens, int eos,
                                                              int beams, int chunks, int steps, int step) {
-  constexpr int kEntries = (DIRECT || HELD * kThreads > kChosenCandidates ? HELD * kThreads : kChosenCandidates) + 8;
+  constexpr int kEntries = DIRECT || HELD * kThreads > kChosenCandidates ? HELD * kThreads : kChosenCandidates;
   // A beam's scores are base + (logit - top), in this order: logits of the lowest value
   // would take the rest of the sum with them. NaN: no candidates.
   __shared__ double base[kMaxBeams];
   __shared__ float tops[kMaxBeams];
   __shared__ bool ended[kMaxBeams];
-  __shared__ u64 list_key[kEntries], list_logit[kEntries];
+  __shared__ __attribute__((aligned(16))) unsigned list_high[kEntries];  // of the keys
+  __shared__ unsigned list_low[kEntries];
+  __shared__ u64 list_logit[kEntries];
   __shared__ int list_at[kEntries];
   __shared__ int chosen[kMaxBeams];
-  __shared__ u64 slots[kWaves], last_first;
+  __shared__ unsigned slots[kWaves];
+  __shared__ u64 last_first;
   __shared__ int lengths[2];
   constexpr int kGroup = 16;  // lanes a beam for its chunks' sums
   const int t = threadIdx.x, lane = t % L2C_WAVE, wave = t / L2C_WAVE;
@@ -392,28 +459,47 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(float *scores_out, 
 #pragma unroll
   for (int r = 0; r < HELD; ++r) held[r] = all[min(t + r * kThreads, entries - 1)];  // together, without a branch
   if (t < 2) lengths[t] = 0;
-  for (int k = t / kGroup; k < beams; k += kThreads / kGroup) {  // whole groups stay together
-    const int member = t % kGroup;
-    // Of an ended row the workspace holds nothing; what is read there is not used.
-    ChunkStat s = {0.0, -INFINITY, 0};
-    if (member < chunks) s = *stat(k, member);
-    const float score = scores[first + k];
-    const bool end = eos >= 0 && tokens[first + k] == eos;
-    float m = s.maximum;
-    for (int c = member + kGroup; c < chunks; c += kGroup) m = fmaxf(m, stat(k, c)->maximum);
+  // The sums of beams t / 16 and, of more than 16, t / 16 + 16. What most rows have is loaded together.
+  // Of an ended row the workspace holds nothing; what is read there is not used.
+  constexpr int kBeams = kThreads / kGroup, kRounds = kMaxBeams / kBeams, kStats = 2;
+  const int member = t % kGroup, row = t / kGroup;
+  ChunkStat held_stat[kRounds][kStats];
+  float score[kRounds];
+  int token[kRounds];
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) {
+    if (r * kBeams >= beams) break;
+    const int k = min(row + r * kBeams, beams - 1);
+#pragma unroll
+    for (int u = 0; u < kStats; ++u) held_stat[r][u] = *stat(k, min(member + u * kGroup, chunks - 1));
+    score[r] = scores[first + k];
+    token[r] = tokens[first + k];
+  }
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) {
+    if (r * kBeams >= beams) break;
+    const int k = min(row + r * kBeams, beams - 1);
+    const bool end = eos >= 0 && token[r] == eos;
+    float m = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < kStats; ++u) m = fmaxf(m, held_stat[r][u].maximum);
+    for (int c = member + kStats * kGroup; c < chunks; c += kGroup) m = fmaxf(m, stat(k, c)->maximum);
     m = row_max(m);
     double sum = 0.0;
-    for (int c = member; c < chunks; c += kGroup) {
-      if (c != member) s = *stat(k, c);
+    auto add = [&](const ChunkStat &s) __attribute__((always_inline)) {
       // A chunk of -Inf has sum 0; NaN stays NaN.
       sum += s.maximum == m ? s.sum
              : s.maximum == -INFINITY ? s.sum * 0.0
                                       : s.sum * exp(static_cast<double>(s.maximum) - static_cast<double>(m));
-    }
+    };
+#pragma unroll
+    for (int u = 0; u < kStats; ++u)
+      if (member + u * kGroup < chunks) add(held_stat[r][u]);
+    for (int c = member + kStats * kGroup; c < chunks; c += kGroup) add(*stat(k, c));
     sum = row_sum(sum);
     if (member == 0) {
       // Of a row of -Inf the sum is 0 and b +Inf, of one with NaN or +Inf it is NaN.
-      const double b = end ? static_cast<double>(score) : static_cast<double>(score) - log(sum);
+      const double b = end ? static_cast<double>(score[r]) : static_cast<double>(score[r]) - log(sum);
       base[k] = b >= -DBL_MAX && b <= DBL_MAX ? b : __longlong_as_double(0x7ff8000000000000LL);
       tops[k] = m;
       ended[k] = end;
@@ -432,25 +518,37 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(float *scores_out, 
   // the lower `at`.
   auto enter = [&](int to, u64 key, int list, Candidate c, int at) __attribute__((always_inline)) {
     const int beam = by_chunks(list);
-    list_key[to] = key;
+    list_high[to] = static_cast<unsigned>(key >> 32), list_low[to] = static_cast<unsigned>(key);
     list_logit[to] = static_cast<u64>(beam) << 32 | (ended[beam] ? 0u : UINT_MAX - key_of(c.logit));
     list_at[to] = at;
   };
   auto token_of = [&](int list, Candidate c) __attribute__((always_inline)) {
     return ended[by_chunks(list)] ? eos : c.token;
   };
-  auto rank_of = [&](int e, int m) __attribute__((always_inline)) {
-    const u64 key = list_key[e], logit = list_logit[e];
-    const int at = list_at[e];
-    const Order among = order(list_key, m, key);
-    int rank = among.larger;
-    if (among.equal > 1)
-      for (int o = 0; o < m; ++o)
-        rank += list_key[o] == key && (list_logit[o] < logit || (list_logit[o] == logit && list_at[o] < at));
-    return rank;
+  auto entry_key = [&](int e) __attribute__((always_inline)) { return static_cast<u64>(list_high[e]) << 32 | list_low[e]; };
+  // act(e, rank) for every entry.
+  auto rank = [&](int m, auto act) __attribute__((always_inline)) {
+    for (int first = 0; first < m; first += L2C_WAVE) {
+      const Order among = order_of_64(list_high, m, first);
+      const int e = first + lane;
+      if (lane / (L2C_WAVE / kWaves) != wave || e >= m) continue;
+      int at = among.larger;
+      if (among.equal > 1) {  // it and others
+        const unsigned high = list_high[e], low = list_low[e];
+        const u64 logit = list_logit[e];
+        const int last = list_at[e];
+#pragma unroll 4
+        for (int o = 0; o < m; ++o) {
+          const bool same = list_low[o] == low, tie = list_logit[o] == logit;
+          at += (list_high[o] == high) & ((list_low[o] > low) | (same & (list_logit[o] < logit)) |
+                                          (same & tie & (list_at[o] < last)));
+        }
+      }
+      act(e, at);
+    }
   };
 
-  // A bound that at least `beams` entries reach, from the lanes' best; equal keys all pass.
+  // A bound that at least `beams` entries reach, from the upper halves of the lanes' best keys.
   u64 best = 0, held_key[HELD];
 #pragma unroll
   for (int r = 0; r < HELD; ++r) {
@@ -459,13 +557,15 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(float *scores_out, 
     held_key[r] = i < entries ? key_at(list, rank, held[r]) : 0ULL;
     best = max(best, held_key[r]);
   }
-  const u64 bound = wave_bound(best, beams);
+  // Of all four waves, if they have entries, a quarter each; else of the one that has the most.
+  const bool quarters = beams > 8 && entries >= kThreads;
+  const unsigned bound = lone_wave_bound(static_cast<unsigned>(best >> 32), quarters ? (beams + 3) / 4 : beams);
   if (lane == 0) slots[wave] = bound;
   __syncthreads();
-  u64 least = slots[0];
+  unsigned most = slots[0];
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w) least = max(least, slots[w]);
-  least = max(least, static_cast<u64>(1));
+  for (int w = 1; w < kWaves; ++w) most = quarters ? min(most, slots[w]) : max(most, slots[w]);
+  u64 least = static_cast<u64>(max(most, 1u)) << 32;  // a candidate's key is larger
   unsigned reach = 0;
 #pragma unroll
   for (int r = 0; r < HELD; ++r) reach |= held_key[r] >= least ? 1u << r : 0u;
@@ -483,35 +583,34 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(float *scores_out, 
     }
   }
   __syncthreads();
-  int m = lengths[0];
+  int m = __builtin_amdgcn_readfirstlane(lengths[0]);
   if (!DIRECT) {
-    for (int e = t; e < m; e += kThreads) {
-      const int rank = rank_of(e, m);
-      if (rank < beams) chosen[rank] = list_at[e];
-      if (rank == beams - 1) last_first = list_key[e];
-    }
+    rank(m, [&](int e, int at) __attribute__((always_inline)) {
+      if (at < beams) chosen[at] = list_at[e];
+      if (at == beams - 1) last_first = entry_key(e);
+    });
     if (m < beams && t == 0) last_first = 1;
     __syncthreads();
     constexpr int kEach = kMaxBeams * kMaxBeams / kThreads;
     const int count = min(m, beams);
     least = last_first;
     Candidate c[kEach];
-    int list[kEach], rank[kEach];
+    int list[kEach], place[kEach];
 #pragma unroll
     for (int u = 0; u < kEach; ++u) {
-      const int i = t + u * kThreads, place = by_beams(i);
-      rank[u] = i - place * beams;
-      list[u] = place < count && place + rank[u] < beams ? chosen[place] : -1;
-      c[u] = all[list[u] >= 0 ? rank[u] * lists + list[u] : 0];
+      const int i = t + u * kThreads, which = by_beams(i);
+      place[u] = i - which * beams;
+      list[u] = which < count && which + place[u] < beams ? chosen[which] : -1;
+      c[u] = all[list[u] >= 0 ? place[u] * lists + list[u] : 0];
     }
 #pragma unroll
     for (int u = 0; u < kEach; ++u) {
       if (list[u] < 0) continue;
-      const u64 key = key_at(list[u], rank[u], c[u]);
+      const u64 key = key_at(list[u], place[u], c[u]);
       if (key >= least) enter(atomicAdd(&lengths[1], 1), key, list[u], c[u], token_of(list[u], c[u]));
     }
     __syncthreads();
-    m = lengths[1];
+    m = __builtin_amdgcn_readfirstlane(lengths[1]);
   }
   auto write = [&](int rank, u64 key, int parent, int token) __attribute__((always_inline)) {
     const int to = first + rank;
@@ -520,10 +619,9 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(float *scores_out, 
     parents[to] = parent;
     if (generated) generated[static_cast<size_t>(to) * steps + step] = token;
   };
-  for (int e = t; e < m; e += kThreads) {
-    const int rank = rank_of(e, m);
-    if (rank < beams) write(rank, list_key[e], static_cast<int>(list_logit[e] >> 32), list_at[e]);
-  }
+  rank(m, [&](int e, int at) __attribute__((always_inline)) {
+    if (at < beams) write(at, entry_key(e), static_cast<int>(list_logit[e] >> 32), list_at[e]);
+  });
   for (int e = m + t; e < beams; e += kThreads) write(e, 0, -1, -1);
 }
 
@@ -583,7 +681,7 @@ extern "C" int l2c_decoder_beam_select(float *scores_out, int *tokens_out, int *
   if (static_cast<long long>(batch) * beams > INT_MAX || grid > INT_MAX || !l2c::launchable(grid, kThreads))
     return hipErrorInvalidValue;
   unsigned char *w = static_cast<unsigned char *>(workspace);
-  const size_t list = sizeof(u64) * (kWaves * static_cast<size_t>(beams) * c.values + 8);
+  const size_t list = 2 * sizeof(unsigned) * (kWaves * static_cast<size_t>(beams) * c.values + 8);
   hipLaunchKernelGGL(c.fn, dim3(static_cast<unsigned>(grid)), dim3(kThreads), list, stream, w, logits, tokens, eos,
                      vocab, beams, c.chunks, c.parts);
   L2C_LAUNCH_CHECK();

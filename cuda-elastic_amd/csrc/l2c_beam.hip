@@ -396,8 +396,8 @@ __global__ __launch_bounds__(kThreads) void beam_chunks_kernel(unsigned char *__
     const int request = row / beams;
     const size_t place = (static_cast<size_t>(request) * beams + t) * beams + (row - request * beams);
     Candidate *const out = reinterpret_cast<Candidate *>(stats + gridDim.x) + place * chunks + chunk;
-    *out = t < count ? Candidate{number_of(kept_key[turn][t]), first + static_cast<int>(UINT_MAX - kept_before[turn][t])}
-                     : Candidate{-INFINITY, -1};
+    *out = {-INFINITY, -1};
+    if (t < count) *out = {number_of(kept_key[turn][t]), first + static_cast<int>(UINT_MAX - kept_before[turn][t])};
   }
   total = wave_scan(total);
   if (lane == L2C_WAVE - 1) sums[wave] = total;
@@ -525,7 +525,9 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(float *scores_out, 
   auto token_of = [&](int list, Candidate c) __attribute__((always_inline)) {
     return ended[by_chunks(list)] ? eos : c.token;
   };
-  auto entry_key = [&](int e) __attribute__((always_inline)) { return static_cast<u64>(list_high[e]) << 32 | list_low[e]; };
+  auto entry_key = [&](int e) __attribute__((always_inline)) {
+    return static_cast<u64>(list_high[e]) << 32 | list_low[e];
+  };
   // act(e, rank) for every entry.
   auto rank = [&](int m, auto act) __attribute__((always_inline)) {
     for (int first = 0; first < m; first += L2C_WAVE) {
@@ -596,19 +598,35 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(float *scores_out, 
     least = last_first;
     Candidate c[kEach];
     int list[kEach], place[kEach];
+    // Neighbours in a list go to different waves: each has its share of the largest.
 #pragma unroll
     for (int u = 0; u < kEach; ++u) {
-      const int i = t + u * kThreads, which = by_beams(i);
+      const int i = lane * kWaves + wave + u * kThreads, which = by_beams(i);
       place[u] = i - which * beams;
       list[u] = which < count && which + place[u] < beams ? chosen[which] : -1;
       c[u] = all[list[u] >= 0 ? place[u] * lists + list[u] : 0];
     }
+    u64 key[kEach];
+    best = 0;
 #pragma unroll
     for (int u = 0; u < kEach; ++u) {
-      if (list[u] < 0) continue;
-      const u64 key = key_at(list[u], place[u], c[u]);
-      if (key >= least) enter(atomicAdd(&lengths[1], 1), key, list[u], c[u], token_of(list[u], c[u]));
+      key[u] = list[u] >= 0 ? key_at(list[u], place[u], c[u]) : 0ULL;
+      best = max(best, key[u]);
     }
+    if (beams > 8) {
+      // Where the lists are hardly more than the beams, the last list's first is a poor bound.
+      const unsigned quarter = lone_wave_bound(static_cast<unsigned>(best >> 32), (beams + 3) / 4);
+      if (lane == 0) slots[wave] = quarter;
+      __syncthreads();
+      most = slots[0];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) most = min(most, slots[w]);
+      least = max(least, static_cast<u64>(most) << 32);
+    }
+#pragma unroll
+    for (int u = 0; u < kEach; ++u)
+      if (list[u] >= 0 && key[u] >= least)
+        enter(atomicAdd(&lengths[1], 1), key[u], list[u], c[u], token_of(list[u], c[u]));
     __syncthreads();
     m = __builtin_amdgcn_readfirstlane(lengths[1]);
   }

@@ -74,11 +74,6 @@ __device__ __forceinline__ float exp_nonpositive(float t) {
   return fmaf(e, low * kLn2, e);
 }
 
-// 64-bit order of a chunk's values: the logit, then the lower place first.
-__device__ __forceinline__ u64 ordered(unsigned key, unsigned place) {
-  return (static_cast<u64>(key) << 32) | (UINT_MAX - place);
-}
-
 // Values of other lanes through the adders' operand paths (DPP), which take a tenth of a
 // trip through LDS: from 1, 2, 4 or 8 lanes before in rows of 16, from the row before's
 // last lane, from the lower half's last lane; or rotated in rows of 16.
@@ -206,22 +201,25 @@ __device__ __forceinline__ Order order(const unsigned *values, int n, unsigned t
   if (o < n) eight(o, n - o);
   return count;
 }
-// The same for the values from `first` on themselves, 64 for the workgroup's four waves: lane l of
-// wave l / 16 gets those of value first + l. The lanes hold the values that a wave's
-// sixteen are compared with, one ballot for 64 comparisons: the chain of a lane that goes
-// through them by itself is four to five times as long.
-__device__ __forceinline__ Order order_of_64(const unsigned *values, int n, int first) {
+// The same for the 64-bit values from `first` on themselves, 64 for the workgroup's four waves:
+// lane l of wave l / 16 gets those of value first + l. The lanes hold the values that a
+// wave's sixteen are compared with, one ballot for 64 comparisons: the chain of a lane that
+// goes through them by itself is four to five times as long. (Where many workgroups share the
+// CUs, as the chunks' do, it costs more than it saves.)
+__device__ __forceinline__ Order order_of_64(const u64 *values, int n, int first) {
   constexpr int kEach = L2C_WAVE / kWaves;
   const int lane = threadIdx.x % L2C_WAVE;
   const int from = kEach * __builtin_amdgcn_readfirstlane(threadIdx.x / L2C_WAVE);
   Order count = {0, 0};
   if (first + from >= n) return count;
-  const unsigned mine = first + lane < n ? values[first + lane] : 0u;
+  const u64 mine = first + lane < n ? values[first + lane] : 0ULL;
   for (int o = 0; o < n; o += L2C_WAVE) {
-    const unsigned v = o == first ? mine : o + lane < n ? values[o + lane] : 0u;
+    const u64 v = o == first ? mine : o + lane < n ? values[o + lane] : 0ULL;
 #pragma unroll
     for (int u = 0; u < kEach; ++u) {
-      const unsigned than = __builtin_amdgcn_readlane(mine, from + u);
+      const unsigned low = __builtin_amdgcn_readlane(static_cast<unsigned>(mine), from + u);
+      const unsigned high = __builtin_amdgcn_readlane(static_cast<unsigned>(mine >> 32), from + u);
+      const u64 than = static_cast<u64>(high) << 32 | low;
       const int larger = __popcll(__ballot(v > than)), equal = __popcll(__ballot(v == than));
       count.larger += lane == from + u ? larger : 0;
       count.equal += lane == from + u ? equal : 0;
@@ -279,7 +277,6 @@ __global__ __launch_bounds__(kThreads) void beam_chunks_kernel(unsigned char *__
   float shift = -INFINITY;     // the largest so far
   int count = 0;               // of `kept`
   int turn = 0;
-  const int quarter = (beams + kWaves - 1) / kWaves;
   for (int start = 0;;) {
     const int n = min(kPart, whole - start);
     const bool more = MANY && whole - start > kPart;
@@ -303,7 +300,9 @@ __global__ __launch_bounds__(kThreads) void beam_chunks_kernel(unsigned char *__
     for (int i = 0; i < 4 * V; ++i) top = fmaxf(top, v[i]);
     const unsigned best = place(0) < n ? key_of(top) : 0u;
     const float largest = wave_top(top);  // of the last lane
-    const unsigned bound = quarter == 1 ? key_of(largest) : wave_bound(best, quarter);
+    // Of the waves whose lanes all have values each has its share of the largest.
+    const int sharing = min(kWaves, max(1, n / (4 * L2C_WAVE))), share = (beams + sharing - 1) / sharing;
+    const unsigned bound = share == 1 ? key_of(largest) : wave_bound(best, share);
     if (lane == L2C_WAVE - 1) {
       bounds[wave] = bound;
       tops[wave] = largest;
@@ -311,7 +310,8 @@ __global__ __launch_bounds__(kThreads) void beam_chunks_kernel(unsigned char *__
     __syncthreads();
     unsigned least = bounds[0];
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) least = min(least, bounds[w]);
+    for (int w = 1; w < kWaves; ++w)
+      if (w < sharing) least = min(least, bounds[w]);
     if (MANY && count == beams) least = max(least, kept_key[turn][beams - 1]);
     least = max(least, 1u);
     float maximum = shift;
@@ -329,27 +329,30 @@ __global__ __launch_bounds__(kThreads) void beam_chunks_kernel(unsigned char *__
     // The values that reach the bound into the list, a wave's after each other's. If more than
     // `beams` of its lanes have such, only those of the `beams` lanes with the largest, and
     // of lanes that tie, with the lowest places of it: no other value can be among the chosen.
-    u64 own = 0;
+    unsigned last = 0;  // of lanes that tie: UINT_MAX - place of the last one's value
     if (wave_reach(best, least) > beams) {
-      const unsigned lanes_bound = wave_bound(best, beams);
-      const int larger = __popcll(__ballot(best > lanes_bound));
-      unsigned before = 0;  // UINT_MAX - place
-      if (best == lanes_bound) {
+      least = wave_bound(best, beams);
+      if (wave_reach(best, least) > beams) {
+        const int larger = __popcll(__ballot(best > least));
+        unsigned before = 0;
+        if (best == least) {
 #pragma unroll
-        for (int i = 4 * V - 1; i >= 0; --i)
-          if (key(i) == lanes_bound) before = UINT_MAX - (static_cast<unsigned>(start) + place(i));
+          for (int i = 4 * V - 1; i >= 0; --i)
+            if (key(i) == least) before = UINT_MAX - (static_cast<unsigned>(start) + place(i));
+        }
+        last = wave_bound(before, beams - larger);
       }
-      own = static_cast<u64>(lanes_bound) << 32 | wave_bound(before, beams - larger);
     }
     unsigned reach = 0;
-    if (own == 0 && least > key_of(-INFINITY)) {  // neither NaN nor what is past the end reaches it
+    if (last == 0 && least > key_of(-INFINITY)) {  // neither NaN nor what is past the end reaches it
       const float limit = number_of(least);
 #pragma unroll
       for (int i = 0; i < 4 * V; ++i) reach |= v[i] >= limit ? 1u << i : 0u;
     } else {
 #pragma unroll
       for (int i = 0; i < 4 * V; ++i)
-        if (key(i) >= least && ordered(key(i), static_cast<unsigned>(start) + place(i)) >= own) reach |= 1u << i;
+        if (key(i) > least || (key(i) == least && UINT_MAX - (static_cast<unsigned>(start) + place(i)) >= last))
+          reach |= 1u << i;
     }
     if (__ballot(reach != 0)) {
       const int count_here = __popc(reach), upto = wave_scan(count_here);
@@ -434,9 +437,7 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(float *scores_out, 
   __shared__ double base[kMaxBeams];
   __shared__ float tops[kMaxBeams];
   __shared__ bool ended[kMaxBeams];
-  __shared__ __attribute__((aligned(16))) unsigned list_high[kEntries];  // of the keys
-  __shared__ unsigned list_low[kEntries];
-  __shared__ u64 list_logit[kEntries];
+  __shared__ u64 list_key[kEntries], list_logit[kEntries];
   __shared__ int list_at[kEntries];
   __shared__ int chosen[kMaxBeams];
   __shared__ unsigned slots[kWaves];
@@ -464,22 +465,19 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(float *scores_out, 
   constexpr int kBeams = kThreads / kGroup, kRounds = kMaxBeams / kBeams, kStats = 2;
   const int member = t % kGroup, row = t / kGroup;
   ChunkStat held_stat[kRounds][kStats];
-  float score[kRounds];
-  int token[kRounds];
+  const float score = scores[first + min(t, beams - 1)];
+  const int token = tokens[first + min(t, beams - 1)];
 #pragma unroll
   for (int r = 0; r < kRounds; ++r) {
     if (r * kBeams >= beams) break;
     const int k = min(row + r * kBeams, beams - 1);
 #pragma unroll
     for (int u = 0; u < kStats; ++u) held_stat[r][u] = *stat(k, min(member + u * kGroup, chunks - 1));
-    score[r] = scores[first + k];
-    token[r] = tokens[first + k];
   }
 #pragma unroll
   for (int r = 0; r < kRounds; ++r) {
     if (r * kBeams >= beams) break;
     const int k = min(row + r * kBeams, beams - 1);
-    const bool end = eos >= 0 && token[r] == eos;
     float m = -INFINITY;
 #pragma unroll
     for (int u = 0; u < kStats; ++u) m = fmaxf(m, held_stat[r][u].maximum);
@@ -497,13 +495,15 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(float *scores_out, 
       if (member + u * kGroup < chunks) add(held_stat[r][u]);
     for (int c = member + kStats * kGroup; c < chunks; c += kGroup) add(*stat(k, c));
     sum = row_sum(sum);
-    if (member == 0) {
-      // Of a row of -Inf the sum is 0 and b +Inf, of one with NaN or +Inf it is NaN.
-      const double b = end ? static_cast<double>(score[r]) : static_cast<double>(score[r]) - log(sum);
-      base[k] = b >= -DBL_MAX && b <= DBL_MAX ? b : __longlong_as_double(0x7ff8000000000000LL);
-      tops[k] = m;
-      ended[k] = end;
-    }
+    if (member == 0) base[k] = sum, tops[k] = m;
+  }
+  __syncthreads();
+  if (t < beams) {
+    // Of a row of -Inf the sum is 0 and b +Inf, of one with NaN or +Inf it is NaN.
+    const bool end = eos >= 0 && token == eos;
+    const double b = end ? static_cast<double>(score) : static_cast<double>(score) - log(base[t]);
+    base[t] = b >= -DBL_MAX && b <= DBL_MAX ? b : __longlong_as_double(0x7ff8000000000000LL);
+    ended[t] = end;
   }
   __syncthreads();
   // The key of candidate `rank` of `list`, 0 where it is none.
@@ -518,33 +518,26 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(float *scores_out, 
   // the lower `at`.
   auto enter = [&](int to, u64 key, int list, Candidate c, int at) __attribute__((always_inline)) {
     const int beam = by_chunks(list);
-    list_high[to] = static_cast<unsigned>(key >> 32), list_low[to] = static_cast<unsigned>(key);
+    list_key[to] = key;
     list_logit[to] = static_cast<u64>(beam) << 32 | (ended[beam] ? 0u : UINT_MAX - key_of(c.logit));
     list_at[to] = at;
   };
   auto token_of = [&](int list, Candidate c) __attribute__((always_inline)) {
     return ended[by_chunks(list)] ? eos : c.token;
   };
-  auto entry_key = [&](int e) __attribute__((always_inline)) {
-    return static_cast<u64>(list_high[e]) << 32 | list_low[e];
-  };
   // act(e, rank) for every entry.
   auto rank = [&](int m, auto act) __attribute__((always_inline)) {
     for (int first = 0; first < m; first += L2C_WAVE) {
-      const Order among = order_of_64(list_high, m, first);
+      const Order among = order_of_64(list_key, m, first);
       const int e = first + lane;
       if (lane / (L2C_WAVE / kWaves) != wave || e >= m) continue;
       int at = among.larger;
       if (among.equal > 1) {  // it and others
-        const unsigned high = list_high[e], low = list_low[e];
-        const u64 logit = list_logit[e];
+        const u64 key = list_key[e], logit = list_logit[e];
         const int last = list_at[e];
 #pragma unroll 4
-        for (int o = 0; o < m; ++o) {
-          const bool same = list_low[o] == low, tie = list_logit[o] == logit;
-          at += (list_high[o] == high) & ((list_low[o] > low) | (same & (list_logit[o] < logit)) |
-                                          (same & tie & (list_at[o] < last)));
-        }
+        for (int o = 0; o < m; ++o)
+          at += (list_key[o] == key) & ((list_logit[o] < logit) | ((list_logit[o] == logit) & (list_at[o] < last)));
       }
       act(e, at);
     }
@@ -560,8 +553,10 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(float *scores_out, 
     best = max(best, held_key[r]);
   }
   // Of all four waves, if they have entries, a quarter each; else of the one that has the most.
-  const bool quarters = beams > 8 && entries >= kThreads;
-  const unsigned bound = lone_wave_bound(static_cast<unsigned>(best >> 32), quarters ? (beams + 3) / 4 : beams);
+  // So few that they are ranked together as quickly as some of them need no bound.
+  const bool few = entries <= L2C_WAVE, quarters = beams > 8 && entries >= kThreads;
+  const unsigned bound =
+      few ? 1u : lone_wave_bound(static_cast<unsigned>(best >> 32), quarters ? (beams + 3) / 4 : beams);
   if (lane == 0) slots[wave] = bound;
   __syncthreads();
   unsigned most = slots[0];
@@ -589,7 +584,7 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(float *scores_out, 
   if (!DIRECT) {
     rank(m, [&](int e, int at) __attribute__((always_inline)) {
       if (at < beams) chosen[at] = list_at[e];
-      if (at == beams - 1) last_first = entry_key(e);
+      if (at == beams - 1) last_first = list_key[e];
     });
     if (m < beams && t == 0) last_first = 1;
     __syncthreads();
@@ -601,6 +596,7 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(float *scores_out, 
     // Neighbours in a list go to different waves: each has its share of the largest.
 #pragma unroll
     for (int u = 0; u < kEach; ++u) {
+      if (u * kThreads >= beams * beams) break;
       const int i = lane * kWaves + wave + u * kThreads, which = by_beams(i);
       place[u] = i - which * beams;
       list[u] = which < count && which + place[u] < beams ? chosen[which] : -1;
@@ -610,6 +606,7 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(float *scores_out, 
     best = 0;
 #pragma unroll
     for (int u = 0; u < kEach; ++u) {
+      if (u * kThreads >= beams * beams) break;
       key[u] = list[u] >= 0 ? key_at(list[u], place[u], c[u]) : 0ULL;
       best = max(best, key[u]);
     }
@@ -624,9 +621,11 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(float *scores_out, 
       least = max(least, static_cast<u64>(most) << 32);
     }
 #pragma unroll
-    for (int u = 0; u < kEach; ++u)
+    for (int u = 0; u < kEach; ++u) {
+      if (u * kThreads >= beams * beams) break;
       if (list[u] >= 0 && key[u] >= least)
         enter(atomicAdd(&lengths[1], 1), key[u], list[u], c[u], token_of(list[u], c[u]));
+    }
     __syncthreads();
     m = __builtin_amdgcn_readfirstlane(lengths[1]);
   }
@@ -638,7 +637,7 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(float *scores_out, 
     if (generated) generated[static_cast<size_t>(to) * steps + step] = token;
   };
   rank(m, [&](int e, int at) __attribute__((always_inline)) {
-    if (at < beams) write(at, entry_key(e), static_cast<int>(list_logit[e] >> 32), list_at[e]);
+    if (at < beams) write(at, list_key[e], static_cast<int>(list_logit[e] >> 32), list_at[e]);
   });
   for (int e = m + t; e < beams; e += kThreads) write(e, 0, -1, -1);
 }

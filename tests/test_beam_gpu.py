@@ -131,6 +131,17 @@ def test_ties(torch_gpu, l2c):
         assert (pa == 0).all()
 
 
+@pytest.mark.parametrize("vocab", [40, 255, 256, 300, 511, 512, 513, 767, 769, 1500, 2560, 4575])
+@pytest.mark.parametrize("beams", [2, 5, 9, 27, 30])
+def test_rows_shorter_than_a_chunk(torch_gpu, l2c, vocab, beams):
+    """Waves with few values and with none, and as many lists as beams; logits as they are, and
+    rounded, so that many are equal."""
+    rng = np.random.default_rng(vocab * 40 + beams)
+    logits, scores, tokens = ordinary(rng, 3, beams, vocab, 0.1, 1)
+    check_select(torch_gpu, l2c, logits, scores, tokens, 1, beams)
+    check_select(torch_gpu, l2c, np.round(2 * logits) / 2, np.round(scores), tokens, 1, beams)
+
+
 @pytest.mark.parametrize("vocab", [300, 5000, 65540, 200001])
 @pytest.mark.parametrize("beams", [1, 4, 16, 32])
 def test_equal_scores_of_many_lists(torch_gpu, l2c, vocab, beams):

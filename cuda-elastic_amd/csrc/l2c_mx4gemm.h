@@ -19,7 +19,7 @@ struct Mx4Tile {
 };
 
 // l2c_mx4gemm_rows.hip, l2c_mx4gemm_slices.hip and l2c_mx4gemm_tiles.hip.
-constexpr int kMx4SliceTiles = 2, kMx4LdsTiles = 5;
+constexpr int kMx4SliceTiles = 3, kMx4LdsTiles = 5;
 extern const Mx4Tile mx4_row_tile, mx4_slice_tiles[kMx4SliceTiles], mx4_lds_tiles[kMx4LdsTiles];
 
 }  // namespace l2c

@@ -3,11 +3,12 @@
 // operands' layout and what happens past the end of K).
 //
 //  * v_mfma_scale_f32_32x32x64_f8f6f4 as in l2c_mx4gemm_tiles.hip. A workgroup computes
-//    32 MI x 32 NI outputs; each of its 8 waves multiplies the whole tile over an eighth
-//    of k, in steps of 256, a cache line of codes a row, and has a stage of LDS of its
-//    own, which LDS DMA fills. So nobody waits for another wave, every fragment is read from
-//    LDS once, and what is under way, (MI + NI) x 32 KB a CU, needs no registers. The
-//    waves' sums are added in wave order at the end.
+//    32 MI x 32 NI outputs; each of its waves multiplies the whole tile over its part of k,
+//    in steps of 256, a cache line of codes a row, and has a stage of LDS of its own,
+//    (MI + NI) x 4 KB, which LDS DMA fills. So nobody waits for another wave, every fragment
+//    is read from LDS once, and what is under way needs no registers. The waves' sums are
+//    added in wave order at the end. Eight waves for few tiles of long K, two for many of
+//    short K (1024 x 288 x 8012: 28 us with eight, 14 with two).
 //  * A wave waits for its stage, reads all of it to registers, asks for the next step
 //    and multiplies. The wait is long, but few steps are a wave's: with a barrier twice a
 //    step, as large tiles have it, a product of few tiles took 0.28 us a step for eight
@@ -31,8 +32,6 @@ typedef unsigned long long u64_any __attribute__((aligned(1)));
 typedef __attribute__((address_space(3))) void lds_ptr;
 
 constexpr int kE2M1 = 4;
-constexpr int kWaves = 8;
-constexpr int kThreads = kWaves * L2C_WAVE;
 constexpr int kRow = 128;  // code bytes of a row and step
 
 __device__ __forceinline__ i32x8 wide(u32x4 v) {
@@ -48,17 +47,19 @@ __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t rsrc, unsigned char
   __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr *)dst, 16, voffset, soffset, 0, 0);
 }
 
-template <int MI, int NI>
-__global__ __launch_bounds__(kThreads) void mxfp4_slice_kernel(float *__restrict__ out, const uint8_t *__restrict__ X,
-                                                               const uint8_t *__restrict__ Xs,
-                                                               const uint8_t *__restrict__ W,
-                                                               const uint8_t *__restrict__ Ws, int M, int N,
-                                                               int blocks) {
+template <int MI, int NI, int WAVES>
+__global__ __launch_bounds__(WAVES *L2C_WAVE) void mxfp4_slice_kernel(float *__restrict__ out,
+                                                                      const uint8_t *__restrict__ X,
+                                                                      const uint8_t *__restrict__ Xs,
+                                                                      const uint8_t *__restrict__ W,
+                                                                      const uint8_t *__restrict__ Ws, int M, int N,
+                                                                      int blocks) {
+  constexpr int kThreads = WAVES * L2C_WAVE;
   constexpr int kBM = 32 * MI, kBN = 32 * NI, kF = MI + NI;
   constexpr int kStage = 32 * kF * kRow;
   constexpr int kSum = 1024 * MI * NI;  // values of a tile
   static_assert(kSum * 4 <= kStage, "the waves' sums fit their stages");
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[kWaves * kStage];
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[WAVES * kStage];
   const int tile = l2c::xcd_tile(blockIdx.x, gridDim.x);
   const int mtiles = (M + kBM - 1) / kBM;
   const int m0 = tile % mtiles * kBM, n0 = tile / mtiles * kBN;
@@ -104,8 +105,8 @@ __global__ __launch_bounds__(kThreads) void mxfp4_slice_kernel(float *__restrict
     for (int j = 0; j < NI; ++j)
 #pragma unroll
       for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.0f;
-  const int end = static_cast<int>((wave + 1LL) * steps / kWaves);
-  int t = static_cast<int>(static_cast<long long>(wave) * steps / kWaves);
+  const int end = static_cast<int>((wave + 1LL) * steps / WAVES);
+  int t = static_cast<int>(static_cast<long long>(wave) * steps / WAVES);
   if (t < end) load(t);
   for (; t < end; ++t) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -157,17 +158,18 @@ __global__ __launch_bounds__(kThreads) void mxfp4_slice_kernel(float *__restrict
     const int e = threadIdx.x + k * kThreads, block = e / 1024, v = e / L2C_WAVE % 16;
     float sum = sums[e];
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) sum += sums[w * (kStage / 4) + e];
+    for (int w = 1; w < WAVES; ++w) sum += sums[w * (kStage / 4) + e];
     const int m = 32 * (block / NI) + 8 * (v / 4) + 4 * h + v % 4, n = 32 * (block % NI) + r;
     if (m < mrows && n < nrows) out[static_cast<size_t>(m0 + m) * N + n0 + n] = sum;
   }
 }
 
-template <int MI, int NI>
+template <int MI, int NI, int WAVES>
 constexpr l2c::Mx4Tile tile(double launch, double per_tile, double per_k) {
-  return {mxfp4_slice_kernel<MI, NI>, 32 * MI, 32 * NI, kThreads, 8, launch, per_tile, per_k};
+  return {mxfp4_slice_kernel<MI, NI, WAVES>, 32 * MI, 32 * NI, WAVES * L2C_WAVE, 8, launch, per_tile, per_k};
 }
 
 }  // namespace
 
-const l2c::Mx4Tile l2c::mx4_slice_tiles[kMx4SliceTiles] = {tile<1, 1>(1884, 595, 0.465), tile<1, 2>(1049, 1747, 0.867)};
+const l2c::Mx4Tile l2c::mx4_slice_tiles[kMx4SliceTiles] = {
+    tile<1, 1, 2>(2401, 142, 0.484), tile<1, 1, 8>(1884, 595, 0.465), tile<1, 2, 8>(1049, 1747, 0.867)};

@@ -136,9 +136,10 @@ def test_product_shapes(torch_gpu, l2c, batch, cols, rows):
 # Every kernel: lanes, batch rows and weight rows of its tile, and shapes that run on it, with
 # ragged edges, one step to many, odd and even steps and a part of one at the end.
 KERNELS = [((256, 16, 16), [(7, 544, 1003), (1, 11008, 500), (16, 4128, 900), (100, 192, 1009), (33, 4128, 1003)]),
+           ((128, 32, 32), [(332, 288, 8012), (1000, 320, 2157), (17, 288, 30001), (200, 544, 3800), (50, 256, 9000)]),
            ((512, 32, 32), [(33, 288, 4001), (61, 1056, 3005), (128, 2080, 1003), (250, 14016, 300), (5, 4096, 8190)]),
-           ((512, 32, 64), [(40, 5024, 8004), (100, 10016, 3003), (20, 736, 13001)]),
-           ((512, 64, 64), [(200, 544, 3800), (64, 4064, 11001), (1021, 2016, 1003), (63, 11008, 9003)]),
+           ((512, 32, 64), [(40, 5024, 8004), (100, 10016, 3003), (100, 1504, 3001)]),
+           ((512, 64, 64), [(200, 1312, 3801), (64, 4064, 11001), (1021, 2016, 1003), (63, 11008, 9003)]),
            ((512, 64, 128), [(120, 3904, 10003), (505, 1312, 3003), (1000, 16384, 2001)]),
            ((512, 128, 128), [(240, 4096, 10001), (513, 2080, 4003), (1010, 11008, 4001)]),
            ((512, 128, 192), [(500, 1120, 10801), (400, 4192, 11002), (384, 608, 10901)]),

@@ -269,30 +269,30 @@ def rmsnorm(out, inp, weight, size, batch, eps=RMS_EPSILON, stream=None):
         _check(code, "l2c_rmsnorm")
 
 
-_types = {}  # of torch's
+_types = {}  # enum l2c_type of torch's types, as they are met
 
 
 def _type(t):
     """The enum l2c_type of a tensor: fp32, or bf16, which two-byte integers may hold, too."""
-    kind = _types.get(t.dtype)
-    if kind is None:
-        known = {"torch.float32": F32, "torch.bfloat16": BF16, "torch.int16": BF16, "torch.uint16": BF16}
-        kind = known.get(str(t.dtype))
-        if kind is None:
-            raise ValueError(f"l2c.residual_rmsnorm takes fp32 and bf16 tensors, not {t.dtype}")
-        _types[t.dtype] = kind
-    return kind
+    known = {"torch.float32": F32, "torch.bfloat16": BF16, "torch.int16": BF16, "torch.uint16": BF16}
+    if str(t.dtype) not in known:
+        raise ValueError(f"l2c.residual_rmsnorm takes fp32 and bf16 tensors, not {t.dtype}")
+    return _types.setdefault(t.dtype, known[str(t.dtype)])
 
 
 def residual_rmsnorm(normalized, residual_out, residual, block, weight, size, batch, block_weight=None, gate=None,
                      rows_per_gate=1, residual_scale=1.0, eps=RMS_EPSILON, stream=None):
     """The types are the tensors'; residual_out, block_weight and gate may be None."""
-    kind = _type(residual)
-    if residual_out is not None and _type(residual_out) != kind:
+    try:
+        kinds = _types[normalized.dtype], _types[residual.dtype], _types[block.dtype]
+        out_kind = None if residual_out is None else _types[residual_out.dtype]
+    except KeyError:
+        kinds = _type(normalized), _type(residual), _type(block)
+        out_kind = None if residual_out is None else _type(residual_out)
+    if out_kind is not None and out_kind != kinds[1]:
         raise ValueError("residual_out has another type than residual")
-    code = _c_residual_rmsnorm(normalized, _type(normalized), residual_out, residual, kind, block, _type(block),
-                               block_weight, gate, rows_per_gate, weight, size, batch, float(residual_scale),
-                               float(eps), stream)
+    code = _c_residual_rmsnorm(normalized, kinds[0], residual_out, residual, kinds[1], block, kinds[2], block_weight,
+                               gate, rows_per_gate, weight, size, batch, residual_scale, eps, stream)
     if code:
         _check(code, "l2c_residual_rmsnorm")
 

@@ -659,9 +659,10 @@ ChunkConfig config(int vocab, int most_chunks) {
 }
 
 // 2048 logits a chunk as long as that makes at most 4096 chunks, and then 4096 logits: small
-// chunks have the least latency (1 x 4 x 32000: 8.1 us in chunks of 2048, 9.3 of 4096, 10.9
-// of 8192). Else 8192, which cost the least instructions a logit (256 x 4 x 32003: 42.6, 35.4,
-// 33.8).
+// chunks have the least latency (1 x 4 x 32000, chunks and join as they were then: 8.1 us in
+// chunks of 2048, 9.3 of 4096, 10.9 of 8192). Else 8192, which cost the least instructions a
+// logit (256 x 4 x 32003: 42.6, 35.4, 33.8, and 31.3 since). No more lists a request than the
+// join takes.
 ChunkConfig chunk_config(int vocab, int beams, int batch) {
   const int most = kJoinLists / beams;
   const double rows = static_cast<double>(batch) * beams;

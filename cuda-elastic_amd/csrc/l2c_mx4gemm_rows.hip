@@ -12,6 +12,7 @@
 //    256 contiguous bytes, two cache lines. The group's 16 scale bytes of a row are one
 //    load; lane q uses byte q of word i for MFMA i. The waves' sums are added in wave
 //    order through LDS.
+//  * Bound by memory's latency: 1 x 4096 x 4096 3.6 us, of which the launch is 2.
 #include "l2c_common.h"
 #include "l2c_mx4gemm.h"
 

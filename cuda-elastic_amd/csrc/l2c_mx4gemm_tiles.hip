@@ -25,6 +25,9 @@
 //  * Rows past the operands re-read the last row, steps past the end the last block, scales
 //    past the last whole step the ones before: every access is inside the operands.
 //    K >= 512.
+//  * 1024 x 16384 x 8192 takes 76 us, 3.6 PFLOP/s at 2.08 GHz, near the device's power limit.
+//    Of a step's 1550 cycles on 256 x 128 LDS is busy 1150, with DMA's writes and the
+//    fragments' reads, and the matrix cores 1024; on 128 x 128 770 and 512 of 1180.
 #include <type_traits>
 
 #include "l2c_common.h"

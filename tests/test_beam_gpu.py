@@ -482,3 +482,39 @@ def test_decoding_captured_and_replayed(torch_gpu, l2c):
         again = d.run(token)
         for got, want in zip(again, eager[token]):
             assert torch.equal(got, want)
+
+
+def test_decoders_on_two_streams(torch_gpu, l2c):
+    """Two decodes whose calls alternate on streams of their own, and two graphs of them replayed
+    at once: each gives what it gives alone."""
+    torch = torch_gpu
+    pair = [Decoder(torch, l2c, 3, 12, 128, 20000, 5, seed=2), Decoder(torch, l2c, 5, 4, 352, 9000, 5, seed=3)]
+    alone = [d.run(11) for d in pair]
+    streams = [torch.cuda.Stream() for _ in pair]
+    graphs = [torch.cuda.CUDAGraph() for _ in pair]
+    for d in pair:
+        d.start(11)
+    torch.cuda.synchronize()
+    for s in range(5):
+        for d, stream in zip(pair, streams):
+            with torch.cuda.stream(stream):
+                d.step(s)
+    torch.cuda.synchronize()
+    for d, want in zip(pair, alone):
+        for got, w in zip((d.scores, d.tokens, d.generated, d.state), want):
+            assert torch.equal(got, w)
+    for d, graph, stream in zip(pair, graphs, streams):
+        with torch.cuda.graph(graph, stream=stream):
+            for s in range(5):
+                d.step(s)
+    for _ in range(3):
+        for d in pair:
+            d.start(11)
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for d, want in zip(pair, alone):
+            for got, w in zip((d.scores, d.tokens, d.generated, d.state), want):
+                assert torch.equal(got, w)

@@ -658,17 +658,18 @@ ChunkConfig config(int vocab, int most_chunks) {
           (parts - 1) / each + 1, each};
 }
 
-// 2048 logits a chunk as long as that makes at most 4096 chunks, and then 4096 logits: small
+// 2048 logits a chunk as long as that makes at most 2048 chunks, and then 4096 logits: small
 // chunks have the least latency (1 x 4 x 32000, chunks and join as they were then: 8.1 us in
 // chunks of 2048, 9.3 of 4096, 10.9 of 8192). Else 8192, which cost the least instructions a
-// logit (256 x 4 x 32003: 42.6, 35.4, 33.8, and 31.3 since). No more lists a request than the
-// join takes.
+// logit (256 x 4 x 32003: 42.6, 35.4, 33.8, and 31.3 since; 8 x 8 x 131072 in 2048 chunks of
+// 4096 18.2, in 4096 of 2048 21.8; 500 x 4 x 2048 in one chunk a row 12.0, in chunks for
+// 8192 17.1). No more lists a request than the join takes.
 ChunkConfig chunk_config(int vocab, int beams, int batch) {
   const int most = kJoinLists / beams;
   const double rows = static_cast<double>(batch) * beams;
   auto fits = [&](int part) {
     const int parts = (vocab - 1) / part + 1;
-    return parts <= most && rows * parts <= 4096;
+    return parts == 1 || (parts <= most && rows * parts <= 2048);
   };
   if (fits(2048)) return config<2>(vocab, most);
   if (fits(4096)) return config<4>(vocab, most);

@@ -368,6 +368,12 @@ def test_reorder_short_and_long_rows(torch_gpu, l2c, length):
     check_reorder(torch_gpu, l2c, (1, 37, 7, 1, 1, length), 1)
 
 
+@pytest.mark.parametrize("beams", [2, 4, 7, 16, 32])
+def test_reorder_many_short_rows(torch_gpu, l2c, beams):
+    check_reorder(torch_gpu, l2c, (1, 301, beams, 1, 128, 4), 25)
+    check_reorder(torch_gpu, l2c, (2, 67, beams, 3, 5, 13), 4, offset=2)
+
+
 # ---------------------------------------------------------------------------
 
 def bf16(x):

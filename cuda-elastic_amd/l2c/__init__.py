@@ -280,9 +280,20 @@ def _type(t):
     return _types.setdefault(t.dtype, known[str(t.dtype)])
 
 
+_f32 = None  # torch.float32, once a weight has shown it
+
+
+def _weight(t):
+    """Raises unless a weight or gate is fp32: the kernel would read one of fewer bits past its end."""
+    global _f32
+    if str(t.dtype) != "torch.float32":
+        raise ValueError(f"l2c.residual_rmsnorm takes fp32 weights and gates, not {t.dtype}")
+    _f32 = t.dtype
+
+
 def residual_rmsnorm(normalized, residual_out, residual, block, weight, size, batch, block_weight=None, gate=None,
                      rows_per_gate=1, residual_scale=1.0, eps=RMS_EPSILON, stream=None):
-    """The types are the tensors'; residual_out, block_weight and gate may be None."""
+    """The types are the tensors', of weights and gates fp32; residual_out, block_weight and gate may be None."""
     try:
         kinds = _types[normalized.dtype], _types[residual.dtype], _types[block.dtype]
         out_kind = None if residual_out is None else _types[residual_out.dtype]
@@ -291,6 +302,12 @@ def residual_rmsnorm(normalized, residual_out, residual, block, weight, size, ba
         out_kind = None if residual_out is None else _type(residual_out)
     if out_kind is not None and out_kind != kinds[1]:
         raise ValueError("residual_out has another type than residual")
+    if weight is not None and weight.dtype is not _f32:
+        _weight(weight)
+    if block_weight is not None and block_weight.dtype is not _f32:
+        _weight(block_weight)
+    if gate is not None and gate.dtype is not _f32:
+        _weight(gate)
     code = _c_residual_rmsnorm(normalized, kinds[0], residual_out, residual, kinds[1], block, kinds[2], block_weight,
                                gate, rows_per_gate, weight, size, batch, residual_scale, eps, stream)
     if code:

@@ -650,12 +650,16 @@ struct ChunkConfig {
   int chunks, parts;  // chunks a row, parts a chunk
 };
 
+// Chunks of several parts: only with 8 float4 a lane, since chunk_config takes fewer only where
+// no chunk needs more than one part.
 template <int V>
 ChunkConfig config(int vocab, int most_chunks) {
   const int parts = (vocab - 1) / (kThreads * 4 * V) + 1;
-  const int each = (parts - 1) / most_chunks + 1;
-  return {each > 1 ? beam_chunks_kernel<V, true> : beam_chunks_kernel<V, false>, 4 * V,
-          (parts - 1) / each + 1, each};
+  if constexpr (V == 8) {
+    const int each = (parts - 1) / most_chunks + 1;
+    if (each > 1) return {beam_chunks_kernel<V, true>, 4 * V, (parts - 1) / each + 1, each};
+  }
+  return {beam_chunks_kernel<V, false>, 4 * V, parts, 1};
 }
 
 // 2048 logits a chunk as long as that makes at most 2048 chunks, and then 4096 logits: small

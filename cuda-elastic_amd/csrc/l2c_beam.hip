@@ -313,7 +313,7 @@ __global__ __launch_bounds__(kThreads, MANY ? 1 : 8) void beam_chunks_kernel(uns
     for (int w = 1; w < kWaves; ++w)
       if (w < sharing) least = min(least, bounds[w]);
     if (MANY && count == beams) least = max(least, kept_key[turn][beams - 1]);
-    least = max(least, key_of(-INFINITY));
+    least = max(least, key_of(-FLT_MAX));  // -Inf is no candidate: no list has it, however many there are
     float maximum = shift;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) maximum = fmaxf(maximum, tops[w]);
@@ -338,20 +338,19 @@ __global__ __launch_bounds__(kThreads, MANY ? 1 : 8) void beam_chunks_kernel(uns
         unsigned before = 0;
 #pragma unroll
         for (int i = 4 * V - 1; i >= 0; --i)
-          if (v[i] == tie && place(i) < n) before = UINT_MAX - (static_cast<unsigned>(start) + place(i));
+          if (v[i] == tie) before = UINT_MAX - (static_cast<unsigned>(start) + place(i));
         last = wave_bound(best == least ? before : 0u, beams - larger);
       }
     }
-    const float limit = number_of(least);  // NaN does not reach it
+    const float limit = number_of(least);  // NaN does not reach it, nor does what is past the end
     unsigned reach = 0;
-    if (last == 0 && limit > -INFINITY) {  // nor does what is past the end
+    if (last == 0) {
 #pragma unroll
       for (int i = 0; i < 4 * V; ++i) reach |= v[i] >= limit ? 1u << i : 0u;
     } else {
 #pragma unroll
       for (int i = 0; i < 4 * V; ++i)
-        if (v[i] > limit ||
-            (v[i] == limit && place(i) < n && UINT_MAX - (static_cast<unsigned>(start) + place(i)) >= last))
+        if (v[i] > limit || (v[i] == limit && UINT_MAX - (static_cast<unsigned>(start) + place(i)) >= last))
           reach |= 1u << i;
     }
     if (__ballot(reach != 0)) {
@@ -511,7 +510,7 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(float *scores_out, 
     const int beam = by_chunks(list);
     const bool end = ended[beam];
     const double score = base[beam] + (end ? 0.0 : static_cast<double>(c.logit) - static_cast<double>(tops[beam]));
-    const bool is = end ? rank == 0 && list == beam * chunks : c.token >= 0 && c.logit > -INFINITY;
+    const bool is = end ? rank == 0 && list == beam * chunks : c.token >= 0;
     return is ? key_of(score) : 0ULL;
   };
   // Entry `to`. What decides between equal keys: the lower beam and its larger logit, then

@@ -242,6 +242,7 @@ __device__ __forceinline__ int earlier(const unsigned *keys, const unsigned *bef
 template <int V, bool MANY>
 __global__ __launch_bounds__(kThreads, MANY ? 1 : 8) void beam_chunks_kernel(unsigned char *__restrict__ workspace,
                                                                const float *__restrict__ logits,
+                                                               const float *__restrict__ scores,
                                                                const int *__restrict__ tokens, int eos, int vocab,
                                                                int beams, int chunks, int parts) {
   constexpr int kPart = kThreads * 4 * V;
@@ -257,7 +258,10 @@ __global__ __launch_bounds__(kThreads, MANY ? 1 : 8) void beam_chunks_kernel(uns
   __shared__ double sums[kWaves];
   __shared__ int length;
   const int row = blockIdx.x / chunks, chunk = blockIdx.x - row * chunks;
-  if (eos >= 0 && tokens[row] == eos) return;  // ended: its logits do not count
+  const int token = tokens[row];  // both loads before either is waited for
+  const float score = scores[row];
+  const bool ended = eos >= 0 && token == eos, dead = !(fabsf(score) <= FLT_MAX);
+  if (ended | dead) return;  // its logits do not count, or it has no continuations
   const int t = threadIdx.x, lane = t % L2C_WAVE, wave = t / L2C_WAVE;
   const long long size = static_cast<long long>(parts) * kPart;
   const int first = static_cast<int>(chunk * size);  // below vocab: no chunk is empty
@@ -460,7 +464,7 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(float *scores_out, 
   for (int r = 0; r < HELD; ++r) held[r] = all[min(t + r * kThreads, entries - 1)];  // together, without a branch
   if (t < 2) lengths[t] = 0;
   // The sums of beams t / 16 and, of more than 16, t / 16 + 16. What most rows have is loaded together.
-  // Of an ended row the workspace holds nothing; what is read there is not used.
+  // Of ended and dead rows the workspace holds nothing; what is read there is not used.
   constexpr int kBeams = kThreads / kGroup, kRounds = kMaxBeams / kBeams, kStats = 2;
   const int member = t % kGroup, row = t / kGroup;
   ChunkStat held_stat[kRounds][kStats];
@@ -641,7 +645,7 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(float *scores_out, 
   for (int e = m + t; e < beams; e += kThreads) write(e, 0, -1, -1);
 }
 
-using ChunkKernel = void (*)(unsigned char *, const float *, const int *, int, int, int, int, int);
+using ChunkKernel = void (*)(unsigned char *, const float *, const float *, const int *, int, int, int, int, int);
 
 struct ChunkConfig {
   ChunkKernel fn;
@@ -704,8 +708,8 @@ extern "C" int l2c_decoder_beam_select(float *scores_out, int *tokens_out, int *
     return hipErrorInvalidValue;
   unsigned char *w = static_cast<unsigned char *>(workspace);
   const size_t list = 2 * sizeof(unsigned) * (kWaves * static_cast<size_t>(beams) * c.values + 8);
-  hipLaunchKernelGGL(c.fn, dim3(static_cast<unsigned>(grid)), dim3(kThreads), list, stream, w, logits, tokens, eos,
-                     vocab, beams, c.chunks, c.parts);
+  hipLaunchKernelGGL(c.fn, dim3(static_cast<unsigned>(grid)), dim3(kThreads), list, stream, w, logits, scores, tokens,
+                     eos, vocab, beams, c.chunks, c.parts);
   L2C_LAUNCH_CHECK();
   const int lists = beams * c.chunks;
   auto join = beams * lists <= kThreads ? beam_join_kernel<1, true>

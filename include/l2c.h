@@ -349,9 +349,10 @@ int l2c_decoder_softmax_argmax(float *probabilities, const float *logits, int *t
  *   by l2c_decoder_beam_reorder).
  *   A beam whose token tokens[row k] is eos (eos >= 0) has ended: its one continuation is
  *   eos at its own score, and its logits are not read. A beam has no continuation if its
- *   score is not finite (start a request with scores 0, -Inf, -Inf, ...), or its row holds a
- *   NaN or a +Inf or nothing but -Inf; nor has a token whose logit is -Inf. Where fewer than
- *   `beams` are left, the other rows get score -Inf, token -1 and parent -1.
+ *   score is not finite (start a request with scores 0, -Inf, -Inf, ...: their logits are not
+ *   read either), or its row holds a NaN or a +Inf or nothing but -Inf; nor has a token whose
+ *   logit is -Inf. Where fewer than `beams` are left, the other rows get score -Inf, token -1
+ *   and parent -1.
  *   Scores are computed in 64 bits (the exponentials in 32) and rounded once.
  *   scores_out may be scores and tokens_out may be tokens. workspace: 16-byte aligned, at
  *   least l2c_decoder_beam_workspace_bytes (0 for sizes that are not supported), which is

@@ -72,3 +72,25 @@ def test_old_contents_do_not_show(torch_gpu, l2c, batch, beams, vocab):
     parents = want[2].reshape(batch, beams)
     for b in range(batch):
         assert set(parents[b]) - {-1} <= set(np.flatnonzero(live[b * beams:(b + 1) * beams]))
+
+
+@pytest.mark.parametrize("eos", [-1, 2])
+@pytest.mark.parametrize("batch,beams,vocab", [(1, 6, 900), (3, 8, 32003), (1, 32, 300001)])
+def test_dead_and_ended_rows_are_left_out(torch_gpu, l2c, batch, beams, vocab, eos):
+    """The first step's scores, 0, -Inf, -Inf, ..., and the other values that end a beam: no chunk of
+    such a row has written anything, whatever its logits, and the others' have."""
+    rows = batch * beams
+    rng = np.random.default_rng(beams)
+    logits = 3 * rng.standard_normal((rows, vocab)).astype(np.float32)
+    scores, tokens = np.full(rows, NEG), np.full(rows, 5)
+    scores[::beams] = 0.0
+    scores[1], scores[2], scores[3] = np.nan, np.inf, -3.0
+    tokens[3] = 2
+    logits[1, 7] = np.nan
+    written = np.isfinite(scores) & ~((tokens == eos) & (eos >= 0))
+    (s, t, p), lists = select(torch_gpu, l2c, logits, scores, tokens, eos, beams, 0xA5)
+    untouched = lists.view(np.uint8).reshape(batch, beams, beams, -1) == 0xA5  # [request][rank][beam][bytes]
+    for b in range(batch):
+        for k in range(beams):
+            assert untouched[b, :, k].all() != written[b * beams + k]
+    assert set(p[:beams]) <= {0, 3} and (p[beams:] == 0).all() and (t >= 0).all() and np.isfinite(s).all()

@@ -70,12 +70,15 @@ __global__ __launch_bounds__(kQuantThreads) void quantize_mxfp4_bf16_kernel(uint
 // ---------------------------------------------------------------------------
 // Choice of the contraction's tile: the one of least estimated time. Fitted to the times of
 // these and 9 other tiles on 132 shapes of 1 to 1024 x 288 to 16384 x 600 to 11008: what a
-// CU takes for its tiles in turn is linear in their number and in K to about 12%, and
-// the choice among these nine is 3% slower than the best of all in the mean. Measured
-// on either side of a border, us: 1 x 4096 x 11008 6.8 on 16 x 16 tiles, 6.0 on 32 x 64,
-// 8.1 on 64 x 64; 332 x 512 x 8012 7.1 on 32 x 32 by two waves, 8.0 on 128 x 128; 64 x 4096 x 11008 11.9 on 32 x 64, 8.9 on 64 x 64; 128 x 4096 x 11008
-// 12.9 on 64 x 64, 11.3 on 64 x 128; 512 x 4096 x 11008 32.3 on 128 x 128, 21.4 on 128 x
-// 192, 24.4 on 256 x 128; 400 x 4096 x 11008 27.2 on 128 x 128, 21.1 on 256 x 128.
+// CU takes for its tiles in turn is linear in their number and in K to about 12% in the mean,
+// and the choice among these nine is 3% slower than the best of all in the mean. Where
+// large tiles keep all CUs busy the estimates are too low, by more the larger the tile, but in
+// order: 1024 x 16384 x 8192 56 us on 256 x 128 where it takes 82, 83 on 128 x 128 (101), 104
+// on 128 x 192 (117). Measured on either side of a border, us: 1 x 4096 x 11008 6.8 on 16 x
+// 16 tiles, 6.0 on 32 x 64, 8.1 on 64 x 64; 332 x 512 x 8012 7.1 on 32 x 32 by two waves, 8.0
+// on 128 x 128; 64 x 4096 x 11008 11.9 on 32 x 64, 8.9 on 64 x 64; 128 x 4096 x 11008 12.9 on
+// 64 x 64, 11.3 on 64 x 128; 512 x 4096 x 11008 32.3 on 128 x 128, 21.4 on 128 x 192, 24.4 on
+// 256 x 128; 400 x 4096 x 11008 27.2 on 128 x 128, 21.1 on 256 x 128.
 
 constexpr int kMaxCols = (1 << 24) - 32;  // a tile's 256 rows of codes stay within 31 bits
 

@@ -25,9 +25,13 @@
 //  * Rows past the operands re-read the last row, steps past the end the last block, scales
 //    past the last whole step the ones before: every access is inside the operands.
 //    K >= 512.
-//  * 1024 x 16384 x 8192 takes 76 us, 3.6 PFLOP/s at 2.08 GHz, near the device's power limit.
-//    Of a step's 1550 cycles on 256 x 128 LDS is busy 1150, with DMA's writes and the
-//    fragments' reads, and the matrix cores 1024; on 128 x 128 770 and 512 of 1180.
+//  * 1024 x 16384 x 8192 takes 77 to 82 us, 3.5 PFLOP/s, with the matrix cores busy 0.46 of
+//    the time. Copies of the kernel with parts left out take 65.5 us with staging alone
+//    and 56 with the products, or the products and the fragments' reads, alone; so staging is the
+//    longer part, and they overlap only in part. Staging brings 805 MB at 12 TB/s, of which 143
+//    MB miss L2, and takes no longer a step where rows are no power of two apart (lengths of 15872 and
+//    16640: 66.8 and 68.4 us). The clock is 1.84 GHz, with the products alone 1.90, with staging
+//    alone 2.35. 256 x 4096 x 11008 on 128 x 128: 16.9, staging alone 13.4, products alone 11.7.
 #include <type_traits>
 
 #include "l2c_common.h"

@@ -11,9 +11,10 @@
 // Bound by HBM: every value read and written once. A workgroup a row of up to 16384
 // values, which its lanes hold in registers from the first load to the last store: eight
 // values a lane and chunk, whole 16-byte loads and stores at any address the types
-// allow. 1024 x 16384, fp32 to fp32 and bf16: 50 us, 4.7 TB/s (74 us with nontemporal
-// loads, which pass the MALL by); 1024 x 16384 bf16 28 us; 1 x 4096 3.0 us. Longer rows are
-// read three times (from HBM once: the later passes hit the caches).
+// allow. 1024 x 16384, fp32 to fp32 and bf16: 53 us, 4.4 TB/s (74 us with nontemporal
+// loads, which pass the MALL by); 1024 x 16384 bf16 30 us; 1 x 4096 2.7 us. Longer rows are
+// read three times (from HBM once: the later passes hit the caches), a value a lane and
+// load, and wait for each: 16 x 20000 fp32 70 us, 200 x 131072 bf16 1310 (0.16 TB/s).
 #include <type_traits>
 
 #include "l2c_common.h"

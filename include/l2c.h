@@ -353,7 +353,10 @@ int l2c_decoder_softmax_argmax(float *probabilities, const float *logits, int *t
  *   read either), or its row holds a NaN or a +Inf or nothing but -Inf; nor has a token whose
  *   logit is -Inf. Where fewer than `beams` are left, the other rows get score -Inf, token -1
  *   and parent -1.
- *   Scores are computed in 64 bits (the exponentials in 32) and rounded once.
+ *   Scores are computed in 64 bits and rounded once (one below fp32's lowest number to -Inf:
+ *   its beam has no continuation on the next step); the exponentials, and sums of 32 of
+ *   them at most, are fp32, which leaves a row's scores within 2^-24 (36 + d) of their values, d the
+ *   mean distance of the row's logits from the largest, weighed by their probabilities.
  *   scores_out may be scores and tokens_out may be tokens. workspace: 16-byte aligned, at
  *   least l2c_decoder_beam_workspace_bytes (0 for sizes that are not supported), which is
  *   at most batch * beams * ceil(vocab / 1024) * (8 * beams + 16); its contents need not be

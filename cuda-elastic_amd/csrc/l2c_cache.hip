@@ -1,0 +1,343 @@
+// The pages of a cache: new tokens' keys and values written into them, the step of the
+// tables that name them, and the copies of pages that two sequences would write.
+#include "l2c_cache.h"
+#include "l2c_formats.h"
+
+namespace {
+
+using l2c::Sequences;
+
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+// ---------------------------------------------------------------------------
+// append
+
+constexpr int kAppendThreads = 256;
+
+__device__ __forceinline__ float low_half(unsigned u) { return __uint_as_float(u << 16); }
+__device__ __forceinline__ float high_half(unsigned u) { return __uint_as_float(u & 0xffff0000u); }
+
+// blockIdx.y: the head. A row's key or value (blockIdx.z) by 32 lanes, eight values a lane.
+template <bool E4M3>
+__global__ __launch_bounds__(kAppendThreads) void append_kernel(void *keys, void *values, float *key_scales,
+                                                                float *value_scales, const uint16_t *k,
+                                                                long long k_stride, const uint16_t *v,
+                                                                long long v_stride, Sequences s, int kv_heads,
+                                                                int width) {
+  constexpr int kLanes = 32;
+  const int row = blockIdx.x * (kAppendThreads / kLanes) + threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
+  const int head = blockIdx.y;
+  const bool value = blockIdx.z != 0;
+  int sequence, position;
+  if (row >= s.rows || !s.find(row, sequence, position) || position < 0 || position >= s.capacity()) return;
+  const int index = s.by_page(position), page = s.page(sequence, index);
+  if (!s.is_page(page)) return;
+  const size_t to = (static_cast<size_t>(page) * kv_heads + head) * s.page_size + (position - index * s.page_size);
+  const uint16_t *const from =
+      (value ? v + row * v_stride : k + row * k_stride) + static_cast<size_t>(head) * width;
+  const bool mine = 8 * lane < width;
+  u32x4 x = {0, 0, 0, 0};
+  if (mine) x = *reinterpret_cast<const u32x4 *>(from + 8 * lane);
+  if constexpr (!E4M3) {
+    if (mine) *reinterpret_cast<u32x4 *>(static_cast<uint16_t *>(value ? values : keys) + to * width + 8 * lane) = x;
+  } else {
+    unsigned largest = 0;  // of the magnitudes' patterns, which order as the numbers do, NaN above all
+#pragma unroll
+    for (int i = 0; i < 4; ++i) largest = max(largest, max(x[i] << 16 & 0x7fff0000u, x[i] & 0x7fff0000u));
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) largest = max(largest, __shfl_xor(largest, o, L2C_WAVE));
+    const bool finite = largest < 0x7f800000u;
+    const float amax = __uint_as_float(largest);
+    const float scale = !finite ? __uint_as_float(0x7fc00000u) : amax > 0.0f ? amax / 448.0f : 1.0f;
+    u32x2 code = {0, 0};
+    if (finite) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const unsigned pair = l2c::e4m3_code(low_half(x[i]) / scale) | l2c::e4m3_code(high_half(x[i]) / scale) << 8;
+        code[i / 2] |= pair << 16 * (i % 2);
+      }
+    }
+    if (mine) *reinterpret_cast<u32x2 *>(static_cast<uint8_t *>(value ? values : keys) + to * width + 8 * lane) = code;
+    if (lane == 0) (value ? value_scales : key_scales)[to] = scale;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// advance
+
+constexpr int kAdvanceThreads = 1024;
+
+struct Step {
+  int *tables_out, *lengths_out, *uses, *copies, *shortage;
+  const int *tables, *lengths, *parents, *starts, *held;
+  int beams, sequences, pages, max_pages, page_size, window;
+
+  __device__ __forceinline__ int pages_of(long long positions) const {  // may be more than max_pages
+    return static_cast<int>((positions + page_size - 1) / page_size);
+  }
+  // Its parent (-1: none), the parent's length and the new tokens of a sequence.
+  __device__ __forceinline__ int parent(int r, int &length, int &n) const {
+    int p = r;
+    if (parents) {
+      const int k = parents[r];
+      p = k >= 0 && k < beams ? r - r % beams + k : -1;
+    }
+    length = p < 0 ? 0 : max(0, lengths[p]);
+    n = p < 0 ? 0 : starts ? static_cast<int>(max(0LL, static_cast<long long>(starts[r + 1]) - starts[r])) : 1;
+    n = min(n, INT_MAX - length);
+    return p;
+  }
+};
+
+// A workgroup a sequence: its parent's entries; and the uses, to be counted from 0.
+__global__ __launch_bounds__(256) void advance_tables_kernel(Step s) {
+  const int r = blockIdx.x;
+  for (long long i = static_cast<long long>(r) * blockDim.x + threadIdx.x; i < s.pages;
+       i += static_cast<long long>(gridDim.x) * blockDim.x)
+    s.uses[i] = 0;
+  int length, n;
+  const int p = s.parent(r, length, n);
+  const int have = min(s.pages_of(length), s.max_pages);
+  const int dropped = s.window ? max(0, length - s.window + 1) / s.page_size : 0;  // entries behind the window
+  int *const to = s.tables_out + static_cast<size_t>(r) * s.max_pages;
+  const int *const from = s.tables + static_cast<size_t>(max(p, 0)) * s.max_pages;
+  for (int i = threadIdx.x; i < s.max_pages; i += blockDim.x) to[i] = i < have && i >= dropped ? from[i] : -1;
+}
+
+__global__ __launch_bounds__(256) void advance_count_kernel(Step s) {
+  const int r = blockIdx.x;
+  int length, n;
+  s.parent(r, length, n);
+  const int have = min(s.pages_of(length), s.max_pages);
+  const int *const table = s.tables_out + static_cast<size_t>(r) * s.max_pages;
+  for (int i = threadIdx.x; i < have; i += blockDim.x)
+    if (static_cast<unsigned>(table[i]) < static_cast<unsigned>(s.pages)) atomicAdd(&s.uses[table[i]], 1);
+}
+
+__device__ __forceinline__ int now(const int *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ void put(int *p, int v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+// The sum over the workgroup's lanes before this one; `all` over all of them.
+__device__ __forceinline__ long long scan_before(long long v, long long *slots, long long &all) {
+  const int lane = threadIdx.x % L2C_WAVE, wave = threadIdx.x / L2C_WAVE, waves = blockDim.x / L2C_WAVE;
+  long long upto = v;
+#pragma unroll
+  for (int o = 1; o < L2C_WAVE; o <<= 1) {
+    const long long before = __shfl_up(upto, o, L2C_WAVE);
+    if (lane >= o) upto += before;
+  }
+  __syncthreads();  // the slots may still be read from the call before
+  if (lane == L2C_WAVE - 1) slots[wave] = upto;
+  __syncthreads();
+  long long base = 0;
+  all = 0;
+  for (int w = 0; w < waves; ++w) {
+    if (w < wave) base += slots[w];
+    all += slots[w];
+  }
+  return base + upto - v;
+}
+
+// One workgroup: which pages are replaced, and the new pages for all sequences. A
+// sequence that writes into a page takes itself off its uses; what is left are those who do not
+// write. Where nobody is, the lowest sequence leaves its number less the number of
+// sequences, a negative one, by which it finds that it keeps the page. Sums and minima of
+// integers: the order of the atomics does not show.
+__global__ __launch_bounds__(kAdvanceThreads) void advance_assign_kernel(Step s) {
+  __shared__ long long slots[kAdvanceThreads / L2C_WAVE];
+  const int t = threadIdx.x;
+  // Entries that sequence r has and needs; the page that it writes into, or -1.
+  auto written = [&](int r, int &first, int &last) {
+    int length, n;
+    s.parent(r, length, n);
+    first = s.pages_of(length), last = s.pages_of(static_cast<long long>(length) + n);
+    if (n == 0 || length % s.page_size == 0 || first > s.max_pages) return -1;
+    const int page = s.tables_out[static_cast<size_t>(r) * s.max_pages + first - 1];
+    return static_cast<unsigned>(page) < static_cast<unsigned>(s.pages) ? page : -1;
+  };
+  int first, last;
+  for (int r = t; r < s.sequences; r += kAdvanceThreads) {
+    const int page = written(r, first, last);
+    if (page >= 0) atomicSub(&s.uses[page], 1);
+  }
+  __syncthreads();
+  for (int r = t; r < s.sequences; r += kAdvanceThreads) {
+    const int page = written(r, first, last);
+    if (page >= 0 && now(&s.uses[page]) <= 0 && !(s.held && s.held[page])) atomicMin(&s.uses[page], r - s.sequences);
+  }
+  __syncthreads();
+  // copies is scratch until the end: the page that is replaced, or -1, and how many new pages the
+  // sequences before need (no more than INT_MAX, which no page's number reaches).
+  long long total = 0, beyond = 0;
+  for (int from = 0; from < s.sequences; from += kAdvanceThreads) {
+    const int r = from + t;
+    int replaced = -1;
+    long long need = 0, lost = 0, all;
+    if (r < s.sequences) {
+      const int page = written(r, first, last);
+      if (page >= 0 && now(&s.uses[page]) != r - s.sequences) replaced = page;
+      const int upto = min(last, s.max_pages);
+      need = max(0, upto - first) + (replaced >= 0);
+      lost = last - max(first, upto);
+    }
+    const long long before = total + scan_before(need, slots, all);
+    if (r < s.sequences) {
+      s.copies[2LL * r] = replaced;
+      s.copies[2LL * r + 1] = static_cast<int>(min(before, static_cast<long long>(INT_MAX)));
+    }
+    total += all;
+    scan_before(lost, slots, all);
+    beyond += all;
+  }
+  __syncthreads();
+  for (int r = t; r < s.sequences; r += kAdvanceThreads) {
+    const int page = written(r, first, last);
+    if (page >= 0 && now(&s.uses[page]) == r - s.sequences) put(&s.uses[page], 1);  // it keeps the page
+  }
+  __syncthreads();
+  // Free pages in order, each to the sequence that its rank falls to.
+  long long given = 0;
+  for (long long from = 0; from < s.pages && given < total; from += kAdvanceThreads) {
+    const int page = static_cast<int>(min(from + t, static_cast<long long>(INT_MAX)));
+    const bool free = page < s.pages && now(&s.uses[page]) == 0 && !(s.held && s.held[page]);
+    long long all;
+    const long long rank = given + scan_before(free, slots, all);
+    if (free && rank < total) {
+      int low = 0, high = s.sequences - 1;  // the last sequence whose first rank is at most this one
+      while (low < high) {
+        const int middle = high - (high - low) / 2;
+        if (s.copies[2LL * middle + 1] <= rank) low = middle;
+        else high = middle - 1;
+      }
+      const int replaced = s.copies[2LL * low] >= 0;
+      int length, n;
+      s.parent(low, length, n);
+      const int entry = s.pages_of(length) - replaced + static_cast<int>(rank - s.copies[2LL * low + 1]);
+      s.tables_out[static_cast<size_t>(low) * s.max_pages + entry] = page;
+      put(&s.uses[page], 1);
+    }
+    given += all;
+  }
+  __syncthreads();
+  for (int r = t; r < s.sequences; r += kAdvanceThreads) {
+    int length, n;
+    s.parent(r, length, n);
+    const int replaced = s.copies[2LL * r];
+    if (replaced >= 0) {
+      int *const entry = s.tables_out + static_cast<size_t>(r) * s.max_pages + s.pages_of(length) - 1;
+      const bool none = s.copies[2LL * r + 1] >= given;
+      if (none) *entry = -1;
+      s.copies[2LL * r] = none ? -1 : replaced;
+      s.copies[2LL * r + 1] = none ? -1 : *entry;
+    } else {
+      s.copies[2LL * r + 1] = -1;
+    }
+    s.lengths_out[r] = length + n;
+  }
+  if (t == 0) *s.shortage = static_cast<int>(min(max(total - given, 0LL) + beyond, static_cast<long long>(INT_MAX)));
+}
+
+// ---------------------------------------------------------------------------
+// copy
+
+constexpr int kCopyThreads = 256;
+
+typedef unsigned u32x4_any __attribute__((ext_vector_type(4), aligned(1)));
+
+// Part `blockIdx.x % parts` of pair blockIdx.x / parts in group blockIdx.y: columns of 16 bytes, and of
+// one byte for what is left of the page.
+__global__ __launch_bounds__(kCopyThreads) void copy_kernel(unsigned char *cache, const int *__restrict__ copies,
+                                                            int pages, unsigned parts, unsigned wide, unsigned columns,
+                                                            long long group_stride, long long page_stride) {
+  const unsigned pair = blockIdx.x / parts, part = blockIdx.x - pair * parts;
+  const int from = copies[2 * static_cast<size_t>(pair)], to = copies[2 * static_cast<size_t>(pair) + 1];
+  if (static_cast<unsigned>(from) >= static_cast<unsigned>(pages) ||
+      static_cast<unsigned>(to) >= static_cast<unsigned>(pages) || from == to)
+    return;
+  const unsigned c = part * kCopyThreads + threadIdx.x;
+  if (c >= columns) return;
+  cache += blockIdx.y * group_stride;
+  const unsigned char *const src = cache + from * page_stride;
+  unsigned char *const dst = cache + to * page_stride;
+  if (c < wide) *reinterpret_cast<u32x4_any *>(dst + 16LL * c) = *reinterpret_cast<const u32x4_any *>(src + 16LL * c);
+  else dst[16LL * wide + (c - wide)] = src[16LL * wide + (c - wide)];
+}
+
+}  // namespace
+
+extern "C" int l2c_cache_append(void *keys, void *values, float *key_scales, float *value_scales, int cache_type,
+                                const uint16_t *k, long long k_stride, const uint16_t *v, long long v_stride,
+                                const int *tables, const int *lengths, const int *starts, int sequences, int rows,
+                                int kv_heads, int width, int page_size, int pages, int max_pages, hipStream_t stream) {
+  if (!l2c::cache_sizes(cache_type, sequences, rows, kv_heads, width, page_size, pages, max_pages))
+    return hipErrorInvalidValue;
+  const long long row = static_cast<long long>(kv_heads) * width;
+  if (k_stride < row || v_stride < row || k_stride % 8 != 0 || v_stride % 8 != 0) return hipErrorInvalidValue;
+  if (sequences == 0 || rows == 0 || pages == 0 || max_pages == 0) return hipSuccess;
+  if (!l2c::cache_arguments(cache_type, keys, values, key_scales, value_scales, tables, lengths, starts, sequences,
+                            rows) ||
+      !k || !v || !l2c_aligned16(k) || !l2c_aligned16(v))
+    return hipErrorInvalidValue;
+  const long long blocks = (static_cast<long long>(rows) + 7) / 8;
+  if (!l2c::launchable(blocks * kv_heads * 2, kAppendThreads)) return hipErrorInvalidValue;
+  const l2c::Sequences s =
+      l2c::sequences_of(tables, lengths, starts, sequences, rows, max_pages, page_size, pages);
+  auto fn = cache_type == L2C_BF16 ? append_kernel<false> : append_kernel<true>;
+  hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(blocks), kv_heads, 2), dim3(kAppendThreads), 0, stream, keys, values,
+                     key_scales, value_scales, k, k_stride, v, v_stride, s, kv_heads, width);
+  L2C_LAUNCH_CHECK();
+  return hipSuccess;
+}
+
+extern "C" int l2c_cache_advance(int *tables_out, int *lengths_out, int *uses, int *copies, int *shortage,
+                                 const int *tables, const int *lengths, const int *parents, int beams,
+                                 const int *starts, const int *held, int sequences, int page_size, int pages,
+                                 int max_pages, int window, hipStream_t stream) {
+  if (sequences < 0 || page_size <= 0 || pages < 0 || max_pages < 0 || window < 0 ||
+      static_cast<long long>(max_pages) * page_size > INT_MAX || (parents && (beams <= 0 || sequences % beams != 0)))
+    return hipErrorInvalidValue;
+  if (sequences == 0) return hipSuccess;
+  if (!lengths_out || !copies || !shortage || !lengths || (pages > 0 && !uses) ||
+      (max_pages > 0 && (!tables_out || !tables)) || (parents && (tables_out == tables || lengths_out == lengths)) ||
+      !l2c::launchable(sequences, 256))
+    return hipErrorInvalidValue;
+  const Step s = {tables_out, lengths_out, uses, copies, shortage, tables, lengths, parents, starts, held,
+                  beams, sequences, pages, max_pages, page_size, window};
+  hipLaunchKernelGGL(advance_tables_kernel, dim3(sequences), dim3(256), 0, stream, s);
+  L2C_LAUNCH_CHECK();
+  hipLaunchKernelGGL(advance_count_kernel, dim3(sequences), dim3(256), 0, stream, s);
+  L2C_LAUNCH_CHECK();
+  hipLaunchKernelGGL(advance_assign_kernel, dim3(1), dim3(kAdvanceThreads), 0, stream, s);
+  L2C_LAUNCH_CHECK();
+  return hipSuccess;
+}
+
+extern "C" int l2c_cache_copy(void *cache, const int *copies, int count, int pages, int groups, long long group_stride,
+                              long long page_stride, long long page_bytes, hipStream_t stream) {
+  if (count < 0 || pages < 0 || groups < 0 || page_bytes < 0) return hipErrorInvalidValue;
+  if (count == 0 || pages == 0 || groups == 0 || page_bytes == 0) return hipSuccess;
+  if (!cache || !copies) return hipErrorInvalidValue;
+  // Pages and groups follow each other without overlap, within 63 bits.
+  typedef __int128 wide_t;
+  const wide_t group = static_cast<wide_t>(pages - 1) * page_stride + page_bytes;
+  const wide_t span = static_cast<wide_t>(groups - 1) * group_stride + group;
+  if ((pages > 1 && page_stride < page_bytes) || (groups > 1 && group_stride < group) || span > LLONG_MAX)
+    return hipErrorInvalidValue;
+  const long long wide = page_bytes / 16, columns = wide + page_bytes % 16;
+  if (columns > INT_MAX) return hipErrorInvalidValue;
+  const long long parts = (columns + kCopyThreads - 1) / kCopyThreads;
+  constexpr int kGridY = 65535;  // groups a launch
+  if (parts > INT_MAX / count || !l2c::launchable(parts * count * min(groups, kGridY), kCopyThreads))
+    return hipErrorInvalidValue;
+  for (int first = 0; first < groups; first += kGridY) {
+    const dim3 grid(static_cast<unsigned>(parts * count), min(groups - first, kGridY));
+    hipLaunchKernelGGL(copy_kernel, grid, dim3(kCopyThreads), 0, stream,
+                       static_cast<unsigned char *>(cache) + first * group_stride, copies, pages,
+                       static_cast<unsigned>(parts), static_cast<unsigned>(wide), static_cast<unsigned>(columns),
+                       group_stride, page_stride);
+    L2C_LAUNCH_CHECK();
+    if (groups - first <= kGridY) break;
+  }
+  return hipSuccess;
+}

@@ -164,7 +164,8 @@ PyObject *fall_back(const char *name, PyObject *const *args, Py_ssize_t n) {
   X(quantize_mxfp8) X(quantize_mxfp4) X(quantize_fp8) X(to_bf16) X(decoder_init_model) X(decoder_rmsnorm)       \
   X(decoder_rmsnorm_absmax) X(decoder_softmax_argmax) X(quantize_mxfp6) X(nvfp4_tensor_scales)                  \
   X(nvfp4_tensor_scales_absmax) X(quantize_nvfp4) X(to_bf16_x4) X(matmul_bf16) X(matmul_mxfp6)                  \
-  X(residual_rmsnorm) X(quantize_mxfp4_bf16) X(matmul_mxfp4) X(decoder_beam_select) X(decoder_beam_reorder)
+  X(residual_rmsnorm) X(quantize_mxfp4_bf16) X(matmul_mxfp4) X(decoder_beam_select) X(decoder_beam_reorder)   \
+  X(decoder_logprobs) X(cache_append) X(cache_attention) X(cache_advance) X(cache_copy)
 L2C_ENTRIES(L2C_ENTRY)
 
 PyObject *initialise(PyObject *, PyObject *args) {

@@ -58,9 +58,14 @@ KERNEL_SYMBOLS = (
     "l2c_copy_to_host",
     "l2c_residual_rmsnorm", "l2c_quantize_mxfp4_bf16", "l2c_matmul_mxfp4",
     "l2c_decoder_beam_select", "l2c_decoder_beam_reorder", "l2c_decoder_beam_workspace_bytes",
+    "l2c_decoder_logprobs", "l2c_decoder_logprobs_workspace_bytes",
+    "l2c_cache_append", "l2c_cache_attention", "l2c_cache_attention_workspace_bytes", "l2c_cache_advance",
+    "l2c_cache_copy",
 )
 MAX_BEAMS = 32  # L2C_MAX_BEAMS
-F32, BF16 = 0, 1  # enum l2c_type
+MAX_ALTERNATIVES = 32  # L2C_MAX_ALTERNATIVES
+MAX_HEAD = 256  # L2C_MAX_HEAD
+F32, BF16, E4M3 = 0, 1, 2  # enum l2c_type
 QS_STATIC_SCRATCH_BYTES = 24 << 20  # L2C_QS_STATIC_SCRATCH_BYTES
 NVFP4_PARTIALS = 1024  # L2C_NVFP4_PARTIALS
 HOST_SYMBOLS = ("l2c_harness_main", "l2c_compare_dumps", "l2c_decoder_main", "l2c_decoder_run",
@@ -98,7 +103,7 @@ def load() -> ctypes.CDLL:
     except ImportError:
         pass
     lib = ctypes.CDLL(LIB_PATH, mode=ctypes.RTLD_GLOBAL)
-    i, f, p, sz = ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t
+    i, f, p, sz, ll = ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_longlong
     sigs = {
         "l2c_rmsnorm": [p, p, p, i, i, f, p],
         "l2c_softmax": [p, p, i, i, p],
@@ -129,7 +134,12 @@ def load() -> ctypes.CDLL:
         "l2c_quantize_mxfp4_bf16": [p, p, p, i, i, p],
         "l2c_matmul_mxfp4": [p, p, p, p, p, i, i, i, p],
         "l2c_decoder_beam_select": [p, p, p, p, p, p, p, i, i, i, i, i, i, p, sz, p],
-        "l2c_decoder_beam_reorder": [p, p, p, i, i, i, i, *[ctypes.c_longlong] * 4, p],
+        "l2c_decoder_beam_reorder": [p, p, p, i, i, i, i, *[ll] * 4, p],
+        "l2c_decoder_logprobs": [p, p, p, p, p, p, i, i, i, p, sz, p],
+        "l2c_cache_append": [p, p, p, p, i, p, ll, p, ll, p, p, p, *[i] * 7, p],
+        "l2c_cache_attention": [p, ll, p, ll, p, p, p, p, i, p, p, p, *[i] * 9, f, p, sz, p],
+        "l2c_cache_advance": [p, p, p, p, p, p, p, p, i, p, p, *[i] * 5, p],
+        "l2c_cache_copy": [p, p, i, i, i, ll, ll, ll, p],
     }
     for name, args in sigs.items():
         fn = getattr(lib, name)
@@ -139,6 +149,10 @@ def load() -> ctypes.CDLL:
     lib.l2c_mxfp8_workspace_bytes.restype = sz
     lib.l2c_decoder_beam_workspace_bytes.argtypes = [i, i, i]
     lib.l2c_decoder_beam_workspace_bytes.restype = sz
+    lib.l2c_decoder_logprobs_workspace_bytes.argtypes = [i, i, i]
+    lib.l2c_decoder_logprobs_workspace_bytes.restype = sz
+    lib.l2c_cache_attention_workspace_bytes.argtypes = [i] * 7
+    lib.l2c_cache_attention_workspace_bytes.restype = sz
     lib.l2c_mxfp6_bytes.argtypes = [i, i, ctypes.POINTER(sz), ctypes.POINTER(sz)]
     lib.l2c_mxfp6_bytes.restype = ctypes.c_int
     lib.l2c_strerror.argtypes = [ctypes.c_int]
@@ -175,7 +189,8 @@ _ENTRIES = ("rmsnorm", "softmax", "matvec", "fused", "matmul", "matmul_q", "matm
             "quantize_mxfp8", "quantize_mxfp4", "quantize_fp8", "to_bf16", "decoder_init_model", "decoder_rmsnorm",
             "decoder_rmsnorm_absmax", "decoder_softmax_argmax", "quantize_mxfp6", "nvfp4_tensor_scales",
             "nvfp4_tensor_scales_absmax", "quantize_nvfp4", "to_bf16_x4", "matmul_bf16", "matmul_mxfp6",
-            "residual_rmsnorm", "quantize_mxfp4_bf16", "matmul_mxfp4", "decoder_beam_select", "decoder_beam_reorder")
+            "residual_rmsnorm", "quantize_mxfp4_bf16", "matmul_mxfp4", "decoder_beam_select", "decoder_beam_reorder",
+            "decoder_logprobs", "cache_append", "cache_attention", "cache_advance", "cache_copy")
 _native = {}
 
 
@@ -439,6 +454,110 @@ def decoder_beam_reorder(out, inp, parents, beams, batch, piece_bytes, row_strid
                                    piece_bytes if row_stride is None else row_stride, piece_stride, piece_bytes, stream)
     if code:
         _check(code, "l2c_decoder_beam_reorder")
+
+
+def _takes(what, dtype, *tensors):
+    """Raises unless the tensors (or None) are of a type, by its name, and on the current device: the
+    kernel would read wider or other elements than theirs, or another device's memory."""
+    import torch
+    wanted = getattr(torch, dtype)
+    device = torch.cuda.current_device() if torch.cuda.is_available() else -1
+    for t in tensors:
+        if t is None:
+            continue
+        if t.dtype is not wanted and not (dtype == "bfloat16" and str(t.dtype) in ("torch.int16", "torch.uint16")):
+            raise ValueError(f"l2c.{what} takes {dtype} here, not {t.dtype}")
+        if t.is_cuda and t.get_device() != device:
+            raise ValueError(f"l2c.{what} takes tensors on the current device, {device}, not on {t.get_device()}")
+
+
+def _bytes(t):
+    return 0 if t is None else t.numel() * t.element_size()
+
+
+def decoder_logprobs_workspace_bytes(vocab, top, rows):
+    return load().l2c_decoder_logprobs_workspace_bytes(vocab, top, rows)
+
+
+def decoder_logprobs(logprobs, entropies, top_tokens, top_logprobs, logits, tokens, vocab, top, rows, workspace=None,
+                     stream=None):
+    """logprobs and tokens may be None together, entropies alone, the alternatives with top 0."""
+    _takes("decoder_logprobs", "float32", logprobs, entropies, top_logprobs, logits)
+    _takes("decoder_logprobs", "int32", top_tokens, tokens)
+    code = _c_decoder_logprobs(logprobs, entropies, top_tokens, top_logprobs, logits, tokens, vocab, top, rows,
+                               workspace, _bytes(workspace), stream)
+    if code:
+        _check(code, "l2c_decoder_logprobs")
+
+
+def _cache_type(what, keys, values, key_scales, value_scales, tables, lengths, starts, *rows):
+    """The pages' enum l2c_type: bf16, or e4m3, which bytes may hold, too."""
+    kind = str(keys.dtype)
+    if values.dtype is not keys.dtype:
+        raise ValueError(f"l2c.{what} takes keys and values of one type")
+    if kind in ("torch.uint8", "torch.float8_e4m3fn"):
+        cache_type = E4M3
+        if key_scales is None or value_scales is None:
+            raise ValueError(f"l2c.{what} needs the scales of e4m3 pages")
+    elif kind in ("torch.bfloat16", "torch.int16", "torch.uint16"):
+        cache_type = BF16
+    else:
+        raise ValueError(f"l2c.{what} takes bf16 and e4m3 pages, not {kind}")
+    _takes(what, kind[len("torch."):], keys, values)
+    _takes(what, "float32", key_scales, value_scales)
+    _takes(what, "int32", tables, lengths, starts)
+    _takes(what, "bfloat16", *rows)
+    return cache_type
+
+
+def cache_append(keys, values, k, v, tables, lengths, kv_heads, width, page_size, pages, max_pages, sequences, rows=None,
+                 starts=None, key_scales=None, value_scales=None, k_stride=None, v_stride=None, stream=None):
+    """Rows of k and v follow each other unless their strides (in values) say otherwise."""
+    cache_type = _cache_type("cache_append", keys, values, key_scales, value_scales, tables, lengths, starts, k, v)
+    code = _c_cache_append(keys, values, key_scales, value_scales, cache_type, k,
+                           kv_heads * width if k_stride is None else k_stride, v,
+                           kv_heads * width if v_stride is None else v_stride, tables, lengths, starts, sequences,
+                           sequences if rows is None else rows, kv_heads, width, page_size, pages, max_pages, stream)
+    if code:
+        _check(code, "l2c_cache_append")
+
+
+def cache_attention_workspace_bytes(sequences, rows, heads, kv_heads, width, page_size, max_pages):
+    return load().l2c_cache_attention_workspace_bytes(sequences, rows, heads, kv_heads, width, page_size, max_pages)
+
+
+def cache_attention(out, q, keys, values, tables, lengths, heads, kv_heads, width, page_size, pages, max_pages, sequences,
+                    workspace=None, rows=None, starts=None, key_scales=None, value_scales=None, window=0, scale=None,
+                    q_stride=None, out_stride=None, stream=None):
+    """scale is 1 / sqrt(width) unless given; rows of q and out follow each other unless their strides say otherwise."""
+    cache_type = _cache_type("cache_attention", keys, values, key_scales, value_scales, tables, lengths, starts, q, out)
+    code = _c_cache_attention(out, heads * width if out_stride is None else out_stride, q,
+                              heads * width if q_stride is None else q_stride, keys, values, key_scales, value_scales,
+                              cache_type, tables, lengths, starts, sequences, sequences if rows is None else rows, heads,
+                              kv_heads, width, page_size, pages, max_pages, window,
+                              width ** -0.5 if scale is None else scale, workspace, _bytes(workspace), stream)
+    if code:
+        _check(code, "l2c_cache_attention")
+
+
+def cache_advance(tables_out, lengths_out, uses, copies, shortage, tables, lengths, sequences, max_pages, page_size, pages,
+                  parents=None, beams=1, starts=None, held=None, window=0, stream=None):
+    _takes("cache_advance", "int32", tables_out, lengths_out, uses, copies, shortage, tables, lengths, parents, starts,
+           held)
+    code = _c_cache_advance(tables_out, lengths_out, uses, copies, shortage, tables, lengths, parents, beams, starts, held,
+                            sequences, page_size, pages, max_pages, window, stream)
+    if code:
+        _check(code, "l2c_cache_advance")
+
+
+def cache_copy(cache, copies, count, pages, page_bytes, page_stride=None, groups=1, group_stride=None, stream=None):
+    """Strides and sizes in bytes; pages, and groups of them, follow each other unless the strides say otherwise."""
+    _takes("cache_copy", "int32", copies)
+    page = page_bytes if page_stride is None else page_stride
+    code = _c_cache_copy(cache, copies, count, pages, groups, pages * page if group_stride is None else group_stride, page,
+                         page_bytes, stream)
+    if code:
+        _check(code, "l2c_cache_copy")
 
 
 def launch_shape(op, batch, cols, rows, variant=0):

@@ -38,6 +38,10 @@
  *                 no kernels in the reference: the norms around a block with its
  *                 residual, the product of 4-bit operands and the beam-search form
  *                 of the decoder's step
+ *   l2c_cache_advance, l2c_cache_copy, l2c_cache_append, l2c_cache_attention,
+ *   l2c_decoder_logprobs
+ *                 no kernels in the reference: a cache in pages that beams share, the
+ *                 attention over it, and the log probabilities of given tokens
  */
 #ifndef L2C_H
 #define L2C_H
@@ -64,10 +68,11 @@ enum l2c_qformat {
                       fp32 scale per row: scales[r] */
 };
 
-/* Element types of l2c_residual_rmsnorm's tensors. */
+/* Element types of l2c_residual_rmsnorm's tensors (fp32, bf16) and of a cache's pages (bf16, e4m3). */
 enum l2c_type {
   L2C_F32 = 0,
-  L2C_BF16 = 1 /* uint16 bit patterns */
+  L2C_BF16 = 1, /* uint16 bit patterns */
+  L2C_E4M3 = 2  /* e4m3 codes (OCP, as L2C_Q_FP8's), one byte each */
 };
 
 /*
@@ -385,6 +390,122 @@ int l2c_decoder_beam_select(float *scores_out, int *tokens_out, int *parents, in
 int l2c_decoder_beam_reorder(void *out, const void *in, const int *parents, int beams, int batch,
                              int groups, int pieces, long long group_stride, long long row_stride,
                              long long piece_stride, long long piece_bytes, hipStream_t stream);
+
+/*
+ * The log probabilities of given tokens, for b < rows, with x = logits[b], m its maximum and
+ * Z = sum_v exp(x[v] - m):
+ *   logprobs[b] = x[tokens[b]] - m - log Z
+ *   entropies[b] = log Z - sum_v exp(x[v] - m) (x[v] - m) / Z
+ *   top_tokens[b * top + i], top_logprobs[b * top + i]: the i-th largest logit's token and log
+ *     probability, i < top (0 to L2C_MAX_ALTERNATIVES), equal logits in the order of their tokens
+ * logprobs and tokens may be NULL together, entropies alone; top_tokens and top_logprobs are not
+ * looked at if top is 0.
+ * A token outside [0, vocab) has log probability NaN. A logit of -Inf has log probability -Inf,
+ * adds nothing to Z or the entropy and is no alternative; where fewer than `top` alternatives are
+ * left, the others are token -1 with log probability -Inf. A row that holds a NaN or a +Inf or
+ * nothing but -Inf has log probabilities and entropy NaN, and tokens -1.
+ * Exponentials are fp32, sums of more than 32 of them and everything after them 64-bit; results
+ * are rounded once (a log probability below fp32's lowest number to -Inf). logits: 4-byte
+ * aligned. workspace: 16-byte aligned (may be NULL if the size below is 0), at least
+ * l2c_decoder_logprobs_workspace_bytes, which is 0 for sizes that are not supported and at most
+ * rows * ceil(vocab / 1024) * (8 * top + 32); its contents need not be kept between calls, and
+ * calls that share one must be ordered.
+ */
+#define L2C_MAX_ALTERNATIVES 32
+size_t l2c_decoder_logprobs_workspace_bytes(int vocab, int top, int rows);
+int l2c_decoder_logprobs(float *logprobs, float *entropies, int *top_tokens, float *top_logprobs, const float *logits,
+                         const int *tokens, int vocab, int top, int rows, void *workspace, size_t workspace_bytes,
+                         hipStream_t stream);
+
+/*
+ * A cache of keys and values in pages, for one layer:
+ *   keys, values [pages][kv_heads][page_size][width]: bf16 (cache_type L2C_BF16), or e4m3 codes
+ *     (L2C_E4M3) with one fp32 scale for every row of `width` codes, key_scales and value_scales
+ *     [pages][kv_heads][page_size]: the cached value is code * scale. Scales are not looked at
+ *     with bf16 pages.
+ *   tables [sequences][max_pages]: position j of sequence s lies in page
+ *     tables[s][j / page_size], in its row j % page_size. An entry outside [0, pages) is no
+ *     page: nothing is written there, and no token attends to its positions.
+ *   lengths [sequences]: the positions of every sequence, the newest tokens' among them
+ *     (below 1: none). Positions past max_pages pages are treated as those without a page.
+ *   starts [sequences + 1], not falling: the newest tokens of sequence s are rows starts[s] to
+ *     starts[s + 1] - 1 of the call's `rows` rows (of q, k, v, out), the last one at position
+ *     lengths[s] - 1, the one before at lengths[s] - 2, and so on. Rows of no sequence (from
+ *     starts[sequences] on, say) are neither read nor written, and rows at positions below 0 are
+ *     in no page. starts NULL: one new token of each sequence, row s (rows == sequences).
+ * width: a multiple of 8, at most L2C_MAX_HEAD. page_size: any from 1 on, max_pages * page_size
+ * below 2^31. Strides are in values between two rows, at least the rows' own length; bf16 rows
+ * hold their heads after each other. keys, values, q, k, v and out are 16-byte aligned, their
+ * strides multiples of 8. tables, lengths and starts are read on the device: a call can be
+ * captured, and replayed as they change.
+ *
+ * l2c_cache_append: writes the new tokens' rows k and v (bf16, kv_heads * width values every
+ *   k_stride and v_stride) into their pages. With e4m3 pages as l2c_quantize_fp8 does it: scale =
+ *   max |x| / 448 over the row's `width` values (1 if that is 0), code = e4m3(x / scale), nearest,
+ *   ties to even, saturating at 448; a row with an Inf or a NaN gets scale NaN and zero codes. Two
+ *   tokens of one call must not lie in the same row of the same page.
+ *
+ * l2c_cache_attention: for every new token, at position p, and head h, with the keys k_j and values
+ *   v_j of head h / (heads / kv_heads):
+ *     out[row][h] = sum_j softmax_j(scale * q[row][h] . k_j) v_j
+ *   over the positions j <= p that have a page, and j > p - window unless window is 0. Whatever the
+ *   other positions hold has no part in it. Where no position is left, or every score is -Inf, out
+ *   is 0. q and out: bf16, heads * width values every q_stride and out_stride. Scores, maxima, sums
+ *   and out are fp32 until out is rounded once, to nearest even; the exponentials are rounded to
+ *   bf16 (at most 2^-8 of each, times the value's scale with e4m3 pages) for the product with the values.
+ *   out overlaps none of the inputs. workspace: 16-byte aligned (may be NULL if the size below is 0),
+ *   at least l2c_cache_attention_workspace_bytes, which is 0 for sizes that are not supported and at
+ *   most 2^19 * (width + 2); its contents need not be kept between calls, and calls that share one
+ *   must be ordered.
+ */
+#define L2C_MAX_HEAD 256
+int l2c_cache_append(void *keys, void *values, float *key_scales, float *value_scales, int cache_type,
+                     const uint16_t *k, long long k_stride, const uint16_t *v, long long v_stride, const int *tables,
+                     const int *lengths, const int *starts, int sequences, int rows, int kv_heads, int width,
+                     int page_size, int pages, int max_pages, hipStream_t stream);
+size_t l2c_cache_attention_workspace_bytes(int sequences, int rows, int heads, int kv_heads, int width, int page_size,
+                                           int max_pages);
+int l2c_cache_attention(uint16_t *out, long long out_stride, const uint16_t *q, long long q_stride, const void *keys,
+                        const void *values, const float *key_scales, const float *value_scales, int cache_type,
+                        const int *tables, const int *lengths, const int *starts, int sequences, int rows, int heads,
+                        int kv_heads, int width, int page_size, int pages, int max_pages, int window, float scale,
+                        void *workspace, size_t workspace_bytes, hipStream_t stream);
+
+/*
+ * l2c_cache_advance: a step of the tables of all sequences that use a set of pages. Sequence r
+ *   becomes what its parent was, with room for n_r more tokens, n_r = starts[r + 1] - starts[r] (or
+ *   1 with starts NULL; below 0 counts as 0). The parent is r itself with parents NULL, else sequence
+ *   r - r % beams + parents[r], as l2c_decoder_beam_select leaves them (sequences a multiple of
+ *   beams); a parent outside [0, beams) ends the sequence: it has length 0, n_r = 0 and no pages.
+ *     lengths_out[r] = lengths[parent] + n_r                     (lengths below 0 count as 0)
+ *     tables_out[r]: the parent's first ceil(lengths[parent] / page_size) entries, then new pages up
+ *       to ceil(lengths_out[r] / page_size), then -1.
+ *   With a window, entries whose positions are all below lengths[parent] - window + 1 become -1: none
+ *   of the new tokens attends to them. A sequence whose new tokens begin within a page that
+ *   something else names too (another entry of tables_out, or `held`) gets a new page in its place;
+ *   but if everything that names it is a sequence with new tokens there, and it is not held, the
+ *   first of these keeps it. copies[2 r], copies[2 r + 1] are that page and the new one, for
+ *   l2c_cache_copy, or -1, -1.
+ *   New pages are those that no entry of tables_out names and `held` (NULL: none) is 0 for, the
+ *   lowest first, given out in the order of the sequences and of their entries. So a page is free as
+ *   soon as no table names it. uses[page] is the number of entries of tables_out that name the page.
+ *   *shortage is the number of new pages that there were none for, or no entry (beyond max_pages):
+ *   their entries are -1, and such a sequence has lost what it would have kept there. A caller that
+ *   keeps as many pages as the sequences can need finds it 0.
+ *   The outputs overlap nothing, but tables_out may be tables and lengths_out lengths if parents is
+ *   NULL.
+ * l2c_cache_copy: for g < groups and i < count with both numbers within [0, pages) and not equal, the
+ *   page_bytes bytes of page copies[2 i + 1] become those of page copies[2 i]:
+ *     cache[g * group_stride + copies[2 i + 1] * page_stride] = cache[g * group_stride + copies[2 i] * page_stride]
+ *   Strides in bytes, at least the extent of what they separate; groups are layers, say, or keys and
+ *   values. No page that one pair writes may be in another pair. Any alignment (16-byte addresses
+ *   and strides are fastest).
+ */
+int l2c_cache_advance(int *tables_out, int *lengths_out, int *uses, int *copies, int *shortage, const int *tables,
+                      const int *lengths, const int *parents, int beams, const int *starts, const int *held,
+                      int sequences, int page_size, int pages, int max_pages, int window, hipStream_t stream);
+int l2c_cache_copy(void *cache, const int *copies, int count, int pages, int groups, long long group_stride,
+                   long long page_stride, long long page_bytes, hipStream_t stream);
 
 /*
  * bytes from device memory `src` to pinned host memory `host_dst`

@@ -1,4 +1,14 @@
 // Attention of new tokens over a cache in pages (include/l2c.h has the formula).
+//
+// The rows of a tile are (token, query head of one key head) pairs, packed token by token: all of
+// them read the same keys and values, once. One pass over the positions, with the running maximum m
+// and sum l of a softmax in base 2: with S = scale log2(e) q.k and p = 2^(S - m), a larger maximum m'
+// multiplies l and the sum of p v by 2^(m - m').
+//
+// Everything is computed transposed, S^T = K Q^T and O^T = V^T P^T: a lane of the matrix
+// instructions' results then has one query and several positions, so that maxima and sums run
+// within lanes, and p is in the lanes and the order in which the second product wants it as an
+// operand; only V has to be transposed, which the LDS does as it is read.
 #include <type_traits>
 
 #include "l2c_cache.h"
@@ -9,92 +19,234 @@ using l2c::Sequences;
 
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / L2C_WAVE;
+constexpr float kLog2e = 1.44269504088896340736f;
 
 struct Attention {
   uint16_t *out;
   const uint16_t *q;
   const void *keys, *values;
   const float *key_scales, *value_scales;
+  float *part_values;  // [row][head][split][width]
+  float2 *part_sums;   // [row][head][split]: maximum and sum
   long long out_stride, q_stride;
   Sequences s;
-  int heads, kv_heads, width, window;
-  float scale;
+  l2c::Quotient31 by_group;
+  int heads, kv_heads, group, width, window, splits, slots;
+  float scale;  // times log2(e)
 };
 
-// Eight cached values as fp32, without their row's scale.
-template <bool E4M3>
-__device__ __forceinline__ void load8(float (&v)[8], const void *cache, size_t at) {
-  if constexpr (E4M3) {
-    const u32x2 q = *reinterpret_cast<const u32x2 *>(static_cast<const uint8_t *>(cache) + at);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const bf16x2 low = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q[i], 1.0f, false);
-      const bf16x2 high = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q[i], 1.0f, true);
-      v[4 * i] = static_cast<float>(low[0]), v[4 * i + 1] = static_cast<float>(low[1]);
-      v[4 * i + 2] = static_cast<float>(high[0]), v[4 * i + 3] = static_cast<float>(high[1]);
-    }
+// ---------------------------------------------------------------------------
+// Which rows and positions a workgroup has.
+
+struct Tile {
+  int sequence, first, count;  // packed rows first .. first + count - 1 of the sequence's new tokens
+  int start;                   // row of its first new token
+  long long before;            // position of that
+  int begin, end;              // positions that any row of the tile sees
+  int chunk, parts;            // positions a part, parts that are not empty (at least 1)
+
+  __device__ __forceinline__ int position(const Attention &a, int packed) const {  // -1: none
+    const long long p = before + a.by_group(packed);
+    return p < -1 ? -1 : p > INT_MAX ? INT_MAX : static_cast<int>(p);
+  }
+  __device__ __forceinline__ int row(const Attention &a, int packed) const { return start + a.by_group(packed); }
+  __device__ __forceinline__ int head(const Attention &a, int kv, int packed) const {
+    return kv * a.group + (packed - a.by_group(packed) * a.group);
+  }
+};
+
+// The parts of a tile's positions: no shorter than 4 STEP, in whole STEPs from the
+// first one's.
+template <int STEP, int LEAST>
+__device__ __forceinline__ void divide(const Attention &a, Tile &t) {
+  const int last = t.position(a, t.first + t.count - 1), low = t.position(a, t.first);
+  t.end = min(last, a.s.capacity() - 1) + 1;
+  t.begin = a.window ? max(0, static_cast<int>(max(0LL, static_cast<long long>(low) - a.window + 1))) / STEP * STEP : 0;
+  const int n = max(0, t.end - t.begin);
+  const int each = (n + a.splits - 1) / a.splits;
+  t.chunk = max((each + STEP - 1) / STEP * STEP, LEAST);
+  t.parts = max(1, (n + t.chunk - 1) / t.chunk);
+}
+
+// Tile `slot` of all. With starts sequence s has the slots from starts[s] group / M + s on, enough of
+// them for its rows: some are empty, but where they begin needs no sum over the sequences before.
+template <int M>
+__device__ __forceinline__ bool tile_of(const Attention &a, int slot, Tile &t) {
+  int n;
+  if (!a.s.starts) {
+    const int each = (a.group + M - 1) / M;
+    t.sequence = slot / each;
+    t.first = (slot - t.sequence * each) * M;
+    t.start = t.sequence;
+    t.before = static_cast<long long>(a.s.lengths[t.sequence]) - 1;
+    n = a.group;
   } else {
-    const u32x4 q = *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(cache) + at);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[2 * i] = __uint_as_float(q[i] << 16);
-      v[2 * i + 1] = __uint_as_float(q[i] & 0xffff0000u);
+    // The last sequence whose slots begin at or before this one: the lanes look at 64 at a time.
+    const int lane = threadIdx.x % L2C_WAVE;
+    int low = 0, count = a.s.sequences;
+    while (true) {
+      const int each = (count + L2C_WAVE - 1) / L2C_WAVE, s = low + lane * each;
+      bool reached = false;
+      if (lane * each < count)
+        reached = static_cast<long long>(a.s.starts[s]) * a.group / M + s <= slot;
+      const int reaches = __popcll(__ballot(reached));
+      if (reaches > 1) low += (reaches - 1) * each;
+      if (each == 1) break;
+      count = min(each, a.s.sequences - low);
     }
+    t.sequence = __builtin_amdgcn_readfirstlane(low);
+    const int from = a.s.starts[t.sequence], to = a.s.starts[t.sequence + 1];
+    const long long tile = slot - (static_cast<long long>(from) * a.group / M + t.sequence);
+    // Of starts that are not in order any answer will do, within the arrays.
+    if (from < 0 || to > a.s.rows || from >= to || tile < 0) return false;
+    const long long packed = static_cast<long long>(to - from) * a.group;
+    if (packed > INT_MAX || tile * M >= packed) return false;
+    n = static_cast<int>(packed);
+    t.first = static_cast<int>(tile) * M;
+    t.start = from;
+    t.before = static_cast<long long>(a.s.lengths[t.sequence]) - (to - from);
+  }
+  t.count = min(M, n - t.first);
+  return true;
+}
+
+// ---------------------------------------------------------------------------
+// Pieces.
+
+__device__ __forceinline__ unsigned pack2(float a, float b) {
+  const f32x2 v = {a, b};
+  return __builtin_bit_cast(unsigned, __builtin_convertvector(v, bf16x2));
+}
+
+// Eight e4m3 codes as bf16, exactly.
+__device__ __forceinline__ u32x4 widen(u32x2 c) {
+  u32x4 v;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    v[2 * i] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[i], 1.0f, false));
+    v[2 * i + 1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[i], 1.0f, true));
+  }
+  return v;
+}
+
+template <bool E4M3>
+using Raw = std::conditional_t<E4M3, u32x2, u32x4>;
+
+// Eight cached values as they lie there, and as bf16.
+template <bool E4M3>
+__device__ __forceinline__ Raw<E4M3> load_raw(const void *cache, size_t at) {
+  if constexpr (E4M3) return *reinterpret_cast<const u32x2 *>(static_cast<const uint8_t *>(cache) + at);
+  else return *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(cache) + at);
+}
+__device__ __forceinline__ u32x4 as_bf16(u32x2 c) { return widen(c); }
+__device__ __forceinline__ u32x4 as_bf16(u32x4 c) { return c; }
+
+__device__ __forceinline__ bool not_finite(u32x4 v) {
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) bad |= (v[i] & 0x7f80u) == 0x7f80u || (v[i] & 0x7f800000u) == 0x7f800000u;
+  return bad;
+}
+__device__ __forceinline__ bool not_finite(float v) { return !(fabsf(v) <= FLT_MAX); }
+
+// Values across lanes without a trip through LDS: of both lanes that differ in bit 5, or bit 4.
+__device__ __forceinline__ float max_halves(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_halves(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float max_rows(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_rows(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+__device__ __forceinline__ float exp2_of(float v) { return __builtin_amdgcn_exp2f(v); }
+
+// What is stored for `head` of `row`: the result, or one part of it.
+__device__ __forceinline__ size_t part_of(const Attention &a, int row, int head, int split) {
+  return (static_cast<size_t>(row) * a.heads + head) * a.splits + split;
+}
+__device__ __forceinline__ float inverse(float total) { return total == 0.0f ? 0.0f : 1.0f / total; }
+
+// Four values of a row's head, from column d on.
+__device__ __forceinline__ void store4(const Attention &a, bool whole, int row, int head, int split, int d, f32x4 v) {
+  if (whole) {
+    const u32x2 packed = {pack2(v[0], v[1]), pack2(v[2], v[3])};
+    *reinterpret_cast<u32x2 *>(a.out + row * a.out_stride + static_cast<size_t>(head) * a.width + d) = packed;
+  } else {
+    *reinterpret_cast<f32x4 *>(a.part_values + part_of(a, row, head, split) * a.width + d) = v;
   }
 }
 
-// A wave a row and head: 64 positions at a time, a lane's score each; then the lanes have
-// values' columns, and go through the positions.
+// One row by one wave, a position a lane and then a column a lane: no product reads a value that the row
+// does not see, whatever that is. For the rare tile that has a value that is not finite where
+// some of its rows see it and some do not (0 times it would be NaN in the matrix product).
 template <bool E4M3>
-__global__ __launch_bounds__(L2C_WAVE) void attention_kernel(Attention a) {
-  __shared__ float q[L2C_MAX_HEAD];
-  const int row = blockIdx.x, head = blockIdx.y, lane = threadIdx.x;
-  int sequence, position;
-  if (!a.s.find(row, sequence, position)) return;
-  const int kv = head / (a.heads / a.kv_heads);
+__device__ __forceinline__ void lone_row(const Attention &a, const Tile &t, int kv, int packed, int split, int begin,
+                                         int end, float *q) {
+  const int lane = threadIdx.x % L2C_WAVE;
+  const int row = t.row(a, packed), head = t.head(a, kv, packed), position = t.position(a, packed);
   for (int i = lane; i < a.width; i += L2C_WAVE)
     q[i] = __uint_as_float(
         static_cast<unsigned>(a.q[row * a.q_stride + static_cast<size_t>(head) * a.width + i]) << 16);
-  __syncthreads();
-  const int end = min(position, a.s.capacity() - 1);
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  const int last = min(position, end - 1);
   float top = -INFINITY, total = 0.0f, acc[L2C_MAX_HEAD / L2C_WAVE] = {};
-  const int begin = a.window ? max(0, position - a.window + 1) : 0;
-  for (int first = begin; first <= end; first += L2C_WAVE) {
+  const int from = a.window ? max(begin, position - a.window + 1) : begin;
+  for (int first = from; first <= last; first += L2C_WAVE) {
     const int j = first + lane;
-    float score = -INFINITY;
+    float score = -INFINITY, value_scale = 1.0f;
     size_t at = 0;
     bool there = false;
-    if (j <= end) {
-      const int index = a.s.by_page(j), page = a.s.page(sequence, index);
+    if (j <= last) {
+      const int index = a.s.by_page(j), page = a.s.page(t.sequence, index);
       if (a.s.is_page(page)) {
         there = true;
         at = (static_cast<size_t>(page) * a.kv_heads + kv) * a.s.page_size + (j - index * a.s.page_size);
         float dot = 0.0f;
         for (int i = 0; i < a.width; i += 8) {
-          float k[8];
-          load8<E4M3>(k, a.keys, at * a.width + i);
+          const u32x4 k = as_bf16(load_raw<E4M3>(a.keys, at * a.width + i));
 #pragma unroll
-          for (int e = 0; e < 8; ++e) dot = fmaf(q[i + e], k[e], dot);
+          for (int e = 0; e < 4; ++e) {
+            dot = fmaf(q[i + 2 * e], __uint_as_float(k[e] << 16), dot);
+            dot = fmaf(q[i + 2 * e + 1], __uint_as_float(k[e] & 0xffff0000u), dot);
+          }
         }
-        if (E4M3) dot *= a.key_scales[at];
+        if (E4M3) dot *= a.key_scales[at], value_scale = a.value_scales[at];
         score = dot * a.scale;
       }
     }
     const float most = fmaxf(top, l2c::wave_max(score));
     const float shift = most == -INFINITY ? 0.0f : most;
-    const float p = !there ? 0.0f : expf(score - shift), again = expf(top - shift);
+    float p = there ? exp2_of(score - shift) : 0.0f;
+    const float again = exp2_of(top - shift);
     total = total * again + l2c::wave_sum(p);
     top = most;
+    p = __uint_as_float(pack2(p * value_scale, 0.0f) << 16);
 #pragma unroll
     for (int c = 0; c < L2C_MAX_HEAD / L2C_WAVE; ++c) acc[c] *= again;
-    for (int i = 0; i < L2C_WAVE && first + i <= end; ++i) {
+    for (int i = 0; i < L2C_WAVE && first + i <= last; ++i) {
       if (!__shfl(static_cast<int>(there), i, L2C_WAVE)) continue;
-      float w = __shfl(p, i, L2C_WAVE);
-      const size_t from = (static_cast<size_t>(static_cast<unsigned>(__shfl(static_cast<int>(at >> 32), i, L2C_WAVE))) << 32) |
-                          static_cast<unsigned>(__shfl(static_cast<int>(at), i, L2C_WAVE));
-      if (E4M3) w *= a.value_scales[from];
+      const float w = __shfl(p, i, L2C_WAVE);
+      const size_t of = (static_cast<size_t>(static_cast<unsigned>(__shfl(static_cast<int>(at >> 32), i, L2C_WAVE))) << 32) |
+                        static_cast<unsigned>(__shfl(static_cast<int>(at), i, L2C_WAVE));
 #pragma unroll
       for (int c = 0; c < L2C_MAX_HEAD / L2C_WAVE; ++c) {
         const int d = c * L2C_WAVE + lane;
@@ -102,26 +254,587 @@ __global__ __launch_bounds__(L2C_WAVE) void attention_kernel(Attention a) {
         float v;
         if constexpr (E4M3)
           v = static_cast<float>(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(
-              static_cast<const uint8_t *>(a.values)[from * a.width + d], 1.0f, false)[0]);
+              static_cast<const uint8_t *>(a.values)[of * a.width + d], 1.0f, false)[0]);
         else
-          v = __uint_as_float(static_cast<unsigned>(static_cast<const uint16_t *>(a.values)[from * a.width + d]) << 16);
+          v = __uint_as_float(static_cast<unsigned>(static_cast<const uint16_t *>(a.values)[of * a.width + d]) << 16);
         acc[c] = fmaf(w, v, acc[c]);
       }
     }
   }
+  const bool whole = t.parts == 1;
+  const size_t part = part_of(a, row, head, split);
 #pragma unroll
   for (int c = 0; c < L2C_MAX_HEAD / L2C_WAVE; ++c) {
     const int d = c * L2C_WAVE + lane;
     if (d >= a.width) continue;
-    const f32x2 o = {total == 0.0f ? 0.0f : acc[c] / total, 0.0f};
-    a.out[row * a.out_stride + static_cast<size_t>(head) * a.width + d] =
-        __builtin_bit_cast(unsigned, __builtin_convertvector(o, bf16x2)) & 0xffffu;
+    if (whole)
+      a.out[row * a.out_stride + static_cast<size_t>(head) * a.width + d] =
+          static_cast<uint16_t>(pack2(total == 0.0f ? 0.0f : acc[c] / total, 0.0f));
+    else a.part_values[part * a.width + d] = acc[c];
   }
+  if (!whole && lane == 0) a.part_sums[part] = make_float2(top, total);
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// Where 16 bytes (`chunk`) of row `key` lie in a tile of values in LDS. Lanes that write
+// together have eight keys and one chunk, lanes that read together the same 32 bytes of four keys: the
+// chunk's lower bits are exchanged so that neither meet in a bank.
+template <int D>
+__device__ __forceinline__ int value_place(int key, int chunk) {
+  const int f = ((key & 3) << 1 | (key >> 2 & 1)) & (D / 8 - 1);
+  return key * D + 8 * (chunk ^ f);
+}
+
+typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+
+// Four keys of a column: lanes l of 16 point to keys l / 4 and columns 4 (l % 4), and get column l.
+__device__ __forceinline__ u32x2 read_column(const uint16_t *at) {
+  return __builtin_bit_cast(
+      u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                 (lds_i16x4 *)(const __attribute__((address_space(3))) uint16_t *)at));
+}
+
+// ---------------------------------------------------------------------------
+// Tiles of up to 16 rows: a step of decoding. Bound by the cache's bytes. The four waves
+// of a workgroup go through positions of their own, 32 at a time, and join at the end. Keys go from
+// memory to the matrix instructions' operands (16 x 16 x 32: a lane has eight values of one
+// key), values through LDS of the wave's own, so that nothing waits for another wave.
+
+constexpr int kNarrow = 16, kNarrowStep = 32;
+
+template <int D, bool E4M3>
+__global__ __launch_bounds__(kThreads) void narrow_kernel(Attention a) {
+  constexpr int kChunks = D / 32;  // chunks of eight values a lane and key
+  constexpr int kTiles = D / 16;   // of columns
+  constexpr int kApart = 68;       // floats from row to row of the join
+  constexpr int kValues = D == 64 ? 2 * kNarrow * kApart : kNarrowStep * D;
+  __shared__ __attribute__((aligned(16))) uint16_t values[kWaves][kValues];
+  __shared__ float tops[kWaves][kNarrow], sums[kWaves][kNarrow];
+  __shared__ int dirty[kWaves];
+  const int lane = threadIdx.x % L2C_WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / L2C_WAVE);
+  const int n = lane % 16, g = lane / 16;
+  int block = blockIdx.x;
+  const int kv = block % a.kv_heads;
+  block /= a.kv_heads;
+  const int split = block % a.splits;
+  Tile t;
+  if (!tile_of<kNarrow>(a, block / a.splits, t)) return;
+  divide<kNarrowStep, 4 * kNarrowStep>(a, t);
+  if (split >= t.parts) return;
+  const int begin = t.begin + split * t.chunk, end = min(t.end, begin + t.chunk);
+  const bool mine = n < t.count;
+  const int packed = t.first + (mine ? n : 0);
+  const int row = t.row(a, packed), head = t.head(a, kv, packed);
+  const int position = mine ? t.position(a, packed) : -1;
+  const int lowest = a.window ? position - a.window : -1;  // it sees those above
+  const int every = t.position(a, t.first);                // all rows see positions up to this one
+  const int nobody = a.window ? t.position(a, t.first + t.count - 1) - a.window : -1;  // and those above this one
+
+  bf16x8 q[kChunks];
+#pragma unroll
+  for (int c = 0; c < kChunks; ++c) {
+    const int d = 8 * (4 * c + g);
+    u32x4 v = {0, 0, 0, 0};
+    if (mine && d < a.width)
+      v = *reinterpret_cast<const u32x4 *>(a.q + row * a.q_stride + static_cast<size_t>(head) * a.width + d);
+    q[c] = __builtin_bit_cast(bf16x8, v);
+  }
+
+  // The pages of a step's keys n and 16 + n.
+  auto look_up = [&](int (&page)[2], int base) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int j = base + 16 * u + n;
+      page[u] = j < end ? a.s.page(t.sequence, a.s.by_page(j)) : -1;
+    }
+  };
+  Raw<E4M3> k[2][kChunks], v[2][kChunks];
+  float key_scale[2], value_scale[2];
+  bool there[2];
+  auto load = [&](const int (&page)[2], int base) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int j = base + 16 * u + n, slot = j - a.s.by_page(j) * a.s.page_size;
+      there[u] = a.s.is_page(page[u]);
+      const size_t at = (static_cast<size_t>(static_cast<unsigned>(page[u])) * a.kv_heads + kv) * a.s.page_size + slot;
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) {
+        const int d = 8 * (4 * c + g);
+        k[u][c] = v[u][c] = Raw<E4M3>{};
+        if (there[u] && d < a.width) {
+          k[u][c] = load_raw<E4M3>(a.keys, at * a.width + d);
+          v[u][c] = load_raw<E4M3>(a.values, at * a.width + d);
+        }
+      }
+      if constexpr (E4M3) {
+        key_scale[u] = there[u] ? a.key_scales[at] : 0.0f;
+        value_scale[u] = there[u] ? a.value_scales[at] : 0.0f;
+      }
+    }
+  };
+
+  constexpr int kStride = kWaves * kNarrowStep;
+  f32x4 acc[kTiles];
+#pragma unroll
+  for (int i = 0; i < kTiles; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  float top = -INFINITY, total = 0.0f;
+  bool bad = false;
+  uint16_t *const mine_values = values[wave];
+  int base = begin + wave * kNarrowStep;
+  int page[2];
+  look_up(page, base);
+  load(page, base);
+  look_up(page, base + kStride);
+  for (; base < end; base += kStride) {
+    // Scores: keys 4 g + i of both halves, of query n.
+    f32x4 s[2];
+    bool seen[2][4];
+    float weight[2][4];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      s[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c)
+        s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, as_bf16(k[u][c])), q[c], s[u], 0, 0, 0);
+      const unsigned pages = static_cast<unsigned>(__ballot(there[u])) >> (4 * g);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int j = base + 16 * u + 4 * g + i;
+        seen[u][i] = (pages >> i & 1) && j <= position && j > lowest;
+        float x = s[u][i];
+        weight[u][i] = 1.0f;
+        if constexpr (E4M3) {
+          x *= __shfl(key_scale[u], 4 * g + i, L2C_WAVE);
+          weight[u][i] = __shfl(value_scale[u], 4 * g + i, L2C_WAVE);
+        }
+        s[u][i] = seen[u][i] ? x * a.scale : -INFINITY;
+      }
+    }
+    // Values into LDS; is there one that some rows see and others do not, and that is not finite?
+    const bool mixed = base + kNarrowStep - 1 > every || base <= nobody;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) {
+        const u32x4 w = as_bf16(v[u][c]);
+        if (mixed) bad |= not_finite(w);
+        *reinterpret_cast<u32x4 *>(mine_values + value_place<D>(16 * u + n, 4 * c + g)) = w;
+      }
+    if constexpr (E4M3)
+      if (mixed) bad |= not_finite(value_scale[0]) || not_finite(value_scale[1]);
+    // The next step's, before anything waits for this one's.
+    load(page, base + kStride);
+    look_up(page, base + 2 * kStride);
+    float most = top;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) most = fmaxf(most, s[u][i]);
+    most = max_halves(max_rows(most));
+    const float shift = most == -INFINITY ? 0.0f : most;
+    const float again = exp2_of(top - shift);
+    top = most;
+    total *= again;
+    u32x4 p;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      float e[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        e[i] = exp2_of(s[u][i] - shift);
+        total += e[i];
+        if constexpr (E4M3) e[i] = seen[u][i] ? e[i] * weight[u][i] : 0.0f;
+      }
+      p[2 * u] = pack2(e[0], e[1]), p[2 * u + 1] = pack2(e[2], e[3]);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) {
+      if (16 * i >= a.width) break;
+      const int d = 16 * i + 4 * (n % 4), key = 4 * g + n / 4;
+      const u32x2 low = read_column(mine_values + value_place<D>(key, d / 8) + d % 8);
+      const u32x2 high = read_column(mine_values + value_place<D>(16 + key, d / 8) + d % 8);
+      const u32x4 w = {low[0], low[1], high[0], high[1]};
+      acc[i] *= again;
+      acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w), __builtin_bit_cast(bf16x8, p), acc[i],
+                                                       0, 0, 0);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+  total = sum_halves(sum_rows(total));
+  if (g == 0) tops[wave][n] = top, sums[wave][n] = total;
+  bad = __ballot(bad) != 0;
+  if (lane == 0) dirty[wave] = bad;
+  __syncthreads();
+  bad = false;
+  float most = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    most = fmaxf(most, tops[w][n]);
+    bad |= dirty[w] != 0;
+  }
+  if (bad) {
+    float *const row_q = reinterpret_cast<float *>(values[wave]);
+    for (int r = wave; r < t.count; r += kWaves) lone_row<E4M3>(a, t, kv, t.first + r, split, begin, end, row_q);
+    return;
+  }
+  const float shift = most == -INFINITY ? 0.0f : most;
+  float all = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) all += sums[w][n] * exp2_of(tops[w][n] - shift);
+  const bool whole = t.parts == 1;
+  const float by = exp2_of(top - shift) * (whole ? inverse(all) : 1.0f);
+  // The waves' sums by way of LDS, 64 columns at a time.
+  float *const shared = reinterpret_cast<float *>(&values[0][0]);
+#pragma unroll
+  for (int part = 0; part < D / 64; ++part) {
+    if (64 * part >= a.width) break;
+    if (part > 0) __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      *reinterpret_cast<f32x4 *>(shared + (wave * kNarrow + n) * kApart + 16 * i + 4 * g) = acc[4 * part + i] * by;
+    __syncthreads();
+    // 16 rows of 64 columns by 256 lanes.
+    const int r = threadIdx.x / 16, c = 4 * (threadIdx.x % 16), d = 64 * part + c;
+    if (r < t.count && d < a.width) {
+      f32x4 sum = *reinterpret_cast<const f32x4 *>(shared + r * kApart + c);
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w)
+        sum += *reinterpret_cast<const f32x4 *>(shared + (w * kNarrow + r) * kApart + c);
+      store4(a, whole, t.row(a, t.first + r), t.head(a, kv, t.first + r), split, d, sum);
+    }
+  }
+  if (!whole && wave == 0 && g == 0 && mine) a.part_sums[part_of(a, row, head, split)] = make_float2(most, all);
+}
+
+// ---------------------------------------------------------------------------
+// Tiles of 128 rows, 32 a wave: chunks of a prompt. Bound by the matrix and the vector units. The
+// workgroup's keys and values, 64 positions at a time (32 of more than 128 columns), lie in LDS, two
+// tiles of them: while one is read, the next is on its way in registers.
+
+constexpr int kWide = 128;
+
+template <int D, bool E4M3>
+__global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void wide_kernel(Attention a) {
+  constexpr int kKeys = D <= 128 ? 64 : 32;
+  constexpr int kLanes = D / 8;               // that hold a row as it is loaded
+  constexpr int kRows = kThreads / kLanes;    // rows loaded together
+  constexpr int kPasses = kKeys / kRows;
+  constexpr int kSteps = D / 16, kTiles = D / 32, kParts = kKeys / 32;
+  __shared__ __attribute__((aligned(16))) uint16_t keys[2][kKeys * D], values[2][kKeys * D];
+  __shared__ __attribute__((aligned(16))) float key_scales[2][kKeys], value_scales[2][kKeys];
+  __shared__ int dirty;
+  const int lane = threadIdx.x % L2C_WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / L2C_WAVE);
+  const int n = lane % 32, h = lane / 32;
+  int block = blockIdx.x;
+  const int kv = block % a.kv_heads;
+  block /= a.kv_heads;
+  const int split = block % a.splits;
+  Tile t;
+  // The last tiles of a sequence see the most positions: they come first.
+  if (!tile_of<kWide>(a, a.slots - 1 - block / a.splits, t)) return;
+  divide<kKeys, 4 * kKeys>(a, t);
+  if (split >= t.parts) return;
+  const int begin = t.begin + split * t.chunk, end = min(t.end, begin + t.chunk);
+  const int first = 32 * wave;                       // of the wave's rows
+  const int count = max(0, min(32, t.count - first));  // of them
+  const bool mine = n < count;
+  const int packed = t.first + (mine ? first + n : 0);
+  const int row = t.row(a, packed), head = t.head(a, kv, packed);
+  const int position = mine ? t.position(a, packed) : -1;
+  const int lowest = a.window ? position - a.window : -1;
+  const int every = t.position(a, t.first);  // all rows of the tile see positions up to this one
+  const int nobody = a.window ? t.position(a, t.first + t.count - 1) - a.window : -1;
+  // Of the wave: all rows see positions in (whole_from, whole_to], none those outside [some_from, some_to].
+  const int whole_to = count > 0 ? t.position(a, t.first + first) : -1;
+  const int some_to = count > 0 ? t.position(a, t.first + first + count - 1) : -1;
+  const int whole_from = a.window ? some_to - a.window : -1, some_from = a.window ? whole_to - a.window + 1 : 0;
+  if (threadIdx.x == 0) dirty = 0;
+  __syncthreads();
+
+  bf16x8 q[kSteps];
+#pragma unroll
+  for (int c = 0; c < kSteps; ++c) {
+    const int d = 16 * c + 8 * h;
+    u32x4 v = {0, 0, 0, 0};
+    if (mine && d < a.width)
+      v = *reinterpret_cast<const u32x4 *>(a.q + row * a.q_stride + static_cast<size_t>(head) * a.width + d);
+    q[c] = __builtin_bit_cast(bf16x8, v);
+  }
+
+  // A tile's pages, a key a lane.
+  auto look_up = [&](int base) __attribute__((always_inline)) {
+    const int j = base + lane % kKeys;
+    return j < end ? a.s.page(t.sequence, a.s.by_page(j)) : -1;
+  };
+  const int load_row = threadIdx.x / kLanes, load_chunk = threadIdx.x % kLanes;
+  Raw<E4M3> k[kPasses], v[kPasses];
+  float key_scale = 0.0f, value_scale = 0.0f;
+  auto row_of = [&](int page, int j) __attribute__((always_inline)) {
+    return (static_cast<size_t>(static_cast<unsigned>(page)) * a.kv_heads + kv) * a.s.page_size +
+           (j - a.s.by_page(j) * a.s.page_size);
+  };
+  auto load = [&](int pages, int base) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      const int r = i * kRows + load_row, page = __shfl(pages, r, L2C_WAVE);
+      k[i] = v[i] = Raw<E4M3>{};
+      if (a.s.is_page(page) && 8 * load_chunk < a.width) {
+        const size_t at = row_of(page, base + r) * a.width + 8 * load_chunk;
+        k[i] = load_raw<E4M3>(a.keys, at);
+        v[i] = load_raw<E4M3>(a.values, at);
+      }
+    }
+    if constexpr (E4M3) {
+      key_scale = value_scale = 0.0f;
+      if (a.s.is_page(pages)) {
+        const size_t at = row_of(pages, base + lane % kKeys);
+        key_scale = a.key_scales[at], value_scale = a.value_scales[at];
+      }
+    }
+  };
+  auto key_place = [](int key, int chunk) __attribute__((always_inline)) {
+    const int f = D == 64 ? key >> 1 & 7 : key & 15;
+    return key * D + 8 * (chunk ^ f);
+  };
+
+  f32x16 acc[kTiles];
+#pragma unroll
+  for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[i][e] = 0.0f;
+  float top = -INFINITY, total = 0.0f;
+  int pages = look_up(begin);
+  load(pages, begin);
+  unsigned long long next_there = __ballot(a.s.is_page(pages));
+  pages = look_up(begin + kKeys);
+  int turn = 0;
+  for (int base = begin; base < end; base += kKeys, turn ^= 1) {
+    const unsigned long long there = next_there;
+    const bool mixed = base + kKeys - 1 > every || base <= nobody;
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      const int r = i * kRows + load_row;
+      const u32x4 kk = as_bf16(k[i]), vv = as_bf16(v[i]);
+      if (mixed) bad |= not_finite(vv);
+      *reinterpret_cast<u32x4 *>(keys[turn] + key_place(r, load_chunk)) = kk;
+      *reinterpret_cast<u32x4 *>(values[turn] + value_place<D>(r, load_chunk)) = vv;
+    }
+    if constexpr (E4M3) {
+      if (mixed) bad |= not_finite(value_scale);
+      if (wave == 0 && lane < kKeys) key_scales[turn][lane] = key_scale, value_scales[turn][lane] = value_scale;
+    }
+    if (mixed && __ballot(bad) && lane == 0) dirty = 1;
+    __syncthreads();
+    load(pages, base + kKeys);
+    next_there = __ballot(a.s.is_page(pages));
+    pages = look_up(base + 2 * kKeys);
+    if (base > some_to || base + kKeys - 1 < some_from) continue;
+    // Scores of positions 32 u + 8 (i / 4) + 4 h + i % 4, of query n.
+    f32x16 s[kParts];
+#pragma unroll
+    for (int u = 0; u < kParts; ++u) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[u][e] = 0.0f;
+#pragma unroll
+      for (int c = 0; c < kSteps; ++c) {
+        const u32x4 kk = *reinterpret_cast<const u32x4 *>(keys[turn] + key_place(32 * u + n, 2 * c + h));
+        s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kk), q[c], s[u], 0, 0, 0);
+      }
+    }
+    if constexpr (E4M3) {
+#pragma unroll
+      for (int u = 0; u < kParts; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const f32x4 x = *reinterpret_cast<const f32x4 *>(&key_scales[turn][32 * u + 8 * i + 4 * h]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[u][4 * i + e] *= x[e];
+        }
+    }
+    constexpr unsigned long long kAll = kKeys == 64 ? ~0ull : 0xffffffffull;
+    if (base + kKeys - 1 > whole_to || base <= whole_from || (there & kAll) != kAll || base + kKeys > end) {
+#pragma unroll
+      for (int u = 0; u < kParts; ++u)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int at = 32 * u + 8 * (i / 4) + 4 * h + i % 4, j = base + at;
+          const bool seen = (there >> at & 1) && j <= position && j > lowest;
+          s[u][i] = seen ? s[u][i] * a.scale : -INFINITY;
+        }
+    } else {
+#pragma unroll
+      for (int u = 0; u < kParts; ++u)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[u][i] *= a.scale;
+    }
+    float most = top;
+#pragma unroll
+    for (int u = 0; u < kParts; ++u)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) most = fmaxf(most, s[u][i]);
+    most = max_halves(most);
+    const float shift = most == -INFINITY ? 0.0f : most;
+    if (__ballot(most > top)) {
+      const float again = exp2_of(top - shift);
+      total *= again;
+#pragma unroll
+      for (int i = 0; i < kTiles; ++i) acc[i] *= again;
+      top = most;
+    }
+#pragma unroll
+    for (int u = 0; u < kParts; ++u) {
+      u32x4 p[2];
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        f32x4 x = {1.0f, 1.0f, 1.0f, 1.0f};
+        if constexpr (E4M3) x = *reinterpret_cast<const f32x4 *>(&value_scales[turn][32 * u + 2 * i + 4 * h]);
+        float e[4];
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          e[m] = exp2_of(s[u][i + m] - shift);
+          total += e[m];
+          if constexpr (E4M3) e[m] = s[u][i + m] == -INFINITY ? 0.0f : e[m] * x[m];
+        }
+        p[i / 8][i / 2 % 4] = pack2(e[0], e[1]);
+        p[i / 8][i / 2 % 4 + 1] = pack2(e[2], e[3]);
+      }
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int key = 32 * u + 16 * half + 4 * h + (n % 16) / 4;
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) {
+          if (32 * i >= a.width) break;
+          const int d = 32 * i + 16 * (n / 16) + 4 * (n % 4);
+          const u32x2 low = read_column(values[turn] + value_place<D>(key, d / 8) + d % 8);
+          const u32x2 high = read_column(values[turn] + value_place<D>(key + 8, d / 8) + d % 8);
+          const u32x4 w = {low[0], low[1], high[0], high[1]};
+          acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, w),
+                                                           __builtin_bit_cast(bf16x8, p[half]), acc[i], 0, 0, 0);
+        }
+      }
+    }
+  }
+  __syncthreads();
+  if (dirty) {
+    float *const row_q = reinterpret_cast<float *>(keys[0]) + wave * L2C_MAX_HEAD;
+    static_assert(sizeof(keys) >= kWaves * L2C_MAX_HEAD * sizeof(float), "room for the queries");
+    for (int r = wave; r < t.count; r += kWaves) lone_row<E4M3>(a, t, kv, t.first + r, split, begin, end, row_q);
+    return;
+  }
+  total = sum_halves(total);
+  const bool whole = t.parts == 1;
+  const float by = whole ? inverse(total) : 1.0f;
+  if (!mine) return;
+#pragma unroll
+  for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+      const int d = 32 * i + 8 * m + 4 * h;
+      if (d >= a.width) continue;
+      const f32x4 o = {acc[i][4 * m] * by, acc[i][4 * m + 1] * by, acc[i][4 * m + 2] * by, acc[i][4 * m + 3] * by};
+      store4(a, whole, row, head, split, d, o);
+    }
+  if (!whole && h == 0) a.part_sums[part_of(a, row, head, split)] = make_float2(top, total);
+}
+
+// ---------------------------------------------------------------------------
+// The parts of tiles that were divided: a wave a row and head.
+
+template <int M, int STEP>
+__global__ __launch_bounds__(kThreads) void join_kernel(Attention a) {
+  const int lane = threadIdx.x % L2C_WAVE;
+  const int item = __builtin_amdgcn_readfirstlane(blockIdx.x * kWaves + threadIdx.x / L2C_WAVE);
+  if (item >= a.s.rows * a.heads) return;
+  const int row = item / a.heads, head = item - row * a.heads;
+  int sequence, position;
+  if (!a.s.find(row, sequence, position)) return;
+  Tile t;
+  t.sequence = sequence;
+  t.start = a.s.starts ? a.s.starts[sequence] : row;
+  const int to = a.s.starts ? a.s.starts[sequence + 1] : row + 1;
+  t.before = static_cast<long long>(a.s.lengths[sequence]) - (to - t.start);
+  const int kv = head / a.group, packed = (row - t.start) * a.group + (head - kv * a.group);
+  t.first = packed / M * M;
+  t.count = min(M, (to - t.start) * a.group - t.first);
+  divide<STEP, 4 * STEP>(a, t);
+  if (t.parts == 1) return;  // whole already
+  const size_t first = part_of(a, row, head, 0);
+  // At most 64 parts: a lane each.
+  const float2 sums = lane < t.parts ? a.part_sums[first + lane] : make_float2(-INFINITY, 0.0f);
+  const float most = l2c::wave_max(sums.x);
+  const float weight = lane < t.parts ? exp2_of(sums.x - (most == -INFINITY ? 0.0f : most)) : 0.0f;
+  const float by = inverse(l2c::wave_sum(sums.y * weight));
+  const float *const values = a.part_values + first * a.width;
+  for (int d = 4 * lane; d < a.width; d += 4 * L2C_WAVE) {
+    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = 0; i < t.parts; ++i)
+      sum += *reinterpret_cast<const f32x4 *>(values + static_cast<size_t>(i) * a.width + d) *
+             __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(weight), i));
+    store4(a, true, row, head, 0, d, sum * by);
+  }
+}
+
+// ---------------------------------------------------------------------------
+
+constexpr int kMaxSplits = 64;
+
+struct Plan {
+  bool narrow;
+  long long slots;
+  int splits;
+};
+
+// Tiles of 16 rows where the sequences have no more on average, else of 128. Positions are divided
+// until there are some workgroups for every CU.
+Plan plan(int sequences, int rows, int heads, int kv_heads, int page_size, int max_pages, bool starts) {
+  const int group = heads / kv_heads;
+  const long long packed = static_cast<long long>(rows) * group;
+  Plan p;
+  p.narrow = packed <= 16LL * sequences;
+  const int m = p.narrow ? kNarrow : kWide;
+  p.slots = starts ? packed / m + sequences : static_cast<long long>(sequences) * ((group + m - 1) / m);
+  const long long tiles = p.slots * kv_heads, wanted = p.narrow ? 2048 : 1024;
+  const long long least = p.narrow ? 4 * kNarrowStep : 256;
+  long long splits = wanted / tiles;
+  splits = min(splits, (static_cast<long long>(max_pages) * page_size + least - 1) / least);
+  splits = min(splits, (1LL << 17) / (static_cast<long long>(rows) * heads));
+  p.splits = static_cast<int>(max(1LL, min(splits, static_cast<long long>(kMaxSplits))));
+  return p;
+}
+
+bool sizes(int sequences, int rows, int heads, int kv_heads, int width, int page_size, int pages, int max_pages) {
+  return l2c::cache_sizes(L2C_BF16, sequences, rows, kv_heads, width, page_size, pages, max_pages) && heads > 0 &&
+         heads <= 65535 && heads % kv_heads == 0;
+}
+
+using Kernel = void (*)(Attention);
+template <int D>
+Kernel kernel(bool narrow, bool e4m3) {
+  return narrow ? (e4m3 ? narrow_kernel<D, true> : narrow_kernel<D, false>)
+                : (e4m3 ? wide_kernel<D, true> : wide_kernel<D, false>);
+}
+
+size_t part_bytes(const Plan &p, int rows, int heads, int width) {
+  return p.splits == 1 ? 0 : static_cast<size_t>(rows) * heads * p.splits * (width + 2) * sizeof(float);
 }
 
 }  // namespace
 
-extern "C" size_t l2c_cache_attention_workspace_bytes(int, int, int, int, int, int, int) { return 0; }
+extern "C" size_t l2c_cache_attention_workspace_bytes(int sequences, int rows, int heads, int kv_heads, int width,
+                                                      int page_size, int max_pages) {
+  if (!sizes(sequences, rows, heads, kv_heads, width, page_size, 0, max_pages) || sequences == 0 || rows == 0) return 0;
+  // What a call with starts needs, or without: the fewer slots, the more parts.
+  const size_t with = part_bytes(plan(sequences, rows, heads, kv_heads, page_size, max_pages, true), rows, heads, width);
+  const size_t without = rows != sequences
+                             ? 0
+                             : part_bytes(plan(sequences, rows, heads, kv_heads, page_size, max_pages, false), rows, heads, width);
+  return with > without ? with : without;
+}
 
 extern "C" int l2c_cache_attention(uint16_t *out, long long out_stride, const uint16_t *q, long long q_stride,
                                    const void *keys, const void *values, const float *key_scales,
@@ -129,23 +842,45 @@ extern "C" int l2c_cache_attention(uint16_t *out, long long out_stride, const ui
                                    const int *starts, int sequences, int rows, int heads, int kv_heads, int width,
                                    int page_size, int pages, int max_pages, int window, float scale, void *workspace,
                                    size_t workspace_bytes, hipStream_t stream) {
-  if (!l2c::cache_sizes(cache_type, sequences, rows, kv_heads, width, page_size, pages, max_pages) || heads <= 0 ||
-      heads > 65535 || heads % kv_heads != 0 || window < 0)
+  if (!sizes(sequences, rows, heads, kv_heads, width, page_size, pages, max_pages) || window < 0 ||
+      (cache_type != L2C_BF16 && cache_type != L2C_E4M3))
     return hipErrorInvalidValue;
   const long long row = static_cast<long long>(heads) * width;
   if (q_stride < row || out_stride < row || q_stride % 8 != 0 || out_stride % 8 != 0) return hipErrorInvalidValue;
   if (sequences == 0 || rows == 0) return hipSuccess;
+  const size_t need = l2c_cache_attention_workspace_bytes(sequences, rows, heads, kv_heads, width, page_size, max_pages);
   if (!l2c::cache_arguments(cache_type, keys, values, key_scales, value_scales, tables, lengths, starts, sequences,
                             rows) ||
-      !q || !out || !l2c_aligned16(q) || !l2c_aligned16(out) ||
-      workspace_bytes < l2c_cache_attention_workspace_bytes(sequences, rows, heads, kv_heads, width, page_size, max_pages))
+      !q || !out || !l2c_aligned16(q) || !l2c_aligned16(out) || workspace_bytes < need ||
+      (need > 0 && (!workspace || !l2c_aligned16(workspace))))
     return hipErrorInvalidValue;
-  if (!l2c::launchable(static_cast<long long>(rows) * heads, L2C_WAVE)) return hipErrorInvalidValue;
-  const Attention a = {out, q, keys, values, key_scales, value_scales, out_stride, q_stride,
-                       l2c::sequences_of(tables, lengths, starts, sequences, rows, max_pages, page_size, pages),
-                       heads, kv_heads, width, window, scale};
-  auto fn = cache_type == L2C_BF16 ? attention_kernel<false> : attention_kernel<true>;
-  hipLaunchKernelGGL(fn, dim3(rows, heads), dim3(L2C_WAVE), 0, stream, a);
+  const Plan p = plan(sequences, rows, heads, kv_heads, page_size, max_pages, starts != nullptr);
+  const long long grid = p.slots * kv_heads * p.splits;
+  if (static_cast<long long>(rows) * heads > INT_MAX || p.slots > INT_MAX || grid > INT_MAX ||
+      !l2c::launchable(grid, kThreads))
+    return hipErrorInvalidValue;
+  float *const parts = static_cast<float *>(workspace);
+  const size_t items = static_cast<size_t>(rows) * heads * p.splits;
+  Attention a = {};
+  a.out = out, a.q = q, a.keys = keys, a.values = values, a.key_scales = key_scales, a.value_scales = value_scales;
+  a.part_values = parts, a.part_sums = reinterpret_cast<float2 *>(parts + (p.splits > 1 ? items * width : 0));
+  a.out_stride = out_stride, a.q_stride = q_stride;
+  a.s = l2c::sequences_of(tables, lengths, starts, sequences, rows, max_pages, page_size, pages);
+  a.group = heads / kv_heads, a.by_group = l2c::Quotient31(a.group);
+  a.heads = heads, a.kv_heads = kv_heads, a.width = width, a.window = window;
+  a.splits = p.splits, a.slots = static_cast<int>(p.slots), a.scale = scale * kLog2e;
+  const bool e4m3 = cache_type == L2C_E4M3;
+  const Kernel fn = width <= 64    ? kernel<64>(p.narrow, e4m3)
+                    : width <= 128 ? kernel<128>(p.narrow, e4m3)
+                                   : kernel<256>(p.narrow, e4m3);
+  hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, stream, a);
+  L2C_LAUNCH_CHECK();
+  if (p.splits == 1) return hipSuccess;
+  const Kernel join = p.narrow      ? join_kernel<kNarrow, kNarrowStep>
+                      : width <= 128 ? join_kernel<kWide, 64>
+                                     : join_kernel<kWide, 32>;
+  const unsigned joins = static_cast<unsigned>((static_cast<long long>(rows) * heads + kWaves - 1) / kWaves);
+  hipLaunchKernelGGL(join, dim3(joins), dim3(kThreads), 0, stream, a);
   L2C_LAUNCH_CHECK();
   return hipSuccess;
 }

@@ -25,6 +25,9 @@ struct Quotient31 {
   }
 };
 
+// Positions that tables may have room for: with some to spare below 2^31, loops may step past the last.
+constexpr long long kMostPositions = 0x7fff0000LL;
+
 struct Sequences {
   const int *tables, *lengths, *starts;
   int sequences, rows, max_pages, page_size, pages;
@@ -73,7 +76,7 @@ inline bool cache_sizes(int cache_type, int sequences, int rows, int kv_heads, i
                         int max_pages) {
   return (cache_type == L2C_BF16 || cache_type == L2C_E4M3) && sequences >= 0 && rows >= 0 && kv_heads > 0 &&
          kv_heads <= 65535 && width > 0 && width <= L2C_MAX_HEAD && width % 8 == 0 && page_size > 0 && pages >= 0 &&
-         max_pages >= 0 && static_cast<long long>(max_pages) * page_size <= INT_MAX;
+         max_pages >= 0 && static_cast<long long>(max_pages) * page_size <= kMostPositions;
 }
 inline Sequences sequences_of(const int *tables, const int *lengths, const int *starts, int sequences, int rows,
                               int max_pages, int page_size, int pages) {

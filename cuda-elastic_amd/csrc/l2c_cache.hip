@@ -295,7 +295,7 @@ extern "C" int l2c_cache_advance(int *tables_out, int *lengths_out, int *uses, i
                                  const int *starts, const int *held, int sequences, int page_size, int pages,
                                  int max_pages, int window, hipStream_t stream) {
   if (sequences < 0 || page_size <= 0 || pages < 0 || max_pages < 0 || window < 0 ||
-      static_cast<long long>(max_pages) * page_size > INT_MAX || (parents && (beams <= 0 || sequences % beams != 0)))
+      static_cast<long long>(max_pages) * page_size > l2c::kMostPositions || (parents && (beams <= 0 || sequences % beams != 0)))
     return hipErrorInvalidValue;
   if (sequences == 0) return hipSuccess;
   if (!lengths_out || !copies || !shortage || !lengths || (pages > 0 && !uses) ||

@@ -434,7 +434,7 @@ int l2c_decoder_logprobs(float *logprobs, float *entropies, int *top_tokens, flo
  *     starts[sequences] on, say) are neither read nor written, and rows at positions below 0 are
  *     in no page. starts NULL: one new token of each sequence, row s (rows == sequences).
  * width: a multiple of 8, at most L2C_MAX_HEAD. page_size: any from 1 on, max_pages * page_size
- * below 2^31. Strides are in values between two rows, at least the rows' own length; bf16 rows
+ * at most 2^31 - 2^16. Strides are in values between two rows, at least the rows' own length; bf16 rows
  * hold their heads after each other. keys, values, q, k, v and out are 16-byte aligned, their
  * strides multiples of 8. tables, lengths and starts are read on the device: a call can be
  * captured, and replayed as they change.

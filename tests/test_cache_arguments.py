@@ -51,6 +51,15 @@ def test_attention_refuses(bad):
     assert attention(**only(attention, bad)) == INVALID
 
 
+def test_attention_refuses_small_workspaces():
+    import l2c
+    sizes = dict(sequences=1, rows=1, heads=8, kv_heads=2, width=128, page_size=16, max_pages=8192)
+    need = l2c.cache_attention_workspace_bytes(*sizes.values())
+    assert 0 < need <= 130 << 19  # one token over 131072 positions is split
+    for bad in (dict(size=need - 1), dict(workspace=None), dict(workspace=P + 8)):
+        assert attention(**{**sizes, "size": need, "workspace": P, **bad}) == INVALID
+
+
 def test_attention_workspace_size():
     import l2c
     for sequences, rows, heads, kv, width, page, most in [

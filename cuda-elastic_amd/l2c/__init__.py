@@ -456,19 +456,26 @@ def decoder_beam_reorder(out, inp, parents, beams, batch, piece_bytes, row_strid
         _check(code, "l2c_decoder_beam_reorder")
 
 
-def _takes(what, dtype, *tensors):
+# Types of torch's and its current device, looked up at the first check of them below.
+_bf16 = _e4m3 = _u8 = _i32 = _device = None
+
+
+def _takes(what, wanted, *tensors):
     """Raises unless the tensors (or None) are of a type, by its name, and on the current device: the
     kernel would read wider or other elements than theirs, or another device's memory."""
-    import torch
-    wanted = getattr(torch, dtype)
-    device = torch.cuda.current_device() if torch.cuda.is_available() else -1
+    global _f32, _bf16, _e4m3, _u8, _i32, _device
+    if _device is None:
+        import torch
+        _f32, _bf16, _e4m3, _u8, _i32 = torch.float32, torch.bfloat16, torch.float8_e4m3fn, torch.uint8, torch.int32
+        _device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+    names = ("torch.int16", "torch.uint16") if wanted == "bfloat16" else ()
     for t in tensors:
         if t is None:
             continue
-        if t.dtype is not wanted and not (dtype == "bfloat16" and str(t.dtype) in ("torch.int16", "torch.uint16")):
-            raise ValueError(f"l2c.{what} takes {dtype} here, not {t.dtype}")
-        if t.is_cuda and t.get_device() != device:
-            raise ValueError(f"l2c.{what} takes tensors on the current device, {device}, not on {t.get_device()}")
+        if str(t.dtype) not in ("torch." + wanted, *names):
+            raise ValueError(f"l2c.{what} takes {wanted} here, not {t.dtype}")
+        if t.is_cuda and t.get_device() != _device():
+            raise ValueError(f"l2c.{what} takes tensors on the current device, {_device()}, not on {t.get_device()}")
 
 
 def _bytes(t):
@@ -482,31 +489,44 @@ def decoder_logprobs_workspace_bytes(vocab, top, rows):
 def decoder_logprobs(logprobs, entropies, top_tokens, top_logprobs, logits, tokens, vocab, top, rows, workspace=None,
                      stream=None):
     """logprobs and tokens may be None together, entropies alone, the alternatives with top 0."""
-    _takes("decoder_logprobs", "float32", logprobs, entropies, top_logprobs, logits)
-    _takes("decoder_logprobs", "int32", top_tokens, tokens)
+    # The usual call in one look; what it does not take goes through every check.
+    if not (logprobs is not None and entropies is not None and top_tokens is not None and tokens is not None
+            and logprobs.dtype is entropies.dtype is top_logprobs.dtype is logits.dtype is _f32
+            and top_tokens.dtype is tokens.dtype is _i32 and logits.is_cuda and logits.get_device() == _device()):
+        _takes("decoder_logprobs", "float32", logprobs, entropies, top_logprobs, logits)
+        _takes("decoder_logprobs", "int32", top_tokens, tokens)
     code = _c_decoder_logprobs(logprobs, entropies, top_tokens, top_logprobs, logits, tokens, vocab, top, rows,
                                workspace, _bytes(workspace), stream)
     if code:
         _check(code, "l2c_decoder_logprobs")
 
 
-def _cache_type(what, keys, values, key_scales, value_scales, tables, lengths, starts, *rows):
-    """The pages' enum l2c_type: bf16, or e4m3, which bytes may hold, too."""
-    kind = str(keys.dtype)
-    if values.dtype is not keys.dtype:
+def _cache_type(what, keys, values, key_scales, value_scales, tables, lengths, starts, x, y):
+    """The pages' enum l2c_type: bf16, or e4m3, which bytes may hold, too. x, y: bf16 rows."""
+    kind = keys.dtype
+    # The usual calls in one look; what it does not take goes through every check.
+    if (_device is not None and values.dtype is kind and x.dtype is y.dtype is _bf16
+            and tables.dtype is lengths.dtype is _i32 and (starts is None or starts.dtype is _i32)
+            and keys.is_cuda and keys.get_device() == _device()):
+        if kind is _bf16:
+            return BF16
+        if (kind is _u8 or kind is _e4m3) and key_scales is not None and value_scales is not None \
+                and key_scales.dtype is value_scales.dtype is _f32:
+            return E4M3
+    if values.dtype is not kind:
         raise ValueError(f"l2c.{what} takes keys and values of one type")
-    if kind in ("torch.uint8", "torch.float8_e4m3fn"):
+    if str(kind) in ("torch.uint8", "torch.float8_e4m3fn"):
         cache_type = E4M3
         if key_scales is None or value_scales is None:
             raise ValueError(f"l2c.{what} needs the scales of e4m3 pages")
-    elif kind in ("torch.bfloat16", "torch.int16", "torch.uint16"):
+    elif str(kind) in ("torch.bfloat16", "torch.int16", "torch.uint16"):
         cache_type = BF16
     else:
         raise ValueError(f"l2c.{what} takes bf16 and e4m3 pages, not {kind}")
-    _takes(what, kind[len("torch."):], keys, values)
+    _takes(what, str(kind)[len("torch."):], keys, values)
     _takes(what, "float32", key_scales, value_scales)
     _takes(what, "int32", tables, lengths, starts)
-    _takes(what, "bfloat16", *rows)
+    _takes(what, "bfloat16", x, y)
     return cache_type
 
 
@@ -542,8 +562,13 @@ def cache_attention(out, q, keys, values, tables, lengths, heads, kv_heads, widt
 
 def cache_advance(tables_out, lengths_out, uses, copies, shortage, tables, lengths, sequences, max_pages, page_size, pages,
                   parents=None, beams=1, starts=None, held=None, window=0, stream=None):
-    _takes("cache_advance", "int32", tables_out, lengths_out, uses, copies, shortage, tables, lengths, parents, starts,
-           held)
+    # The usual calls in one look; what it does not take goes through every check.
+    if not (tables_out.dtype is lengths_out.dtype is uses.dtype is copies.dtype is shortage.dtype is tables.dtype
+            is lengths.dtype is _i32 and (parents is None or parents.dtype is _i32)
+            and (starts is None or starts.dtype is _i32) and (held is None or held.dtype is _i32)
+            and tables.is_cuda and tables.get_device() == _device()):
+        _takes("cache_advance", "int32", tables_out, lengths_out, uses, copies, shortage, tables, lengths, parents, starts,
+               held)
     code = _c_cache_advance(tables_out, lengths_out, uses, copies, shortage, tables, lengths, parents, beams, starts, held,
                             sequences, page_size, pages, max_pages, window, stream)
     if code:
@@ -552,7 +577,8 @@ def cache_advance(tables_out, lengths_out, uses, copies, shortage, tables, lengt
 
 def cache_copy(cache, copies, count, pages, page_bytes, page_stride=None, groups=1, group_stride=None, stream=None):
     """Strides and sizes in bytes; pages, and groups of them, follow each other unless the strides say otherwise."""
-    _takes("cache_copy", "int32", copies)
+    if not (copies.dtype is _i32 and copies.is_cuda and copies.get_device() == _device()):
+        _takes("cache_copy", "int32", copies)
     page = page_bytes if page_stride is None else page_stride
     code = _c_cache_copy(cache, copies, count, pages, groups, pages * page if group_stride is None else group_stride, page,
                          page_bytes, stream)

@@ -129,7 +129,7 @@ def logprobs(logprobs=P, entropies=P, top_tokens=P, top_logprobs=P, logits=P, to
 @pytest.mark.parametrize("bad", [
     dict(logprobs=None), dict(tokens=None), dict(top_tokens=None), dict(top_logprobs=None), dict(logits=None),
     dict(logits=P + 2), dict(vocab=0), dict(vocab=-1), dict(top=-1), dict(top=33), dict(rows=-1),
-    dict(rows=0x7fffffff, size=1 << 62)], ids=str)
+    dict(workspace=None), dict(workspace=P + 8), dict(size=0), dict(rows=0x7fffffff, size=1 << 62)], ids=str)
 def test_logprobs_refuses(bad):
     assert logprobs(**bad) == INVALID
 

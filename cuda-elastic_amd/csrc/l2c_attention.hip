@@ -511,16 +511,23 @@ __global__ __launch_bounds__(kThreads) void narrow_kernel(Attention a) {
 }
 
 // ---------------------------------------------------------------------------
-// Tiles of 128 rows, 32 a wave: chunks of a prompt. Bound by the matrix and the vector units. The
-// workgroup's keys and values, 64 positions at a time (32 of more than 128 columns), lie in LDS, two
-// tiles of them: while one is read, the next is on its way in registers.
+// Tiles of 128 rows, 32 a wave: chunks of a prompt. Bound by the matrix and the vector units, and by
+// LDS, which each wave reads whole tiles from. The workgroup's keys and values, 64 positions
+// at a time (32 of more than 128 columns), lie in LDS, two tiles of them: while one is read, the
+// next is on its way. bf16 pages go to LDS without registers between, rows that are not there
+// from a row of zeros; e4m3 pages through registers, where they become bf16.
 
 constexpr int kWide = 128;
+
+__device__ const u32x4 zero_row[L2C_MAX_HEAD / 8] = {};
+
+typedef __attribute__((address_space(1))) const void global_ptr;
+typedef __attribute__((address_space(3))) void lds_ptr;
 
 template <int D, bool E4M3>
 __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void wide_kernel(Attention a) {
   constexpr int kKeys = D <= 128 ? 64 : 32;
-  constexpr int kLanes = D / 8;               // that hold a row as it is loaded
+  constexpr int kLanes = D / 8;               // that load a row
   constexpr int kRows = kThreads / kLanes;    // rows loaded together
   constexpr int kPasses = kKeys / kRows;
   constexpr int kSteps = D / 16, kTiles = D / 32, kParts = kKeys / 32;
@@ -553,8 +560,10 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void wide_kernel(Attent
   const int some_to = count > 0 ? t.position(a, t.first + first + count - 1) : -1;
   const int whole_from = a.window ? some_to - a.window : -1, some_from = a.window ? whole_to - a.window + 1 : 0;
   if (threadIdx.x == 0) dirty = 0;
-  __syncthreads();
 
+  // The scale's sign goes to the queries, and 0 is the least number instead, so that the largest of the products
+  // is the largest score, and -Inf stays that.
+  const float scale = fmaxf(fabsf(a.scale), FLT_MIN);
   bf16x8 q[kSteps];
 #pragma unroll
   for (int c = 0; c < kSteps; ++c) {
@@ -562,6 +571,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void wide_kernel(Attent
     u32x4 v = {0, 0, 0, 0};
     if (mine && d < a.width)
       v = *reinterpret_cast<const u32x4 *>(a.q + row * a.q_stride + static_cast<size_t>(head) * a.width + d);
+    if (a.scale < 0.0f) v ^= 0x80008000u;
     q[c] = __builtin_bit_cast(bf16x8, v);
   }
 
@@ -570,22 +580,42 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void wide_kernel(Attent
     const int j = base + lane % kKeys;
     return j < end ? a.s.page(t.sequence, a.s.by_page(j)) : -1;
   };
-  const int load_row = threadIdx.x / kLanes, load_chunk = threadIdx.x % kLanes;
-  Raw<E4M3> k[kPasses], v[kPasses];
-  float key_scale = 0.0f, value_scale = 0.0f;
   auto row_of = [&](int page, int j) __attribute__((always_inline)) {
     return (static_cast<size_t>(static_cast<unsigned>(page)) * a.kv_heads + kv) * a.s.page_size +
            (j - a.s.by_page(j) * a.s.page_size);
   };
-  auto load = [&](int pages, int base) __attribute__((always_inline)) {
+  // Lanes that read a chunk of eight (sixteen) keys together: each in other banks.
+  auto key_swap = [](int key) __attribute__((always_inline)) { return D == 64 ? key >> 1 & 7 : key & 15; };
+  auto value_swap = [](int key) __attribute__((always_inline)) { return ((key & 3) << 1 | (key >> 2 & 1)) & (D / 8 - 1); };
+  const int load_row = threadIdx.x / kLanes, load_chunk = threadIdx.x % kLanes;
+  Raw<E4M3> k[kPasses], v[kPasses];
+  float key_scale = 0.0f, value_scale = 0.0f;
+  // Begins to load a tile: into LDS, or registers.
+  auto load = [&](int pages, int base, int to) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < kPasses; ++i) {
       const int r = i * kRows + load_row, page = __shfl(pages, r, L2C_WAVE);
-      k[i] = v[i] = Raw<E4M3>{};
-      if (a.s.is_page(page) && 8 * load_chunk < a.width) {
-        const size_t at = row_of(page, base + r) * a.width + 8 * load_chunk;
-        k[i] = load_raw<E4M3>(a.keys, at);
-        v[i] = load_raw<E4M3>(a.values, at);
+      if constexpr (E4M3) {
+        k[i] = v[i] = Raw<E4M3>{};
+        if (a.s.is_page(page) && 8 * load_chunk < a.width) {
+          const size_t at = row_of(page, base + r) * a.width + 8 * load_chunk;
+          k[i] = load_raw<E4M3>(a.keys, at);
+          v[i] = load_raw<E4M3>(a.values, at);
+        }
+      } else {
+        // A lane's 16 bytes go to LDS after those of the lane before.
+        const int key_chunk = load_chunk ^ key_swap(r), value_chunk = load_chunk ^ value_swap(r);
+        const size_t at = row_of(page, base + r) * a.width;
+        const bool there = a.s.is_page(page);
+        const uint16_t *const from_key = there && 8 * key_chunk < a.width
+                                             ? static_cast<const uint16_t *>(a.keys) + at + 8 * key_chunk
+                                             : reinterpret_cast<const uint16_t *>(zero_row);
+        const uint16_t *const from_value = there && 8 * value_chunk < a.width
+                                               ? static_cast<const uint16_t *>(a.values) + at + 8 * value_chunk
+                                               : reinterpret_cast<const uint16_t *>(zero_row);
+        const int place = i * kRows * D + wave * 8 * L2C_WAVE;
+        __builtin_amdgcn_global_load_lds((global_ptr *)from_key, (lds_ptr *)(keys[to] + place), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((global_ptr *)from_value, (lds_ptr *)(values[to] + place), 16, 0, 0);
       }
     }
     if constexpr (E4M3) {
@@ -596,19 +626,15 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void wide_kernel(Attent
       }
     }
   };
-  auto key_place = [](int key, int chunk) __attribute__((always_inline)) {
-    const int f = D == 64 ? key >> 1 & 7 : key & 15;
-    return key * D + 8 * (chunk ^ f);
-  };
 
   f32x16 acc[kTiles];
 #pragma unroll
   for (int i = 0; i < kTiles; ++i)
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[i][e] = 0.0f;
-  float top = -INFINITY, total = 0.0f;
+  float top = -INFINITY, total = 0.0f;  // of the products, without the scale
   int pages = look_up(begin);
-  load(pages, begin);
+  load(pages, begin, 0);
   unsigned long long next_there = __ballot(a.s.is_page(pages));
   pages = look_up(begin + kKeys);
   int turn = 0;
@@ -616,21 +642,29 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void wide_kernel(Attent
     const unsigned long long there = next_there;
     const bool mixed = base + kKeys - 1 > every || base <= nobody;
     bool bad = false;
-#pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-      const int r = i * kRows + load_row;
-      const u32x4 kk = as_bf16(k[i]), vv = as_bf16(v[i]);
-      if (mixed) bad |= not_finite(vv);
-      *reinterpret_cast<u32x4 *>(keys[turn] + key_place(r, load_chunk)) = kk;
-      *reinterpret_cast<u32x4 *>(values[turn] + value_place<D>(r, load_chunk)) = vv;
-    }
     if constexpr (E4M3) {
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i) {
+        const int r = i * kRows + load_row;
+        const u32x4 kk = as_bf16(k[i]), vv = as_bf16(v[i]);
+        if (mixed) bad |= not_finite(vv);
+        *reinterpret_cast<u32x4 *>(keys[turn] + r * D + 8 * (load_chunk ^ key_swap(r))) = kk;
+        *reinterpret_cast<u32x4 *>(values[turn] + r * D + 8 * (load_chunk ^ value_swap(r))) = vv;
+      }
       if (mixed) bad |= not_finite(value_scale);
       if (wave == 0 && lane < kKeys) key_scales[turn][lane] = key_scale, value_scales[turn][lane] = value_scale;
+      __syncthreads();
+    } else {
+      __builtin_amdgcn_sched_barrier(0);
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+      if (mixed)
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i)
+          bad |= not_finite(*reinterpret_cast<const u32x4 *>(values[turn] + 8 * (i * kThreads + threadIdx.x)));
     }
     if (mixed && __ballot(bad) && lane == 0) dirty = 1;
-    __syncthreads();
-    load(pages, base + kKeys);
+    load(pages, base + kKeys, turn ^ 1);
     next_there = __ballot(a.s.is_page(pages));
     pages = look_up(base + 2 * kKeys);
     if (base > some_to || base + kKeys - 1 < some_from) continue;
@@ -642,7 +676,8 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void wide_kernel(Attent
       for (int e = 0; e < 16; ++e) s[u][e] = 0.0f;
 #pragma unroll
       for (int c = 0; c < kSteps; ++c) {
-        const u32x4 kk = *reinterpret_cast<const u32x4 *>(keys[turn] + key_place(32 * u + n, 2 * c + h));
+        const u32x4 kk =
+            *reinterpret_cast<const u32x4 *>(keys[turn] + (32 * u + n) * D + 8 * ((2 * c + h) ^ key_swap(32 * u + n)));
         s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kk), q[c], s[u], 0, 0, 0);
       }
     }
@@ -657,20 +692,16 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void wide_kernel(Attent
         }
     }
     constexpr unsigned long long kAll = kKeys == 64 ? ~0ull : 0xffffffffull;
-    if (base + kKeys - 1 > whole_to || base <= whole_from || (there & kAll) != kAll || base + kKeys > end) {
+    if (base + kKeys - 1 > whole_to || base <= whole_from || (there & kAll) != kAll) {
+      const unsigned long long mine_there = there >> (4 * h);
+      const int to = position - base - 4 * h, from = lowest - base - 4 * h;
 #pragma unroll
       for (int u = 0; u < kParts; ++u)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const int at = 32 * u + 8 * (i / 4) + 4 * h + i % 4, j = base + at;
-          const bool seen = (there >> at & 1) && j <= position && j > lowest;
-          s[u][i] = seen ? s[u][i] * a.scale : -INFINITY;
+          const int at = 32 * u + 8 * (i / 4) + i % 4;
+          if (!((mine_there >> at & 1) && at <= to && at > from)) s[u][i] = -INFINITY;
         }
-    } else {
-#pragma unroll
-      for (int u = 0; u < kParts; ++u)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[u][i] *= a.scale;
     }
     float most = top;
 #pragma unroll
@@ -678,14 +709,14 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void wide_kernel(Attent
 #pragma unroll
       for (int i = 0; i < 16; ++i) most = fmaxf(most, s[u][i]);
     most = max_halves(most);
-    const float shift = most == -INFINITY ? 0.0f : most;
     if (__ballot(most > top)) {
-      const float again = exp2_of(top - shift);
+      const float again = top == -INFINITY ? 0.0f : exp2_of((top - most) * scale);
       total *= again;
 #pragma unroll
       for (int i = 0; i < kTiles; ++i) acc[i] *= again;
       top = most;
     }
+    const float shift = most == -INFINITY ? 0.0f : most * scale;
 #pragma unroll
     for (int u = 0; u < kParts; ++u) {
       u32x4 p[2];
@@ -696,7 +727,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void wide_kernel(Attent
         float e[4];
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-          e[m] = exp2_of(s[u][i + m] - shift);
+          e[m] = exp2_of(fmaf(s[u][i + m], scale, -shift));
           total += e[m];
           if constexpr (E4M3) e[m] = s[u][i + m] == -INFINITY ? 0.0f : e[m] * x[m];
         }
@@ -719,6 +750,8 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void wide_kernel(Attent
       }
     }
   }
+  // The last tile's load, of no positions, may still be writing zeros to LDS.
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
   __syncthreads();
   if (dirty) {
     float *const row_q = reinterpret_cast<float *>(keys[0]) + wave * L2C_MAX_HEAD;
@@ -739,7 +772,8 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void wide_kernel(Attent
       const f32x4 o = {acc[i][4 * m] * by, acc[i][4 * m + 1] * by, acc[i][4 * m + 2] * by, acc[i][4 * m + 3] * by};
       store4(a, whole, row, head, split, d, o);
     }
-  if (!whole && h == 0) a.part_sums[part_of(a, row, head, split)] = make_float2(top, total);
+  if (!whole && h == 0)
+    a.part_sums[part_of(a, row, head, split)] = make_float2(top == -INFINITY ? top : top * scale, total);
 }
 
 // ---------------------------------------------------------------------------

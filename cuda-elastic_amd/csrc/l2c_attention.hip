@@ -518,21 +518,29 @@ __global__ __launch_bounds__(kThreads) void narrow_kernel(Attention a) {
 // from a row of zeros; e4m3 pages through registers, where they become bf16.
 
 constexpr int kWide = 128;
+constexpr int kSchedMfma = 0x008, kSchedDsRead = 0x100;  // sched_group_barrier classes
 
 __device__ const u32x4 zero_row[L2C_MAX_HEAD / 8] = {};
 
 typedef __attribute__((address_space(1))) const void global_ptr;
 typedef __attribute__((address_space(3))) void lds_ptr;
 
-template <int D, bool E4M3>
-__global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void wide_kernel(Attention a) {
+// kTiles: tiles of 32 columns, of which there are some; a row has D columns in LDS.
+template <int kTiles, bool E4M3>
+__global__ __launch_bounds__(kThreads, kTiles <= 4 ? 2 : 1) void wide_kernel(Attention a) {
+  constexpr int D = kTiles <= 2 ? 64 : kTiles <= 4 ? 128 : 256;
   constexpr int kKeys = D <= 128 ? 64 : 32;
   constexpr int kLanes = D / 8;               // that load a row
   constexpr int kRows = kThreads / kLanes;    // rows loaded together
   constexpr int kPasses = kKeys / kRows;
-  constexpr int kSteps = D / 16, kTiles = D / 32, kParts = kKeys / 32;
-  __shared__ __attribute__((aligned(16))) uint16_t keys[2][kKeys * D], values[2][kKeys * D];
-  __shared__ __attribute__((aligned(16))) float key_scales[2][kKeys], value_scales[2][kKeys];
+  constexpr int kTogether = kRows / kWaves;   // of them by one wave
+  constexpr int kSteps = 2 * kTiles, kParts = kKeys / 32;
+  // Two of each, with names of their own: of one array's halves the compiler would wait for the loads into one
+  // before it reads the other.
+  constexpr int kSecond = E4M3 ? 8 : kKeys * D;
+  __shared__ __attribute__((aligned(16))) uint16_t keys_0[kKeys * D], keys_1[kSecond], values_0[kKeys * D],
+      values_1[kSecond];
+  __shared__ __attribute__((aligned(16))) float key_scales[kKeys], value_scales[kKeys];
   __shared__ int dirty;
   const int lane = threadIdx.x % L2C_WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / L2C_WAVE);
   const int n = lane % 32, h = lane / 32;
@@ -560,6 +568,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void wide_kernel(Attent
   const int some_to = count > 0 ? t.position(a, t.first + first + count - 1) : -1;
   const int whole_from = a.window ? some_to - a.window : -1, some_from = a.window ? whole_to - a.window + 1 : 0;
   if (threadIdx.x == 0) dirty = 0;
+  __syncthreads();
 
   // The scale's sign goes to the queries, and 0 is the least number instead, so that the largest of the products
   // is the largest score, and -Inf stays that.
@@ -590,12 +599,16 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void wide_kernel(Attent
   const int load_row = threadIdx.x / kLanes, load_chunk = threadIdx.x % kLanes;
   Raw<E4M3> k[kPasses], v[kPasses];
   float key_scale = 0.0f, value_scale = 0.0f;
+  // A wave's rows lie in one page, and their places in it follow each other.
+  const bool together = a.s.page_size % kTogether == 0;
+  const int lane_key = load_row % kTogether;
   // Begins to load a tile: into LDS, or registers.
-  auto load = [&](int pages, int base, int to) __attribute__((always_inline)) {
+  auto load = [&](int pages, int base, uint16_t *to_keys, uint16_t *to_values) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < kPasses; ++i) {
-      const int r = i * kRows + load_row, page = __shfl(pages, r, L2C_WAVE);
+      const int r = i * kRows + load_row;
       if constexpr (E4M3) {
+        const int page = __shfl(pages, r, L2C_WAVE);
         k[i] = v[i] = Raw<E4M3>{};
         if (a.s.is_page(page) && 8 * load_chunk < a.width) {
           const size_t at = row_of(page, base + r) * a.width + 8 * load_chunk;
@@ -605,17 +618,36 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void wide_kernel(Attent
       } else {
         // A lane's 16 bytes go to LDS after those of the lane before.
         const int key_chunk = load_chunk ^ key_swap(r), value_chunk = load_chunk ^ value_swap(r);
-        const size_t at = row_of(page, base + r) * a.width;
-        const bool there = a.s.is_page(page);
-        const uint16_t *const from_key = there && 8 * key_chunk < a.width
-                                             ? static_cast<const uint16_t *>(a.keys) + at + 8 * key_chunk
-                                             : reinterpret_cast<const uint16_t *>(zero_row);
-        const uint16_t *const from_value = there && 8 * value_chunk < a.width
-                                               ? static_cast<const uint16_t *>(a.values) + at + 8 * value_chunk
-                                               : reinterpret_cast<const uint16_t *>(zero_row);
         const int place = i * kRows * D + wave * 8 * L2C_WAVE;
-        __builtin_amdgcn_global_load_lds((global_ptr *)from_key, (lds_ptr *)(keys[to] + place), 16, 0, 0);
-        __builtin_amdgcn_global_load_lds((global_ptr *)from_value, (lds_ptr *)(values[to] + place), 16, 0, 0);
+        const int first_row = i * kRows + wave * kTogether;
+        const int page = __builtin_amdgcn_readlane(pages, first_row);
+        if (together && a.s.is_page(page) && base + first_row + kTogether <= end) {
+          // One page for the wave: an address in scalar registers, and the lanes' offsets, which stay the same.
+          const size_t at = 2 * (row_of(page, base + first_row) * a.width);
+          const unsigned char *const page_keys = static_cast<const unsigned char *>(a.keys) + at;
+          const unsigned char *const page_values = static_cast<const unsigned char *>(a.values) + at;
+          const unsigned key_at = 2 * (lane_key * a.width + 8 * key_chunk), value_at = 2 * (lane_key * a.width + 8 * value_chunk);
+          if (a.width == D) {
+            __builtin_amdgcn_global_load_lds((global_ptr *)(page_keys + key_at), (lds_ptr *)(to_keys + place), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((global_ptr *)(page_values + value_at), (lds_ptr *)(to_values + place), 16, 0, 0);
+          } else {
+            const unsigned char *const zeros = reinterpret_cast<const unsigned char *>(zero_row);
+            __builtin_amdgcn_global_load_lds((global_ptr *)(8 * key_chunk < a.width ? page_keys + key_at : zeros),
+                                             (lds_ptr *)(to_keys + place), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((global_ptr *)(8 * value_chunk < a.width ? page_values + value_at : zeros),
+                                             (lds_ptr *)(to_values + place), 16, 0, 0);
+          }
+        } else {
+          const int own = __shfl(pages, r, L2C_WAVE);
+          const size_t at = row_of(own, base + r) * a.width;
+          const uint16_t *from_key = reinterpret_cast<const uint16_t *>(zero_row), *from_value = from_key;
+          if (a.s.is_page(own) && 8 * key_chunk < a.width)
+            from_key = static_cast<const uint16_t *>(a.keys) + at + 8 * key_chunk;
+          if (a.s.is_page(own) && 8 * value_chunk < a.width)
+            from_value = static_cast<const uint16_t *>(a.values) + at + 8 * value_chunk;
+          __builtin_amdgcn_global_load_lds((global_ptr *)from_key, (lds_ptr *)(to_keys + place), 16, 0, 0);
+          __builtin_amdgcn_global_load_lds((global_ptr *)from_value, (lds_ptr *)(to_values + place), 16, 0, 0);
+        }
       }
     }
     if constexpr (E4M3) {
@@ -634,11 +666,11 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void wide_kernel(Attent
     for (int e = 0; e < 16; ++e) acc[i][e] = 0.0f;
   float top = -INFINITY, total = 0.0f;  // of the products, without the scale
   int pages = look_up(begin);
-  load(pages, begin, 0);
+  load(pages, begin, keys_0, values_0);
   unsigned long long next_there = __ballot(a.s.is_page(pages));
   pages = look_up(begin + kKeys);
-  int turn = 0;
-  for (int base = begin; base < end; base += kKeys, turn ^= 1) {
+  auto step = [&](int base, uint16_t *keys, uint16_t *values, uint16_t *next_keys, uint16_t *next_values)
+      __attribute__((always_inline)) {
     const unsigned long long there = next_there;
     const bool mixed = base + kKeys - 1 > every || base <= nobody;
     bool bad = false;
@@ -648,11 +680,11 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void wide_kernel(Attent
         const int r = i * kRows + load_row;
         const u32x4 kk = as_bf16(k[i]), vv = as_bf16(v[i]);
         if (mixed) bad |= not_finite(vv);
-        *reinterpret_cast<u32x4 *>(keys[turn] + r * D + 8 * (load_chunk ^ key_swap(r))) = kk;
-        *reinterpret_cast<u32x4 *>(values[turn] + r * D + 8 * (load_chunk ^ value_swap(r))) = vv;
+        *reinterpret_cast<u32x4 *>(keys + r * D + 8 * (load_chunk ^ key_swap(r))) = kk;
+        *reinterpret_cast<u32x4 *>(values + r * D + 8 * (load_chunk ^ value_swap(r))) = vv;
       }
       if (mixed) bad |= not_finite(value_scale);
-      if (wave == 0 && lane < kKeys) key_scales[turn][lane] = key_scale, value_scales[turn][lane] = value_scale;
+      if (wave == 0 && lane < kKeys) key_scales[lane] = key_scale, value_scales[lane] = value_scale;
       __syncthreads();
     } else {
       __builtin_amdgcn_sched_barrier(0);
@@ -661,13 +693,13 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void wide_kernel(Attent
       if (mixed)
 #pragma unroll
         for (int i = 0; i < kPasses; ++i)
-          bad |= not_finite(*reinterpret_cast<const u32x4 *>(values[turn] + 8 * (i * kThreads + threadIdx.x)));
+          bad |= not_finite(*reinterpret_cast<const u32x4 *>(values + 8 * (i * kThreads + threadIdx.x)));
     }
     if (mixed && __ballot(bad) && lane == 0) dirty = 1;
-    load(pages, base + kKeys, turn ^ 1);
+    load(pages, base + kKeys, next_keys, next_values);
     next_there = __ballot(a.s.is_page(pages));
     pages = look_up(base + 2 * kKeys);
-    if (base > some_to || base + kKeys - 1 < some_from) continue;
+    if (base > some_to || base + kKeys - 1 < some_from) return;
     // Scores of positions 32 u + 8 (i / 4) + 4 h + i % 4, of query n.
     f32x16 s[kParts];
 #pragma unroll
@@ -677,16 +709,25 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void wide_kernel(Attent
 #pragma unroll
       for (int c = 0; c < kSteps; ++c) {
         const u32x4 kk =
-            *reinterpret_cast<const u32x4 *>(keys[turn] + (32 * u + n) * D + 8 * ((2 * c + h) ^ key_swap(32 * u + n)));
+            *reinterpret_cast<const u32x4 *>(keys + (32 * u + n) * D + 8 * ((2 * c + h) ^ key_swap(32 * u + n)));
         s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kk), q[c], s[u], 0, 0, 0);
       }
     }
+    // Reads of keys stay kAhead ahead of the instruction that takes them.
+    constexpr int kAhead = 6;
+    __builtin_amdgcn_sched_group_barrier(kSchedDsRead, kAhead, 0);
+#pragma unroll
+    for (int i = 0; i < kParts * kSteps - kAhead; ++i) {
+      __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(kSchedDsRead, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(kSchedMfma, kAhead, 0);
     if constexpr (E4M3) {
 #pragma unroll
       for (int u = 0; u < kParts; ++u)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const f32x4 x = *reinterpret_cast<const f32x4 *>(&key_scales[turn][32 * u + 8 * i + 4 * h]);
+          const f32x4 x = *reinterpret_cast<const f32x4 *>(&key_scales[32 * u + 8 * i + 4 * h]);
 #pragma unroll
           for (int e = 0; e < 4; ++e) s[u][4 * i + e] *= x[e];
         }
@@ -709,21 +750,23 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void wide_kernel(Attent
 #pragma unroll
       for (int i = 0; i < 16; ++i) most = fmaxf(most, s[u][i]);
     most = max_halves(most);
-    if (__ballot(most > top)) {
+    // Sums stay relative to an older maximum until a new one is 2^8 times as large: floats, and bf16 weights,
+    // are as exact there.
+    if (__ballot((most - top) * scale > 8.0f)) {
       const float again = top == -INFINITY ? 0.0f : exp2_of((top - most) * scale);
       total *= again;
 #pragma unroll
       for (int i = 0; i < kTiles; ++i) acc[i] *= again;
       top = most;
     }
-    const float shift = most == -INFINITY ? 0.0f : most * scale;
+    const float shift = top == -INFINITY ? 0.0f : top * scale;
 #pragma unroll
     for (int u = 0; u < kParts; ++u) {
       u32x4 p[2];
 #pragma unroll
       for (int i = 0; i < 16; i += 4) {
         f32x4 x = {1.0f, 1.0f, 1.0f, 1.0f};
-        if constexpr (E4M3) x = *reinterpret_cast<const f32x4 *>(&value_scales[turn][32 * u + 2 * i + 4 * h]);
+        if constexpr (E4M3) x = *reinterpret_cast<const f32x4 *>(&value_scales[32 * u + 2 * i + 4 * h]);
         float e[4];
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
@@ -739,23 +782,34 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void wide_kernel(Attent
         const int key = 32 * u + 16 * half + 4 * h + (n % 16) / 4;
 #pragma unroll
         for (int i = 0; i < kTiles; ++i) {
-          if (32 * i >= a.width) break;
           const int d = 32 * i + 16 * (n / 16) + 4 * (n % 4);
-          const u32x2 low = read_column(values[turn] + value_place<D>(key, d / 8) + d % 8);
-          const u32x2 high = read_column(values[turn] + value_place<D>(key + 8, d / 8) + d % 8);
+          const u32x2 low = read_column(values + value_place<D>(key, d / 8) + d % 8);
+          const u32x2 high = read_column(values + value_place<D>(key + 8, d / 8) + d % 8);
           const u32x4 w = {low[0], low[1], high[0], high[1]};
           acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, w),
                                                            __builtin_bit_cast(bf16x8, p[half]), acc[i], 0, 0, 0);
         }
       }
     }
+    };
+  if constexpr (E4M3) {
+    for (int base = begin; base < end; base += kKeys) {
+      step(base, keys_0, values_0, nullptr, nullptr);
+      __syncthreads();
+    }
+  } else {
+    for (int base = begin; base < end; base += 2 * kKeys) {
+      step(base, keys_0, values_0, keys_1, values_1);
+      if (base + kKeys >= end) break;
+      step(base + kKeys, keys_1, values_1, keys_0, values_0);
+    }
   }
   // The last tile's load, of no positions, may still be writing zeros to LDS.
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
   __syncthreads();
   if (dirty) {
-    float *const row_q = reinterpret_cast<float *>(keys[0]) + wave * L2C_MAX_HEAD;
-    static_assert(sizeof(keys) >= kWaves * L2C_MAX_HEAD * sizeof(float), "room for the queries");
+    float *const row_q = reinterpret_cast<float *>(keys_0) + wave * L2C_MAX_HEAD;
+    static_assert(sizeof(keys_0) >= kWaves * L2C_MAX_HEAD * sizeof(float), "room for the queries");
     for (int r = wave; r < t.count; r += kWaves) lone_row<E4M3>(a, t, kv, t.first + r, split, begin, end, row_q);
     return;
   }
@@ -847,10 +901,14 @@ bool sizes(int sequences, int rows, int heads, int kv_heads, int width, int page
 }
 
 using Kernel = void (*)(Attention);
-template <int D>
-Kernel kernel(bool narrow, bool e4m3) {
-  return narrow ? (e4m3 ? narrow_kernel<D, true> : narrow_kernel<D, false>)
-                : (e4m3 ? wide_kernel<D, true> : wide_kernel<D, false>);
+template <bool E4M3>
+Kernel kernel(bool narrow, int width) {
+  if (narrow) return width <= 64 ? narrow_kernel<64, E4M3> : width <= 128 ? narrow_kernel<128, E4M3> : narrow_kernel<256, E4M3>;
+  return width <= 64    ? wide_kernel<2, E4M3>
+         : width <= 96  ? wide_kernel<3, E4M3>
+         : width <= 128 ? wide_kernel<4, E4M3>
+         : width <= 192 ? wide_kernel<6, E4M3>
+                        : wide_kernel<8, E4M3>;
 }
 
 size_t part_bytes(const Plan &p, int rows, int heads, int width) {
@@ -903,10 +961,7 @@ extern "C" int l2c_cache_attention(uint16_t *out, long long out_stride, const ui
   a.group = heads / kv_heads, a.by_group = l2c::Quotient31(a.group);
   a.heads = heads, a.kv_heads = kv_heads, a.width = width, a.window = window;
   a.splits = p.splits, a.slots = static_cast<int>(p.slots), a.scale = scale * kLog2e;
-  const bool e4m3 = cache_type == L2C_E4M3;
-  const Kernel fn = width <= 64    ? kernel<64>(p.narrow, e4m3)
-                    : width <= 128 ? kernel<128>(p.narrow, e4m3)
-                                   : kernel<256>(p.narrow, e4m3);
+  const Kernel fn = cache_type == L2C_E4M3 ? kernel<true>(p.narrow, width) : kernel<false>(p.narrow, width);
   hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, stream, a);
   L2C_LAUNCH_CHECK();
   if (p.splits == 1) return hipSuccess;

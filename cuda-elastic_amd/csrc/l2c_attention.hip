@@ -41,7 +41,8 @@ struct Attention {
   Sequences s;
   l2c::Quotient31 by_group;
   int heads, kv_heads, group, width, window, splits, slots;
-  float scale;  // times log2(e)
+  unsigned long long page_bytes;  // of bf16 keys
+  float scale;                    // times log2(e)
 };
 
 // ---------------------------------------------------------------------------
@@ -277,15 +278,6 @@ __device__ __forceinline__ void lone_row(const Attention &a, const Tile &t, int 
   __builtin_amdgcn_wave_barrier();
 }
 
-// Where 16 bytes (`chunk`) of row `key` lie in a tile of values in LDS. Lanes that write
-// together have eight keys and one chunk, lanes that read together the same 32 bytes of four keys: the
-// chunk's lower bits are exchanged so that neither meet in a bank.
-template <int D>
-__device__ __forceinline__ int value_place(int key, int chunk) {
-  const int f = ((key & 3) << 1 | (key >> 2 & 1)) & (D / 8 - 1);
-  return key * D + 8 * (chunk ^ f);
-}
-
 typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
 
 // Four keys of a column: lanes l of 16 point to keys l / 4 and columns 4 (l % 4), and get column l.
@@ -302,6 +294,14 @@ __device__ __forceinline__ u32x2 read_column(const uint16_t *at) {
 // key), values through LDS of the wave's own, so that nothing waits for another wave.
 
 constexpr int kNarrow = 16, kNarrowStep = 32;
+
+// Where 16 bytes (`chunk`) of row `key` lie in a wave's values in LDS. Lanes that write together have sixteen keys
+// and one chunk, lanes that read together the same 32 bytes of eight keys: chunks are exchanged so that
+// neither meet in a bank.
+template <int D>
+__device__ __forceinline__ int value_place(int key, int chunk) {
+  return key * D + 8 * (chunk ^ ((D == 64 ? key >> 1 & 3 : key & 7) << 1 | (key >> 3 & 1)));
+}
 
 template <int D, bool E4M3>
 __global__ __launch_bounds__(kThreads) void narrow_kernel(Attention a) {
@@ -595,66 +595,72 @@ __global__ __launch_bounds__(kThreads, kTiles <= 4 ? 2 : 1) void wide_kernel(Att
   };
   // Lanes that read a chunk of eight (sixteen) keys together: each in other banks.
   auto key_swap = [](int key) __attribute__((always_inline)) { return D == 64 ? key >> 1 & 7 : key & 15; };
-  auto value_swap = [](int key) __attribute__((always_inline)) { return ((key & 3) << 1 | (key >> 2 & 1)) & (D / 8 - 1); };
+  // Lanes that read four keys of 32 columns together, the same.
+  auto value_swap = [](int key) __attribute__((always_inline)) { return D == 64 ? (key >> 1 & 1) << 2 : (key & 3) << 2; };
+  auto value_place = [&](int key, int chunk) __attribute__((always_inline)) { return key * D + 8 * (chunk ^ value_swap(key)); };
   const int load_row = threadIdx.x / kLanes, load_chunk = threadIdx.x % kLanes;
   Raw<E4M3> k[kPasses], v[kPasses];
   float key_scale = 0.0f, value_scale = 0.0f;
-  // A wave's rows lie in one page, and their places in it follow each other.
-  const bool together = a.s.page_size % kTogether == 0;
-  const int lane_key = load_row % kTogether;
-  // Begins to load a tile: into LDS, or registers.
-  auto load = [&](int pages, int base, uint16_t *to_keys, uint16_t *to_values) __attribute__((always_inline)) {
+  // Begins to load a tile, `there` of which have a page: into LDS, or registers.
+  constexpr unsigned long long kAll = kKeys == 64 ? ~0ull : 0xffffffffull;
+  const bool together = a.s.page_size % kTogether == 0;  // a wave's rows lie in one page
+  const unsigned row_bytes = 2u * static_cast<unsigned>(a.width);
+  const unsigned long long head_bytes = static_cast<unsigned long long>(kv) * a.s.page_size * row_bytes;
+  auto load = [&](int pages, unsigned long long there, int base, uint16_t *to_keys, uint16_t *to_values)
+                  __attribute__((always_inline)) {
+    if constexpr (E4M3) {
 #pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-      const int r = i * kRows + load_row;
-      if constexpr (E4M3) {
-        const int page = __shfl(pages, r, L2C_WAVE);
+      for (int i = 0; i < kPasses; ++i) {
+        const int r = i * kRows + load_row, page = __shfl(pages, r, L2C_WAVE);
         k[i] = v[i] = Raw<E4M3>{};
         if (a.s.is_page(page) && 8 * load_chunk < a.width) {
           const size_t at = row_of(page, base + r) * a.width + 8 * load_chunk;
           k[i] = load_raw<E4M3>(a.keys, at);
           v[i] = load_raw<E4M3>(a.values, at);
         }
-      } else {
-        // A lane's 16 bytes go to LDS after those of the lane before.
-        const int key_chunk = load_chunk ^ key_swap(r), value_chunk = load_chunk ^ value_swap(r);
-        const int place = i * kRows * D + wave * 8 * L2C_WAVE;
-        const int first_row = i * kRows + wave * kTogether;
-        const int page = __builtin_amdgcn_readlane(pages, first_row);
-        if (together && a.s.is_page(page) && base + first_row + kTogether <= end) {
-          // One page for the wave: an address in scalar registers, and the lanes' offsets, which stay the same.
-          const size_t at = 2 * (row_of(page, base + first_row) * a.width);
-          const unsigned char *const page_keys = static_cast<const unsigned char *>(a.keys) + at;
-          const unsigned char *const page_values = static_cast<const unsigned char *>(a.values) + at;
-          const unsigned key_at = 2 * (lane_key * a.width + 8 * key_chunk), value_at = 2 * (lane_key * a.width + 8 * value_chunk);
-          if (a.width == D) {
-            __builtin_amdgcn_global_load_lds((global_ptr *)(page_keys + key_at), (lds_ptr *)(to_keys + place), 16, 0, 0);
-            __builtin_amdgcn_global_load_lds((global_ptr *)(page_values + value_at), (lds_ptr *)(to_values + place), 16, 0, 0);
-          } else {
-            const unsigned char *const zeros = reinterpret_cast<const unsigned char *>(zero_row);
-            __builtin_amdgcn_global_load_lds((global_ptr *)(8 * key_chunk < a.width ? page_keys + key_at : zeros),
-                                             (lds_ptr *)(to_keys + place), 16, 0, 0);
-            __builtin_amdgcn_global_load_lds((global_ptr *)(8 * value_chunk < a.width ? page_values + value_at : zeros),
-                                             (lds_ptr *)(to_values + place), 16, 0, 0);
-          }
-        } else {
-          const int own = __shfl(pages, r, L2C_WAVE);
-          const size_t at = row_of(own, base + r) * a.width;
-          const uint16_t *from_key = reinterpret_cast<const uint16_t *>(zero_row), *from_value = from_key;
-          if (a.s.is_page(own) && 8 * key_chunk < a.width)
-            from_key = static_cast<const uint16_t *>(a.keys) + at + 8 * key_chunk;
-          if (a.s.is_page(own) && 8 * value_chunk < a.width)
-            from_value = static_cast<const uint16_t *>(a.values) + at + 8 * value_chunk;
-          __builtin_amdgcn_global_load_lds((global_ptr *)from_key, (lds_ptr *)(to_keys + place), 16, 0, 0);
-          __builtin_amdgcn_global_load_lds((global_ptr *)from_value, (lds_ptr *)(to_values + place), 16, 0, 0);
-        }
       }
-    }
-    if constexpr (E4M3) {
       key_scale = value_scale = 0.0f;
       if (a.s.is_page(pages)) {
         const size_t at = row_of(pages, base + lane % kKeys);
         key_scale = a.key_scales[at], value_scale = a.value_scales[at];
+      }
+    } else {
+      // Where the lane's key lies; then a lane's 16 bytes go to LDS after those of the lane before.
+      const int j = base + lane % kKeys;
+      const unsigned long long offset = static_cast<unsigned long long>(static_cast<unsigned>(pages)) * a.page_bytes +
+                                        head_bytes +
+                                        static_cast<unsigned long long>(j - a.s.by_page(j) * a.s.page_size) * row_bytes;
+      const unsigned low = static_cast<unsigned>(offset), high = static_cast<unsigned>(offset >> 32);
+      const bool whole = together && (there & kAll) == kAll;
+#pragma unroll
+      for (int i = 0; i < kPasses; ++i) {
+        const int r = i * kRows + load_row, first_row = i * kRows + wave * kTogether;
+        const unsigned key_at = 16u * (load_chunk ^ key_swap(r)), value_at = 16u * (load_chunk ^ value_swap(r));
+        const unsigned char *from_key, *from_value;
+        if (whole) {
+          const unsigned long long at =
+              static_cast<unsigned long long>(static_cast<unsigned>(__builtin_amdgcn_readlane(high, first_row))) << 32 |
+              static_cast<unsigned>(__builtin_amdgcn_readlane(low, first_row));
+          const unsigned row_at = (load_row % kTogether) * row_bytes;
+          from_key = static_cast<const unsigned char *>(a.keys) + at + (row_at + key_at);
+          from_value = static_cast<const unsigned char *>(a.values) + at + (row_at + value_at);
+        } else {
+          const unsigned long long at = static_cast<unsigned long long>(static_cast<unsigned>(__shfl(high, r, L2C_WAVE)))
+                                            << 32 |
+                                        static_cast<unsigned>(__shfl(low, r, L2C_WAVE));
+          const bool is = there >> r & 1;
+          from_key = is ? static_cast<const unsigned char *>(a.keys) + at + key_at
+                        : reinterpret_cast<const unsigned char *>(zero_row);
+          from_value = is ? static_cast<const unsigned char *>(a.values) + at + value_at
+                          : reinterpret_cast<const unsigned char *>(zero_row);
+        }
+        if (a.width != D) {  // columns past the row's
+          if (key_at >= row_bytes) from_key = reinterpret_cast<const unsigned char *>(zero_row);
+          if (value_at >= row_bytes) from_value = reinterpret_cast<const unsigned char *>(zero_row);
+        }
+        const int place = i * kRows * D + wave * 8 * L2C_WAVE;
+        __builtin_amdgcn_global_load_lds((global_ptr *)from_key, (lds_ptr *)(to_keys + place), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((global_ptr *)from_value, (lds_ptr *)(to_values + place), 16, 0, 0);
       }
     }
   };
@@ -666,8 +672,8 @@ __global__ __launch_bounds__(kThreads, kTiles <= 4 ? 2 : 1) void wide_kernel(Att
     for (int e = 0; e < 16; ++e) acc[i][e] = 0.0f;
   float top = -INFINITY, total = 0.0f;  // of the products, without the scale
   int pages = look_up(begin);
-  load(pages, begin, keys_0, values_0);
   unsigned long long next_there = __ballot(a.s.is_page(pages));
+  load(pages, next_there, begin, keys_0, values_0);
   pages = look_up(begin + kKeys);
   auto step = [&](int base, uint16_t *keys, uint16_t *values, uint16_t *next_keys, uint16_t *next_values)
       __attribute__((always_inline)) {
@@ -696,8 +702,8 @@ __global__ __launch_bounds__(kThreads, kTiles <= 4 ? 2 : 1) void wide_kernel(Att
           bad |= not_finite(*reinterpret_cast<const u32x4 *>(values + 8 * (i * kThreads + threadIdx.x)));
     }
     if (mixed && __ballot(bad) && lane == 0) dirty = 1;
-    load(pages, base + kKeys, next_keys, next_values);
     next_there = __ballot(a.s.is_page(pages));
+    load(pages, next_there, base + kKeys, next_keys, next_values);
     pages = look_up(base + 2 * kKeys);
     if (base > some_to || base + kKeys - 1 < some_from) return;
     // Scores of positions 32 u + 8 (i / 4) + 4 h + i % 4, of query n.
@@ -732,7 +738,6 @@ __global__ __launch_bounds__(kThreads, kTiles <= 4 ? 2 : 1) void wide_kernel(Att
           for (int e = 0; e < 4; ++e) s[u][4 * i + e] *= x[e];
         }
     }
-    constexpr unsigned long long kAll = kKeys == 64 ? ~0ull : 0xffffffffull;
     if (base + kKeys - 1 > whole_to || base <= whole_from || (there & kAll) != kAll) {
       const unsigned long long mine_there = there >> (4 * h);
       const int to = position - base - 4 * h, from = lowest - base - 4 * h;
@@ -783,8 +788,8 @@ __global__ __launch_bounds__(kThreads, kTiles <= 4 ? 2 : 1) void wide_kernel(Att
 #pragma unroll
         for (int i = 0; i < kTiles; ++i) {
           const int d = 32 * i + 16 * (n / 16) + 4 * (n % 4);
-          const u32x2 low = read_column(values + value_place<D>(key, d / 8) + d % 8);
-          const u32x2 high = read_column(values + value_place<D>(key + 8, d / 8) + d % 8);
+          const u32x2 low = read_column(values + value_place(key, d / 8) + d % 8);
+          const u32x2 high = read_column(values + value_place(key + 8, d / 8) + d % 8);
           const u32x4 w = {low[0], low[1], high[0], high[1]};
           acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, w),
                                                            __builtin_bit_cast(bf16x8, p[half]), acc[i], 0, 0, 0);
@@ -957,6 +962,7 @@ extern "C" int l2c_cache_attention(uint16_t *out, long long out_stride, const ui
   a.out = out, a.q = q, a.keys = keys, a.values = values, a.key_scales = key_scales, a.value_scales = value_scales;
   a.part_values = parts, a.part_sums = reinterpret_cast<float2 *>(parts + (p.splits > 1 ? items * width : 0));
   a.out_stride = out_stride, a.q_stride = q_stride;
+  a.page_bytes = 2ull * kv_heads * page_size * width;
   a.s = l2c::sequences_of(tables, lengths, starts, sequences, rows, max_pages, page_size, pages);
   a.group = heads / kv_heads, a.by_group = l2c::Quotient31(a.group);
   a.heads = heads, a.kv_heads = kv_heads, a.width = width, a.window = window;

@@ -518,7 +518,7 @@ __global__ __launch_bounds__(kThreads) void narrow_kernel(Attention a) {
 // from a row of zeros; e4m3 pages through registers, where they become bf16.
 
 constexpr int kWide = 128;
-constexpr int kSchedMfma = 0x008, kSchedDsRead = 0x100;  // sched_group_barrier classes
+constexpr int kSchedValu = 0x002, kSchedMfma = 0x008, kSchedDsRead = 0x100;  // sched_group_barrier classes
 
 __device__ const u32x4 zero_row[L2C_MAX_HEAD / 8] = {};
 
@@ -706,28 +706,38 @@ __global__ __launch_bounds__(kThreads, kTiles <= 4 ? 2 : 1) void wide_kernel(Att
     load(pages, next_there, base + kKeys, next_keys, next_values);
     pages = look_up(base + 2 * kKeys);
     if (base > some_to || base + kKeys - 1 < some_from) return;
-    // Scores of positions 32 u + 8 (i / 4) + 4 h + i % 4, of query n.
+    // Scores of positions 32 u + 8 (i / 4) + 4 h + i % 4, of query n. Keys are read four operands ahead, in
+    // this order and no other: left to itself the compiler reads one, waits, and multiplies.
     f32x16 s[kParts];
+    constexpr int kAhead = 4, kGroups = kParts * kSteps / kAhead;
+    u32x4 operand[2][kAhead];
+    auto read_keys = [&](u32x4 (&to)[kAhead], int group) __attribute__((always_inline)) {
 #pragma unroll
-    for (int u = 0; u < kParts; ++u) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e) s[u][e] = 0.0f;
-#pragma unroll
-      for (int c = 0; c < kSteps; ++c) {
-        const u32x4 kk =
+      for (int e = 0; e < kAhead; ++e) {
+        const int u = (group * kAhead + e) / kSteps, c = (group * kAhead + e) % kSteps;
+        to[e] =
             *reinterpret_cast<const u32x4 *>(keys + (32 * u + n) * D + 8 * ((2 * c + h) ^ key_swap(32 * u + n)));
-        s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kk), q[c], s[u], 0, 0, 0);
       }
-    }
-    // Reads of keys stay kAhead ahead of the instruction that takes them.
-    constexpr int kAhead = 6;
-    __builtin_amdgcn_sched_group_barrier(kSchedDsRead, kAhead, 0);
+    };
+    read_keys(operand[0], 0);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int i = 0; i < kParts * kSteps - kAhead; ++i) {
-      __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(kSchedDsRead, 1, 0);
+    for (int group = 0; group < kGroups; ++group) {
+      if (group + 1 < kGroups) read_keys(operand[(group + 1) % 2], group + 1);
+#pragma unroll
+      for (int e = 0; e < kAhead; ++e) {
+        const int u = (group * kAhead + e) / kSteps, c = (group * kAhead + e) % kSteps;
+        f32x16 before = s[u];
+        if (c == 0)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) before[i] = 0.0f;
+        s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, operand[group % 2][e]), q[c], before, 0, 0,
+                                                       0);
+      }
+      __builtin_amdgcn_sched_group_barrier(kSchedDsRead, kAhead, 0);
+      __builtin_amdgcn_sched_group_barrier(kSchedMfma, kAhead, 0);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    __builtin_amdgcn_sched_group_barrier(kSchedMfma, kAhead, 0);
     if constexpr (E4M3) {
 #pragma unroll
       for (int u = 0; u < kParts; ++u)
@@ -765,38 +775,62 @@ __global__ __launch_bounds__(kThreads, kTiles <= 4 ? 2 : 1) void wide_kernel(Att
       top = most;
     }
     const float shift = top == -INFINITY ? 0.0f : top * scale;
+    // 16 positions at a time: while the matrix unit has their product, the next ones' weights are computed and
+    // their values read.
+    u32x4 weight[2], column[2][kTiles];
+    auto weigh = [&](u32x4 &to, int group) __attribute__((always_inline)) {
+      const int u = group / 2;
 #pragma unroll
-    for (int u = 0; u < kParts; ++u) {
-      u32x4 p[2];
-#pragma unroll
-      for (int i = 0; i < 16; i += 4) {
+      for (int i = 0; i < 8; i += 4) {
+        const int at = 8 * (group % 2) + i;
         f32x4 x = {1.0f, 1.0f, 1.0f, 1.0f};
-        if constexpr (E4M3) x = *reinterpret_cast<const f32x4 *>(&value_scales[32 * u + 2 * i + 4 * h]);
+        if constexpr (E4M3) x = *reinterpret_cast<const f32x4 *>(&value_scales[32 * u + 2 * at + 4 * h]);
         float e[4];
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-          e[m] = exp2_of(fmaf(s[u][i + m], scale, -shift));
+          e[m] = exp2_of(fmaf(s[u][at + m], scale, -shift));
           total += e[m];
-          if constexpr (E4M3) e[m] = s[u][i + m] == -INFINITY ? 0.0f : e[m] * x[m];
+          if constexpr (E4M3) e[m] = s[u][at + m] == -INFINITY ? 0.0f : e[m] * x[m];
         }
-        p[i / 8][i / 2 % 4] = pack2(e[0], e[1]);
-        p[i / 8][i / 2 % 4 + 1] = pack2(e[2], e[3]);
+        to[i / 2] = pack2(e[0], e[1]);
+        to[i / 2 + 1] = pack2(e[2], e[3]);
+      }
+    };
+    auto read_values = [&](u32x4 (&to)[kTiles], int group) __attribute__((always_inline)) {
+      const int key = 16 * group + 4 * h + (n % 16) / 4;
+#pragma unroll
+      for (int i = 0; i < kTiles; ++i) {
+        const int d = 32 * i + 16 * (n / 16) + 4 * (n % 4);
+        const u32x2 low = read_column(values + value_place(key, d / 8) + d % 8);
+        const u32x2 high = read_column(values + value_place(key + 8, d / 8) + d % 8);
+        to[i] = u32x4{low[0], low[1], high[0], high[1]};
+      }
+    };
+    read_values(column[0], 0);
+    weigh(weight[0], 0);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int group = 0; group < 2 * kParts; ++group) {
+      const bool more = group + 1 < 2 * kParts;
+      if (more) {
+        read_values(column[(group + 1) % 2], group + 1);
+        weigh(weight[(group + 1) % 2], group + 1);
       }
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int key = 32 * u + 16 * half + 4 * h + (n % 16) / 4;
+      for (int i = 0; i < kTiles; ++i)
+        acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, column[group % 2][i]),
+                                                         __builtin_bit_cast(bf16x8, weight[group % 2]), acc[i], 0, 0, 0);
+      if (more) {
+        __builtin_amdgcn_sched_group_barrier(kSchedDsRead, 2 * kTiles, 0);
 #pragma unroll
         for (int i = 0; i < kTiles; ++i) {
-          const int d = 32 * i + 16 * (n / 16) + 4 * (n % 4);
-          const u32x2 low = read_column(values + value_place(key, d / 8) + d % 8);
-          const u32x2 high = read_column(values + value_place(key + 8, d / 8) + d % 8);
-          const u32x4 w = {low[0], low[1], high[0], high[1]};
-          acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, w),
-                                                           __builtin_bit_cast(bf16x8, p[half]), acc[i], 0, 0, 0);
+          __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(kSchedValu, 28 / kTiles, 0);
         }
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
-    };
+  };
   if constexpr (E4M3) {
     for (int base = begin; base < end; base += kKeys) {
       step(base, keys_0, values_0, nullptr, nullptr);

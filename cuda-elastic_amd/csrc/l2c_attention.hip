@@ -870,12 +870,16 @@ __global__ __launch_bounds__(kThreads, kTiles <= 4 ? 2 : 1) void wide_kernel(Att
 }
 
 // ---------------------------------------------------------------------------
-// The parts of tiles that were divided: a wave a row and head.
+// The parts of tiles that were divided. A wave a row and head, or, of many parts, a workgroup, whose halves of
+// waves have every eighth part: one wave went through 64 of them in 28 us (4 x 32 rows and heads).
+constexpr int kFewParts = 8;
 
-template <int M, int STEP>
+template <int M, int STEP, bool MANY>
 __global__ __launch_bounds__(kThreads) void join_kernel(Attention a) {
-  const int lane = threadIdx.x % L2C_WAVE;
-  const int item = __builtin_amdgcn_readfirstlane(blockIdx.x * kWaves + threadIdx.x / L2C_WAVE);
+  constexpr int kBlock = 128;  // columns of a half wave
+  __shared__ __attribute__((aligned(16))) float shared[MANY ? 2 * kWaves * kBlock : 4];
+  const int lane = threadIdx.x % L2C_WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / L2C_WAVE);
+  const int item = MANY ? blockIdx.x : __builtin_amdgcn_readfirstlane(blockIdx.x * kWaves + wave);
   if (item >= a.s.rows * a.heads) return;
   const int row = item / a.heads, head = item - row * a.heads;
   int sequence, position;
@@ -897,12 +901,29 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Attention a) {
   const float weight = lane < t.parts ? exp2_of(sums.x - (most == -INFINITY ? 0.0f : most)) : 0.0f;
   const float by = inverse(l2c::wave_sum(sums.y * weight));
   const float *const values = a.part_values + first * a.width;
-  for (int d = 4 * lane; d < a.width; d += 4 * L2C_WAVE) {
+  constexpr int kLanes = kBlock / 4, kStride = MANY ? 2 * kWaves : 2;
+  const int half = (MANY ? 2 * wave : 0) + lane / kLanes, column = 4 * (lane % kLanes);
+  for (int block = 0; block < a.width; block += kBlock) {
+    const int d = block + column;
     f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int i = 0; i < t.parts; ++i)
-      sum += *reinterpret_cast<const f32x4 *>(values + static_cast<size_t>(i) * a.width + d) *
-             __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(weight), i));
-    store4(a, true, row, head, 0, d, sum * by);
+#pragma unroll 4
+    for (int i = 0; i < t.parts; i += kStride) {
+      const int part = i + half;
+      const float w = __shfl(weight, part & (L2C_WAVE - 1), L2C_WAVE);
+      if (part < t.parts && d < a.width)
+        sum += *reinterpret_cast<const f32x4 *>(values + static_cast<size_t>(part) * a.width + d) * w;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum[e] = sum_halves(sum[e]);
+    if constexpr (MANY) {
+      if (block > 0) __syncthreads();
+      if (lane < kLanes) *reinterpret_cast<f32x4 *>(shared + wave * kBlock + column) = sum;
+      __syncthreads();
+      if (wave > 0 || lane >= kLanes) continue;
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) sum += *reinterpret_cast<const f32x4 *>(shared + w * kBlock + column);
+    }
+    if (lane < kLanes && d < a.width) store4(a, true, row, head, 0, d, sum * by);
   }
 }
 
@@ -1005,10 +1026,12 @@ extern "C" int l2c_cache_attention(uint16_t *out, long long out_stride, const ui
   hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, stream, a);
   L2C_LAUNCH_CHECK();
   if (p.splits == 1) return hipSuccess;
-  const Kernel join = p.narrow      ? join_kernel<kNarrow, kNarrowStep>
-                      : width <= 128 ? join_kernel<kWide, 64>
-                                     : join_kernel<kWide, 32>;
-  const unsigned joins = static_cast<unsigned>((static_cast<long long>(rows) * heads + kWaves - 1) / kWaves);
+  const bool many = p.splits > kFewParts;
+  const Kernel join = p.narrow       ? (many ? join_kernel<kNarrow, kNarrowStep, true> : join_kernel<kNarrow, kNarrowStep, false>)
+                      : width <= 128 ? (many ? join_kernel<kWide, 64, true> : join_kernel<kWide, 64, false>)
+                                     : (many ? join_kernel<kWide, 32, true> : join_kernel<kWide, 32, false>);
+  const long long pairs = static_cast<long long>(rows) * heads;
+  const unsigned joins = static_cast<unsigned>(many ? pairs : (pairs + kWaves - 1) / kWaves);
   hipLaunchKernelGGL(join, dim3(joins), dim3(kThreads), 0, stream, a);
   L2C_LAUNCH_CHECK();
   return hipSuccess;

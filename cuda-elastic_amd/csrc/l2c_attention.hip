@@ -24,11 +24,14 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / L2C_WAVE;
 constexpr float kLog2e = 1.44269504088896340736f;
+
+__device__ const u32x4 zero_row[L2C_MAX_HEAD / 8] = {};  // of a position without a page
 
 struct Attention {
   uint16_t *out;
@@ -40,9 +43,9 @@ struct Attention {
   long long out_stride, q_stride;
   Sequences s;
   l2c::Quotient31 by_group;
-  int heads, kv_heads, group, width, window, splits, slots;
-  unsigned long long page_bytes;  // of bf16 keys
-  float scale;                    // times log2(e)
+  int heads, kv_heads, group, width, window, splits, slots, least;
+  unsigned long long page_rows;  // of all heads
+  float scale;                   // times log2(e)
 };
 
 // ---------------------------------------------------------------------------
@@ -52,7 +55,8 @@ struct Tile {
   int sequence, first, count;  // packed rows first .. first + count - 1 of the sequence's new tokens
   int start;                   // row of its first new token
   long long before;            // position of that
-  int begin, end;              // positions that any row of the tile sees
+  int from, end;               // positions that any row of the tile sees
+  int begin;                   // the last multiple of the step up to the first of them
   int chunk, parts;            // positions a part, parts that are not empty (at least 1)
 
   __device__ __forceinline__ int position(const Attention &a, int packed) const {  // -1: none
@@ -65,16 +69,16 @@ struct Tile {
   }
 };
 
-// The parts of a tile's positions: no shorter than 4 STEP, in whole STEPs from the
-// first one's.
-template <int STEP, int LEAST>
+// The parts of a tile's positions: no shorter than a.least, in whole STEPs from the first one's.
+template <int STEP>
 __device__ __forceinline__ void divide(const Attention &a, Tile &t) {
   const int last = t.position(a, t.first + t.count - 1), low = t.position(a, t.first);
   t.end = min(last, a.s.capacity() - 1) + 1;
-  t.begin = a.window ? max(0, static_cast<int>(max(0LL, static_cast<long long>(low) - a.window + 1))) / STEP * STEP : 0;
+  t.from = a.window ? max(0, low - a.window + 1) : 0;
+  t.begin = t.from / STEP * STEP;
   const int n = max(0, t.end - t.begin);
   const int each = (n + a.splits - 1) / a.splits;
-  t.chunk = max((each + STEP - 1) / STEP * STEP, LEAST);
+  t.chunk = max((each + STEP - 1) / STEP * STEP, a.least);
   t.parts = max(1, (n + t.chunk - 1) / t.chunk);
 }
 
@@ -303,10 +307,14 @@ __device__ __forceinline__ int value_place(int key, int chunk) {
   return key * D + 8 * (chunk ^ ((D == 64 ? key >> 1 & 3 : key & 7) << 1 | (key >> 3 & 1)));
 }
 
-template <int D, bool E4M3>
-__global__ __launch_bounds__(kThreads) void narrow_kernel(Attention a) {
-  constexpr int kChunks = D / 32;  // chunks of eight values a lane and key
-  constexpr int kTiles = D / 16;   // of columns
+// kChunks: of 32 columns, of which a lane has eight; those from kSure on may end before. A row has D columns in LDS.
+// Three waves a SIMD for e4m3 pages and short rows, whose bytes in flight are few (4 x 131072 in e4m3 220 us, 235
+// with two; 16 x 5 of 2500, 80 wide, 21.0 and 24.3), two for others (64 x 4096 159 us, 167 with three).
+template <int kChunks, bool E4M3>
+__global__ __launch_bounds__(kThreads, kChunks > 4 ? 1 : E4M3 || kChunks < 4 ? 3 : 2) void narrow_kernel(Attention a) {
+  constexpr int kSure = kChunks == 2 ? 0 : kChunks <= 4 ? kChunks - 1 : kChunks - 2;
+  constexpr int D = kChunks <= 2 ? 64 : kChunks <= 4 ? 128 : 256;
+  constexpr int kTiles = 2 * kChunks;  // of columns
   constexpr int kApart = 68;       // floats from row to row of the join
   constexpr int kValues = D == 64 ? 2 * kNarrow * kApart : kNarrowStep * D;
   __shared__ __attribute__((aligned(16))) uint16_t values[kWaves][kValues];
@@ -320,7 +328,7 @@ __global__ __launch_bounds__(kThreads) void narrow_kernel(Attention a) {
   const int split = block % a.splits;
   Tile t;
   if (!tile_of<kNarrow>(a, block / a.splits, t)) return;
-  divide<kNarrowStep, 4 * kNarrowStep>(a, t);
+  divide<kNarrowStep>(a, t);
   if (split >= t.parts) return;
   const int begin = t.begin + split * t.chunk, end = min(t.end, begin + t.chunk);
   const bool mine = n < t.count;
@@ -329,8 +337,12 @@ __global__ __launch_bounds__(kThreads) void narrow_kernel(Attention a) {
   const int position = mine ? t.position(a, packed) : -1;
   const int lowest = a.window ? position - a.window : -1;  // it sees those above
   const int every = t.position(a, t.first);                // all rows see positions up to this one
+  const unsigned long long head_rows = static_cast<unsigned long long>(kv) * a.s.page_size;
   const int nobody = a.window ? t.position(a, t.first + t.count - 1) - a.window : -1;  // and those above this one
 
+  // The scale's sign goes to the queries, and 0 is the least number instead, so that the largest of the products
+  // is the largest score, and -Inf stays that.
+  const float scale = fmaxf(fabsf(a.scale), FLT_MIN);
   bf16x8 q[kChunks];
 #pragma unroll
   for (int c = 0; c < kChunks; ++c) {
@@ -338,6 +350,7 @@ __global__ __launch_bounds__(kThreads) void narrow_kernel(Attention a) {
     u32x4 v = {0, 0, 0, 0};
     if (mine && d < a.width)
       v = *reinterpret_cast<const u32x4 *>(a.q + row * a.q_stride + static_cast<size_t>(head) * a.width + d);
+    if (a.scale < 0.0f) v ^= 0x80008000u;
     q[c] = __builtin_bit_cast(bf16x8, v);
   }
 
@@ -349,27 +362,52 @@ __global__ __launch_bounds__(kThreads) void narrow_kernel(Attention a) {
       page[u] = j < end ? a.s.page(t.sequence, a.s.by_page(j)) : -1;
     }
   };
+  // Where a key's row lies.
+  auto row_of = [&](int page, int j) __attribute__((always_inline)) {
+    return static_cast<unsigned long long>(static_cast<unsigned>(page)) * a.page_rows + head_rows +
+           static_cast<unsigned>(j - a.s.by_page(j) * a.s.page_size);
+  };
   Raw<E4M3> k[2][kChunks], v[2][kChunks];
-  float key_scale[2], value_scale[2];
-  bool there[2];
+  f32x4 key_scale[2], value_scale[2];  // of keys 4 g + i, which the lane has scores of
+  unsigned there;                      // keys with a page that some row sees
+  const bool fours = a.s.page_size % 4 == 0;  // four keys from a multiple of four on lie in one page
+  // The lane's part of a chunk is inside the row.
+  auto inside = [&](int c) __attribute__((always_inline)) { return c < kSure || 32 * c + 8 * g < a.width; };
   auto load = [&](const int (&page)[2], int base) __attribute__((always_inline)) {
+    const bool seen[2] = {a.s.is_page(page[0]) && base + n >= t.from, a.s.is_page(page[1]) && base + 16 + n >= t.from};
+    there = (static_cast<unsigned>(__ballot(seen[0])) & 0xffffu) | static_cast<unsigned>(__ballot(seen[1])) << 16;
+    typedef std::conditional_t<E4M3, uint8_t, uint16_t> Element;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const int j = base + 16 * u + n, slot = j - a.s.by_page(j) * a.s.page_size;
-      there[u] = a.s.is_page(page[u]);
-      const size_t at = (static_cast<size_t>(static_cast<unsigned>(page[u])) * a.kv_heads + kv) * a.s.page_size + slot;
+      const bool is = seen[u];
+      const unsigned long long of = row_of(page[u], base + 16 * u + n), at = of * a.width;
+      // Of a key without a page zeros; past the row's end its beginning, which becomes zeros, or ends in columns
+      // that nobody stores.
+      const Element *const none = reinterpret_cast<const Element *>(zero_row);
+      const Element *const key = is ? static_cast<const Element *>(a.keys) + at : none;
+      const Element *const value = is ? static_cast<const Element *>(a.values) + at : none;
 #pragma unroll
       for (int c = 0; c < kChunks; ++c) {
-        const int d = 8 * (4 * c + g);
-        k[u][c] = v[u][c] = Raw<E4M3>{};
-        if (there[u] && d < a.width) {
-          k[u][c] = load_raw<E4M3>(a.keys, at * a.width + d);
-          v[u][c] = load_raw<E4M3>(a.values, at * a.width + d);
-        }
+        const int from = inside(c) ? 32 * c + 8 * g : 0;
+        k[u][c] = *reinterpret_cast<const Raw<E4M3> *>(key + from);
+        v[u][c] = *reinterpret_cast<const Raw<E4M3> *>(value + from);
       }
       if constexpr (E4M3) {
-        key_scale[u] = there[u] ? a.key_scales[at] : 0.0f;
-        value_scale[u] = there[u] ? a.value_scales[at] : 0.0f;
+        const float *const zero = reinterpret_cast<const float *>(zero_row);
+        if (fours) {
+          const int page_of_four = __shfl(page[u], 4 * g, L2C_WAVE);
+          const unsigned long long four = row_of(page_of_four, base + 16 * u + 4 * g);
+          const bool are = a.s.is_page(page_of_four);
+          key_scale[u] = *reinterpret_cast<const f32x4_any *>(are ? a.key_scales + four : zero);
+          value_scale[u] = *reinterpret_cast<const f32x4_any *>(are ? a.value_scales + four : zero);
+        } else {
+          const float x = *(is ? a.key_scales + of : zero), y = *(is ? a.value_scales + of : zero);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            key_scale[u][i] = __shfl(x, 4 * g + i, L2C_WAVE);
+            value_scale[u][i] = __shfl(y, 4 * g + i, L2C_WAVE);
+          }
+        }
       }
     }
   };
@@ -378,7 +416,7 @@ __global__ __launch_bounds__(kThreads) void narrow_kernel(Attention a) {
   f32x4 acc[kTiles];
 #pragma unroll
   for (int i = 0; i < kTiles; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  float top = -INFINITY, total = 0.0f;
+  float top = -INFINITY, total = 0.0f;  // of the products, without the scale
   bool bad = false;
   uint16_t *const mine_values = values[wave];
   int base = begin + wave * kNarrowStep;
@@ -387,32 +425,30 @@ __global__ __launch_bounds__(kThreads) void narrow_kernel(Attention a) {
   load(page, base);
   look_up(page, base + kStride);
   for (; base < end; base += kStride) {
-    // Scores: keys 4 g + i of both halves, of query n.
-    f32x4 s[2];
-    bool seen[2][4];
-    float weight[2][4];
+    // Products of keys 4 g + i of both halves with query n.
+    f32x4 s[2], factor[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       s[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int c = 0; c < kChunks; ++c)
-        s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, as_bf16(k[u][c])), q[c], s[u], 0, 0, 0);
-      const unsigned pages = static_cast<unsigned>(__ballot(there[u])) >> (4 * g);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int j = base + 16 * u + 4 * g + i;
-        seen[u][i] = (pages >> i & 1) && j <= position && j > lowest;
-        float x = s[u][i];
-        weight[u][i] = 1.0f;
-        if constexpr (E4M3) {
-          x *= __shfl(key_scale[u], 4 * g + i, L2C_WAVE);
-          weight[u][i] = __shfl(value_scale[u], 4 * g + i, L2C_WAVE);
-        }
-        s[u][i] = seen[u][i] ? x * a.scale : -INFINITY;
+      for (int c = 0; c < kChunks; ++c) {
+        u32x4 x = as_bf16(k[u][c]);
+        if (!inside(c)) x = u32x4{0, 0, 0, 0};  // q's zeros alone would make NaN of an infinity
+        s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), q[c], s[u], 0, 0, 0);
       }
+      if constexpr (E4M3) s[u] *= key_scale[u], factor[u] = value_scale[u];
+    }
+    const bool mixed = base + kNarrowStep - 1 > every || base <= nobody;
+    if (mixed || there != 0xffffffffu) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = 16 * u + 4 * g + i, j = base + key;
+          if (!((there >> key & 1) && j <= position && j > lowest)) s[u][i] = -INFINITY;
+        }
     }
     // Values into LDS; is there one that some rows see and others do not, and that is not finite?
-    const bool mixed = base + kNarrowStep - 1 > every || base <= nobody;
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -422,7 +458,11 @@ __global__ __launch_bounds__(kThreads) void narrow_kernel(Attention a) {
         *reinterpret_cast<u32x4 *>(mine_values + value_place<D>(16 * u + n, 4 * c + g)) = w;
       }
     if constexpr (E4M3)
-      if (mixed) bad |= not_finite(value_scale[0]) || not_finite(value_scale[1]);
+      if (mixed)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)  // a scale beside one that is there may be anything
+          bad |= ((there >> (4 * g + i) & 1) && not_finite(factor[0][i])) ||
+                 ((there >> (16 + 4 * g + i) & 1) && not_finite(factor[1][i]));
     // The next step's, before anything waits for this one's.
     load(page, base + kStride);
     look_up(page, base + 2 * kStride);
@@ -432,19 +472,25 @@ __global__ __launch_bounds__(kThreads) void narrow_kernel(Attention a) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) most = fmaxf(most, s[u][i]);
     most = max_halves(max_rows(most));
-    const float shift = most == -INFINITY ? 0.0f : most;
-    const float again = exp2_of(top - shift);
-    top = most;
-    total *= again;
+    // Sums stay relative to an older maximum until a new one is 2^8 times as large: floats, and bf16 weights,
+    // are as exact there.
+    if (__ballot((most - top) * scale > 8.0f)) {
+      const float again = top == -INFINITY ? 0.0f : exp2_of((top - most) * scale);
+      total *= again;
+#pragma unroll
+      for (int i = 0; i < kTiles; ++i) acc[i] *= again;
+      top = most;
+    }
+    const float shift = top == -INFINITY ? 0.0f : top * scale;
     u32x4 p;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       float e[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        e[i] = exp2_of(s[u][i] - shift);
+        e[i] = exp2_of(fmaf(s[u][i], scale, -shift));
         total += e[i];
-        if constexpr (E4M3) e[i] = seen[u][i] ? e[i] * weight[u][i] : 0.0f;
+        if constexpr (E4M3) e[i] = s[u][i] == -INFINITY ? 0.0f : e[i] * factor[u][i];
       }
       p[2 * u] = pack2(e[0], e[1]), p[2 * u + 1] = pack2(e[2], e[3]);
     }
@@ -452,18 +498,17 @@ __global__ __launch_bounds__(kThreads) void narrow_kernel(Attention a) {
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int i = 0; i < kTiles; ++i) {
-      if (16 * i >= a.width) break;
       const int d = 16 * i + 4 * (n % 4), key = 4 * g + n / 4;
       const u32x2 low = read_column(mine_values + value_place<D>(key, d / 8) + d % 8);
       const u32x2 high = read_column(mine_values + value_place<D>(16 + key, d / 8) + d % 8);
       const u32x4 w = {low[0], low[1], high[0], high[1]};
-      acc[i] *= again;
       acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w), __builtin_bit_cast(bf16x8, p), acc[i],
                                                        0, 0, 0);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
   }
+  if (top > -INFINITY) top *= scale;
   total = sum_halves(sum_rows(total));
   if (g == 0) tops[wave][n] = top, sums[wave][n] = total;
   bad = __ballot(bad) != 0;
@@ -490,12 +535,12 @@ __global__ __launch_bounds__(kThreads) void narrow_kernel(Attention a) {
   // The waves' sums by way of LDS, 64 columns at a time.
   float *const shared = reinterpret_cast<float *>(&values[0][0]);
 #pragma unroll
-  for (int part = 0; part < D / 64; ++part) {
-    if (64 * part >= a.width) break;
+  for (int part = 0; part < (kTiles + 3) / 4; ++part) {
     if (part > 0) __syncthreads();
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      *reinterpret_cast<f32x4 *>(shared + (wave * kNarrow + n) * kApart + 16 * i + 4 * g) = acc[4 * part + i] * by;
+      if (4 * part + i < kTiles)
+        *reinterpret_cast<f32x4 *>(shared + (wave * kNarrow + n) * kApart + 16 * i + 4 * g) = acc[4 * part + i] * by;
     __syncthreads();
     // 16 rows of 64 columns by 256 lanes.
     const int r = threadIdx.x / 16, c = 4 * (threadIdx.x % 16), d = 64 * part + c;
@@ -519,8 +564,6 @@ __global__ __launch_bounds__(kThreads) void narrow_kernel(Attention a) {
 
 constexpr int kWide = 128;
 constexpr int kSchedValu = 0x002, kSchedMfma = 0x008, kSchedDsRead = 0x100;  // sched_group_barrier classes
-
-__device__ const u32x4 zero_row[L2C_MAX_HEAD / 8] = {};
 
 typedef __attribute__((address_space(1))) const void global_ptr;
 typedef __attribute__((address_space(3))) void lds_ptr;
@@ -551,7 +594,7 @@ __global__ __launch_bounds__(kThreads, kTiles <= 4 ? 2 : 1) void wide_kernel(Att
   Tile t;
   // The last tiles of a sequence see the most positions: they come first.
   if (!tile_of<kWide>(a, a.slots - 1 - block / a.splits, t)) return;
-  divide<kKeys, 4 * kKeys>(a, t);
+  divide<kKeys>(a, t);
   if (split >= t.parts) return;
   const int begin = t.begin + split * t.chunk, end = min(t.end, begin + t.chunk);
   const int first = 32 * wave;                       // of the wave's rows
@@ -587,7 +630,7 @@ __global__ __launch_bounds__(kThreads, kTiles <= 4 ? 2 : 1) void wide_kernel(Att
   // A tile's pages, a key a lane.
   auto look_up = [&](int base) __attribute__((always_inline)) {
     const int j = base + lane % kKeys;
-    return j < end ? a.s.page(t.sequence, a.s.by_page(j)) : -1;
+    return j >= t.from && j < end ? a.s.page(t.sequence, a.s.by_page(j)) : -1;
   };
   auto row_of = [&](int page, int j) __attribute__((always_inline)) {
     return (static_cast<size_t>(static_cast<unsigned>(page)) * a.kv_heads + kv) * a.s.page_size +
@@ -605,6 +648,7 @@ __global__ __launch_bounds__(kThreads, kTiles <= 4 ? 2 : 1) void wide_kernel(Att
   constexpr unsigned long long kAll = kKeys == 64 ? ~0ull : 0xffffffffull;
   const bool together = a.s.page_size % kTogether == 0;  // a wave's rows lie in one page
   const unsigned row_bytes = 2u * static_cast<unsigned>(a.width);
+  const unsigned long long page_bytes = a.page_rows * row_bytes;
   const unsigned long long head_bytes = static_cast<unsigned long long>(kv) * a.s.page_size * row_bytes;
   auto load = [&](int pages, unsigned long long there, int base, uint16_t *to_keys, uint16_t *to_values)
                   __attribute__((always_inline)) {
@@ -627,8 +671,7 @@ __global__ __launch_bounds__(kThreads, kTiles <= 4 ? 2 : 1) void wide_kernel(Att
     } else {
       // Where the lane's key lies; then a lane's 16 bytes go to LDS after those of the lane before.
       const int j = base + lane % kKeys;
-      const unsigned long long offset = static_cast<unsigned long long>(static_cast<unsigned>(pages)) * a.page_bytes +
-                                        head_bytes +
+      const unsigned long long offset = static_cast<unsigned long long>(static_cast<unsigned>(pages)) * page_bytes + head_bytes +
                                         static_cast<unsigned long long>(j - a.s.by_page(j) * a.s.page_size) * row_bytes;
       const unsigned low = static_cast<unsigned>(offset), high = static_cast<unsigned>(offset >> 32);
       const bool whole = together && (there & kAll) == kAll;
@@ -892,7 +935,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Attention a) {
   const int kv = head / a.group, packed = (row - t.start) * a.group + (head - kv * a.group);
   t.first = packed / M * M;
   t.count = min(M, (to - t.start) * a.group - t.first);
-  divide<STEP, 4 * STEP>(a, t);
+  divide<STEP>(a, t);
   if (t.parts == 1) return;  // whole already
   const size_t first = part_of(a, row, head, 0);
   // At most 64 parts: a lane each.
@@ -934,11 +977,13 @@ constexpr int kMaxSplits = 64;
 struct Plan {
   bool narrow;
   long long slots;
-  int splits;
+  int splits, least;  // the least positions of a part: a multiple of the kernels' steps
 };
 
 // Tiles of 16 rows where the sequences have no more on average, else of 128. Positions are divided
-// until there are some workgroups for every CU.
+// until there are some workgroups for every CU, but not into parts that are mostly beginnings and
+// ends: 256 positions, or, where that leaves CUs idle, 128 (16 x 5 of 2500 in tiles of 10
+// heads: 19.9 us with 256, 21.0 with 128).
 Plan plan(int sequences, int rows, int heads, int kv_heads, int page_size, int max_pages, bool starts) {
   const int group = heads / kv_heads;
   const long long packed = static_cast<long long>(rows) * group;
@@ -947,10 +992,11 @@ Plan plan(int sequences, int rows, int heads, int kv_heads, int page_size, int m
   const int m = p.narrow ? kNarrow : kWide;
   p.slots = starts ? packed / m + sequences : static_cast<long long>(sequences) * ((group + m - 1) / m);
   const long long tiles = p.slots * kv_heads, wanted = p.narrow ? 2048 : 1024;
-  const long long least = p.narrow ? 4 * kNarrowStep : 256;
+  const long long least = p.narrow && tiles < 128 ? 128 : 256;
   long long splits = wanted / tiles;
   splits = min(splits, (static_cast<long long>(max_pages) * page_size + least - 1) / least);
   splits = min(splits, (1LL << 17) / (static_cast<long long>(rows) * heads));
+  p.least = static_cast<int>(least);
   p.splits = static_cast<int>(max(1LL, min(splits, static_cast<long long>(kMaxSplits))));
   return p;
 }
@@ -963,7 +1009,12 @@ bool sizes(int sequences, int rows, int heads, int kv_heads, int width, int page
 using Kernel = void (*)(Attention);
 template <bool E4M3>
 Kernel kernel(bool narrow, int width) {
-  if (narrow) return width <= 64 ? narrow_kernel<64, E4M3> : width <= 128 ? narrow_kernel<128, E4M3> : narrow_kernel<256, E4M3>;
+  if (narrow)
+    return width <= 64    ? narrow_kernel<2, E4M3>
+           : width <= 96  ? narrow_kernel<3, E4M3>
+           : width <= 128 ? narrow_kernel<4, E4M3>
+           : width <= 192 ? narrow_kernel<6, E4M3>
+                          : narrow_kernel<8, E4M3>;
   return width <= 64    ? wide_kernel<2, E4M3>
          : width <= 96  ? wide_kernel<3, E4M3>
          : width <= 128 ? wide_kernel<4, E4M3>
@@ -1017,11 +1068,11 @@ extern "C" int l2c_cache_attention(uint16_t *out, long long out_stride, const ui
   a.out = out, a.q = q, a.keys = keys, a.values = values, a.key_scales = key_scales, a.value_scales = value_scales;
   a.part_values = parts, a.part_sums = reinterpret_cast<float2 *>(parts + (p.splits > 1 ? items * width : 0));
   a.out_stride = out_stride, a.q_stride = q_stride;
-  a.page_bytes = 2ull * kv_heads * page_size * width;
+  a.page_rows = static_cast<unsigned long long>(kv_heads) * page_size;
   a.s = l2c::sequences_of(tables, lengths, starts, sequences, rows, max_pages, page_size, pages);
   a.group = heads / kv_heads, a.by_group = l2c::Quotient31(a.group);
   a.heads = heads, a.kv_heads = kv_heads, a.width = width, a.window = window;
-  a.splits = p.splits, a.slots = static_cast<int>(p.slots), a.scale = scale * kLog2e;
+  a.splits = p.splits, a.slots = static_cast<int>(p.slots), a.least = p.least, a.scale = scale * kLog2e;
   const Kernel fn = cache_type == L2C_E4M3 ? kernel<true>(p.narrow, width) : kernel<false>(p.narrow, width);
   hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, stream, a);
   L2C_LAUNCH_CHECK();

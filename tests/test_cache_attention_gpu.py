@@ -161,6 +161,27 @@ def test_keys_of_nan_in_masked_places(torch_gpu, l2c):
         check(l2c, c, 4)
 
 
+@pytest.mark.parametrize("cache", ["bf16", "e4m3"])
+@pytest.mark.parametrize("new,window", [(1, 0), (1, 37), (3, 9), (30, 0), (30, 21), (150, 77)])
+def test_what_nobody_sees_leaves_no_trace(torch_gpu, l2c, new, window, cache):
+    """Rows of pages without a position, and positions behind the window: the same bits whatever they hold."""
+    bits = []
+    for poison in (0.0, NAN, 1.0e30, math.inf):
+        c = Cache(new + window, [new + 50, new + 7], [new, new], 2, 64, 16, cache, poison=poison)
+        q = fused(c.rows, 8 * 64, c.gen)
+        if window:
+            for s, length in enumerate(c.lengths):
+                behind = length - new - window + 1
+                if behind > 0:
+                    page, slot = c.place(s, 0, behind)
+                    for which in ("keys", "values"):
+                        getattr(c, which)[page, :, slot] = poison if cache == "bf16" else 0x7f
+                        if cache == "e4m3":
+                            getattr(c, which[:-1] + "_scales")[page, :, slot] = poison
+        bits.append(call(l2c, c, q, 8, window).view(torch.int16))
+        assert all(torch.equal(bits[0], b) for b in bits)
+
+
 @pytest.mark.parametrize("new", [1, 20])
 def test_scores_of_minus_infinity(torch_gpu, l2c, new):
     """Keys whose score is -Inf weigh nothing; a row with no other is 0."""

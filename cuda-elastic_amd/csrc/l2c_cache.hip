@@ -139,31 +139,6 @@ struct Step {
   }
 };
 
-// A workgroup a sequence: its parent's entries; and the uses, to be counted from 0.
-__global__ __launch_bounds__(256) void advance_tables_kernel(Step s) {
-  const int r = blockIdx.x;
-  for (long long i = static_cast<long long>(r) * blockDim.x + threadIdx.x; i < s.pages;
-       i += static_cast<long long>(gridDim.x) * blockDim.x)
-    s.uses[i] = 0;
-  int length, n;
-  const int p = s.parent(r, length, n);
-  const int have = min(s.pages_of(length), s.max_pages);
-  const int dropped = s.window ? max(0, length - s.window + 1) / s.page_size : 0;  // entries behind the window
-  int *const to = s.tables_out + static_cast<size_t>(r) * s.max_pages;
-  const int *const from = s.tables + static_cast<size_t>(max(p, 0)) * s.max_pages;
-  for (int i = threadIdx.x; i < s.max_pages; i += blockDim.x) to[i] = i < have && i >= dropped ? from[i] : -1;
-}
-
-__global__ __launch_bounds__(256) void advance_count_kernel(Step s) {
-  const int r = blockIdx.x;
-  int length, n;
-  s.parent(r, length, n);
-  const int have = min(s.pages_of(length), s.max_pages);
-  const int *const table = s.tables_out + static_cast<size_t>(r) * s.max_pages;
-  for (int i = threadIdx.x; i < have; i += blockDim.x)
-    if (static_cast<unsigned>(table[i]) < static_cast<unsigned>(s.pages)) atomicAdd(&s.uses[table[i]], 1);
-}
-
 __device__ __forceinline__ int now(const int *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 __device__ __forceinline__ void put(int *p, int v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
@@ -186,6 +161,33 @@ __device__ __forceinline__ long long scan_before(long long v, long long *slots, 
     all += slots[w];
   }
   return base + upto - v;
+}
+
+// A workgroup a sequence: its parent's entries; and the uses, where they are counted in place, from 0.
+template <bool USES>
+__global__ __launch_bounds__(256) void advance_tables_kernel(Step s) {
+  const int r = blockIdx.x;
+  if constexpr (USES)
+    for (long long i = static_cast<long long>(r) * blockDim.x + threadIdx.x; i < s.pages;
+         i += static_cast<long long>(gridDim.x) * blockDim.x)
+      s.uses[i] = 0;
+  int length, n;
+  const int p = s.parent(r, length, n);
+  const int have = min(s.pages_of(length), s.max_pages);
+  const int dropped = s.window ? max(0, length - s.window + 1) / s.page_size : 0;  // entries behind the window
+  int *const to = s.tables_out + static_cast<size_t>(r) * s.max_pages;
+  const int *const from = s.tables + static_cast<size_t>(max(p, 0)) * s.max_pages;
+  for (int i = threadIdx.x; i < s.max_pages; i += blockDim.x) to[i] = i < have && i >= dropped ? from[i] : -1;
+}
+
+__global__ __launch_bounds__(256) void advance_count_kernel(Step s) {
+  const int r = blockIdx.x;
+  int length, n;
+  s.parent(r, length, n);
+  const int have = min(s.pages_of(length), s.max_pages);
+  const int *const table = s.tables_out + static_cast<size_t>(r) * s.max_pages;
+  for (int i = threadIdx.x; i < have; i += blockDim.x)
+    if (static_cast<unsigned>(table[i]) < static_cast<unsigned>(s.pages)) atomicAdd(&s.uses[table[i]], 1);
 }
 
 // One workgroup: which pages are replaced, and the new pages for all sequences. A
@@ -287,6 +289,128 @@ __global__ __launch_bounds__(kAdvanceThreads) void advance_assign_kernel(Step s)
   if (t == 0) *s.shortage = static_cast<int>(min(max(total - given, 0LL) + beyond, static_cast<long long>(INT_MAX)));
 }
 
+// The same for up to 1024 sequences and as many pages as LDS has counters for, in one workgroup with a lane a
+// sequence: the steps below wait for LDS instead of memory. COPY: the tables, too, where they are small
+// enough for one workgroup to be the sooner done.
+constexpr int kLdsPages = 32768, kLdsSequences = kAdvanceThreads, kCopyEntries = 8192, kLdsEntries = 1 << 18;
+
+typedef int i32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+
+template <bool COPY>
+__global__ __launch_bounds__(kAdvanceThreads) void advance_lds_kernel(Step s) {
+  __shared__ int uses[kLdsPages];
+  __shared__ int parent[kLdsSequences], have[kLdsSequences], dropped[kLdsSequences];
+  __shared__ int base[kLdsSequences], entry[kLdsSequences], fresh[kLdsSequences];
+  __shared__ long long slots[kAdvanceThreads / L2C_WAVE];
+  const int t = threadIdx.x, lane = t % L2C_WAVE, wave = t / L2C_WAVE;
+  constexpr int kWaves = kAdvanceThreads / L2C_WAVE;
+  const bool is = t < s.sequences;
+  int length = 0, n = 0, first = 0, last = 0, page = -1;
+  if (is) {
+    const int p = s.parent(t, length, n);
+    first = s.pages_of(length), last = s.pages_of(static_cast<long long>(length) + n);
+    // The page that the sequence writes into, or -1.
+    if (n > 0 && length % s.page_size != 0 && first <= s.max_pages)
+      page = s.tables[static_cast<size_t>(p) * s.max_pages + first - 1];
+    parent[t] = max(p, 0), have[t] = min(first, s.max_pages);
+    dropped[t] = s.window ? max(0, length - s.window + 1) / s.page_size : 0;
+  }
+  for (int i = t; i < s.pages; i += kAdvanceThreads) uses[i] = 0;
+  __syncthreads();
+  auto count = [&](int e) __attribute__((always_inline)) {
+    if (static_cast<unsigned>(e) < static_cast<unsigned>(s.pages)) atomicAdd(&uses[e], 1);
+  };
+  if constexpr (COPY) {
+    // A wave a sequence, four of them at a time.
+    constexpr int kEach = 4;
+    for (int from = wave; from < s.sequences; from += kEach * kWaves)
+      for (int i = lane; i < s.max_pages; i += L2C_WAVE) {
+        int e[kEach];
+#pragma unroll
+        for (int u = 0; u < kEach; ++u) {
+          const int r = from + u * kWaves;
+          e[u] = -1;
+          if (r < s.sequences && i >= dropped[r] && i < have[r])
+            e[u] = s.tables[static_cast<size_t>(parent[r]) * s.max_pages + i];
+        }
+#pragma unroll
+        for (int u = 0; u < kEach; ++u) {
+          const int r = from + u * kWaves;
+          count(e[u]);
+          if (r < s.sequences) s.tables_out[static_cast<size_t>(r) * s.max_pages + i] = e[u];
+        }
+      }
+  } else {
+    // The tables as one array, in which all that is no sequence's is -1.
+    constexpr int kEach = 8;
+    const int all = s.sequences * s.max_pages, whole = all / 4;
+    for (int from = t; from < whole; from += kEach * kAdvanceThreads) {
+      i32x4_any e[kEach];
+#pragma unroll
+      for (int u = 0; u < kEach; ++u) {
+        const int i = from + u * kAdvanceThreads;
+        e[u] = i32x4_any{-1, -1, -1, -1};
+        if (i < whole) e[u] = *reinterpret_cast<const i32x4_any *>(s.tables_out + 4 * i);
+      }
+#pragma unroll
+      for (int u = 0; u < kEach; ++u)
+#pragma unroll
+        for (int m = 0; m < 4; ++m) count(e[u][m]);
+    }
+    if (t < all % 4) count(s.tables_out[4 * whole + t]);
+  }
+  if (static_cast<unsigned>(page) >= static_cast<unsigned>(s.pages)) page = -1;
+  const bool held = page >= 0 && s.held && s.held[page];
+  __syncthreads();
+  if (page >= 0) atomicSub(&uses[page], 1);
+  __syncthreads();
+  if (page >= 0 && uses[page] <= 0 && !held) atomicMin(&uses[page], t - s.sequences);
+  __syncthreads();
+  const bool keeps = page >= 0 && uses[page] == t - s.sequences, replaced = page >= 0 && !keeps;
+  const int upto = min(last, s.max_pages);
+  long long total, beyond;
+  const long long before = scan_before(is ? max(0, upto - first) + replaced : 0, slots, total);
+  scan_before(is ? last - max(first, upto) : 0, slots, beyond);  // its barriers part the reads of uses above from what follows
+  if (keeps) uses[page] = 1;
+  if (is) {
+    base[t] = static_cast<int>(min(before, static_cast<long long>(INT_MAX)));
+    entry[t] = first - replaced;
+    fresh[t] = -1;
+  }
+  __syncthreads();
+  // Free pages in order, each to the sequence that its rank falls to.
+  long long given = 0;
+  for (int from = 0; from < s.pages && given < total; from += kAdvanceThreads) {
+    const int of = from + t;
+    const bool free = of < s.pages && uses[of] == 0 && !(s.held && s.held[of]);
+    long long all;
+    const long long rank = given + scan_before(free, slots, all);
+    if (free && rank < total) {
+      int low = 0, high = s.sequences - 1;  // the last sequence whose first rank is at most this one
+      while (low < high) {
+        const int middle = high - (high - low) / 2;
+        if (base[middle] <= rank) low = middle;
+        else high = middle - 1;
+      }
+      const int at = static_cast<int>(rank - base[low]);
+      s.tables_out[static_cast<size_t>(low) * s.max_pages + entry[low] + at] = of;
+      if (at == 0) fresh[low] = of;
+      uses[of] = 1;
+    }
+    given += all;
+  }
+  __syncthreads();
+  if (is) {
+    const bool copied = replaced && fresh[t] >= 0;
+    if (replaced && !copied) s.tables_out[static_cast<size_t>(t) * s.max_pages + first - 1] = -1;
+    s.copies[2 * t] = copied ? page : -1;
+    s.copies[2 * t + 1] = copied ? fresh[t] : -1;
+    s.lengths_out[t] = length + n;
+  }
+  for (int i = t; i < s.pages; i += kAdvanceThreads) s.uses[i] = uses[i];
+  if (t == 0) *s.shortage = static_cast<int>(min(max(total - given, 0LL) + beyond, static_cast<long long>(INT_MAX)));
+}
+
 // ---------------------------------------------------------------------------
 // copy
 
@@ -359,7 +483,19 @@ extern "C" int l2c_cache_advance(int *tables_out, int *lengths_out, int *uses, i
     return hipErrorInvalidValue;
   const Step s = {tables_out, lengths_out, uses, copies, shortage, tables, lengths, parents, starts, held,
                   beams, sequences, pages, max_pages, page_size, window};
-  hipLaunchKernelGGL(advance_tables_kernel, dim3(sequences), dim3(256), 0, stream, s);
+  const long long entries = static_cast<long long>(sequences) * max_pages;
+  if (sequences <= kLdsSequences && pages <= kLdsPages && entries <= kLdsEntries) {
+    const bool copy = entries <= kCopyEntries;
+    if (!copy) {
+      hipLaunchKernelGGL(advance_tables_kernel<false>, dim3(sequences), dim3(256), 0, stream, s);
+      L2C_LAUNCH_CHECK();
+    }
+    hipLaunchKernelGGL(copy ? advance_lds_kernel<true> : advance_lds_kernel<false>, dim3(1), dim3(kAdvanceThreads), 0,
+                       stream, s);
+    L2C_LAUNCH_CHECK();
+    return hipSuccess;
+  }
+  hipLaunchKernelGGL(advance_tables_kernel<true>, dim3(sequences), dim3(256), 0, stream, s);
   L2C_LAUNCH_CHECK();
   hipLaunchKernelGGL(advance_count_kernel, dim3(sequences), dim3(256), 0, stream, s);
   L2C_LAUNCH_CHECK();

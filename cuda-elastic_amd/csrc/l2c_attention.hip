@@ -124,6 +124,39 @@ __device__ __forceinline__ bool tile_of(const Attention &a, int slot, Tile &t) {
   return true;
 }
 
+// The same with the tiles in the order of what they have to do, the most first: that of their sequences'
+// lengths, and of a sequence its last tile first. For up to 64 sequences, a lane each; the tiles of many are
+// in the order of the sequences, from the last. (Of three chunks of 750 to 1000 tokens over 3100 to 5000
+// positions, 680 workgroups for 512 places, the longest began last.)
+template <int M>
+__device__ __forceinline__ bool longest_tile_of(const Attention &a, int slot, Tile &t) {
+  if (!a.s.starts || a.s.sequences > L2C_WAVE) return tile_of<M>(a, a.slots - 1 - slot, t);
+  const int s = threadIdx.x % L2C_WAVE;
+  int from = 0, packed = 0, length = 0, tiles = 0;
+  if (s < a.s.sequences) {
+    from = a.s.starts[s];
+    const int to = a.s.starts[s + 1];
+    length = a.s.lengths[s];
+    // Of starts that are not in order any answer will do, within the arrays.
+    if (from >= 0 && to <= a.s.rows && from < to) packed = (to - from) * a.group, tiles = (packed + M - 1) / M;
+  }
+  int before = 0;  // tiles of longer sequences
+  for (int o = 0; o < a.s.sequences; ++o) {
+    const int other = __builtin_amdgcn_readlane(length, o), its = __builtin_amdgcn_readlane(tiles, o);
+    before += other > length || (other == length && o < s) ? its : 0;
+  }
+  const unsigned long long here = __ballot(slot >= before && slot < before + tiles);
+  if (here == 0) return false;
+  const int lane = __ffsll(here) - 1;
+  t.sequence = lane;
+  t.start = __builtin_amdgcn_readlane(from, lane);
+  packed = __builtin_amdgcn_readlane(packed, lane);
+  t.before = static_cast<long long>(__builtin_amdgcn_readlane(length, lane)) - packed / a.group;
+  t.first = (__builtin_amdgcn_readlane(tiles, lane) - 1 - (slot - __builtin_amdgcn_readlane(before, lane))) * M;
+  t.count = min(M, packed - t.first);
+  return true;
+}
+
 // ---------------------------------------------------------------------------
 // Pieces.
 
@@ -592,8 +625,7 @@ __global__ __launch_bounds__(kThreads, kTiles <= 4 ? 2 : 1) void wide_kernel(Att
   block /= a.kv_heads;
   const int split = block % a.splits;
   Tile t;
-  // The last tiles of a sequence see the most positions: they come first.
-  if (!tile_of<kWide>(a, a.slots - 1 - block / a.splits, t)) return;
+  if (!longest_tile_of<kWide>(a, block / a.splits, t)) return;
   divide<kKeys>(a, t);
   if (split >= t.parts) return;
   const int begin = t.begin + split * t.chunk, end = min(t.end, begin + t.chunk);

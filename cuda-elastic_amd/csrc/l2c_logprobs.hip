@@ -84,11 +84,12 @@ struct Row {
 template <int V, bool WHOLE>
 __global__ __launch_bounds__(kThreads) void logprobs_kernel(Args a) {
   constexpr int kPart = kThreads * 4 * V;
-  // Keys and UINT_MAX - place of the list: `top` lanes' values of each wave at most, and what
-  // order() may read.
+  // Keys and UINT_MAX - place of the list: of two parts `top` lanes' values of each wave at most, and
+  // what order() may read.
   extern __shared__ uint4 lists[];
   unsigned *const list_key = reinterpret_cast<unsigned *>(lists);
-  unsigned *const list_before = list_key + kWaves * 4 * V * a.top + 8;
+  const int unit = kWaves * 4 * V * a.top;  // values that one part can add
+  unsigned *const list_before = list_key + 2 * unit + 8;
   __shared__ __attribute__((aligned(16))) unsigned kept_key[2][kMost + 8];  // the largest so far, in order
   __shared__ unsigned kept_before[2][kMost + 8];
   __shared__ unsigned bounds[kWaves];
@@ -129,7 +130,8 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(Args a) {
   if (t < 3) lengths[t] = 0;
   double z = 0.0, s = 0.0;
   float m = -INFINITY;
-  int count = 0, turn = 0, part = 0;  // `kept` has count values
+  int count = 0, turn = 0, part = 0;  // `kept` has count values,
+  int pending = 0;                    // and the list as many
   if (top > 0) __syncthreads();
   for (int start = 0;; ++part) {
     const int n = min(kPart, whole - start);
@@ -206,23 +208,26 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(Args a) {
         const int count_here = __popc(reach), upto = wave_scan(count_here);
         int base = 0;
         if (lane == L2C_WAVE - 1) base = atomicAdd(&lengths[part % 3], upto);
-        int to = __builtin_amdgcn_readlane(base, L2C_WAVE - 1) + upto - count_here;
-#pragma unroll
-        for (int c = 0; c < V; ++c) {
-          if (__ballot(reach >> 4 * c & 15u) == 0) continue;
-#pragma unroll
-          for (int i = 4 * c; i < 4 * c + 4; ++i)
-            if (reach >> i & 1) {
-              list_key[to] = key_of(v[i]);
-              list_before[to++] = UINT_MAX - (static_cast<unsigned>(start) + place(i));
-            }
+        int to = pending + __builtin_amdgcn_readlane(base, L2C_WAVE - 1) + upto - count_here;
+        // Their places alone; the values are read again where they are put in order.
+        while (__ballot(reach != 0)) {
+          if (reach != 0) {
+            const int i = __ffs(reach) - 1;
+            list_before[to++] = UINT_MAX - (static_cast<unsigned>(start) + place(i));
+            reach &= reach - 1;
+          }
         }
       }
       __syncthreads();
-      const int listed = __builtin_amdgcn_readfirstlane(lengths[part % 3]);
+      pending += __builtin_amdgcn_readfirstlane(lengths[part % 3]);
       if (t == 0) lengths[(part + 2) % 3] = 0;  // read before this barrier, used after the next
-      if (listed > 0) {
-        const int all = count + listed;
+      // While there is a bound the list only grows, until there are enough of them to find a closer bound by (2048 x
+      // 32003, top 20: 70 us with 64, 74 with 128, 77 as long as they fit); then, or at the end, its values and
+      // the kept ones are put in order.
+      if (pending > 0 && (!more || count < top || pending > min(unit, 64))) {
+        const int listed = pending, all = count + listed;
+        for (int e = t; e < listed; e += kThreads) list_key[e] = key_of(x[UINT_MAX - list_before[e]]);
+        __syncthreads();
         for (int e = t; e < all; e += kThreads) {
           const bool old = e < count;
           const unsigned mine = old ? kept_key[turn][e] : list_key[e - count];
@@ -237,6 +242,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(Args a) {
           if (among.larger < top) kept_key[turn ^ 1][among.larger] = mine, kept_before[turn ^ 1][among.larger] = before;
         }
         count = min(all, top);
+        pending = 0;
         turn ^= 1;
         __syncthreads();
       }
@@ -329,7 +335,8 @@ struct Plan {
 };
 
 // A row a workgroup from 512 rows on (or of no more than 2048 logits), else chunks for about 1024
-// workgroups, of 2048 logits at least.
+// workgroups, of 2048 logits at least. No more than 4096 logits in registers at a time: 8192 leave two
+// waves a SIMD (2048 x 32003 78 us, 96 so).
 Plan plan(int vocab, int rows) {
   int chunks = 1;
   if (rows < 512) {
@@ -339,7 +346,7 @@ Plan plan(int vocab, int rows) {
   Plan p;
   p.chunk = (vocab - 1) / chunks + 1;
   p.chunks = (vocab - 1) / p.chunk + 1;
-  p.v = p.chunk <= 1024 ? 1 : p.chunk <= 2048 ? 2 : p.chunk <= 4096 ? 4 : 8;
+  p.v = p.chunk <= 1024 ? 1 : p.chunk <= 2048 ? 2 : 4;
   return p;
 }
 
@@ -372,8 +379,8 @@ extern "C" int l2c_decoder_logprobs(float *logprobs, float *entropies, int *top_
   const Args a = {logprobs, entropies, top_tokens, top_logprobs, logits, tokens, static_cast<unsigned char *>(workspace),
                   vocab, top, p.chunks, p.chunk};
   const bool whole = p.chunks == 1;
-  const Kernel fn = p.v == 1 ? kernel<1>(whole) : p.v == 2 ? kernel<2>(whole) : p.v == 4 ? kernel<4>(whole) : kernel<8>(whole);
-  const size_t list = 2 * sizeof(unsigned) * (kWaves * static_cast<size_t>(top) * 4 * p.v + 8);
+  const Kernel fn = p.v == 1 ? kernel<1>(whole) : p.v == 2 ? kernel<2>(whole) : kernel<4>(whole);
+  const size_t list = 2 * sizeof(unsigned) * (2 * kWaves * static_cast<size_t>(top) * 4 * p.v + 8);
   hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(grid)), dim3(kThreads), list, stream, a);
   L2C_LAUNCH_CHECK();
   if (whole) return hipSuccess;

@@ -196,6 +196,13 @@ __device__ __forceinline__ bool not_finite(u32x4 v) {
 }
 __device__ __forceinline__ bool not_finite(float v) { return !(fabsf(v) <= FLT_MAX); }
 
+// Which of 32 positions in a row a row sees: those with a page, up to the `to`-th, after the `from`-th.
+__device__ __forceinline__ unsigned seen_of_32(unsigned there, int to, int from) {
+  const unsigned upto = to < 0 ? 0u : to >= 31 ? ~0u : (2u << to) - 1u;
+  const unsigned behind = from < 0 ? 0u : from >= 31 ? ~0u : (2u << from) - 1u;
+  return there & upto & ~behind;
+}
+
 // Values across lanes without a trip through LDS: of both lanes that differ in bit 5, or bit 4.
 __device__ __forceinline__ float max_halves(float v) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -473,13 +480,12 @@ __global__ __launch_bounds__(kThreads, kChunks > 4 ? 1 : E4M3 || kChunks < 4 ? 3
     }
     const bool mixed = base + kNarrowStep - 1 > every || base <= nobody;
     if (mixed || there != 0xffffffffu) {
+      const unsigned seen = seen_of_32(there, position - base, lowest - base);
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int key = 16 * u + 4 * g + i, j = base + key;
-          if (!((there >> key & 1) && j <= position && j > lowest)) s[u][i] = -INFINITY;
-        }
+        for (int i = 0; i < 4; ++i)
+          if (!(seen >> (16 * u + 4 * g + i) & 1)) s[u][i] = -INFINITY;
     }
     // Values into LDS; is there one that some rows see and others do not, and that is not finite?
 #pragma unroll
@@ -824,15 +830,15 @@ __global__ __launch_bounds__(kThreads, kTiles <= 4 ? 2 : 1) void wide_kernel(Att
         }
     }
     if (base + kKeys - 1 > whole_to || base <= whole_from || (there & kAll) != kAll) {
-      const unsigned long long mine_there = there >> (4 * h);
-      const int to = position - base - 4 * h, from = lowest - base - 4 * h;
 #pragma unroll
-      for (int u = 0; u < kParts; ++u)
+      for (int u = 0; u < kParts; ++u) {
+        const unsigned seen = seen_of_32(static_cast<unsigned>(there >> (32 * u)), position - base - 32 * u,
+                                         lowest - base - 32 * u) >>
+                              (4 * h);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int at = 32 * u + 8 * (i / 4) + i % 4;
-          if (!((mine_there >> at & 1) && at <= to && at > from)) s[u][i] = -INFINITY;
-        }
+        for (int i = 0; i < 16; ++i)
+          if (!(seen >> (8 * (i / 4) + i % 4) & 1)) s[u][i] = -INFINITY;
+      }
     }
     float most = top;
 #pragma unroll

@@ -300,3 +300,35 @@ def test_repeated_and_captured(torch_gpu, l2c, new):
         assert torch.equal(out.view(torch.int16), want[i % 2].view(torch.int16))
         again = call(l2c, (d, c)[i % 2], qs[1 - i % 2], heads, workspace=ws)
         assert torch.equal(again.view(torch.int16), want[1 - i % 2].view(torch.int16))
+
+
+# Chunks long enough, over heads enough, for tiles of 256 rows (64 key heads, and 2048 rows for each).
+@pytest.mark.parametrize("width,page,window", [(64, 16, 0), (128, 16, 0), (80, 48, 0), (96, 5, 0), (128, 64, 130), (40, 16, 1),
+                                               (120, 16, 1000)])
+def test_many_rows_and_heads(torch_gpu, l2c, width, page, window):
+    lengths, new = [1500, 700, 3, 90, 1333], [1400, 650, 0, 90, 1]
+    c = Cache(width + window, lengths, new, 64, width, page, rows_behind=3)
+    q = fused(c.rows, 64 * width, c.gen, 8)
+    peaked(c, q, 64, [0, 1, 63, 64, 65, 127, 128, 700, 1435, 1436, 1498, 1499])
+    check(l2c, c, 64, window=window, q=q)
+
+
+@pytest.mark.parametrize("scale", [None, -0.7, 0.0])
+def test_many_rows_of_shared_heads(torch_gpu, l2c, scale):
+    c = Cache(3, [800, 1111], [260, 777], 31, 64, 16)
+    check(l2c, c, 31 * 4, scale=scale)
+
+
+@pytest.mark.parametrize("bad", [NAN, math.inf])
+def test_many_rows_over_masked_places(torch_gpu, l2c, bad):
+    """Values that are not finite where some rows of a tile see them; pages that are not there; -Inf scores."""
+    c = Cache(4, [2200, 300], [2000, 100], 64, 64, 16)
+    for at in (2199, 1700, 201, 5):
+        row = torch.zeros(1, 64, 64, device="cuda")
+        row[:, 3, 5::7] = bad
+        c.dense[0][1][:, at] = c.put(0, at, "values", row)[:, 0]
+    none = [(0, 0), (0, 3), (0, 77), (1, 2)] + [(0, i) for i in range(100, 109)]
+    for s, column in none:
+        c.tables[s, column] = -1
+    check(l2c, c, 64, no_page=none)
+    check(l2c, c, 64, no_page=none, window=90)

@@ -595,27 +595,31 @@ __global__ __launch_bounds__(kThreads, kChunks > 4 ? 1 : E4M3 || kChunks < 4 ? 3
 }
 
 // ---------------------------------------------------------------------------
-// Tiles of 128 rows, 32 a wave: chunks of a prompt. Bound by the matrix and the vector units, and by
-// LDS, which each wave reads whole tiles from. The workgroup's keys and values, 64 positions
-// at a time (32 of more than 128 columns), lie in LDS, two tiles of them: while one is read, the
-// next is on its way. bf16 pages go to LDS without registers between, rows that are not there
-// from a row of zeros; e4m3 pages through registers, where they become bf16.
+// Tiles of 32 rows a wave: chunks of a prompt. Bound by the matrix and the vector units, and by LDS, which each
+// wave reads whole tiles from. The workgroup's keys and values, 64 positions at a time (32 of more than 128
+// columns), lie in LDS, two tiles of them: while one is read, the next is on its way. bf16 pages go to LDS
+// without registers between, rows that are not there from a row of zeros; e4m3 pages through registers, where
+// they become bf16. Four waves share a tile, so that two workgroups fit a CU, or eight, for which half as much is
+// loaded (a chunk of 4096 over 16384 positions 896 us, 982 with four; three of 1000 over 5000 208 and 223), where
+// 128 columns make that worth it and the tiles are enough (four chunks of 300 over 2000 57 us with four, 64 with
+// eight; 64 columns the same with both). Four waves of more than 128 columns need the registers of eight.
 
-constexpr int kWide = 128;
+constexpr int kManyWaves = 8, kWide = 32 * kWaves, kWideMany = 32 * kManyWaves;
 constexpr int kSchedValu = 0x002, kSchedMfma = 0x008, kSchedDsRead = 0x100;  // sched_group_barrier classes
 
 typedef __attribute__((address_space(1))) const void global_ptr;
 typedef __attribute__((address_space(3))) void lds_ptr;
 
 // kTiles: tiles of 32 columns, of which there are some; a row has D columns in LDS.
-template <int kTiles, bool E4M3>
-__global__ __launch_bounds__(kThreads, kTiles <= 4 ? 2 : 1) void wide_kernel(Attention a) {
+template <int kTiles, int kTileWaves, bool E4M3>
+__global__ __launch_bounds__(kTileWaves * L2C_WAVE, kTiles <= 4 && kTileWaves == kWaves ? 2 : 1) void wide_kernel(Attention a) {
+  constexpr int kLaneCount = kTileWaves * L2C_WAVE;
   constexpr int D = kTiles <= 2 ? 64 : kTiles <= 4 ? 128 : 256;
   constexpr int kKeys = D <= 128 ? 64 : 32;
   constexpr int kLanes = D / 8;               // that load a row
-  constexpr int kRows = kThreads / kLanes;    // rows loaded together
+  constexpr int kRows = kLaneCount / kLanes;    // rows loaded together
   constexpr int kPasses = kKeys / kRows;
-  constexpr int kTogether = kRows / kWaves;   // of them by one wave
+  constexpr int kTogether = kRows / kTileWaves;   // of them by one wave
   constexpr int kSteps = 2 * kTiles, kParts = kKeys / 32;
   // Two of each, with names of their own: of one array's halves the compiler would wait for the loads into one
   // before it reads the other.
@@ -631,7 +635,7 @@ __global__ __launch_bounds__(kThreads, kTiles <= 4 ? 2 : 1) void wide_kernel(Att
   block /= a.kv_heads;
   const int split = block % a.splits;
   Tile t;
-  if (!longest_tile_of<kWide>(a, block / a.splits, t)) return;
+  if (!longest_tile_of<32 * kTileWaves>(a, block / a.splits, t)) return;
   divide<kKeys>(a, t);
   if (split >= t.parts) return;
   const int begin = t.begin + split * t.chunk, end = min(t.end, begin + t.chunk);
@@ -780,7 +784,7 @@ __global__ __launch_bounds__(kThreads, kTiles <= 4 ? 2 : 1) void wide_kernel(Att
       if (mixed)
 #pragma unroll
         for (int i = 0; i < kPasses; ++i)
-          bad |= not_finite(*reinterpret_cast<const u32x4 *>(values + 8 * (i * kThreads + threadIdx.x)));
+          bad |= not_finite(*reinterpret_cast<const u32x4 *>(values + 8 * (i * kLaneCount + threadIdx.x)));
     }
     if (mixed && __ballot(bad) && lane == 0) dirty = 1;
     next_there = __ballot(a.s.is_page(pages));
@@ -929,8 +933,8 @@ __global__ __launch_bounds__(kThreads, kTiles <= 4 ? 2 : 1) void wide_kernel(Att
   __syncthreads();
   if (dirty) {
     float *const row_q = reinterpret_cast<float *>(keys_0) + wave * L2C_MAX_HEAD;
-    static_assert(sizeof(keys_0) >= kWaves * L2C_MAX_HEAD * sizeof(float), "room for the queries");
-    for (int r = wave; r < t.count; r += kWaves) lone_row<E4M3>(a, t, kv, t.first + r, split, begin, end, row_q);
+    static_assert(sizeof(keys_0) >= kTileWaves * L2C_MAX_HEAD * sizeof(float), "room for the queries");
+    for (int r = wave; r < t.count; r += kTileWaves) lone_row<E4M3>(a, t, kv, t.first + r, split, begin, end, row_q);
     return;
   }
   total = sum_halves(total);
@@ -1013,24 +1017,25 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Attention a) {
 constexpr int kMaxSplits = 64;
 
 struct Plan {
-  bool narrow;
+  int rows;  // of a tile: kNarrow, kWide or kWideMany
   long long slots;
   int splits, least;  // the least positions of a part: a multiple of the kernels' steps
 };
 
-// Tiles of 16 rows where the sequences have no more on average, else of 128. Positions are divided
+// Tiles of 16 rows where the sequences have no more on average, else of 128, or of 256. Positions are divided
 // until there are some workgroups for every CU, but not into parts that are mostly beginnings and
 // ends: 256 positions, or, where that leaves CUs idle, 128 (16 x 5 of 2500 in tiles of 10
 // heads: 19.9 us with 256, 21.0 with 128).
-Plan plan(int sequences, int rows, int heads, int kv_heads, int page_size, int max_pages, bool starts) {
+Plan plan(int sequences, int rows, int heads, int kv_heads, int width, int page_size, int max_pages, bool starts) {
   const int group = heads / kv_heads;
   const long long packed = static_cast<long long>(rows) * group;
   Plan p;
-  p.narrow = packed <= 16LL * sequences;
-  const int m = p.narrow ? kNarrow : kWide;
+  const bool narrow = packed <= 16LL * sequences;
+  const bool many = width > 96 && width <= 128 && packed / kWideMany * kv_heads >= 256;
+  const int m = p.rows = narrow ? kNarrow : many ? kWideMany : kWide;
   p.slots = starts ? packed / m + sequences : static_cast<long long>(sequences) * ((group + m - 1) / m);
-  const long long tiles = p.slots * kv_heads, wanted = p.narrow ? 2048 : 1024;
-  const long long least = p.narrow && tiles < 128 ? 128 : 256;
+  const long long tiles = p.slots * kv_heads, wanted = narrow ? 2048 : 512;
+  const long long least = narrow && tiles < 128 ? 128 : 256;
   long long splits = wanted / tiles;
   splits = min(splits, (static_cast<long long>(max_pages) * page_size + least - 1) / least);
   splits = min(splits, (1LL << 17) / (static_cast<long long>(rows) * heads));
@@ -1046,18 +1051,24 @@ bool sizes(int sequences, int rows, int heads, int kv_heads, int width, int page
 
 using Kernel = void (*)(Attention);
 template <bool E4M3>
-Kernel kernel(bool narrow, int width) {
-  if (narrow)
+Kernel kernel(int rows, int width) {
+  if (rows == kNarrow)
     return width <= 64    ? narrow_kernel<2, E4M3>
            : width <= 96  ? narrow_kernel<3, E4M3>
            : width <= 128 ? narrow_kernel<4, E4M3>
            : width <= 192 ? narrow_kernel<6, E4M3>
                           : narrow_kernel<8, E4M3>;
-  return width <= 64    ? wide_kernel<2, E4M3>
-         : width <= 96  ? wide_kernel<3, E4M3>
-         : width <= 128 ? wide_kernel<4, E4M3>
-         : width <= 192 ? wide_kernel<6, E4M3>
-                        : wide_kernel<8, E4M3>;
+  return width <= 64         ? wide_kernel<2, kWaves, E4M3>
+         : width <= 96       ? wide_kernel<3, kWaves, E4M3>
+         : rows == kWideMany ? wide_kernel<4, kManyWaves, E4M3>
+         : width <= 128      ? wide_kernel<4, kWaves, E4M3>
+         : width <= 192      ? wide_kernel<6, kWaves, E4M3>
+                             : wide_kernel<8, kWaves, E4M3>;
+}
+
+template <int M, int STEP>
+Kernel join_of(bool many) {
+  return many ? join_kernel<M, STEP, true> : join_kernel<M, STEP, false>;
 }
 
 size_t part_bytes(const Plan &p, int rows, int heads, int width) {
@@ -1070,10 +1081,10 @@ extern "C" size_t l2c_cache_attention_workspace_bytes(int sequences, int rows, i
                                                       int page_size, int max_pages) {
   if (!sizes(sequences, rows, heads, kv_heads, width, page_size, 0, max_pages) || sequences == 0 || rows == 0) return 0;
   // What a call with starts needs, or without: the fewer slots, the more parts.
-  const size_t with = part_bytes(plan(sequences, rows, heads, kv_heads, page_size, max_pages, true), rows, heads, width);
+  const size_t with = part_bytes(plan(sequences, rows, heads, kv_heads, width, page_size, max_pages, true), rows, heads, width);
   const size_t without = rows != sequences
                              ? 0
-                             : part_bytes(plan(sequences, rows, heads, kv_heads, page_size, max_pages, false), rows, heads, width);
+                             : part_bytes(plan(sequences, rows, heads, kv_heads, width, page_size, max_pages, false), rows, heads, width);
   return with > without ? with : without;
 }
 
@@ -1095,7 +1106,7 @@ extern "C" int l2c_cache_attention(uint16_t *out, long long out_stride, const ui
       !q || !out || !l2c_aligned16(q) || !l2c_aligned16(out) || workspace_bytes < need ||
       (need > 0 && (!workspace || !l2c_aligned16(workspace))))
     return hipErrorInvalidValue;
-  const Plan p = plan(sequences, rows, heads, kv_heads, page_size, max_pages, starts != nullptr);
+  const Plan p = plan(sequences, rows, heads, kv_heads, width, page_size, max_pages, starts != nullptr);
   const long long grid = p.slots * kv_heads * p.splits;
   if (static_cast<long long>(rows) * heads > INT_MAX || p.slots > INT_MAX || grid > INT_MAX ||
       !l2c::launchable(grid, kThreads))
@@ -1111,14 +1122,16 @@ extern "C" int l2c_cache_attention(uint16_t *out, long long out_stride, const ui
   a.group = heads / kv_heads, a.by_group = l2c::Quotient31(a.group);
   a.heads = heads, a.kv_heads = kv_heads, a.width = width, a.window = window;
   a.splits = p.splits, a.slots = static_cast<int>(p.slots), a.least = p.least, a.scale = scale * kLog2e;
-  const Kernel fn = cache_type == L2C_E4M3 ? kernel<true>(p.narrow, width) : kernel<false>(p.narrow, width);
-  hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, stream, a);
+  const Kernel fn = cache_type == L2C_E4M3 ? kernel<true>(p.rows, width) : kernel<false>(p.rows, width);
+  hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(grid)), dim3(p.rows == kWideMany ? kManyWaves * L2C_WAVE : kThreads), 0, stream,
+                     a);
   L2C_LAUNCH_CHECK();
   if (p.splits == 1) return hipSuccess;
   const bool many = p.splits > kFewParts;
-  const Kernel join = p.narrow       ? (many ? join_kernel<kNarrow, kNarrowStep, true> : join_kernel<kNarrow, kNarrowStep, false>)
-                      : width <= 128 ? (many ? join_kernel<kWide, 64, true> : join_kernel<kWide, 64, false>)
-                                     : (many ? join_kernel<kWide, 32, true> : join_kernel<kWide, 32, false>);
+  const Kernel join = p.rows == kNarrow     ? join_of<kNarrow, kNarrowStep>(many)
+                      : p.rows == kWideMany ? join_of<kWideMany, 64>(many)
+                      : width <= 128        ? join_of<kWide, 64>(many)
+                                            : join_of<kWide, 32>(many);
   const long long pairs = static_cast<long long>(rows) * heads;
   const unsigned joins = static_cast<unsigned>(many ? pairs : (pairs + kWaves - 1) / kWaves);
   hipLaunchKernelGGL(join, dim3(joins), dim3(kThreads), 0, stream, a);

@@ -313,6 +313,15 @@ def test_many_rows_and_heads(torch_gpu, l2c, width, page, window):
     check(l2c, c, 64, window=window, q=q)
 
 
+@pytest.mark.parametrize("width,page,window", [(128, 16, 0), (104, 20, 300)])
+def test_many_rows_of_e4m3(torch_gpu, l2c, width, page, window):
+    lengths, new = [1500, 3, 900], [1400, 1, 850]
+    c = Cache(width, lengths, new, 64, width, page, "e4m3")
+    q = fused(c.rows, 64 * width, c.gen)
+    peaked(c, q, 64, [0, 63, 64, 700, 1499])
+    check(l2c, c, 64, window=window, q=q)
+
+
 @pytest.mark.parametrize("scale", [None, -0.7, 0.0])
 def test_many_rows_of_shared_heads(torch_gpu, l2c, scale):
     c = Cache(3, [800, 1111], [260, 777], 31, 64, 16)

@@ -348,11 +348,14 @@ __device__ __forceinline__ int value_place(int key, int chunk) {
 }
 
 // kChunks: of 32 columns, of which a lane has eight; those from kSure on may end before. A row has D columns in LDS.
+// PAIRS: of e4m3 pages a lane has sixteen columns in a row for two chunks, so that it loads 16 bytes at a time, too
+// (4 x 131072 166 us, 215 with eight, and as long without any arithmetic; rows of an odd number of eights are loaded so).
 // Three waves a SIMD for e4m3 pages and short rows, whose bytes in flight are few (4 x 131072 in e4m3 220 us, 235
 // with two; 16 x 5 of 2500, 80 wide, 21.0 and 24.3), two for others (64 x 4096 159 us, 167 with three).
-template <int kChunks, bool E4M3>
+template <int kChunks, bool E4M3, bool PAIRS>
 __global__ __launch_bounds__(kThreads, kChunks > 4 ? 1 : E4M3 || kChunks < 4 ? 3 : 2) void narrow_kernel(Attention a) {
-  constexpr int kSure = kChunks == 2 ? 0 : kChunks <= 4 ? kChunks - 1 : kChunks - 2;
+  static_assert(!PAIRS || kChunks % 2 == 0, "two chunks a load");
+  constexpr int kSure = PAIRS ? kChunks - 2 : kChunks == 2 ? 0 : kChunks <= 4 ? kChunks - 1 : kChunks - 2;
   constexpr int D = kChunks <= 2 ? 64 : kChunks <= 4 ? 128 : 256;
   constexpr int kTiles = 2 * kChunks;  // of columns
   constexpr int kApart = 68;       // floats from row to row of the join
@@ -383,10 +386,13 @@ __global__ __launch_bounds__(kThreads, kChunks > 4 ? 1 : E4M3 || kChunks < 4 ? 3
   // The scale's sign goes to the queries, and 0 is the least number instead, so that the largest of the products
   // is the largest score, and -Inf stays that.
   const float scale = fmaxf(fabsf(a.scale), FLT_MIN);
+  auto column = [&](int c) __attribute__((always_inline)) {  // the lane's first of a chunk
+    return PAIRS ? 64 * (c / 2) + 16 * g + 8 * (c % 2) : 32 * c + 8 * g;
+  };
   bf16x8 q[kChunks];
 #pragma unroll
   for (int c = 0; c < kChunks; ++c) {
-    const int d = 8 * (4 * c + g);
+    const int d = column(c);
     u32x4 v = {0, 0, 0, 0};
     if (mine && d < a.width)
       v = *reinterpret_cast<const u32x4 *>(a.q + row * a.q_stride + static_cast<size_t>(head) * a.width + d);
@@ -412,7 +418,7 @@ __global__ __launch_bounds__(kThreads, kChunks > 4 ? 1 : E4M3 || kChunks < 4 ? 3
   unsigned there;                      // keys with a page that some row sees
   const bool fours = a.s.page_size % 4 == 0;  // four keys from a multiple of four on lie in one page
   // The lane's part of a chunk is inside the row.
-  auto inside = [&](int c) __attribute__((always_inline)) { return c < kSure || 32 * c + 8 * g < a.width; };
+  auto inside = [&](int c) __attribute__((always_inline)) { return c < kSure || column(c) < a.width; };
   auto load = [&](const int (&page)[2], int base) __attribute__((always_inline)) {
     const bool seen[2] = {a.s.is_page(page[0]) && base + n >= t.from, a.s.is_page(page[1]) && base + 16 + n >= t.from};
     there = (static_cast<unsigned>(__ballot(seen[0])) & 0xffffu) | static_cast<unsigned>(__ballot(seen[1])) << 16;
@@ -427,10 +433,16 @@ __global__ __launch_bounds__(kThreads, kChunks > 4 ? 1 : E4M3 || kChunks < 4 ? 3
       const Element *const key = is ? static_cast<const Element *>(a.keys) + at : none;
       const Element *const value = is ? static_cast<const Element *>(a.values) + at : none;
 #pragma unroll
-      for (int c = 0; c < kChunks; ++c) {
-        const int from = inside(c) ? 32 * c + 8 * g : 0;
-        k[u][c] = *reinterpret_cast<const Raw<E4M3> *>(key + from);
-        v[u][c] = *reinterpret_cast<const Raw<E4M3> *>(value + from);
+      for (int c = 0; c < kChunks; c += PAIRS ? 2 : 1) {
+        const int from = inside(c) ? column(c) : 0;
+        if constexpr (PAIRS) {
+          const u32x4 x = *reinterpret_cast<const u32x4 *>(key + from), y = *reinterpret_cast<const u32x4 *>(value + from);
+          k[u][c] = u32x2{x[0], x[1]}, k[u][c + 1] = u32x2{x[2], x[3]};
+          v[u][c] = u32x2{y[0], y[1]}, v[u][c + 1] = u32x2{y[2], y[3]};
+        } else {
+          k[u][c] = *reinterpret_cast<const Raw<E4M3> *>(key + from);
+          v[u][c] = *reinterpret_cast<const Raw<E4M3> *>(value + from);
+        }
       }
       if constexpr (E4M3) {
         const float *const zero = reinterpret_cast<const float *>(zero_row);
@@ -494,7 +506,7 @@ __global__ __launch_bounds__(kThreads, kChunks > 4 ? 1 : E4M3 || kChunks < 4 ? 3
       for (int c = 0; c < kChunks; ++c) {
         const u32x4 w = as_bf16(v[u][c]);
         if (mixed) bad |= not_finite(w);
-        *reinterpret_cast<u32x4 *>(mine_values + value_place<D>(16 * u + n, 4 * c + g)) = w;
+        *reinterpret_cast<u32x4 *>(mine_values + value_place<D>(16 * u + n, column(c) / 8)) = w;
       }
     if constexpr (E4M3)
       if (mixed)
@@ -1052,12 +1064,18 @@ bool sizes(int sequences, int rows, int heads, int kv_heads, int width, int page
 using Kernel = void (*)(Attention);
 template <bool E4M3>
 Kernel kernel(int rows, int width) {
-  if (rows == kNarrow)
-    return width <= 64    ? narrow_kernel<2, E4M3>
-           : width <= 96  ? narrow_kernel<3, E4M3>
-           : width <= 128 ? narrow_kernel<4, E4M3>
-           : width <= 192 ? narrow_kernel<6, E4M3>
-                          : narrow_kernel<8, E4M3>;
+  if (rows == kNarrow) {
+    if (E4M3 && width % 16 == 0)
+      return width <= 64    ? narrow_kernel<2, E4M3, E4M3>
+             : width <= 128 ? narrow_kernel<4, E4M3, E4M3>
+             : width <= 192 ? narrow_kernel<6, E4M3, E4M3>
+                            : narrow_kernel<8, E4M3, E4M3>;
+    return width <= 64    ? narrow_kernel<2, E4M3, false>
+           : width <= 96  ? narrow_kernel<3, E4M3, false>
+           : width <= 128 ? narrow_kernel<4, E4M3, false>
+           : width <= 192 ? narrow_kernel<6, E4M3, false>
+                          : narrow_kernel<8, E4M3, false>;
+  }
   return width <= 64         ? wide_kernel<2, kWaves, E4M3>
          : width <= 96       ? wide_kernel<3, kWaves, E4M3>
          : rows == kWideMany ? wide_kernel<4, kManyWaves, E4M3>

@@ -30,6 +30,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / L2C_WAVE;
 constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kSlack = 8.0f;
 
 __device__ const u32x4 zero_row[L2C_MAX_HEAD / 8] = {};  // of a position without a page
 
@@ -378,7 +379,7 @@ __global__ __launch_bounds__(kThreads, kChunks > 4 ? 1 : E4M3 || kChunks < 4 ? 3
   const int packed = t.first + (mine ? n : 0);
   const int row = t.row(a, packed), head = t.head(a, kv, packed);
   const int position = mine ? t.position(a, packed) : -1;
-  const int lowest = a.window ? position - a.window : -1;  // it sees those above
+  const int lowest = a.window ? max(-1, position - a.window) : -1;  // it sees those above
   const int every = t.position(a, t.first);                // all rows see positions up to this one
   const unsigned long long head_rows = static_cast<unsigned long long>(kv) * a.s.page_size;
   const int nobody = a.window ? t.position(a, t.first + t.count - 1) - a.window : -1;  // and those above this one
@@ -523,16 +524,16 @@ __global__ __launch_bounds__(kThreads, kChunks > 4 ? 1 : E4M3 || kChunks < 4 ? 3
 #pragma unroll
       for (int i = 0; i < 4; ++i) most = fmaxf(most, s[u][i]);
     most = max_halves(max_rows(most));
-    // Sums stay relative to an older maximum until a new one is 2^8 times as large: floats, and bf16 weights,
-    // are as exact there.
-    if (__ballot((most - top) * scale > 8.0f)) {
+    // Sums stay relative to an older maximum until a new one is more than 2^kSlack times as large. Weights are
+    // 2^-kSlack of the softmax's, so that none is above 1 and large values do not overflow.
+    if (__ballot((most - top) * scale > kSlack)) {
       const float again = top == -INFINITY ? 0.0f : exp2_of((top - most) * scale);
       total *= again;
 #pragma unroll
       for (int i = 0; i < kTiles; ++i) acc[i] *= again;
       top = most;
     }
-    const float shift = top == -INFINITY ? 0.0f : top * scale;
+    const float shift = top == -INFINITY ? 0.0f : fmaf(top, scale, kSlack);
     u32x4 p;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -559,7 +560,7 @@ __global__ __launch_bounds__(kThreads, kChunks > 4 ? 1 : E4M3 || kChunks < 4 ? 3
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
   }
-  if (top > -INFINITY) top *= scale;
+  if (top > -INFINITY) top = fmaf(top, scale, kSlack);  // what its sums are relative to
   total = sum_halves(sum_rows(total));
   if (g == 0) tops[wave][n] = top, sums[wave][n] = total;
   bad = __ballot(bad) != 0;
@@ -657,7 +658,7 @@ __global__ __launch_bounds__(kTileWaves * L2C_WAVE, kTiles <= 4 && kTileWaves ==
   const int packed = t.first + (mine ? first + n : 0);
   const int row = t.row(a, packed), head = t.head(a, kv, packed);
   const int position = mine ? t.position(a, packed) : -1;
-  const int lowest = a.window ? position - a.window : -1;
+  const int lowest = a.window ? max(-1, position - a.window) : -1;
   const int every = t.position(a, t.first);  // all rows of the tile see positions up to this one
   const int nobody = a.window ? t.position(a, t.first + t.count - 1) - a.window : -1;
   // Of the wave: all rows see positions in (whole_from, whole_to], none those outside [some_from, some_to].
@@ -862,16 +863,16 @@ __global__ __launch_bounds__(kTileWaves * L2C_WAVE, kTiles <= 4 && kTileWaves ==
 #pragma unroll
       for (int i = 0; i < 16; ++i) most = fmaxf(most, s[u][i]);
     most = max_halves(most);
-    // Sums stay relative to an older maximum until a new one is 2^8 times as large: floats, and bf16 weights,
-    // are as exact there.
-    if (__ballot((most - top) * scale > 8.0f)) {
+    // Sums stay relative to an older maximum until a new one is more than 2^kSlack times as large. Weights are
+    // 2^-kSlack of the softmax's, so that none is above 1 and large values do not overflow.
+    if (__ballot((most - top) * scale > kSlack)) {
       const float again = top == -INFINITY ? 0.0f : exp2_of((top - most) * scale);
       total *= again;
 #pragma unroll
       for (int i = 0; i < kTiles; ++i) acc[i] *= again;
       top = most;
     }
-    const float shift = top == -INFINITY ? 0.0f : top * scale;
+    const float shift = top == -INFINITY ? 0.0f : fmaf(top, scale, kSlack);
     // 16 positions at a time: while the matrix unit has their product, the next ones' weights are computed and
     // their values read.
     u32x4 weight[2], column[2][kTiles];
@@ -963,7 +964,7 @@ __global__ __launch_bounds__(kTileWaves * L2C_WAVE, kTiles <= 4 && kTileWaves ==
       store4(a, whole, row, head, split, d, o);
     }
   if (!whole && h == 0)
-    a.part_sums[part_of(a, row, head, split)] = make_float2(top == -INFINITY ? top : top * scale, total);
+    a.part_sums[part_of(a, row, head, split)] = make_float2(top == -INFINITY ? top : fmaf(top, scale, kSlack), total);
 }
 
 // ---------------------------------------------------------------------------
@@ -1112,7 +1113,7 @@ extern "C" int l2c_cache_attention(uint16_t *out, long long out_stride, const ui
                                    const int *starts, int sequences, int rows, int heads, int kv_heads, int width,
                                    int page_size, int pages, int max_pages, int window, float scale, void *workspace,
                                    size_t workspace_bytes, hipStream_t stream) {
-  if (!sizes(sequences, rows, heads, kv_heads, width, page_size, pages, max_pages) || window < 0 ||
+  if (!sizes(sequences, rows, heads, kv_heads, width, page_size, pages, max_pages) || window < 0 || !(fabsf(scale) <= FLT_MAX) ||
       (cache_type != L2C_BF16 && cache_type != L2C_E4M3))
     return hipErrorInvalidValue;
   const long long row = static_cast<long long>(heads) * width;

@@ -492,7 +492,9 @@ def decoder_logprobs(logprobs, entropies, top_tokens, top_logprobs, logits, toke
     # The usual call in one look; what it does not take goes through every check.
     if not (logprobs is not None and entropies is not None and top_tokens is not None and tokens is not None
             and logprobs.dtype is entropies.dtype is top_logprobs.dtype is logits.dtype is _f32
-            and top_tokens.dtype is tokens.dtype is _i32 and logits.is_cuda and logits.get_device() == _device()):
+            and top_tokens.dtype is tokens.dtype is _i32 and logits.is_cuda and logprobs.get_device()
+            == entropies.get_device() == top_tokens.get_device() == top_logprobs.get_device() == logits.get_device()
+            == tokens.get_device() == _device()):
         _takes("decoder_logprobs", "float32", logprobs, entropies, top_logprobs, logits)
         _takes("decoder_logprobs", "int32", top_tokens, tokens)
     code = _c_decoder_logprobs(logprobs, entropies, top_tokens, top_logprobs, logits, tokens, vocab, top, rows,
@@ -507,11 +509,14 @@ def _cache_type(what, keys, values, key_scales, value_scales, tables, lengths, s
     # The usual calls in one look; what it does not take goes through every check.
     if (_device is not None and values.dtype is kind and x.dtype is y.dtype is _bf16
             and tables.dtype is lengths.dtype is _i32 and (starts is None or starts.dtype is _i32)
-            and keys.is_cuda and keys.get_device() == _device()):
+            and keys.is_cuda and keys.get_device() == values.get_device() == x.get_device() == y.get_device()
+            == tables.get_device() == lengths.get_device() == _device()
+            and (starts is None or starts.get_device() == _device())):
         if kind is _bf16:
             return BF16
         if (kind is _u8 or kind is _e4m3) and key_scales is not None and value_scales is not None \
-                and key_scales.dtype is value_scales.dtype is _f32:
+                and key_scales.dtype is value_scales.dtype is _f32 \
+                and key_scales.get_device() == value_scales.get_device() == keys.get_device():
             return E4M3
     if values.dtype is not kind:
         raise ValueError(f"l2c.{what} takes keys and values of one type")
@@ -566,7 +571,10 @@ def cache_advance(tables_out, lengths_out, uses, copies, shortage, tables, lengt
     if not (tables_out.dtype is lengths_out.dtype is uses.dtype is copies.dtype is shortage.dtype is tables.dtype
             is lengths.dtype is _i32 and (parents is None or parents.dtype is _i32)
             and (starts is None or starts.dtype is _i32) and (held is None or held.dtype is _i32)
-            and tables.is_cuda and tables.get_device() == _device()):
+            and tables.is_cuda and tables_out.get_device() == lengths_out.get_device() == uses.get_device()
+            == copies.get_device() == shortage.get_device() == tables.get_device() == lengths.get_device() == _device()
+            and (parents is None or parents.get_device() == _device())
+            and (starts is None or starts.get_device() == _device()) and (held is None or held.get_device() == _device())):
         _takes("cache_advance", "int32", tables_out, lengths_out, uses, copies, shortage, tables, lengths, parents, starts,
                held)
     code = _c_cache_advance(tables_out, lengths_out, uses, copies, shortage, tables, lengths, parents, beams, starts, held,
@@ -577,8 +585,10 @@ def cache_advance(tables_out, lengths_out, uses, copies, shortage, tables, lengt
 
 def cache_copy(cache, copies, count, pages, page_bytes, page_stride=None, groups=1, group_stride=None, stream=None):
     """Strides and sizes in bytes; pages, and groups of them, follow each other unless the strides say otherwise."""
-    if not (copies.dtype is _i32 and copies.is_cuda and copies.get_device() == _device()):
+    if not (copies.dtype is _i32 and copies.is_cuda and copies.get_device() == cache.get_device() == _device()):
         _takes("cache_copy", "int32", copies)
+        if cache.is_cuda and cache.get_device() != _device():
+            raise ValueError(f"l2c.cache_copy takes tensors on the current device, {_device()}, not on {cache.get_device()}")
     page = page_bytes if page_stride is None else page_stride
     code = _c_cache_copy(cache, copies, count, pages, groups, pages * page if group_stride is None else group_stride, page,
                          page_bytes, stream)

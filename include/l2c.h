@@ -428,7 +428,7 @@ int l2c_decoder_logprobs(float *logprobs, float *entropies, int *top_tokens, flo
  *     page: nothing is written there, and no token attends to its positions.
  *   lengths [sequences]: the positions of every sequence, the newest tokens' among them
  *     (below 1: none). Positions past max_pages pages are treated as those without a page.
- *   starts [sequences + 1], not falling: the newest tokens of sequence s are rows starts[s] to
+ *   starts [sequences + 1], not falling, at most `rows`: the newest tokens of sequence s are rows starts[s] to
  *     starts[s + 1] - 1 of the call's `rows` rows (of q, k, v, out), the last one at position
  *     lengths[s] - 1, the one before at lengths[s] - 2, and so on. Rows of no sequence (from
  *     starts[sequences] on, say) are neither read nor written, and rows at positions below 0 are
@@ -448,11 +448,14 @@ int l2c_decoder_logprobs(float *logprobs, float *entropies, int *top_tokens, flo
  * l2c_cache_attention: for every new token, at position p, and head h, with the keys k_j and values
  *   v_j of head h / (heads / kv_heads):
  *     out[row][h] = sum_j softmax_j(scale * q[row][h] . k_j) v_j
- *   over the positions j <= p that have a page, and j > p - window unless window is 0. Whatever the
+ *   over the positions j <= p that have a page, and j > p - window unless window is 0; scale is
+ *   finite. Whatever the
  *   other positions hold has no part in it. Where no position is left, or every score is -Inf, out
  *   is 0. q and out: bf16, heads * width values every q_stride and out_stride. Scores, maxima, sums
  *   and out are fp32 until out is rounded once, to nearest even; the exponentials are rounded to
  *   bf16 (at most 2^-8 of each, times the value's scale with e4m3 pages) for the product with the values.
+ *   None is above 1 before they are divided by their sum, so values below 2^128 over the number of positions
+ *   that a token sees do not overflow.
  *   out overlaps none of the inputs. workspace: 16-byte aligned (may be NULL if the size below is 0),
  *   at least l2c_cache_attention_workspace_bytes, which is 0 for sizes that are not supported and at
  *   most 2^19 * (width + 2); its contents need not be kept between calls, and calls that share one

@@ -16,9 +16,9 @@ def append(keys=P, values=2 * P, key_scales=3 * P, value_scales=4 * P, cache_typ
 
 def attention(out=P, out_stride=1024, q=2 * P, q_stride=1024, keys=3 * P, values=4 * P, key_scales=P, value_scales=P,
               cache_type=BF16, tables=P, lengths=P, starts=P, sequences=2, rows=5, heads=8, kv_heads=2, width=128,
-              page_size=16, pages=10, max_pages=4, window=0, workspace=P, size=1 << 40):
+              page_size=16, pages=10, max_pages=4, window=0, workspace=P, size=1 << 40, scale=1.0):
     return call("l2c_cache_attention", out, out_stride, q, q_stride, keys, values, key_scales, value_scales, cache_type,
-                tables, lengths, starts, sequences, rows, heads, kv_heads, width, page_size, pages, max_pages, window, 1.0,
+                tables, lengths, starts, sequences, rows, heads, kv_heads, width, page_size, pages, max_pages, window, scale,
                 workspace, size, None)
 
 
@@ -45,6 +45,7 @@ def test_append_refuses(bad):
 @pytest.mark.parametrize("bad", BOTH + [
     dict(q=None), dict(out=None), dict(q=P + 4), dict(out=P + 8), dict(q_stride=1016), dict(q_stride=1028),
     dict(out_stride=-1024), dict(out_stride=1025), dict(heads=0), dict(heads=7), dict(window=-1),
+    dict(scale=float("nan")), dict(scale=float("-inf")),
     dict(heads=65536, kv_heads=1, q_stride=1 << 23, out_stride=1 << 23),
     dict(rows=0x7fffffff, heads=64, q_stride=1 << 14, out_stride=1 << 14)], ids=str)
 def test_attention_refuses(bad):

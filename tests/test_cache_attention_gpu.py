@@ -202,6 +202,26 @@ def test_scales(torch_gpu, l2c, new, scale):
     check(l2c, Cache(4, [200, 31], [new, new], 2, 64, 16), 8, scale=scale)
 
 
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 2, 2 ** 31 - 200, 2 ** 30])
+@pytest.mark.parametrize("new", [1, 5, 300])
+def test_windows_past_everything(torch_gpu, l2c, new, window):
+    check(l2c, Cache(new, [new + 350, new, 1], [new, new, 1], 2, 64, 16), 8, window=window)
+
+
+@pytest.mark.parametrize("cache", ["bf16", "e4m3"])
+@pytest.mark.parametrize("length,new", [(3000, 1), (3000, 4), (900, 600)])
+def test_large_values(torch_gpu, l2c, length, new, cache):
+    """Values as large as `length` of them may be, 2^128 / length, and scores that grow from tile to tile: weights are
+    never above 1, so their sums do not overflow."""
+    c = Cache(length, [length], [new], 1, 64, 16, cache, spread=0.0)
+    q = torch.ones(c.rows, 2 * 64, device="cuda").bfloat16()
+    j = torch.arange(length, device="cuda").float().reshape(-1, 1, 1)
+    c.dense[0][0] = c.put(0, 0, "keys", (j * (8.0 / length)).floor().expand(-1, 1, 64).contiguous() / 8)
+    c.dense[0][1] = c.put(0, 0, "values", torch.full((length, 1, 64), 1e35, device="cuda"))
+    out = check(l2c, c, 2, q=q)
+    assert bool(out.isfinite().all())
+
+
 def peaked(c, q, heads, at):
     """Keys along the first query row of head 0 at the given positions of sequence 0: they share the weight."""
     k = torch.zeros(1, c.kv, c.width, device="cuda")

@@ -291,8 +291,9 @@ __device__ __forceinline__ void lone_row(const Attention &a, const Tile &t, int 
     for (int i = 0; i < L2C_WAVE && first + i <= last; ++i) {
       if (!__shfl(static_cast<int>(there), i, L2C_WAVE)) continue;
       const float w = __shfl(p, i, L2C_WAVE);
-      const size_t of = (static_cast<size_t>(static_cast<unsigned>(__shfl(static_cast<int>(at >> 32), i, L2C_WAVE))) << 32) |
-                        static_cast<unsigned>(__shfl(static_cast<int>(at), i, L2C_WAVE));
+      const unsigned high = __shfl(static_cast<int>(at >> 32), i, L2C_WAVE);
+      const unsigned low = __shfl(static_cast<int>(at), i, L2C_WAVE);
+      const size_t of = static_cast<size_t>(high) << 32 | low;
 #pragma unroll
       for (int c = 0; c < L2C_MAX_HEAD / L2C_WAVE; ++c) {
         const int d = c * L2C_WAVE + lane;
@@ -350,11 +351,11 @@ __device__ __forceinline__ int value_place(int key, int chunk) {
 
 // kChunks: of 32 columns, of which a lane has eight; those from kSure on may end before. A row has D columns in LDS.
 // PAIRS: of e4m3 pages a lane has sixteen columns in a row for two chunks, so that it loads 16 bytes at a time, too
-// (4 x 131072 166 us, 215 with eight, and as long without any arithmetic; rows of an odd number of eights are loaded so).
-// Three waves a SIMD for e4m3 pages and short rows, whose bytes in flight are few (4 x 131072 in e4m3 220 us, 235
-// with two; 16 x 5 of 2500, 80 wide, 21.0 and 24.3), two for others (64 x 4096 159 us, 167 with three).
+// (4 x 131072 in e4m3 166-169 us, 4.9 TB/s, 215 with eight, and as long without any arithmetic; rows of an odd number
+// of eights are loaded so). 64 x 4096 in bf16 takes 153-157 us, 4.9 TB/s; 16 x 5 of 2500, 80 wide, 20, of which the
+// kernel 15. Three waves a SIMD up to 128 columns (e4m3 168 us, 172 with two; the others are the same).
 template <int kChunks, bool E4M3, bool PAIRS>
-__global__ __launch_bounds__(kThreads, kChunks > 4 ? 1 : E4M3 || kChunks < 4 ? 3 : 2) void narrow_kernel(Attention a) {
+__global__ __launch_bounds__(kThreads, kChunks > 4 ? 1 : 3) void narrow_kernel(Attention a) {
   static_assert(!PAIRS || kChunks % 2 == 0, "two chunks a load");
   constexpr int kSure = PAIRS ? kChunks - 2 : kChunks == 2 ? 0 : kChunks <= 4 ? kChunks - 1 : kChunks - 2;
   constexpr int D = kChunks <= 2 ? 64 : kChunks <= 4 ? 128 : 256;
@@ -437,7 +438,8 @@ __global__ __launch_bounds__(kThreads, kChunks > 4 ? 1 : E4M3 || kChunks < 4 ? 3
       for (int c = 0; c < kChunks; c += PAIRS ? 2 : 1) {
         const int from = inside(c) ? column(c) : 0;
         if constexpr (PAIRS) {
-          const u32x4 x = *reinterpret_cast<const u32x4 *>(key + from), y = *reinterpret_cast<const u32x4 *>(value + from);
+          const u32x4 x = *reinterpret_cast<const u32x4 *>(key + from);
+          const u32x4 y = *reinterpret_cast<const u32x4 *>(value + from);
           k[u][c] = u32x2{x[0], x[1]}, k[u][c + 1] = u32x2{x[2], x[3]};
           v[u][c] = u32x2{y[0], y[1]}, v[u][c + 1] = u32x2{y[2], y[3]};
         } else {
@@ -554,8 +556,8 @@ __global__ __launch_bounds__(kThreads, kChunks > 4 ? 1 : E4M3 || kChunks < 4 ? 3
       const u32x2 low = read_column(mine_values + value_place<D>(key, d / 8) + d % 8);
       const u32x2 high = read_column(mine_values + value_place<D>(16 + key, d / 8) + d % 8);
       const u32x4 w = {low[0], low[1], high[0], high[1]};
-      acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w), __builtin_bit_cast(bf16x8, p), acc[i],
-                                                       0, 0, 0);
+      acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w), __builtin_bit_cast(bf16x8, p),
+                                                       acc[i], 0, 0, 0);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -625,7 +627,8 @@ typedef __attribute__((address_space(3))) void lds_ptr;
 
 // kTiles: tiles of 32 columns, of which there are some; a row has D columns in LDS.
 template <int kTiles, int kTileWaves, bool E4M3>
-__global__ __launch_bounds__(kTileWaves * L2C_WAVE, kTiles <= 4 && kTileWaves == kWaves ? 2 : 1) void wide_kernel(Attention a) {
+__global__ __launch_bounds__(kTileWaves * L2C_WAVE,
+                             kTiles <= 4 && kTileWaves == kWaves ? 2 : 1) void wide_kernel(Attention a) {
   constexpr int kLaneCount = kTileWaves * L2C_WAVE;
   constexpr int D = kTiles <= 2 ? 64 : kTiles <= 4 ? 128 : 256;
   constexpr int kKeys = D <= 128 ? 64 : 32;
@@ -694,8 +697,12 @@ __global__ __launch_bounds__(kTileWaves * L2C_WAVE, kTiles <= 4 && kTileWaves ==
   // Lanes that read a chunk of eight (sixteen) keys together: each in other banks.
   auto key_swap = [](int key) __attribute__((always_inline)) { return D == 64 ? key >> 1 & 7 : key & 15; };
   // Lanes that read four keys of 32 columns together, the same.
-  auto value_swap = [](int key) __attribute__((always_inline)) { return D == 64 ? (key >> 1 & 1) << 2 : (key & 3) << 2; };
-  auto value_place = [&](int key, int chunk) __attribute__((always_inline)) { return key * D + 8 * (chunk ^ value_swap(key)); };
+  auto value_swap = [](int key) __attribute__((always_inline)) {
+    return D == 64 ? (key >> 1 & 1) << 2 : (key & 3) << 2;
+  };
+  auto value_place = [&](int key, int chunk) __attribute__((always_inline)) {
+    return key * D + 8 * (chunk ^ value_swap(key));
+  };
   const int load_row = threadIdx.x / kLanes, load_chunk = threadIdx.x % kLanes;
   Raw<E4M3> k[kPasses], v[kPasses];
   float key_scale = 0.0f, value_scale = 0.0f;
@@ -726,8 +733,8 @@ __global__ __launch_bounds__(kTileWaves * L2C_WAVE, kTiles <= 4 && kTileWaves ==
     } else {
       // Where the lane's key lies; then a lane's 16 bytes go to LDS after those of the lane before.
       const int j = base + lane % kKeys;
-      const unsigned long long offset = static_cast<unsigned long long>(static_cast<unsigned>(pages)) * page_bytes + head_bytes +
-                                        static_cast<unsigned long long>(j - a.s.by_page(j) * a.s.page_size) * row_bytes;
+      const unsigned long long page = static_cast<unsigned>(pages), of_page = j - a.s.by_page(j) * a.s.page_size;
+      const unsigned long long offset = page * page_bytes + head_bytes + of_page * row_bytes;
       const unsigned low = static_cast<unsigned>(offset), high = static_cast<unsigned>(offset >> 32);
       const bool whole = together && (there & kAll) == kAll;
 #pragma unroll
@@ -743,9 +750,8 @@ __global__ __launch_bounds__(kTileWaves * L2C_WAVE, kTiles <= 4 && kTileWaves ==
           from_key = static_cast<const unsigned char *>(a.keys) + at + (row_at + key_at);
           from_value = static_cast<const unsigned char *>(a.values) + at + (row_at + value_at);
         } else {
-          const unsigned long long at = static_cast<unsigned long long>(static_cast<unsigned>(__shfl(high, r, L2C_WAVE)))
-                                            << 32 |
-                                        static_cast<unsigned>(__shfl(low, r, L2C_WAVE));
+          const unsigned long long above = static_cast<unsigned>(__shfl(high, r, L2C_WAVE));
+          const unsigned long long at = above << 32 | static_cast<unsigned>(__shfl(low, r, L2C_WAVE));
           const bool is = there >> r & 1;
           from_key = is ? static_cast<const unsigned char *>(a.keys) + at + key_at
                         : reinterpret_cast<const unsigned char *>(zero_row);
@@ -829,8 +835,8 @@ __global__ __launch_bounds__(kTileWaves * L2C_WAVE, kTiles <= 4 && kTileWaves ==
         if (c == 0)
 #pragma unroll
           for (int i = 0; i < 16; ++i) before[i] = 0.0f;
-        s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, operand[group % 2][e]), q[c], before, 0, 0,
-                                                       0);
+        s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, operand[group % 2][e]), q[c], before,
+                                                       0, 0, 0);
       }
       __builtin_amdgcn_sched_group_barrier(kSchedDsRead, kAhead, 0);
       __builtin_amdgcn_sched_group_barrier(kSchedMfma, kAhead, 0);
@@ -917,7 +923,8 @@ __global__ __launch_bounds__(kTileWaves * L2C_WAVE, kTiles <= 4 && kTileWaves ==
 #pragma unroll
       for (int i = 0; i < kTiles; ++i)
         acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, column[group % 2][i]),
-                                                         __builtin_bit_cast(bf16x8, weight[group % 2]), acc[i], 0, 0, 0);
+                                                         __builtin_bit_cast(bf16x8, weight[group % 2]), acc[i],
+                                                         0, 0, 0);
       if (more) {
         __builtin_amdgcn_sched_group_barrier(kSchedDsRead, 2 * kTiles, 0);
 #pragma unroll
@@ -1044,7 +1051,7 @@ Plan plan(int sequences, int rows, int heads, int kv_heads, int width, int page_
   const long long packed = static_cast<long long>(rows) * group;
   Plan p;
   const bool narrow = packed <= 16LL * sequences;
-  const bool many = width > 96 && width <= 128 && packed / kWideMany * kv_heads >= 256;
+  const bool many = width > 96 && width <= 128 && packed / kWideMany * kv_heads > 256;
   const int m = p.rows = narrow ? kNarrow : many ? kWideMany : kWide;
   p.slots = starts ? packed / m + sequences : static_cast<long long>(sequences) * ((group + m - 1) / m);
   const long long tiles = p.slots * kv_heads, wanted = narrow ? 2048 : 512;
@@ -1085,9 +1092,12 @@ Kernel kernel(int rows, int width) {
                              : wide_kernel<8, kWaves, E4M3>;
 }
 
-template <int M, int STEP>
-Kernel join_of(bool many) {
-  return many ? join_kernel<M, STEP, true> : join_kernel<M, STEP, false>;
+// Tiles of 256 rows are more than 256 and not divided.
+Kernel join(const Plan &p, int width, bool many) {
+  if (p.rows == kNarrow)
+    return many ? join_kernel<kNarrow, kNarrowStep, true> : join_kernel<kNarrow, kNarrowStep, false>;
+  if (width <= 128) return many ? join_kernel<kWide, 64, true> : join_kernel<kWide, 64, false>;
+  return many ? join_kernel<kWide, 32, true> : join_kernel<kWide, 32, false>;
 }
 
 size_t part_bytes(const Plan &p, int rows, int heads, int width) {
@@ -1100,11 +1110,12 @@ extern "C" size_t l2c_cache_attention_workspace_bytes(int sequences, int rows, i
                                                       int page_size, int max_pages) {
   if (!sizes(sequences, rows, heads, kv_heads, width, page_size, 0, max_pages) || sequences == 0 || rows == 0) return 0;
   // What a call with starts needs, or without: the fewer slots, the more parts.
-  const size_t with = part_bytes(plan(sequences, rows, heads, kv_heads, width, page_size, max_pages, true), rows, heads, width);
-  const size_t without = rows != sequences
-                             ? 0
-                             : part_bytes(plan(sequences, rows, heads, kv_heads, width, page_size, max_pages, false), rows, heads, width);
-  return with > without ? with : without;
+  size_t most = 0;
+  for (const bool starts : {true, false})
+    if (starts || rows == sequences)
+      most = max(most, part_bytes(plan(sequences, rows, heads, kv_heads, width, page_size, max_pages, starts), rows,
+                                  heads, width));
+  return most;
 }
 
 extern "C" int l2c_cache_attention(uint16_t *out, long long out_stride, const uint16_t *q, long long q_stride,
@@ -1113,13 +1124,15 @@ extern "C" int l2c_cache_attention(uint16_t *out, long long out_stride, const ui
                                    const int *starts, int sequences, int rows, int heads, int kv_heads, int width,
                                    int page_size, int pages, int max_pages, int window, float scale, void *workspace,
                                    size_t workspace_bytes, hipStream_t stream) {
-  if (!sizes(sequences, rows, heads, kv_heads, width, page_size, pages, max_pages) || window < 0 || !(fabsf(scale) <= FLT_MAX) ||
-      (cache_type != L2C_BF16 && cache_type != L2C_E4M3))
+  scale *= kLog2e;
+  if (!sizes(sequences, rows, heads, kv_heads, width, page_size, pages, max_pages) || window < 0 ||
+      !(fabsf(scale) <= FLT_MAX) || (cache_type != L2C_BF16 && cache_type != L2C_E4M3))
     return hipErrorInvalidValue;
   const long long row = static_cast<long long>(heads) * width;
   if (q_stride < row || out_stride < row || q_stride % 8 != 0 || out_stride % 8 != 0) return hipErrorInvalidValue;
   if (sequences == 0 || rows == 0) return hipSuccess;
-  const size_t need = l2c_cache_attention_workspace_bytes(sequences, rows, heads, kv_heads, width, page_size, max_pages);
+  const size_t need =
+      l2c_cache_attention_workspace_bytes(sequences, rows, heads, kv_heads, width, page_size, max_pages);
   if (!l2c::cache_arguments(cache_type, keys, values, key_scales, value_scales, tables, lengths, starts, sequences,
                             rows) ||
       !q || !out || !l2c_aligned16(q) || !l2c_aligned16(out) || workspace_bytes < need ||
@@ -1127,8 +1140,9 @@ extern "C" int l2c_cache_attention(uint16_t *out, long long out_stride, const ui
     return hipErrorInvalidValue;
   const Plan p = plan(sequences, rows, heads, kv_heads, width, page_size, max_pages, starts != nullptr);
   const long long grid = p.slots * kv_heads * p.splits;
+  const int threads = p.rows == kWideMany ? kManyWaves * L2C_WAVE : kThreads;
   if (static_cast<long long>(rows) * heads > INT_MAX || p.slots > INT_MAX || grid > INT_MAX ||
-      !l2c::launchable(grid, kThreads))
+      !l2c::launchable(grid, threads))
     return hipErrorInvalidValue;
   float *const parts = static_cast<float *>(workspace);
   const size_t items = static_cast<size_t>(rows) * heads * p.splits;
@@ -1140,20 +1154,15 @@ extern "C" int l2c_cache_attention(uint16_t *out, long long out_stride, const ui
   a.s = l2c::sequences_of(tables, lengths, starts, sequences, rows, max_pages, page_size, pages);
   a.group = heads / kv_heads, a.by_group = l2c::Quotient31(a.group);
   a.heads = heads, a.kv_heads = kv_heads, a.width = width, a.window = window;
-  a.splits = p.splits, a.slots = static_cast<int>(p.slots), a.least = p.least, a.scale = scale * kLog2e;
+  a.splits = p.splits, a.slots = static_cast<int>(p.slots), a.least = p.least, a.scale = scale;
   const Kernel fn = cache_type == L2C_E4M3 ? kernel<true>(p.rows, width) : kernel<false>(p.rows, width);
-  hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(grid)), dim3(p.rows == kWideMany ? kManyWaves * L2C_WAVE : kThreads), 0, stream,
-                     a);
+  hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(grid)), dim3(threads), 0, stream, a);
   L2C_LAUNCH_CHECK();
   if (p.splits == 1) return hipSuccess;
   const bool many = p.splits > kFewParts;
-  const Kernel join = p.rows == kNarrow     ? join_of<kNarrow, kNarrowStep>(many)
-                      : p.rows == kWideMany ? join_of<kWideMany, 64>(many)
-                      : width <= 128        ? join_of<kWide, 64>(many)
-                                            : join_of<kWide, 32>(many);
   const long long pairs = static_cast<long long>(rows) * heads;
   const unsigned joins = static_cast<unsigned>(many ? pairs : (pairs + kWaves - 1) / kWaves);
-  hipLaunchKernelGGL(join, dim3(joins), dim3(kThreads), 0, stream, a);
+  hipLaunchKernelGGL(join(p, width, many), dim3(joins), dim3(kThreads), 0, stream, a);
   L2C_LAUNCH_CHECK();
   return hipSuccess;
 }

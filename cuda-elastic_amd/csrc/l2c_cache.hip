@@ -21,7 +21,7 @@ __device__ __forceinline__ float high_half(unsigned u) { return __uint_as_float(
 // Keys, then values of a row's heads, then the next row's: an item each, by G lanes with eight values a lane,
 // kItems items one after the other by the same lanes, all of them on their way before the first is looked at.
 // Bound by memory; where a row goes is found once for the workgroup, meanwhile. 8192 rows of 8 x 128 into e4m3 pages
-// 12 us (4.2 TB/s), 39 with an item a lane and every lane's own search; 64 rows into bf16 pages 2.4.
+// 12.6-14.3 us (3.2 TB/s), 39 with an item a lane and every lane's own search; 64 rows into bf16 pages 2.4-2.7.
 template <int G, int kItems, bool E4M3>
 __global__ __launch_bounds__(kAppendThreads) void append_kernel(void *keys, void *values, float *key_scales,
                                                                 float *value_scales, const uint16_t *k,
@@ -64,7 +64,8 @@ __global__ __launch_bounds__(kAppendThreads) void append_kernel(void *keys, void
     const bool value = of >= kv_heads, mine = place >= 0 && 8 * lane < width;
     const size_t to = place + static_cast<size_t>(value ? of - kv_heads : of) * s.page_size;
     if constexpr (!E4M3) {
-      if (mine) *reinterpret_cast<u32x4 *>(static_cast<uint16_t *>(value ? values : keys) + to * width + 8 * lane) = x[i];
+      uint16_t *const cache = static_cast<uint16_t *>(value ? values : keys);
+      if (mine) *reinterpret_cast<u32x4 *>(cache + to * width + 8 * lane) = x[i];
     } else {
       unsigned largest = 0;  // of the magnitudes' patterns, which order as the numbers do, NaN above all
 #pragma unroll
@@ -104,8 +105,8 @@ __global__ __launch_bounds__(kAppendThreads) void append_kernel(void *keys, void
   }
 }
 
-using AppendKernel = void (*)(void *, void *, float *, float *, const uint16_t *, long long, const uint16_t *, long long,
-                              Sequences, int, int, l2c::Quotient31);
+using AppendKernel = void (*)(void *, void *, float *, float *, const uint16_t *, long long, const uint16_t *,
+                              long long, Sequences, int, int, l2c::Quotient31);
 template <int G>
 AppendKernel append_of(bool many, bool e4m3) {
   return many ? (e4m3 ? append_kernel<G, 4, true> : append_kernel<G, 4, false>)
@@ -139,8 +140,12 @@ struct Step {
   }
 };
 
-__device__ __forceinline__ int now(const int *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-__device__ __forceinline__ void put(int *p, int v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ int now(const int *p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void put(int *p, int v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
 
 // The sum over the workgroup's lanes before this one; `all` over all of them.
 __device__ __forceinline__ long long scan_before(long long v, long long *slots, long long &all) {
@@ -370,7 +375,8 @@ __global__ __launch_bounds__(kAdvanceThreads) void advance_lds_kernel(Step s) {
   const int upto = min(last, s.max_pages);
   long long total, beyond;
   const long long before = scan_before(is ? max(0, upto - first) + replaced : 0, slots, total);
-  scan_before(is ? last - max(first, upto) : 0, slots, beyond);  // its barriers part the reads of uses above from what follows
+  // Its barriers part the reads of uses above from what follows.
+  scan_before(is ? last - max(first, upto) : 0, slots, beyond);
   if (keeps) uses[page] = 1;
   if (is) {
     base[t] = static_cast<int>(min(before, static_cast<long long>(INT_MAX)));
@@ -474,7 +480,8 @@ extern "C" int l2c_cache_advance(int *tables_out, int *lengths_out, int *uses, i
                                  const int *starts, const int *held, int sequences, int page_size, int pages,
                                  int max_pages, int window, hipStream_t stream) {
   if (sequences < 0 || page_size <= 0 || pages < 0 || max_pages < 0 || window < 0 ||
-      static_cast<long long>(max_pages) * page_size > l2c::kMostPositions || (parents && (beams <= 0 || sequences % beams != 0)))
+      static_cast<long long>(max_pages) * page_size > l2c::kMostPositions ||
+      (parents && (beams <= 0 || sequences % beams != 0)))
     return hipErrorInvalidValue;
   if (sequences == 0) return hipSuccess;
   if (!lengths_out || !copies || !shortage || !lengths || (pages > 0 && !uses) ||

@@ -144,7 +144,8 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(Args a) {
     float best_value = -INFINITY;  // the lane's largest, -Inf where all are NaN
 #pragma unroll
     for (int i = 0; i < 4 * V; ++i) best_value = fmaxf(best_value, v[i]);
-    const float largest = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(wave_top(best_value)), L2C_WAVE - 1));
+    const unsigned last = __builtin_amdgcn_readlane(__float_as_uint(wave_top(best_value)), L2C_WAVE - 1);
+    const float largest = __uint_as_float(last);
     if (largest > m) raise(z, s, m, largest);
     const float subtract = m == -INFINITY ? 0.0f : m;
     float sum = 0.0f, product = 0.0f;
@@ -351,9 +352,9 @@ Plan plan(int vocab, int rows) {
 }
 
 using Kernel = void (*)(Args);
-template <int V>
-Kernel kernel(bool whole) {
-  return whole ? logprobs_kernel<V, true> : logprobs_kernel<V, false>;
+Kernel kernel(const Plan &p) {  // chunks of a row have more than 1024 logits
+  if (p.chunks > 1) return p.v == 2 ? logprobs_kernel<2, false> : logprobs_kernel<4, false>;
+  return p.v == 1 ? logprobs_kernel<1, true> : p.v == 2 ? logprobs_kernel<2, true> : logprobs_kernel<4, true>;
 }
 
 }  // namespace
@@ -376,14 +377,12 @@ extern "C" int l2c_decoder_logprobs(float *logprobs, float *entropies, int *top_
   const Plan p = plan(vocab, rows);
   const long long grid = static_cast<long long>(rows) * p.chunks;
   if (!l2c::launchable(grid, kThreads)) return hipErrorInvalidValue;
-  const Args a = {logprobs, entropies, top_tokens, top_logprobs, logits, tokens, static_cast<unsigned char *>(workspace),
-                  vocab, top, p.chunks, p.chunk};
-  const bool whole = p.chunks == 1;
-  const Kernel fn = p.v == 1 ? kernel<1>(whole) : p.v == 2 ? kernel<2>(whole) : kernel<4>(whole);
+  const Args a = {logprobs, entropies, top_tokens, top_logprobs, logits, tokens,
+                  static_cast<unsigned char *>(workspace), vocab, top, p.chunks, p.chunk};
   const size_t list = 2 * sizeof(unsigned) * (2 * kWaves * static_cast<size_t>(top) * 4 * p.v + 8);
-  hipLaunchKernelGGL(fn, dim3(static_cast<unsigned>(grid)), dim3(kThreads), list, stream, a);
+  hipLaunchKernelGGL(kernel(p), dim3(static_cast<unsigned>(grid)), dim3(kThreads), list, stream, a);
   L2C_LAUNCH_CHECK();
-  if (whole) return hipSuccess;
+  if (p.chunks == 1) return hipSuccess;
   hipLaunchKernelGGL(logprobs_join_kernel, dim3(rows), dim3(L2C_WAVE),
                      sizeof(Candidate) * static_cast<size_t>(p.chunks) * top, stream, a, static_cast<unsigned>(rows));
   L2C_LAUNCH_CHECK();

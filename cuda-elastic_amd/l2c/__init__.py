@@ -535,8 +535,8 @@ def _cache_type(what, keys, values, key_scales, value_scales, tables, lengths, s
     return cache_type
 
 
-def cache_append(keys, values, k, v, tables, lengths, kv_heads, width, page_size, pages, max_pages, sequences, rows=None,
-                 starts=None, key_scales=None, value_scales=None, k_stride=None, v_stride=None, stream=None):
+def cache_append(keys, values, k, v, tables, lengths, kv_heads, width, page_size, pages, max_pages, sequences,
+                 rows=None, starts=None, key_scales=None, value_scales=None, k_stride=None, v_stride=None, stream=None):
     """Rows of k and v follow each other unless their strides (in values) say otherwise."""
     cache_type = _cache_type("cache_append", keys, values, key_scales, value_scales, tables, lengths, starts, k, v)
     code = _c_cache_append(keys, values, key_scales, value_scales, cache_type, k,
@@ -551,10 +551,11 @@ def cache_attention_workspace_bytes(sequences, rows, heads, kv_heads, width, pag
     return load().l2c_cache_attention_workspace_bytes(sequences, rows, heads, kv_heads, width, page_size, max_pages)
 
 
-def cache_attention(out, q, keys, values, tables, lengths, heads, kv_heads, width, page_size, pages, max_pages, sequences,
-                    workspace=None, rows=None, starts=None, key_scales=None, value_scales=None, window=0, scale=None,
+def cache_attention(out, q, keys, values, tables, lengths, heads, kv_heads, width, page_size, pages, max_pages,
+                    sequences, workspace=None, rows=None, starts=None, key_scales=None, value_scales=None, window=0, scale=None,
                     q_stride=None, out_stride=None, stream=None):
-    """scale is 1 / sqrt(width) unless given; rows of q and out follow each other unless their strides say otherwise."""
+    """scale is 1 / sqrt(width) unless given; rows of q and out follow each other unless their strides say
+    otherwise."""
     cache_type = _cache_type("cache_attention", keys, values, key_scales, value_scales, tables, lengths, starts, q, out)
     code = _c_cache_attention(out, heads * width if out_stride is None else out_stride, q,
                               heads * width if q_stride is None else q_stride, keys, values, key_scales, value_scales,
@@ -565,8 +566,8 @@ def cache_attention(out, q, keys, values, tables, lengths, heads, kv_heads, widt
         _check(code, "l2c_cache_attention")
 
 
-def cache_advance(tables_out, lengths_out, uses, copies, shortage, tables, lengths, sequences, max_pages, page_size, pages,
-                  parents=None, beams=1, starts=None, held=None, window=0, stream=None):
+def cache_advance(tables_out, lengths_out, uses, copies, shortage, tables, lengths, sequences, max_pages, page_size,
+                  pages, parents=None, beams=1, starts=None, held=None, window=0, stream=None):
     # The usual calls in one look; what it does not take goes through every check.
     if not (tables_out.dtype is lengths_out.dtype is uses.dtype is copies.dtype is shortage.dtype is tables.dtype
             is lengths.dtype is _i32 and (parents is None or parents.dtype is _i32)
@@ -574,11 +575,12 @@ def cache_advance(tables_out, lengths_out, uses, copies, shortage, tables, lengt
             and tables.is_cuda and tables_out.get_device() == lengths_out.get_device() == uses.get_device()
             == copies.get_device() == shortage.get_device() == tables.get_device() == lengths.get_device() == _device()
             and (parents is None or parents.get_device() == _device())
-            and (starts is None or starts.get_device() == _device()) and (held is None or held.get_device() == _device())):
-        _takes("cache_advance", "int32", tables_out, lengths_out, uses, copies, shortage, tables, lengths, parents, starts,
-               held)
-    code = _c_cache_advance(tables_out, lengths_out, uses, copies, shortage, tables, lengths, parents, beams, starts, held,
-                            sequences, page_size, pages, max_pages, window, stream)
+            and (starts is None or starts.get_device() == _device())
+            and (held is None or held.get_device() == _device())):
+        _takes("cache_advance", "int32", tables_out, lengths_out, uses, copies, shortage, tables, lengths, parents,
+               starts, held)
+    code = _c_cache_advance(tables_out, lengths_out, uses, copies, shortage, tables, lengths, parents, beams, starts,
+                            held, sequences, page_size, pages, max_pages, window, stream)
     if code:
         _check(code, "l2c_cache_advance")
 
@@ -588,10 +590,11 @@ def cache_copy(cache, copies, count, pages, page_bytes, page_stride=None, groups
     if not (copies.dtype is _i32 and copies.is_cuda and copies.get_device() == cache.get_device() == _device()):
         _takes("cache_copy", "int32", copies)
         if cache.is_cuda and cache.get_device() != _device():
-            raise ValueError(f"l2c.cache_copy takes tensors on the current device, {_device()}, not on {cache.get_device()}")
+            raise ValueError(
+                f"l2c.cache_copy takes tensors on the current device, {_device()}, not on {cache.get_device()}")
     page = page_bytes if page_stride is None else page_stride
-    code = _c_cache_copy(cache, copies, count, pages, groups, pages * page if group_stride is None else group_stride, page,
-                         page_bytes, stream)
+    code = _c_cache_copy(cache, copies, count, pages, groups, pages * page if group_stride is None else group_stride,
+                         page, page_bytes, stream)
     if code:
         _check(code, "l2c_cache_copy")
 

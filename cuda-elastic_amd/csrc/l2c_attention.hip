@@ -611,13 +611,16 @@ __global__ __launch_bounds__(kThreads, kChunks > 4 ? 1 : 3) void narrow_kernel(A
 
 // ---------------------------------------------------------------------------
 // Tiles of 32 rows a wave: chunks of a prompt. Bound by the matrix and the vector units, and by LDS, which each
-// wave reads whole tiles from. The workgroup's keys and values, 64 positions at a time (32 of more than 128
-// columns), lie in LDS, two tiles of them: while one is read, the next is on its way. bf16 pages go to LDS
-// without registers between, rows that are not there from a row of zeros; e4m3 pages through registers, where
-// they become bf16. Four waves share a tile, so that two workgroups fit a CU, or eight, for which half as much is
-// loaded (a chunk of 4096 over 16384 positions 896 us, 982 with four; three of 1000 over 5000 208 and 223), where
-// 128 columns make that worth it and the tiles are enough (four chunks of 300 over 2000 57 us with four, 64 with
-// eight; 64 columns the same with both). Four waves of more than 128 columns need the registers of eight.
+// wave reads whole tiles from. The workgroup's keys and values, 64 positions at a time, lie in LDS, two tiles of
+// them: while one is read, the next is on its way. bf16 pages go to LDS without registers between, rows that are
+// not there from a row of zeros; e4m3 pages through registers, where they become bf16 (a chunk each of 2000 over up
+// to 4000 positions of 8 sequences 648 us, 548 in bf16; two tiles in LDS here, too, 676: they cost registers). Of
+// more than 128 columns a tile of 64 positions needs all 512 registers and 128 KB, and is still better than one of 32
+// (200 over 10000 positions, 256 wide, 116 us and 130; 192 wide, 1000 over 4000 of 4, 139 and 157). Four waves share
+// a tile, so that two workgroups fit a CU, or eight, for which half as much is loaded (a chunk of 4096 over 16384
+// positions 896 us, 982 with four; three of 1000 over 5000 208 and 223), where 128 columns make that worth it and the
+// tiles are enough (four chunks of 300 over 2000 57 us with four, 64 with eight; 64 columns the same with both). Four
+// waves of more than 128 columns need the registers of eight.
 
 constexpr int kManyWaves = 8, kWide = 32 * kWaves, kWideMany = 32 * kManyWaves;
 constexpr int kSchedValu = 0x002, kSchedMfma = 0x008, kSchedDsRead = 0x100;  // sched_group_barrier classes
@@ -631,7 +634,7 @@ __global__ __launch_bounds__(kTileWaves * L2C_WAVE,
                              kTiles <= 4 && kTileWaves == kWaves ? 2 : 1) void wide_kernel(Attention a) {
   constexpr int kLaneCount = kTileWaves * L2C_WAVE;
   constexpr int D = kTiles <= 2 ? 64 : kTiles <= 4 ? 128 : 256;
-  constexpr int kKeys = D <= 128 ? 64 : 32;
+  constexpr int kKeys = 64;
   constexpr int kLanes = D / 8;               // that load a row
   constexpr int kRows = kLaneCount / kLanes;    // rows loaded together
   constexpr int kPasses = kKeys / kRows;
@@ -687,7 +690,7 @@ __global__ __launch_bounds__(kTileWaves * L2C_WAVE,
 
   // A tile's pages, a key a lane.
   auto look_up = [&](int base) __attribute__((always_inline)) {
-    const int j = base + lane % kKeys;
+    const int j = base + lane;
     return j >= t.from && j < end ? a.s.page(t.sequence, a.s.by_page(j)) : -1;
   };
   auto row_of = [&](int page, int j) __attribute__((always_inline)) {
@@ -707,7 +710,7 @@ __global__ __launch_bounds__(kTileWaves * L2C_WAVE,
   Raw<E4M3> k[kPasses], v[kPasses];
   float key_scale = 0.0f, value_scale = 0.0f;
   // Begins to load a tile, `there` of which have a page: into LDS, or registers.
-  constexpr unsigned long long kAll = kKeys == 64 ? ~0ull : 0xffffffffull;
+  static_assert(kKeys == L2C_WAVE, "a key a lane");
   const bool together = a.s.page_size % kTogether == 0;  // a wave's rows lie in one page
   const unsigned row_bytes = 2u * static_cast<unsigned>(a.width);
   const unsigned long long page_bytes = a.page_rows * row_bytes;
@@ -727,16 +730,16 @@ __global__ __launch_bounds__(kTileWaves * L2C_WAVE,
       }
       key_scale = value_scale = 0.0f;
       if (a.s.is_page(pages)) {
-        const size_t at = row_of(pages, base + lane % kKeys);
+        const size_t at = row_of(pages, base + lane);
         key_scale = a.key_scales[at], value_scale = a.value_scales[at];
       }
     } else {
       // Where the lane's key lies; then a lane's 16 bytes go to LDS after those of the lane before.
-      const int j = base + lane % kKeys;
+      const int j = base + lane;
       const unsigned long long page = static_cast<unsigned>(pages), of_page = j - a.s.by_page(j) * a.s.page_size;
       const unsigned long long offset = page * page_bytes + head_bytes + of_page * row_bytes;
       const unsigned low = static_cast<unsigned>(offset), high = static_cast<unsigned>(offset >> 32);
-      const bool whole = together && (there & kAll) == kAll;
+      const bool whole = together && there == ~0ull;
 #pragma unroll
       for (int i = 0; i < kPasses; ++i) {
         const int r = i * kRows + load_row, first_row = i * kRows + wave * kTogether;
@@ -794,7 +797,7 @@ __global__ __launch_bounds__(kTileWaves * L2C_WAVE,
         *reinterpret_cast<u32x4 *>(values + r * D + 8 * (load_chunk ^ value_swap(r))) = vv;
       }
       if (mixed) bad |= not_finite(value_scale);
-      if (wave == 0 && lane < kKeys) key_scales[lane] = key_scale, value_scales[lane] = value_scale;
+      if (wave == 0) key_scales[lane] = key_scale, value_scales[lane] = value_scale;
       __syncthreads();
     } else {
       __builtin_amdgcn_sched_barrier(0);
@@ -852,7 +855,7 @@ __global__ __launch_bounds__(kTileWaves * L2C_WAVE,
           for (int e = 0; e < 4; ++e) s[u][4 * i + e] *= x[e];
         }
     }
-    if (base + kKeys - 1 > whole_to || base <= whole_from || (there & kAll) != kAll) {
+    if (base + kKeys - 1 > whole_to || base <= whole_from || there != ~0ull) {
 #pragma unroll
       for (int u = 0; u < kParts; ++u) {
         const unsigned seen = seen_of_32(static_cast<unsigned>(there >> (32 * u)), position - base - 32 * u,
@@ -875,7 +878,13 @@ __global__ __launch_bounds__(kTileWaves * L2C_WAVE,
       const float again = top == -INFINITY ? 0.0f : exp2_of((top - most) * scale);
       total *= again;
 #pragma unroll
-      for (int i = 0; i < kTiles; ++i) acc[i] *= again;
+      for (int i = 0; i < kTiles; ++i) {
+        // The sums of more than 128 columns lie in accumulation registers, and leave them here alone: where the
+        // compiler chose, they were copied to others and back on every step (256 wide, 200 over 10000: 130 us, 155).
+        if constexpr (kTiles > 4) asm volatile("" : "+a"(acc[i]));
+        acc[i] *= again;
+        if constexpr (kTiles > 4) asm volatile("" : "+a"(acc[i]));
+      }
       top = most;
     }
     const float shift = top == -INFINITY ? 0.0f : fmaf(top, scale, kSlack);
@@ -894,7 +903,7 @@ __global__ __launch_bounds__(kTileWaves * L2C_WAVE,
         for (int m = 0; m < 4; ++m) {
           e[m] = exp2_of(fmaf(s[u][at + m], scale, -shift));
           total += e[m];
-          if constexpr (E4M3) e[m] = s[u][at + m] == -INFINITY ? 0.0f : e[m] * x[m];
+          if constexpr (E4M3) e[m] *= x[m];
         }
         to[i / 2] = pack2(e[0], e[1]);
         to[i / 2 + 1] = pack2(e[2], e[3]);
@@ -1045,8 +1054,13 @@ struct Plan {
 // Tiles of 16 rows where the sequences have no more on average, else of 128, or of 256. Positions are divided
 // until there are some workgroups for every CU, but not into parts that are mostly beginnings and
 // ends: 256 positions, or, where that leaves CUs idle, 128 (16 x 5 of 2500 in tiles of 10
-// heads: 19.9 us with 256, 21.0 with 128).
-Plan plan(int sequences, int rows, int heads, int kv_heads, int width, int page_size, int max_pages, bool starts) {
+// heads: 19.9 us with 256, 21.0 with 128). Of larger tiles the join has as much to write and read as a part of 256
+// positions takes, so the more tiles there are, the longer their parts (700 over 700 positions of 3 sequences, 152
+// tiles: 30 us in parts of 256, 24 undivided; 700 over 5000 of 4, 240 tiles: 80 in two parts, 110 undivided). A CU
+// has room for two workgroups of four waves of up to 128 columns, and one of wider ones (200 over 10000, 256 wide:
+// 116 us with 256 workgroups, 130 with 512). With a window, a tile sees no more positions than that and its tokens.
+Plan plan(int sequences, int rows, int heads, int kv_heads, int width, int page_size, int max_pages, int window,
+          bool starts) {
   const int group = heads / kv_heads;
   const long long packed = static_cast<long long>(rows) * group;
   Plan p;
@@ -1054,10 +1068,12 @@ Plan plan(int sequences, int rows, int heads, int kv_heads, int width, int page_
   const bool many = width > 96 && width <= 128 && packed / kWideMany * kv_heads > 256;
   const int m = p.rows = narrow ? kNarrow : many ? kWideMany : kWide;
   p.slots = starts ? packed / m + sequences : static_cast<long long>(sequences) * ((group + m - 1) / m);
-  const long long tiles = p.slots * kv_heads, wanted = narrow ? 2048 : 512;
-  const long long least = narrow && tiles < 128 ? 128 : 256;
+  const long long tiles = p.slots * kv_heads, wanted = narrow ? 2048 : width > 128 ? 256 : 512;
+  const long long least = narrow ? (tiles < 128 ? 128 : 256) : max(256LL, min(tiles, 512LL) / 8 * 64);
+  long long positions = static_cast<long long>(max_pages) * page_size;
+  if (window > 0) positions = min(positions, window + 2LL * m);
   long long splits = wanted / tiles;
-  splits = min(splits, (static_cast<long long>(max_pages) * page_size + least - 1) / least);
+  splits = min(splits, (positions + least - 1) / least);
   splits = min(splits, (1LL << 17) / (static_cast<long long>(rows) * heads));
   p.least = static_cast<int>(least);
   p.splits = static_cast<int>(max(1LL, min(splits, static_cast<long long>(kMaxSplits))));
@@ -1096,8 +1112,7 @@ Kernel kernel(int rows, int width) {
 Kernel join(const Plan &p, int width, bool many) {
   if (p.rows == kNarrow)
     return many ? join_kernel<kNarrow, kNarrowStep, true> : join_kernel<kNarrow, kNarrowStep, false>;
-  if (width <= 128) return many ? join_kernel<kWide, 64, true> : join_kernel<kWide, 64, false>;
-  return many ? join_kernel<kWide, 32, true> : join_kernel<kWide, 32, false>;
+  return many ? join_kernel<kWide, 64, true> : join_kernel<kWide, 64, false>;
 }
 
 size_t part_bytes(const Plan &p, int rows, int heads, int width) {
@@ -1113,7 +1128,7 @@ extern "C" size_t l2c_cache_attention_workspace_bytes(int sequences, int rows, i
   size_t most = 0;
   for (const bool starts : {true, false})
     if (starts || rows == sequences)
-      most = max(most, part_bytes(plan(sequences, rows, heads, kv_heads, width, page_size, max_pages, starts), rows,
+      most = max(most, part_bytes(plan(sequences, rows, heads, kv_heads, width, page_size, max_pages, 0, starts), rows,
                                   heads, width));
   return most;
 }
@@ -1138,7 +1153,7 @@ extern "C" int l2c_cache_attention(uint16_t *out, long long out_stride, const ui
       !q || !out || !l2c_aligned16(q) || !l2c_aligned16(out) || workspace_bytes < need ||
       (need > 0 && (!workspace || !l2c_aligned16(workspace))))
     return hipErrorInvalidValue;
-  const Plan p = plan(sequences, rows, heads, kv_heads, width, page_size, max_pages, starts != nullptr);
+  const Plan p = plan(sequences, rows, heads, kv_heads, width, page_size, max_pages, window, starts != nullptr);
   const long long grid = p.slots * kv_heads * p.splits;
   const int threads = p.rows == kWideMany ? kManyWaves * L2C_WAVE : kThreads;
   if (static_cast<long long>(rows) * heads > INT_MAX || p.slots > INT_MAX || grid > INT_MAX ||

@@ -450,7 +450,7 @@ int l2c_decoder_logprobs(float *logprobs, float *entropies, int *top_tokens, flo
  *     out[row][h] = sum_j softmax_j(scale * q[row][h] . k_j) v_j
  *   over the positions j <= p that have a page, and j > p - window unless window is 0; scale times
  *   log2(e) is finite. Whatever the other positions hold has no part in it. Where no position is left, or
- *   every score is -Inf, out is 0. q and out: bf16, heads * width values every q_stride and out_stride. Scores, maxima, sums
+ *   every score is -Inf, out is 0 (0 times a value that is not finite is NaN, though). q and out: bf16, heads * width values every q_stride and out_stride. Scores, maxima, sums
  *   and out are fp32 until out is rounded once, to nearest even; the exponentials are rounded to
  *   bf16 (at most 2^-8 of each, times the value's scale with e4m3 pages) for the product with the values.
  *   None is above 1 before they are divided by their sum, so values below 2^128 over the number of positions

@@ -20,8 +20,8 @@ def attention(sequences, rows, heads, kv_heads, width, page_size, max_pages, sta
     m = 16 if narrow else 256 if many else 128
     slots = packed // m + sequences if starts else sequences * -(-group // m)
     tiles = slots * kv_heads
-    least = 128 if narrow and tiles < 128 else 256
-    splits = min((2048 if narrow else 512) // tiles, -(-max_pages * page_size // least), 64)
+    least = (128 if tiles < 128 else 256) if narrow else max(256, min(tiles, 512) // 8 * 64)
+    splits = min((2048 if narrow else 256 if width > 128 else 512) // tiles, -(-max_pages * page_size // least), 64)
     splits = max(1, min(splits, (1 << 17) // (rows * heads)))
     columns = next(c for c in (2, 3, 4, 6, 8) if width <= 32 * c)
     if narrow:
@@ -29,7 +29,7 @@ def attention(sequences, rows, heads, kv_heads, width, page_size, max_pages, sta
         kernel = "narrow", 4 if pairs and columns == 3 else columns, e4m3, pairs
     else:
         kernel = "wide", columns, 8 if many else 4, e4m3
-    join = None if splits == 1 else (m, 32 if narrow or width > 128 else 64, splits > 8)
+    join = None if splits == 1 else (m, 32 if narrow else 64, splits > 8)
     return kernel, join, 0 if splits == 1 else rows * heads * splits * (width + 2) * 4
 
 

@@ -1051,7 +1051,9 @@ struct Plan {
   int splits, least;  // the least positions of a part: a multiple of the kernels' steps
 };
 
-// Tiles of 16 rows where the sequences have no more on average, else of 128, or of 256. Positions are divided
+// Tiles of 16 rows where the sequences have no more on average, or, of e4m3 pages, up to 24, which two of them read
+// sooner than one large one (5 rows of 4 heads a key head, 64 over up to 1000 positions: 29 us and 33, 2 over up to
+// 100000: 97 and 107; of bf16 pages 64 over up to 4000 188 and 150), else of 128, or of 256. Positions are divided
 // until there are some workgroups for every CU, but not into parts that are mostly beginnings and
 // ends: 256 positions, or, where that leaves CUs idle, 128 (16 x 5 of 2500 in tiles of 10
 // heads: 19.9 us with 256, 21.0 with 128). Of larger tiles the join has as much to write and read as a part of 256
@@ -1060,11 +1062,11 @@ struct Plan {
 // has room for two workgroups of four waves of up to 128 columns, and one of wider ones (200 over 10000, 256 wide:
 // 116 us with 256 workgroups, 130 with 512). With a window, a tile sees no more positions than that and its tokens.
 Plan plan(int sequences, int rows, int heads, int kv_heads, int width, int page_size, int max_pages, int window,
-          bool starts) {
+          bool starts, bool e4m3) {
   const int group = heads / kv_heads;
   const long long packed = static_cast<long long>(rows) * group;
   Plan p;
-  const bool narrow = packed <= 16LL * sequences;
+  const bool narrow = packed <= (e4m3 ? 24LL : 16LL) * sequences;
   const bool many = width > 96 && width <= 128 && packed / kWideMany * kv_heads > 256;
   const int m = p.rows = narrow ? kNarrow : many ? kWideMany : kWide;
   p.slots = starts ? packed / m + sequences : static_cast<long long>(sequences) * ((group + m - 1) / m);
@@ -1124,12 +1126,14 @@ size_t part_bytes(const Plan &p, int rows, int heads, int width) {
 extern "C" size_t l2c_cache_attention_workspace_bytes(int sequences, int rows, int heads, int kv_heads, int width,
                                                       int page_size, int max_pages) {
   if (!sizes(sequences, rows, heads, kv_heads, width, page_size, 0, max_pages) || sequences == 0 || rows == 0) return 0;
-  // What a call with starts needs, or without: the fewer slots, the more parts.
+  // The most that a call with starts or without, of either type's pages, needs: the fewer slots, the more parts.
   size_t most = 0;
   for (const bool starts : {true, false})
-    if (starts || rows == sequences)
-      most = max(most, part_bytes(plan(sequences, rows, heads, kv_heads, width, page_size, max_pages, 0, starts), rows,
-                                  heads, width));
+    for (const bool e4m3 : {true, false})
+      if (starts || rows == sequences)
+        most = max(most, part_bytes(plan(sequences, rows, heads, kv_heads, width, page_size, max_pages, 0, starts,
+                                         e4m3),
+                                    rows, heads, width));
   return most;
 }
 
@@ -1153,7 +1157,8 @@ extern "C" int l2c_cache_attention(uint16_t *out, long long out_stride, const ui
       !q || !out || !l2c_aligned16(q) || !l2c_aligned16(out) || workspace_bytes < need ||
       (need > 0 && (!workspace || !l2c_aligned16(workspace))))
     return hipErrorInvalidValue;
-  const Plan p = plan(sequences, rows, heads, kv_heads, width, page_size, max_pages, window, starts != nullptr);
+  const Plan p = plan(sequences, rows, heads, kv_heads, width, page_size, max_pages, window, starts != nullptr,
+                      cache_type == L2C_E4M3);
   const long long grid = p.slots * kv_heads * p.splits;
   const int threads = p.rows == kWideMany ? kManyWaves * L2C_WAVE : kThreads;
   if (static_cast<long long>(rows) * heads > INT_MAX || p.slots > INT_MAX || grid > INT_MAX ||

@@ -87,6 +87,15 @@ def test_windows(torch_gpu, l2c, window, new):
     check(l2c, Cache(window + new, lengths, [new] * 4, 2, 64, 16), 8, window=window)
 
 
+@pytest.mark.parametrize("cache", ["bf16", "e4m3"])
+@pytest.mark.parametrize("width", [64, 136, 256])
+@pytest.mark.parametrize("window", [0, 300, 700, 3001])
+@pytest.mark.parametrize("new", [[1, 1], [5, 7], [6, 20], [150, 10], [600, 500]], ids=str)
+def test_parts_of_long_sequences(torch_gpu, l2c, new, window, width, cache):
+    """Tiles of every kind, divided where a window leaves enough of their positions."""
+    check(l2c, Cache(sum(new) + width, [5000, 2300], new, 2, width, 16, cache), 8, window=window)
+
+
 @pytest.mark.parametrize("page", [16, 24])
 @pytest.mark.parametrize("new", [1, 9, 200])
 def test_pages_that_are_not_there(torch_gpu, l2c, new, page):

@@ -147,21 +147,24 @@ __device__ __forceinline__ void put(int *p, int v) {
   __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// The sum over the workgroup's lanes before this one; `all` over all of them.
-__device__ __forceinline__ long long scan_before(long long v, long long *slots, long long &all) {
-  const int lane = threadIdx.x % L2C_WAVE, wave = threadIdx.x / L2C_WAVE, waves = blockDim.x / L2C_WAVE;
-  long long upto = v;
+// The sum over the workgroup's kAdvanceThreads lanes before this one; `all` over all of them.
+template <class T>
+__device__ __forceinline__ T scan_before(T v, T *slots, T &all) {
+  constexpr int kWaves = kAdvanceThreads / L2C_WAVE;
+  const int lane = threadIdx.x % L2C_WAVE, wave = threadIdx.x / L2C_WAVE;
+  T upto = v;
 #pragma unroll
   for (int o = 1; o < L2C_WAVE; o <<= 1) {
-    const long long before = __shfl_up(upto, o, L2C_WAVE);
+    const T before = __shfl_up(upto, o, L2C_WAVE);
     if (lane >= o) upto += before;
   }
   __syncthreads();  // the slots may still be read from the call before
   if (lane == L2C_WAVE - 1) slots[wave] = upto;
   __syncthreads();
-  long long base = 0;
+  T base = 0;
   all = 0;
-  for (int w = 0; w < waves; ++w) {
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
     if (w < wave) base += slots[w];
     all += slots[w];
   }
@@ -199,7 +202,8 @@ __global__ __launch_bounds__(256) void advance_count_kernel(Step s) {
 // sequence that writes into a page takes itself off its uses; what is left are those who do not
 // write. Where nobody is, the lowest sequence leaves its number less the number of
 // sequences, a negative one, by which it finds that it keeps the page. Sums and minima of
-// integers: the order of the atomics does not show.
+// integers: the order of the atomics does not show. 512 sequences over 13433 pages take the three kernels 34.8 us;
+// the next one, with the tables', does so in 21.
 __global__ __launch_bounds__(kAdvanceThreads) void advance_assign_kernel(Step s) {
   __shared__ long long slots[kAdvanceThreads / L2C_WAVE];
   const int t = threadIdx.x;
@@ -237,13 +241,13 @@ __global__ __launch_bounds__(kAdvanceThreads) void advance_assign_kernel(Step s)
       need = max(0, upto - first) + (replaced >= 0);
       lost = last - max(first, upto);
     }
-    const long long before = total + scan_before(need, slots, all);
+    const long long before = total + scan_before<long long>(need, slots, all);
     if (r < s.sequences) {
       s.copies[2LL * r] = replaced;
       s.copies[2LL * r + 1] = static_cast<int>(min(before, static_cast<long long>(INT_MAX)));
     }
     total += all;
-    scan_before(lost, slots, all);
+    scan_before<long long>(lost, slots, all);
     beyond += all;
   }
   __syncthreads();
@@ -258,7 +262,7 @@ __global__ __launch_bounds__(kAdvanceThreads) void advance_assign_kernel(Step s)
     const int page = static_cast<int>(min(from + t, static_cast<long long>(INT_MAX)));
     const bool free = page < s.pages && now(&s.uses[page]) == 0 && !(s.held && s.held[page]);
     long long all;
-    const long long rank = given + scan_before(free, slots, all);
+    const long long rank = given + scan_before<long long>(free, slots, all);
     if (free && rank < total) {
       int low = 0, high = s.sequences - 1;  // the last sequence whose first rank is at most this one
       while (low < high) {
@@ -296,7 +300,9 @@ __global__ __launch_bounds__(kAdvanceThreads) void advance_assign_kernel(Step s)
 
 // The same for up to 1024 sequences and as many pages as LDS has counters for, in one workgroup with a lane a
 // sequence: the steps below wait for LDS instead of memory. COPY: the tables, too, where they are small
-// enough for one workgroup to be the sooner done.
+// enough for one workgroup to be the sooner done. 32 sequences over 312 pages take 5.6 us, lengths and parents 1, the
+// tables 0.6, who writes 1.4, free pages 2.4; 512 over 13433 pages, whose 132000 entries one CU reads, 18: 1.4,
+// 6.5, 1.5 and 5.5. (Equal entries of sequences below each other counted together took 21 in all.)
 constexpr int kLdsPages = 32768, kLdsSequences = kAdvanceThreads, kCopyEntries = 8192, kLdsEntries = 1 << 18;
 
 typedef int i32x4_any __attribute__((ext_vector_type(4), aligned(4)));
@@ -306,9 +312,10 @@ __global__ __launch_bounds__(kAdvanceThreads) void advance_lds_kernel(Step s) {
   __shared__ int uses[kLdsPages];
   __shared__ int parent[kLdsSequences], have[kLdsSequences], dropped[kLdsSequences];
   __shared__ int base[kLdsSequences], entry[kLdsSequences], fresh[kLdsSequences];
-  __shared__ long long slots[kAdvanceThreads / L2C_WAVE];
-  const int t = threadIdx.x, lane = t % L2C_WAVE, wave = t / L2C_WAVE;
   constexpr int kWaves = kAdvanceThreads / L2C_WAVE;
+  __shared__ int slots[kWaves], ranks[kLdsPages / L2C_WAVE];
+  __shared__ unsigned long long beyond;
+  const int t = threadIdx.x, lane = t % L2C_WAVE, wave = __builtin_amdgcn_readfirstlane(t / L2C_WAVE);
   const bool is = t < s.sequences;
   int length = 0, n = 0, first = 0, last = 0, page = -1;
   if (is) {
@@ -321,6 +328,7 @@ __global__ __launch_bounds__(kAdvanceThreads) void advance_lds_kernel(Step s) {
     dropped[t] = s.window ? max(0, length - s.window + 1) / s.page_size : 0;
   }
   for (int i = t; i < s.pages; i += kAdvanceThreads) uses[i] = 0;
+  if (t == 0) beyond = 0;
   __syncthreads();
   auto count = [&](int e) __attribute__((always_inline)) {
     if (static_cast<unsigned>(e) < static_cast<unsigned>(s.pages)) atomicAdd(&uses[e], 1);
@@ -373,37 +381,54 @@ __global__ __launch_bounds__(kAdvanceThreads) void advance_lds_kernel(Step s) {
   __syncthreads();
   const bool keeps = page >= 0 && uses[page] == t - s.sequences, replaced = page >= 0 && !keeps;
   const int upto = min(last, s.max_pages);
-  long long total, beyond;
-  const long long before = scan_before(is ? max(0, upto - first) + replaced : 0, slots, total);
+  if (is && last > max(first, upto)) atomicAdd(&beyond, static_cast<unsigned long long>(last - max(first, upto)));
+  int total;  // no more than the tables' entries, and a page that each sequence replaces
   // Its barriers part the reads of uses above from what follows.
-  scan_before(is ? last - max(first, upto) : 0, slots, beyond);
+  const int before = scan_before(is ? max(0, upto - first) + replaced : 0, slots, total);
   if (keeps) uses[page] = 1;
   if (is) {
-    base[t] = static_cast<int>(min(before, static_cast<long long>(INT_MAX)));
+    base[t] = before;
     entry[t] = first - replaced;
     fresh[t] = -1;
   }
   __syncthreads();
-  // Free pages in order, each to the sequence that its rank falls to.
-  long long given = 0;
-  for (int from = 0; from < s.pages && given < total; from += kAdvanceThreads) {
-    const int of = from + t;
-    const bool free = of < s.pages && uses[of] == 0 && !(s.held && s.held[of]);
-    long long all;
-    const long long rank = given + scan_before(free, slots, all);
-    if (free && rank < total) {
+  // Free pages in order, each to the sequence that its rank falls to. A wave's 64 of the i-th 1024 are lane i's mask,
+  // and all of those are ranked by one sum.
+  static_assert(kLdsPages / kAdvanceThreads <= L2C_WAVE, "a lane each");
+  const int rounds = (s.pages + kAdvanceThreads - 1) / kAdvanceThreads, masks = rounds * kWaves;
+  unsigned low_mask = 0, high_mask = 0;
+#pragma unroll 4
+  for (int i = 0; i < rounds; ++i) {
+    const int of = i * kAdvanceThreads + t;
+    const unsigned long long free = __ballot(of < s.pages && uses[of] == 0 && !(s.held && s.held[of]));
+    if (lane == i) low_mask = static_cast<unsigned>(free), high_mask = static_cast<unsigned>(free >> 32);
+  }
+  if (lane < rounds) ranks[lane * kWaves + wave] = __popc(low_mask) + __popc(high_mask);
+  __syncthreads();
+  int given;
+  const int before_mask = scan_before(t < masks ? ranks[t] : 0, slots, given);
+  if (t < masks) ranks[t] = before_mask;
+  __syncthreads();
+  const int rank_of = lane < rounds ? ranks[lane * kWaves + wave] : 0;
+  for (int i = 0; i < rounds; ++i) {
+    const unsigned long long free =
+        static_cast<unsigned long long>(static_cast<unsigned>(__builtin_amdgcn_readlane(high_mask, i))) << 32 |
+        static_cast<unsigned>(__builtin_amdgcn_readlane(low_mask, i));
+    const int first_rank = __builtin_amdgcn_readlane(rank_of, i);
+    if (first_rank >= total) break;
+    const int rank = first_rank + __popcll(free & ((1ull << lane) - 1));
+    if ((free >> lane & 1) && rank < total) {
       int low = 0, high = s.sequences - 1;  // the last sequence whose first rank is at most this one
       while (low < high) {
         const int middle = high - (high - low) / 2;
         if (base[middle] <= rank) low = middle;
         else high = middle - 1;
       }
-      const int at = static_cast<int>(rank - base[low]);
+      const int of = i * kAdvanceThreads + t, at = rank - base[low];
       s.tables_out[static_cast<size_t>(low) * s.max_pages + entry[low] + at] = of;
       if (at == 0) fresh[low] = of;
       uses[of] = 1;
     }
-    given += all;
   }
   __syncthreads();
   if (is) {
@@ -414,7 +439,8 @@ __global__ __launch_bounds__(kAdvanceThreads) void advance_lds_kernel(Step s) {
     s.lengths_out[t] = length + n;
   }
   for (int i = t; i < s.pages; i += kAdvanceThreads) s.uses[i] = uses[i];
-  if (t == 0) *s.shortage = static_cast<int>(min(max(total - given, 0LL) + beyond, static_cast<long long>(INT_MAX)));
+  constexpr unsigned long long kMost = INT_MAX;
+  if (t == 0) *s.shortage = static_cast<int>(min(max(total - given, 0) + beyond, kMost));
 }
 
 // ---------------------------------------------------------------------------
@@ -425,7 +451,8 @@ constexpr int kCopyThreads = 256;
 typedef unsigned u32x4_any __attribute__((ext_vector_type(4), aligned(1)));
 
 // Part `blockIdx.x % parts` of pair blockIdx.x / parts in group blockIdx.y: columns of 16 bytes, and of
-// one byte for what is left of the page.
+// one byte for what is left of the page. Bound by memory: about 160 pairs of 4 x 8 KB (10 MB read and written) 6 us, a
+// few 1 to 2.
 __global__ __launch_bounds__(kCopyThreads) void copy_kernel(unsigned char *cache, const int *__restrict__ copies,
                                                             int pages, unsigned parts, unsigned wide, unsigned columns,
                                                             long long group_stride, long long page_stride) {

@@ -8,7 +8,8 @@
 // that its sums wait for nobody; the largest logits so far lie in LDS, in order, and the least of them is
 // a bound that most parts have nothing above. Where there is none yet, the bound comes from the lanes'
 // maxima by ballots, as in the beam selection. Chunks leave their sums and their lists, which a second
-// kernel joins.
+// kernel joins. 2048 rows of 32003 take 51 us without alternatives (5.2 TB/s), 67 to 70 with 20; one of 32000
+// in 16 chunks 6.2 and the join 3.6, where every step waits for the one before.
 #include "l2c_select.h"
 #include "../../include/l2c.h"
 

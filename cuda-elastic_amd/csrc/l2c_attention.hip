@@ -1053,8 +1053,9 @@ struct Plan {
 
 // Tiles of 16 rows where the sequences have no more on average, or, of e4m3 pages, up to 24, which two of them read
 // sooner than one large one (5 rows of 4 heads a key head, 64 over up to 1000 positions: 29 us and 33, 2 over up to
-// 100000: 97 and 107; of bf16 pages 64 over up to 4000 188 and 150), else of 128, or of 256. Positions are divided
-// until there are some workgroups for every CU, but not into parts that are mostly beginnings and
+// 100000: 97 and 107; of bf16 pages 64 over up to 4000 188 and 150), and of 64 columns up to 48, three of them
+// (16 over up to 3000, 48 rows: 33 and 48; 32 over up to 300, 32 rows: 18 and 15), else of 128, or of 256. Positions
+// are divided until there are some workgroups for every CU, but not into parts that are mostly beginnings and
 // ends: 256 positions, or, where that leaves CUs idle, 128 (16 x 5 of 2500 in tiles of 10
 // heads: 19.9 us with 256, 21.0 with 128). Of larger tiles the join has as much to write and read as a part of 256
 // positions takes, so the more tiles there are, the longer their parts (700 over 700 positions of 3 sequences, 152
@@ -1066,7 +1067,7 @@ Plan plan(int sequences, int rows, int heads, int kv_heads, int width, int page_
   const int group = heads / kv_heads;
   const long long packed = static_cast<long long>(rows) * group;
   Plan p;
-  const bool narrow = packed <= (e4m3 ? 24LL : 16LL) * sequences;
+  const bool narrow = packed <= (!e4m3 ? 16LL : width <= 64 ? 48LL : 24LL) * sequences;
   const bool many = width > 96 && width <= 128 && packed / kWideMany * kv_heads > 256;
   const int m = p.rows = narrow ? kNarrow : many ? kWideMany : kWide;
   p.slots = starts ? packed / m + sequences : static_cast<long long>(sequences) * ((group + m - 1) / m);

@@ -15,7 +15,7 @@ def attention(sequences, rows, heads, kv_heads, width, page_size, max_pages, sta
     """(The tiles' kernel, the join's or None, the parts' bytes) by the rules that the entry point's comments state."""
     group = heads // kv_heads
     packed = rows * group
-    narrow = packed <= (24 if e4m3 else 16) * sequences
+    narrow = packed <= (16 if not e4m3 else 48 if width <= 64 else 24) * sequences
     many = 96 < width <= 128 and packed // 256 * kv_heads > 256
     m = 16 if narrow else 256 if many else 128
     slots = packed // m + sequences if starts else sequences * -(-group // m)

@@ -166,6 +166,19 @@ __device__ __forceinline__ unsigned pack2(float a, float b) {
   return __builtin_bit_cast(unsigned, __builtin_convertvector(v, bf16x2));
 }
 
+// A weight as the sum of two bf16 numbers: its upper 16 bits, which are no larger, and the bf16 of what they leave, to
+// 2^-15 of it together. 2^-20 of the weight is added to the second: it has the weight's sign even where the first is
+// the whole of it, so that both times an infinity are the same infinity. BOUNDED: of a weight that is no infinity.
+__device__ __forceinline__ float upper(float v) { return __uint_as_float(__float_as_uint(v) & 0xffff0000u); }
+__device__ __forceinline__ unsigned pack_upper(float a, float b) {
+  return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+}
+template <bool BOUNDED>
+__device__ __forceinline__ float lower(float v) {
+  const float left = v - upper(v);  // NaN of an infinity, for which any other number does
+  return fmaf(v, 0x1p-20f, BOUNDED ? left : fmaxf(left, -FLT_MAX));
+}
+
 // Eight e4m3 codes as bf16, exactly.
 __device__ __forceinline__ u32x4 widen(u32x2 c) {
   u32x4 v;
@@ -285,7 +298,7 @@ __device__ __forceinline__ void lone_row(const Attention &a, const Tile &t, int 
     const float again = exp2_of(top - shift);
     total = total * again + l2c::wave_sum(p);
     top = most;
-    p = __uint_as_float(pack2(p * value_scale, 0.0f) << 16);
+    p *= value_scale;
 #pragma unroll
     for (int c = 0; c < L2C_MAX_HEAD / L2C_WAVE; ++c) acc[c] *= again;
     for (int i = 0; i < L2C_WAVE && first + i <= last; ++i) {
@@ -353,9 +366,14 @@ __device__ __forceinline__ int value_place(int key, int chunk) {
 // PAIRS: of e4m3 pages a lane has sixteen columns in a row for two chunks, so that it loads 16 bytes at a time, too
 // (4 x 131072 in e4m3 166-169 us, 4.9 TB/s, 215 with eight, and as long without any arithmetic; rows of an odd number
 // of eights are loaded so). 64 x 4096 in bf16 takes 153-157 us, 4.9 TB/s; 16 x 5 of 2500, 80 wide, 20, of which the
-// kernel 15. Three waves a SIMD up to 128 columns (e4m3 168 us, 172 with two; the others are the same).
+// kernel 15. Three waves a SIMD up to 128 columns (e4m3 168 us, 172 with two; bf16 of more than 96 columns lacks the
+// registers: 174 us, 154 with two; the others are the same).
+//
+// The weights are two bf16 numbers each, and the second product is taken of both: the matrix units have the time (busy
+// 4 to 7% of it with one number; 64 x 4096 153.7 us with one and with two, 4 x 131072 in e4m3 165, 16 x 5 of 2500 18.3
+// and 18.5, 1 x 2048 10.8 and 11.3). Rounded to one, a weight would be off by up to 2^-8 of it.
 template <int kChunks, bool E4M3, bool PAIRS>
-__global__ __launch_bounds__(kThreads, kChunks > 4 ? 1 : 3) void narrow_kernel(Attention a) {
+__global__ __launch_bounds__(kThreads, kChunks > 4 ? 1 : kChunks == 4 && !E4M3 ? 2 : 3) void narrow_kernel(Attention a) {
   static_assert(!PAIRS || kChunks % 2 == 0, "two chunks a load");
   constexpr int kSure = PAIRS ? kChunks - 2 : kChunks == 2 ? 0 : kChunks <= 4 ? kChunks - 1 : kChunks - 2;
   constexpr int D = kChunks <= 2 ? 64 : kChunks <= 4 ? 128 : 256;
@@ -536,17 +554,19 @@ __global__ __launch_bounds__(kThreads, kChunks > 4 ? 1 : 3) void narrow_kernel(A
       top = most;
     }
     const float shift = top == -INFINITY ? 0.0f : fmaf(top, scale, kSlack);
-    u32x4 p;
+    u32x4 p, rest;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      float e[4];
+      float e[4], left[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         e[i] = exp2_of(fmaf(s[u][i], scale, -shift));
         total += e[i];
         if constexpr (E4M3) e[i] = s[u][i] == -INFINITY ? 0.0f : e[i] * factor[u][i];
+        left[i] = lower<!E4M3>(e[i]);
       }
-      p[2 * u] = pack2(e[0], e[1]), p[2 * u + 1] = pack2(e[2], e[3]);
+      p[2 * u] = pack_upper(e[0], e[1]), p[2 * u + 1] = pack_upper(e[2], e[3]);
+      rest[2 * u] = pack2(left[0], left[1]), rest[2 * u + 1] = pack2(left[2], left[3]);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -557,6 +577,8 @@ __global__ __launch_bounds__(kThreads, kChunks > 4 ? 1 : 3) void narrow_kernel(A
       const u32x2 high = read_column(mine_values + value_place<D>(16 + key, d / 8) + d % 8);
       const u32x4 w = {low[0], low[1], high[0], high[1]};
       acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w), __builtin_bit_cast(bf16x8, p),
+                                                       acc[i], 0, 0, 0);
+      acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w), __builtin_bit_cast(bf16x8, rest),
                                                        acc[i], 0, 0, 0);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -621,6 +643,10 @@ __global__ __launch_bounds__(kThreads, kChunks > 4 ? 1 : 3) void narrow_kernel(A
 // positions 896 us, 982 with four; three of 1000 over 5000 208 and 223), where 128 columns make that worth it and the
 // tiles are enough (four chunks of 300 over 2000 57 us with four, 64 with eight; 64 columns the same with both). Four
 // waves of more than 128 columns need the registers of eight.
+//
+// The weights are rounded to bf16, by up to 2^-8 of each, as operands of the second product: another product for what
+// the rounding leaves, as tiles of 16 rows have it, takes 1215 us for 883 (4096 over 16384) and 278 for 210 (three of 1000
+// over 5000), since the matrix units are busy half of the time here.
 
 constexpr int kManyWaves = 8, kWide = 32 * kWaves, kWideMany = 32 * kManyWaves;
 constexpr int kSchedValu = 0x002, kSchedMfma = 0x008, kSchedDsRead = 0x100;  // sched_group_barrier classes

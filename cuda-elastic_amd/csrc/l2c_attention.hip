@@ -518,7 +518,10 @@ __global__ __launch_bounds__(kThreads, kChunks > 4 ? 1 : kChunks == 4 && !E4M3 ?
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (!(seen >> (16 * u + 4 * g + i) & 1)) s[u][i] = -INFINITY;
+          if (!(seen >> (16 * u + 4 * g + i) & 1)) {
+            s[u][i] = -INFINITY;
+            if constexpr (E4M3) factor[u][i] = 0.0f;  // a scale beside those that the row sees may be anything
+          }
     }
     // Values into LDS; is there one that some rows see and others do not, and that is not finite?
 #pragma unroll
@@ -529,12 +532,6 @@ __global__ __launch_bounds__(kThreads, kChunks > 4 ? 1 : kChunks == 4 && !E4M3 ?
         if (mixed) bad |= not_finite(w);
         *reinterpret_cast<u32x4 *>(mine_values + value_place<D>(16 * u + n, column(c) / 8)) = w;
       }
-    if constexpr (E4M3)
-      if (mixed)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)  // a scale beside one that is there may be anything
-          bad |= ((there >> (4 * g + i) & 1) && not_finite(factor[0][i])) ||
-                 ((there >> (16 + 4 * g + i) & 1) && not_finite(factor[1][i]));
     // The next step's, before anything waits for this one's.
     load(page, base + kStride);
     look_up(page, base + 2 * kStride);
@@ -562,7 +559,7 @@ __global__ __launch_bounds__(kThreads, kChunks > 4 ? 1 : kChunks == 4 && !E4M3 ?
       for (int i = 0; i < 4; ++i) {
         e[i] = exp2_of(fmaf(s[u][i], scale, -shift));
         total += e[i];
-        if constexpr (E4M3) e[i] = s[u][i] == -INFINITY ? 0.0f : e[i] * factor[u][i];
+        if constexpr (E4M3) e[i] *= factor[u][i];
         left[i] = lower<!E4M3>(e[i]);
       }
       p[2 * u] = pack_upper(e[0], e[1]), p[2 * u + 1] = pack_upper(e[2], e[3]);

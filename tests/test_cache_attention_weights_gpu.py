@@ -9,8 +9,8 @@ import math
 
 import pytest
 import torch
-from paged import Cache
-from test_cache_attention_gpu import call
+from paged import E4M3, NAN, Cache
+from test_cache_attention_gpu import call, check
 
 pytestmark = pytest.mark.gpu
 
@@ -39,3 +39,25 @@ def test_weights_are_not_rounded_to_bf16(torch_gpu, l2c, below, length, new, hea
         tol = 2.0 ** -15 + 2 * (0.01 * (width + 4) * 2.0 ** -24 + 2.0 ** -21) + 2 * n * 2.0 ** -24 + want.abs() * 2.0 ** -8
         off = (out[i] - want).abs()
         assert bool((off <= 1.02 * tol).all()), (off / tol).max()
+
+
+@pytest.mark.parametrize("bad", [NAN, math.inf, -math.inf])
+@pytest.mark.parametrize("page", [5, 16])
+@pytest.mark.parametrize("width", [64, 72, 128])
+@pytest.mark.parametrize("new,window", [(1, 0), (5, 0), (5, 99), (40, 0), (150, 0)])
+def test_scales_beside_scores_of_minus_infinity(torch_gpu, l2c, new, window, width, page, bad):
+    """A value that is not finite times the weight 0 is NaN in every kind of tile, also where the weight is 0 because the
+    score is -Inf, and also where the value is not finite by its scale; rows that do not see it have none of it."""
+    c = Cache(width, [new + 130, new + 3], [new, new], 1, width, page, "e4m3")
+    q = torch.ones(c.rows, 4 * width, device="cuda").bfloat16()
+    low = torch.zeros(1, 1, width, device="cuda")
+    low[..., 0] = -1
+    for at in (4, 40, new + 90, new + 128):
+        where, slot = c.place(0, at, 1)
+        c.keys[where, :, slot] = low.to(E4M3).view(torch.uint8)
+        c.key_scales[where, :, slot] = math.inf
+        c.dense[0][0][:, at] = torch.where(low[0] < 0, -math.inf, 0.0).double()  # the score of ones is -Inf
+        c.values[where, :, slot] = torch.ones_like(low).to(E4M3).view(torch.uint8)
+        c.value_scales[where, :, slot] = bad
+        c.dense[0][1][:, at] = bad
+    check(l2c, c, 4, window=window, q=q)

@@ -32,6 +32,8 @@ __global__ __launch_bounds__(kAppendThreads) void append_kernel(void *keys, void
   __shared__ long long places[kBlock + 1];  // of the block's rows: in the cache's rows of head 0; -1: nowhere
   const int t = threadIdx.x, lane = t % G;
   const int each = 2 * kv_heads, all = each * s.rows, first = blockIdx.x * kBlock, first_row = by_each(first);
+  // k and v may end where the sequences' rows do.
+  const int begin = s.starts ? s.starts[0] : 0, end = s.starts ? min(s.starts[s.sequences], s.rows) : s.rows;
   u32x4 x[kItems];
 #pragma unroll
   for (int i = 0; i < kItems; ++i) {
@@ -39,6 +41,7 @@ __global__ __launch_bounds__(kAppendThreads) void append_kernel(void *keys, void
     x[i] = u32x4{0, 0, 0, 0};
     if (item >= all || 8 * lane >= width) continue;
     const int row = by_each(item), of = item - row * each;
+    if (row < begin || row >= end) continue;
     const bool value = of >= kv_heads;
     const uint16_t *const from = value ? v + row * v_stride + static_cast<long long>(of - kv_heads) * width
                                        : k + row * k_stride + static_cast<long long>(of) * width;

@@ -478,8 +478,13 @@ def _takes(what, wanted, *tensors):
             raise ValueError(f"l2c.{what} takes tensors on the current device, {_device()}, not on {t.get_device()}")
 
 
-def _bytes(t):
-    return 0 if t is None else t.numel() * t.element_size()
+def _workspace_bytes(what, t):
+    """Its size; raises unless it is on the current device: the kernels write through it."""
+    if t is None:
+        return 0
+    if t.is_cuda and t.get_device() != _device():
+        raise ValueError(f"l2c.{what} takes a workspace on the current device, {_device()}, not on {t.get_device()}")
+    return t.numel() * t.element_size()
 
 
 def decoder_logprobs_workspace_bytes(vocab, top, rows):
@@ -498,7 +503,7 @@ def decoder_logprobs(logprobs, entropies, top_tokens, top_logprobs, logits, toke
         _takes("decoder_logprobs", "float32", logprobs, entropies, top_logprobs, logits)
         _takes("decoder_logprobs", "int32", top_tokens, tokens)
     code = _c_decoder_logprobs(logprobs, entropies, top_tokens, top_logprobs, logits, tokens, vocab, top, rows,
-                               workspace, _bytes(workspace), stream)
+                               workspace, _workspace_bytes("decoder_logprobs", workspace), stream)
     if code:
         _check(code, "l2c_decoder_logprobs")
 
@@ -561,7 +566,8 @@ def cache_attention(out, q, keys, values, tables, lengths, heads, kv_heads, widt
                               heads * width if q_stride is None else q_stride, keys, values, key_scales, value_scales,
                               cache_type, tables, lengths, starts, sequences, sequences if rows is None else rows, heads,
                               kv_heads, width, page_size, pages, max_pages, window,
-                              width ** -0.5 if scale is None else scale, workspace, _bytes(workspace), stream)
+                              width ** -0.5 if scale is None else scale, workspace,
+                              _workspace_bytes("cache_attention", workspace), stream)
     if code:
         _check(code, "l2c_cache_attention")
 

@@ -495,8 +495,8 @@ def decoder_logprobs(logprobs, entropies, top_tokens, top_logprobs, logits, toke
                      stream=None):
     """logprobs and tokens may be None together, entropies alone, the alternatives with top 0."""
     # The usual call in one look; what it does not take goes through every check.
-    if not (logprobs is not None and entropies is not None and top_tokens is not None and tokens is not None
-            and logprobs.dtype is entropies.dtype is top_logprobs.dtype is logits.dtype is _f32
+    if not (logprobs is not None and entropies is not None and top_tokens is not None and top_logprobs is not None
+            and tokens is not None and logprobs.dtype is entropies.dtype is top_logprobs.dtype is logits.dtype is _f32
             and top_tokens.dtype is tokens.dtype is _i32 and logits.is_cuda and logprobs.get_device()
             == entropies.get_device() == top_tokens.get_device() == top_logprobs.get_device() == logits.get_device()
             == tokens.get_device() == _device()):
@@ -574,9 +574,11 @@ def cache_attention(out, q, keys, values, tables, lengths, heads, kv_heads, widt
 
 def cache_advance(tables_out, lengths_out, uses, copies, shortage, tables, lengths, sequences, max_pages, page_size,
                   pages, parents=None, beams=1, starts=None, held=None, window=0, stream=None):
+    """uses may be None of no pages, tables_out and tables of no columns, and what has a default."""
     # The usual calls in one look; what it does not take goes through every check.
-    if not (tables_out.dtype is lengths_out.dtype is uses.dtype is copies.dtype is shortage.dtype is tables.dtype
-            is lengths.dtype is _i32 and (parents is None or parents.dtype is _i32)
+    if not (tables_out is not None and uses is not None and tables is not None and tables_out.dtype
+            is lengths_out.dtype is uses.dtype is copies.dtype is shortage.dtype is tables.dtype is lengths.dtype
+            is _i32 and (parents is None or parents.dtype is _i32)
             and (starts is None or starts.dtype is _i32) and (held is None or held.dtype is _i32)
             and tables.is_cuda and tables_out.get_device() == lengths_out.get_device() == uses.get_device()
             == copies.get_device() == shortage.get_device() == tables.get_device() == lengths.get_device() == _device()
@@ -592,10 +594,12 @@ def cache_advance(tables_out, lengths_out, uses, copies, shortage, tables, lengt
 
 
 def cache_copy(cache, copies, count, pages, page_bytes, page_stride=None, groups=1, group_stride=None, stream=None):
-    """Strides and sizes in bytes; pages, and groups of them, follow each other unless the strides say otherwise."""
-    if not (copies.dtype is _i32 and copies.is_cuda and copies.get_device() == cache.get_device() == _device()):
+    """Strides and sizes in bytes; pages, and groups of them, follow each other unless the strides say otherwise.
+    cache and copies may be None where there is nothing to copy."""
+    if not (cache is not None and copies is not None and copies.dtype is _i32 and copies.is_cuda
+            and copies.get_device() == cache.get_device() == _device()):
         _takes("cache_copy", "int32", copies)
-        if cache.is_cuda and cache.get_device() != _device():
+        if cache is not None and cache.is_cuda and cache.get_device() != _device():
             raise ValueError(
                 f"l2c.cache_copy takes tensors on the current device, {_device()}, not on {cache.get_device()}")
     page = page_bytes if page_stride is None else page_stride

@@ -70,3 +70,16 @@ def test_a_tensor_of_another_device_is_refused(calls, operator, which):
     with pytest.raises(ValueError, match="current device"):
         call(operator, elsewhere=which)
     assert not calls
+
+
+@pytest.mark.parametrize("operator,without", [
+    ("logprobs", (0, 5)), ("logprobs", (1,)), ("logprobs", (2, 3)), ("logprobs", (2,)), ("logprobs", (3,)),
+    ("logprobs", ("workspace",)), ("attention", ("workspace", "starts")), ("append", ("starts",)),
+    ("advance", ("parents", "starts", "held")),
+    ("advance", (0, 5)), ("advance", (2,)), ("advance", (0, 2, 5)),  # of no columns, of no pages
+    ("copy", (0,)), ("copy", (1,)), ("copy", (0, 1)),                # of nothing
+], ids=str)
+def test_what_the_entry_point_may_get_as_null(calls, operator, without):
+    call(operator, without=without)
+    (_, args), = calls
+    assert sum(a is None for a in args[:-1]) >= len(without)

@@ -555,17 +555,21 @@ extern "C" int l2c_cache_copy(void *cache, const int *copies, int count, int pag
   const long long wide = page_bytes / 16, columns = wide + page_bytes % 16;
   if (columns > INT_MAX) return hipErrorInvalidValue;
   const long long parts = (columns + kCopyThreads - 1) / kCopyThreads;
-  constexpr int kGridY = 65535;  // groups a launch
-  if (parts > INT_MAX / count || !l2c::launchable(parts * count * min(groups, kGridY), kCopyThreads))
-    return hipErrorInvalidValue;
-  for (int first = 0; first < groups; first += kGridY) {
-    const dim3 grid(static_cast<unsigned>(parts * count), min(groups - first, kGridY));
-    hipLaunchKernelGGL(copy_kernel, grid, dim3(kCopyThreads), 0, stream,
-                       static_cast<unsigned char *>(cache) + first * group_stride, copies, pages,
-                       static_cast<unsigned>(parts), static_cast<unsigned>(wide), static_cast<unsigned>(columns),
-                       group_stride, page_stride);
-    L2C_LAUNCH_CHECK();
-    if (groups - first <= kGridY) break;
-  }
+  // As many pairs and groups a launch as HIP takes; no more than some hundred launches for it.
+  constexpr long long kGridY = 65535, kMostBlocks = 0xffffffffLL / kCopyThreads, kMostWork = 1LL << 31;
+  const long long pairs = min(static_cast<long long>(count), kMostBlocks / parts);
+  if (pairs == 0) return hipErrorInvalidValue;
+  const long long deep = min(kGridY, kMostBlocks / (parts * pairs));
+  if ((pairs < count || deep < kGridY) && parts * count > kMostWork / groups) return hipErrorInvalidValue;
+  for (long long group = 0; group < groups; group += deep)
+    for (long long pair = 0; pair < count; pair += pairs) {
+      const dim3 grid(static_cast<unsigned>(parts * min(pairs, count - pair)),
+                      static_cast<unsigned>(min(deep, groups - group)));
+      hipLaunchKernelGGL(copy_kernel, grid, dim3(kCopyThreads), 0, stream,
+                         static_cast<unsigned char *>(cache) + group * group_stride, copies + 2 * pair, pages,
+                         static_cast<unsigned>(parts), static_cast<unsigned>(wide), static_cast<unsigned>(columns),
+                         group_stride, page_stride);
+      L2C_LAUNCH_CHECK();
+    }
   return hipSuccess;
 }

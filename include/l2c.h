@@ -503,7 +503,7 @@ int l2c_cache_attention(uint16_t *out, long long out_stride, const uint16_t *q, 
  *     cache[g * group_stride + copies[2 i + 1] * page_stride] = cache[g * group_stride + copies[2 i] * page_stride]
  *   Strides in bytes, at least the extent of what they separate; groups are layers, say, or keys and
  *   values. No page that one pair writes may be in another pair. Any alignment (16-byte addresses
- *   and strides are fastest).
+ *   and strides are fastest). A call may have at least 2^30 / ceil(page_bytes / 4096) copies, count * groups.
  */
 int l2c_cache_advance(int *tables_out, int *lengths_out, int *uses, int *copies, int *shortage, const int *tables,
                       const int *lengths, const int *parents, int beams, const int *starts, const int *held,

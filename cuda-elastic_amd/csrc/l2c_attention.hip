@@ -1014,7 +1014,7 @@ constexpr int kFewParts = 8;
 template <int M, int STEP, bool MANY>
 __global__ __launch_bounds__(kThreads) void join_kernel(Attention a) {
   constexpr int kBlock = 128;  // columns of a half wave
-  __shared__ __attribute__((aligned(16))) float shared[MANY ? 2 * kWaves * kBlock : 4];
+  __shared__ __attribute__((aligned(16))) float shared[MANY ? kWaves * kBlock : 4];
   const int lane = threadIdx.x % L2C_WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / L2C_WAVE);
   const int item = MANY ? blockIdx.x : __builtin_amdgcn_readfirstlane(blockIdx.x * kWaves + wave);
   if (item >= a.s.rows * a.heads) return;

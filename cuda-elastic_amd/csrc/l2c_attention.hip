@@ -1177,7 +1177,7 @@ extern "C" int l2c_cache_attention(uint16_t *out, long long out_stride, const ui
   const size_t need =
       l2c_cache_attention_workspace_bytes(sequences, rows, heads, kv_heads, width, page_size, max_pages);
   if (!l2c::cache_arguments(cache_type, keys, values, key_scales, value_scales, tables, lengths, starts, sequences,
-                            rows) ||
+                            rows, pages, max_pages) ||
       !q || !out || !l2c_aligned16(q) || !l2c_aligned16(out) || workspace_bytes < need ||
       (need > 0 && (!workspace || !l2c_aligned16(workspace))))
     return hipErrorInvalidValue;

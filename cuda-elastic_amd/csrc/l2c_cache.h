@@ -65,12 +65,14 @@ struct Sequences {
   }
 };
 
-// The arguments that append and attention have in common; false where they are refused.
+// The arguments that append and attention have in common; false where they are refused. Arrays of no pages, and tables of
+// no columns, are nowhere.
 inline bool cache_arguments(int cache_type, const void *keys, const void *values, const float *key_scales,
                             const float *value_scales, const int *tables, const int *lengths, const int *starts,
-                            int sequences, int rows) {
-  return (cache_type == L2C_BF16 || (key_scales && value_scales)) && keys && values && l2c_aligned16(keys) &&
-         l2c_aligned16(values) && tables && lengths && (starts || rows == sequences);
+                            int sequences, int rows, int pages, int max_pages) {
+  return (pages == 0 || ((cache_type == L2C_BF16 || (key_scales && value_scales)) && keys && values)) &&
+         l2c_aligned16(keys) && l2c_aligned16(values) && (max_pages == 0 || tables) && lengths &&
+         (starts || rows == sequences);
 }
 inline bool cache_sizes(int cache_type, int sequences, int rows, int kv_heads, int width, int page_size, int pages,
                         int max_pages) {

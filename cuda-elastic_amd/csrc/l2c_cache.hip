@@ -485,7 +485,7 @@ extern "C" int l2c_cache_append(void *keys, void *values, float *key_scales, flo
   if (k_stride < row || v_stride < row || k_stride % 8 != 0 || v_stride % 8 != 0) return hipErrorInvalidValue;
   if (sequences == 0 || rows == 0 || pages == 0 || max_pages == 0) return hipSuccess;
   if (!l2c::cache_arguments(cache_type, keys, values, key_scales, value_scales, tables, lengths, starts, sequences,
-                            rows) ||
+                            rows, pages, max_pages) ||
       !k || !v || !l2c_aligned16(k) || !l2c_aligned16(v))
     return hipErrorInvalidValue;
   const int lanes = width <= 64 ? 8 : width <= 128 ? 16 : 32;

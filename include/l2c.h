@@ -436,7 +436,7 @@ int l2c_decoder_logprobs(float *logprobs, float *entropies, int *top_tokens, flo
  * width: a multiple of 8, at most L2C_MAX_HEAD. page_size: any from 1 on, max_pages * page_size
  * at most 2^31 - 2^16. Strides are in values between two rows, at least the rows' own length; bf16 rows
  * hold their heads after each other. keys, values, q, k, v and out are 16-byte aligned, their
- * strides multiples of 8. tables, lengths and starts are read on the device: a call can be
+ * strides multiples of 8. keys, values and scales may be NULL if pages is 0, tables if max_pages is 0. tables, lengths and starts are read on the device: a call can be
  * captured, and replayed as they change.
  *
  * l2c_cache_append: writes the new tokens' rows k and v (bf16, kv_heads * width values every

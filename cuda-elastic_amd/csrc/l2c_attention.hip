@@ -347,14 +347,14 @@ __device__ __forceinline__ int value_place(int key, int chunk) {
 // PAIRS: of e4m3 pages a lane has sixteen columns in a row for two chunks, so that it loads 16 bytes at a time, too
 // (4 x 131072 in e4m3 166-169 us, 4.9 TB/s, 215 with eight, and as long without any arithmetic; rows of an odd number
 // of eights are loaded so). 64 x 4096 in bf16 takes 153-157 us, 4.9 TB/s; 16 x 5 of 2500, 80 wide, 20, of which the
-// kernel 15. Three waves a SIMD up to 128 columns (e4m3 168 us, 172 with two; bf16 of more than 96 columns lacks the
-// registers: 174 us, 154 with two; the others are the same).
+// kernel 15. Three waves a SIMD up to 128 columns (e4m3 168 us, 172 with two; 64 x 4 over 1000 in bf16 82 and 90), four up
+// to 64.
 //
 // The weights are two bf16 numbers each, and the second product is taken of both: the matrix units have the time (busy
 // 4 to 7% of it with one number; 64 x 4096 153.7 us with one and with two, 4 x 131072 in e4m3 165, 16 x 5 of 2500 18.3
 // and 18.5, 1 x 2048 10.8 and 11.3). Rounded to one, a weight would be off by up to 2^-8 of it.
 template <int kChunks, bool E4M3, bool PAIRS>
-__global__ __launch_bounds__(kThreads, kChunks > 4 ? 1 : kChunks == 4 && !E4M3 ? 2 : 3) void narrow_kernel(Attention a) {
+__global__ __launch_bounds__(kThreads, kChunks > 4 ? 1 : kChunks == 2 ? 4 : 3) void narrow_kernel(Attention a) {
   static_assert(!PAIRS || kChunks % 2 == 0, "two chunks a load");
   constexpr int kSure = PAIRS ? kChunks - 2 : kChunks == 2 ? 0 : kChunks <= 4 ? kChunks - 1 : kChunks - 2;
   constexpr int D = kChunks <= 2 ? 64 : kChunks <= 4 ? 128 : 256;
@@ -472,6 +472,8 @@ __global__ __launch_bounds__(kThreads, kChunks > 4 ? 1 : kChunks == 4 && !E4M3 ?
   float top = -INFINITY, total = 0.0f;  // of the products, without the scale
   bool odd = false;                     // there were values for odd_positions()
   uint16_t *const mine_values = values[wave];
+  // Where the lane writes its first chunk of key n, and reads keys 4 g + n / 4 of the first tile of columns.
+  int to_place = value_place<D>(n, PAIRS ? 2 * g : g), from_place = value_place<D>(4 * g + n / 4, n % 4 / 2) + 4 * (n % 2);
   int base = begin + wave * kNarrowStep;
   int page[2];
   look_up(page, base);
@@ -505,13 +507,18 @@ __global__ __launch_bounds__(kThreads, kChunks > 4 ? 1 : kChunks == 4 && !E4M3 ?
     }
     // Values into LDS; where some rows see them and others do not, 0 in the place of those that are not finite.
     bool bad = false;
+    // The places differ by bits of their own from chunk to chunk: found anew in every step, not kept in registers.
+    asm volatile("" : "+v"(to_place));
+    auto place = [&](int u, int c) __attribute__((always_inline)) {
+      return reinterpret_cast<u32x4 *>(mine_values + (to_place ^ 8 * (PAIRS ? 8 * (c / 2) + c % 2 : 4 * c)) + 16 * D * u);
+    };
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int c = 0; c < kChunks; ++c) {
         const u32x4 w = as_bf16(v[u][c]);
         if (mixed) bad |= not_finite(w);
-        *reinterpret_cast<u32x4 *>(mine_values + value_place<D>(16 * u + n, column(c) / 8)) = w;
+        *place(u, c) = w;
       }
     if (mixed && __ballot(bad)) {
       odd = true;
@@ -519,8 +526,7 @@ __global__ __launch_bounds__(kThreads, kChunks > 4 ? 1 : kChunks == 4 && !E4M3 ?
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int c = 0; c < kChunks; ++c)
-          *reinterpret_cast<u32x4 *>(mine_values + value_place<D>(16 * u + n, column(c) / 8)) =
-              finite_part(as_bf16(v[u][c]));
+          *place(u, c) = finite_part(as_bf16(v[u][c]));
     }
     // The next step's, before anything waits for this one's.
     load(page, base + kStride);
@@ -557,11 +563,11 @@ __global__ __launch_bounds__(kThreads, kChunks > 4 ? 1 : kChunks == 4 && !E4M3 ?
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
+    asm volatile("" : "+v"(from_place));
 #pragma unroll
     for (int i = 0; i < kTiles; ++i) {
-      const int d = 16 * i + 4 * (n % 4), key = 4 * g + n / 4;
-      const u32x2 low = read_column(mine_values + value_place<D>(key, d / 8) + d % 8);
-      const u32x2 high = read_column(mine_values + value_place<D>(16 + key, d / 8) + d % 8);
+      const uint16_t *const from = mine_values + (from_place ^ 16 * i);
+      const u32x2 low = read_column(from), high = read_column(from + 16 * D);
       const u32x4 w = {low[0], low[1], high[0], high[1]};
       acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w), __builtin_bit_cast(bf16x8, p),
                                                        acc[i], 0, 0, 0);

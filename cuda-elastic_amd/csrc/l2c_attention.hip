@@ -345,14 +345,15 @@ __device__ __forceinline__ int value_place(int key, int chunk) {
 
 // kChunks: of 32 columns, of which a lane has eight; those from kSure on may end before. A row has D columns in LDS.
 // PAIRS: of e4m3 pages a lane has sixteen columns in a row for two chunks, so that it loads 16 bytes at a time, too
-// (4 x 131072 in e4m3 166-169 us, 4.9 TB/s, 215 with eight, and as long without any arithmetic; rows of an odd number
-// of eights are loaded so). 64 x 4096 in bf16 takes 153-157 us, 4.9 TB/s; 16 x 5 of 2500, 80 wide, 20, of which the
-// kernel 15. Three waves a SIMD up to 128 columns (e4m3 168 us, 172 with two; 64 x 4 over 1000 in bf16 82 and 90), four up
-// to 64.
+// (4 x 131072 in e4m3 158 us, 5.2 TB/s; when eight took 215, that was as long as without any arithmetic; rows of an odd
+// number of eights are loaded so). 64 x 4096 in bf16 takes 153 us, 4.9 TB/s; 16 x 5 of 2500, 80 wide, 18.7, of which the
+// kernel 14.5 and the join 4.2. Three waves a SIMD up to 128 columns (64 x 4 over 1000 in bf16 82 us, 90 with two), four
+// up to 64.
 //
 // The weights are two bf16 numbers each, and the second product is taken of both: the matrix units have the time (busy
-// 4 to 7% of it with one number; 64 x 4096 153.7 us with one and with two, 4 x 131072 in e4m3 165, 16 x 5 of 2500 18.3
-// and 18.5, 1 x 2048 10.8 and 11.3). Rounded to one, a weight would be off by up to 2^-8 of it.
+// 4 to 7% of it with one number, 6 to 12 with two). With one and with two numbers, us: 153.7 and 153.3 (64 x 4096), 117.6
+// and 111.4 (64 x 4096 in e4m3), 18.3 and 18.7 (16 x 5 of 2500), 10.8 and 11.0 (1 x 2048), 30.6 and 32.7 (16 x 8 of 3000,
+// 64 wide, in e4m3). Rounded to one, a weight would be off by up to 2^-8 of it.
 template <int kChunks, bool E4M3, bool PAIRS>
 __global__ __launch_bounds__(kThreads, kChunks > 4 ? 1 : kChunks == 2 ? 4 : 3) void narrow_kernel(Attention a) {
   static_assert(!PAIRS || kChunks % 2 == 0, "two chunks a load");
@@ -643,7 +644,7 @@ __global__ __launch_bounds__(kThreads, kChunks > 4 ? 1 : kChunks == 2 ? 4 : 3) v
 // more than 128 columns a tile of 64 positions needs all 512 registers and 128 KB, and is still better than one of 32
 // (200 over 10000 positions, 256 wide, 116 us and 130; 192 wide, 1000 over 4000 of 4, 139 and 157). Four waves share
 // a tile, so that two workgroups fit a CU, or eight, for which half as much is loaded (a chunk of 4096 over 16384
-// positions 896 us, 982 with four; three of 1000 over 5000 208 and 223), where 128 columns make that worth it and the
+// positions 880 to 920 us, 982 with four; three of 1000 over 5000 209 and 223), where 128 columns make that worth it and the
 // tiles are enough (four chunks of 300 over 2000 57 us with four, 64 with eight; 64 columns the same with both). Four
 // waves of more than 128 columns need the registers of eight.
 //
@@ -1119,13 +1120,19 @@ struct Plan {
   int splits, least;  // the least positions of a part: a multiple of the kernels' steps
 };
 
-// Tiles of 16 rows where the sequences have no more on average, or, of e4m3 pages, up to 24, which two of them read
-// sooner than one large one (5 rows of 4 heads a key head, 64 over up to 1000 positions: 29 us and 33, 2 over up to
-// 100000: 97 and 107; of bf16 pages 64 over up to 4000 188 and 150), and of 64 columns up to 48, three of them
-// (16 over up to 3000, 48 rows: 33 and 48; 32 over up to 300, 32 rows: 18 and 15), else of 128, or of 256. Positions
-// are divided until there are some workgroups for every CU, but not into parts that are mostly beginnings and
-// ends: 256 positions, or, where that leaves CUs idle, 128 (16 x 5 of 2500 in tiles of 10
-// heads: 19.9 us with 256, 21.0 with 128). Of larger tiles the join has as much to write and read as a part of 256
+// Tiles of 16 rows where the sequences have no more on average, whose weights are the more precise, or, of e4m3 pages, up
+// to 24, and of 64 columns up to 48, else of 128, or of 256. In tiles of 16 and of 128 rows, us: single tokens 11.1 and
+// 15.1 (1 x 2048), 153 and 145 (64 x 4096), 158 and 294 (4 x 131072 in e4m3), 18.7 and 30 (16 x 5 of 2500); of 8 rows for
+// each of 8 key heads in bf16 58 and 52 (64 x 1000), 47 and 42 (16 x 3000), and of 24 rows 70 and 52, 62 and 43; in e4m3
+// of 24 rows 52 and 49, 44 and 55, of 32 rows 58 and 50, 48 and 57; of 64 columns in e4m3 of 32 rows 33 and 39, 31 and
+// 43, of 48 rows 46 and 40, 38 and 46, of 64 rows 47 and 40, 44 and 48: where the rule ends the one is as often the
+// sooner as the other. It goes by the average of a call, so a chunk among many single tokens is cut into small tiles, and
+// single tokens beside a large chunk have a large tile each (1 of 1000 over 5000 and 3 of 1 over 131072: 2770 us in one
+// call, 119 and 300 in two).
+//
+// Positions are divided until there are some workgroups for every CU, but not into parts that are mostly beginnings and
+// ends: 256 positions, or, where that leaves CUs idle, 128 (16 x 5 of 2500 in tiles of 10 heads, when it took longer in
+// all: 19.9 us with 256, 21.0 with 128). Of larger tiles the join has as much to write and read as a part of 256
 // positions takes, so the more tiles there are, the longer their parts (700 over 700 positions of 3 sequences, 152
 // tiles: 30 us in parts of 256, 24 undivided; 700 over 5000 of 4, 240 tiles: 80 in two parts, 110 undivided). A CU
 // has room for two workgroups of four waves of up to 128 columns, and one of wider ones (200 over 10000, 256 wide:

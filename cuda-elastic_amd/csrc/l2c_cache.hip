@@ -21,7 +21,7 @@ __device__ __forceinline__ float high_half(unsigned u) { return __uint_as_float(
 // Keys, then values of a row's heads, then the next row's: an item each, by G lanes with eight values a lane,
 // kItems items one after the other by the same lanes, all of them on their way before the first is looked at.
 // Bound by memory; where a row goes is found once for the workgroup, meanwhile. 8192 rows of 8 x 128 into e4m3 pages
-// 12.6-14.3 us (3.2 TB/s), 39 with an item a lane and every lane's own search; 64 rows into bf16 pages 2.4-2.7.
+// 12.0-14.7 us (3.1 TB/s), 39 with an item a lane and every lane's own search; 64 rows into bf16 pages 2.4-2.7.
 template <int G, int kItems, bool E4M3>
 __global__ __launch_bounds__(kAppendThreads) void append_kernel(void *keys, void *values, float *key_scales,
                                                                 float *value_scales, const uint16_t *k,
@@ -454,8 +454,8 @@ constexpr int kCopyThreads = 256;
 typedef unsigned u32x4_any __attribute__((ext_vector_type(4), aligned(1)));
 
 // Part `blockIdx.x % parts` of pair blockIdx.x / parts in group blockIdx.y: columns of 16 bytes, and of
-// one byte for what is left of the page. Bound by memory: about 160 pairs of 4 x 8 KB (10 MB read and written) 6 us, a
-// few 1 to 2.
+// one byte for what is left of the page. Bound by memory: about 160 pairs of 4 x 8 KB (10 MB read and written) 4.2
+// us, a few 1 to 2.6.
 __global__ __launch_bounds__(kCopyThreads) void copy_kernel(unsigned char *cache, const int *__restrict__ copies,
                                                             int pages, unsigned parts, unsigned wide, unsigned columns,
                                                             long long group_stride, long long page_stride) {

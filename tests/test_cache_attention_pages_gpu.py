@@ -8,9 +8,9 @@ pytestmark = pytest.mark.gpu
 
 
 # Widths that are multiples of 16 and of 8 only, for both ways of reading a row.
-@pytest.mark.parametrize("width", [64, 72, 120, 128, 136, 256])
-@pytest.mark.parametrize("new", [1, 3, 7, 100])
-@pytest.mark.parametrize("page", [1, 2, 3, 5, 7, 50])
+@pytest.mark.parametrize("width", [64, 72, 128, 136])
+@pytest.mark.parametrize("new", [1, 7, 100])
+@pytest.mark.parametrize("page", [1, 3, 6, 50])
 def test_page_sizes_of_e4m3(torch_gpu, l2c, page, new, width):
     lengths = [max(new, n) for n in (page, page + 1, 3 * page, 34, 211)]
     check(l2c, Cache(page + new + width, lengths, [new] * 5, 2, width, page, "e4m3"), 8)

@@ -289,9 +289,10 @@ __device__ __forceinline__ float dot8(u32x4 x, u32x4 y, float sum) {
 
 // Values that are not finite, in steps of positions that some rows of a tile see and others do not: in the product they
 // would be NaN times the weight 0 of those, so their places have 0 there, and afterwards the rows that see them get
-// them here. A wave goes through its steps of KEYS positions from `base` on; add(row, j) for each position j that has such a
-// value, or, SCALED, such a scale, and its row in the cache. After all steps, since the registers for it are free then: one
-// infinity in 4096 over 16384 positions 1030 us, 960 without; computed beside the products it spilled others, 1740.
+// them here. A wave goes through its steps of KEYS positions from `base` on; add(row, j) for each position j that has
+// such a value, or, SCALED, such a scale, and its row in the cache. After all steps, since the registers for it are
+// free then: one infinity in 4096 over 16384 positions 1030 us, 960 without; computed beside the products it spilled
+// others, 1740.
 template <int KEYS, bool E4M3, bool SCALED, class Add>
 __device__ __forceinline__ void odd_positions(const Attention &a, const Tile &t, int kv, int base, int stride, int end,
                                               int every, int nobody, Add add) {
@@ -344,16 +345,16 @@ __device__ __forceinline__ int value_place(int key, int chunk) {
 }
 
 // kChunks: of 32 columns, of which a lane has eight; those from kSure on may end before. A row has D columns in LDS.
-// PAIRS: of e4m3 pages a lane has sixteen columns in a row for two chunks, so that it loads 16 bytes at a time, too
-// (4 x 131072 in e4m3 158 us, 5.2 TB/s; when eight took 215, that was as long as without any arithmetic; rows of an odd
-// number of eights are loaded so). 64 x 4096 in bf16 takes 153 us, 4.9 TB/s; 16 x 5 of 2500, 80 wide, 18.7, of which the
-// kernel 14.5 and the join 4.2. Three waves a SIMD up to 128 columns (64 x 4 over 1000 in bf16 82 us, 90 with two), four
-// up to 64.
+// PAIRS: of e4m3 pages a lane has sixteen columns in a row for two chunks, so that it loads 16 bytes at a time, too (4
+// x 131072 in e4m3 158 us, 5.2 TB/s; when eight took 215, that was as long as without any arithmetic; rows of an odd
+// number of eights are loaded so). 64 x 4096 in bf16 takes 153 us, 4.9 TB/s; 16 x 5 of 2500, 80 wide, 18.7, of which
+// the kernel 14.5 and the join 4.2. Three waves a SIMD up to 128 columns (64 x 4 over 1000 in bf16 82 us, 90 with two),
+// four up to 64.
 //
 // The weights are two bf16 numbers each, and the second product is taken of both: the matrix units have the time (busy
-// 4 to 7% of it with one number, 6 to 12 with two). With one and with two numbers, us: 153.7 and 153.3 (64 x 4096), 117.6
-// and 111.4 (64 x 4096 in e4m3), 18.3 and 18.7 (16 x 5 of 2500), 10.8 and 11.0 (1 x 2048), 30.6 and 32.7 (16 x 8 of 3000,
-// 64 wide, in e4m3). Rounded to one, a weight would be off by up to 2^-8 of it.
+// 4 to 7% of it with one number, 6 to 12 with two). With one and with two numbers, us: 153.7 and 153.3 (64 x 4096),
+// 117.6 and 111.4 (64 x 4096 in e4m3), 18.3 and 18.7 (16 x 5 of 2500), 10.8 and 11.0 (1 x 2048), 30.6 and 32.7 (16 x 8
+// of 3000, 64 wide, in e4m3). Rounded to one, a weight would be off by up to 2^-8 of it.
 template <int kChunks, bool E4M3, bool PAIRS>
 __global__ __launch_bounds__(kThreads, kChunks > 4 ? 1 : kChunks == 2 ? 4 : 3) void narrow_kernel(Attention a) {
   static_assert(!PAIRS || kChunks % 2 == 0, "two chunks a load");
@@ -474,7 +475,8 @@ __global__ __launch_bounds__(kThreads, kChunks > 4 ? 1 : kChunks == 2 ? 4 : 3) v
   bool odd = false;                     // there were values for odd_positions()
   uint16_t *const mine_values = values[wave];
   // Where the lane writes its first chunk of key n, and reads keys 4 g + n / 4 of the first tile of columns.
-  int to_place = value_place<D>(n, PAIRS ? 2 * g : g), from_place = value_place<D>(4 * g + n / 4, n % 4 / 2) + 4 * (n % 2);
+  int to_place = value_place<D>(n, PAIRS ? 2 * g : g);
+  int from_place = value_place<D>(4 * g + n / 4, n % 4 / 2) + 4 * (n % 2);
   int base = begin + wave * kNarrowStep;
   int page[2];
   look_up(page, base);
@@ -511,7 +513,8 @@ __global__ __launch_bounds__(kThreads, kChunks > 4 ? 1 : kChunks == 2 ? 4 : 3) v
     // The places differ by bits of their own from chunk to chunk: found anew in every step, not kept in registers.
     asm volatile("" : "+v"(to_place));
     auto place = [&](int u, int c) __attribute__((always_inline)) {
-      return reinterpret_cast<u32x4 *>(mine_values + (to_place ^ 8 * (PAIRS ? 8 * (c / 2) + c % 2 : 4 * c)) + 16 * D * u);
+      const int chunk = PAIRS ? 8 * (c / 2) + c % 2 : 4 * c;
+      return reinterpret_cast<u32x4 *>(mine_values + (to_place ^ 8 * chunk) + 16 * D * u);
     };
 #pragma unroll
     for (int u = 0; u < 2; ++u)
@@ -586,7 +589,8 @@ __global__ __launch_bounds__(kThreads, kChunks > 4 ? 1 : kChunks == 2 ? 4 : 3) v
 #pragma unroll
           for (int c = 0; c < kChunks; ++c)
             if (inside(c))
-              score = dot8(as_bf16(load_raw<E4M3>(a.keys, at * a.width + column(c))), __builtin_bit_cast(u32x4, q[c]), score);
+              score = dot8(as_bf16(load_raw<E4M3>(a.keys, at * a.width + column(c))),
+                           __builtin_bit_cast(u32x4, q[c]), score);
           score = sum_halves(sum_rows(score));
           if constexpr (E4M3) score *= a.key_scales[at];
           float weight = exp2_of(fmaf(score, scale, top > -INFINITY ? -top : 0.0f));
@@ -636,21 +640,21 @@ __global__ __launch_bounds__(kThreads, kChunks > 4 ? 1 : kChunks == 2 ? 4 : 3) v
 }
 
 // ---------------------------------------------------------------------------
-// Tiles of 32 rows a wave: chunks of a prompt. Bound by the matrix and the vector units, and by LDS, which each
-// wave reads whole tiles from. The workgroup's keys and values, 64 positions at a time, lie in LDS, two tiles of
-// them: while one is read, the next is on its way. bf16 pages go to LDS without registers between, rows that are
-// not there from a row of zeros; e4m3 pages through registers, where they become bf16 (a chunk each of 2000 over up
-// to 4000 positions of 8 sequences 648 us, 548 in bf16; two tiles in LDS here, too, 676: they cost registers). Of
-// more than 128 columns a tile of 64 positions needs all 512 registers and 128 KB, and is still better than one of 32
-// (200 over 10000 positions, 256 wide, 116 us and 130; 192 wide, 1000 over 4000 of 4, 139 and 157). Four waves share
-// a tile, so that two workgroups fit a CU, or eight, for which half as much is loaded (a chunk of 4096 over 16384
-// positions 880 to 920 us, 982 with four; three of 1000 over 5000 209 and 223), where 128 columns make that worth it and the
-// tiles are enough (four chunks of 300 over 2000 57 us with four, 64 with eight; 64 columns the same with both). Four
-// waves of more than 128 columns need the registers of eight.
+// Tiles of 32 rows a wave: chunks of a prompt. Bound by the matrix and the vector units, and by LDS, which each wave
+// reads whole tiles from. The workgroup's keys and values, 64 positions at a time, lie in LDS, two tiles of them: while
+// one is read, the next is on its way. bf16 pages go to LDS without registers between, rows that are not there from a
+// row of zeros; e4m3 pages through registers, where they become bf16 (a chunk each of 2000 over up to 4000 positions of
+// 8 sequences 648 us, 548 in bf16; two tiles in LDS here, too, 676: they cost registers). Of more than 128 columns a
+// tile of 64 positions needs all 512 registers and 128 KB, and is still better than one of 32 (200 over 10000
+// positions, 256 wide, 116 us and 130; 192 wide, 1000 over 4000 of 4, 139 and 157). Four waves share a tile, so that
+// two workgroups fit a CU, or eight, for which half as much is loaded (a chunk of 4096 over 16384 positions 880 to 920
+// us, 982 with four; three of 1000 over 5000 209 and 223), where 128 columns make that worth it and the tiles are
+// enough (four chunks of 300 over 2000 57 us with four, 64 with eight; 64 columns the same with both). Four waves of
+// more than 128 columns need the registers of eight.
 //
 // The weights are rounded to bf16, by up to 2^-8 of each, as operands of the second product: another product for what
-// the rounding leaves, as tiles of 16 rows have it, takes 1215 us for 883 (4096 over 16384) and 278 for 210 (three of 1000
-// over 5000), since the matrix units are busy half of the time here.
+// the rounding leaves, as tiles of 16 rows have it, takes 1215 us for 883 (4096 over 16384) and 278 for 210 (three of
+// 1000 over 5000), since the matrix units are busy half of the time here.
 
 constexpr int kManyWaves = 8, kWide = 32 * kWaves, kWideMany = 32 * kManyWaves;
 constexpr int kSchedValu = 0x002, kSchedMfma = 0x008, kSchedDsRead = 0x100;  // sched_group_barrier classes
@@ -1120,15 +1124,15 @@ struct Plan {
   int splits, least;  // the least positions of a part: a multiple of the kernels' steps
 };
 
-// Tiles of 16 rows where the sequences have no more on average, whose weights are the more precise, or, of e4m3 pages, up
-// to 24, and of 64 columns up to 48, else of 128, or of 256. In tiles of 16 and of 128 rows, us: single tokens 11.1 and
-// 15.1 (1 x 2048), 153 and 145 (64 x 4096), 158 and 294 (4 x 131072 in e4m3), 18.7 and 30 (16 x 5 of 2500); of 8 rows for
-// each of 8 key heads in bf16 58 and 52 (64 x 1000), 47 and 42 (16 x 3000), and of 24 rows 70 and 52, 62 and 43; in e4m3
-// of 24 rows 52 and 49, 44 and 55, of 32 rows 58 and 50, 48 and 57; of 64 columns in e4m3 of 32 rows 33 and 39, 31 and
-// 43, of 48 rows 46 and 40, 38 and 46, of 64 rows 47 and 40, 44 and 48: where the rule ends the one is as often the
-// sooner as the other. It goes by the average of a call, so a chunk among many single tokens is cut into small tiles, and
-// single tokens beside a large chunk have a large tile each (1 of 1000 over 5000 and 3 of 1 over 131072: 2770 us in one
-// call, 119 and 300 in two).
+// Tiles of 16 rows where the sequences have no more on average, whose weights are the more precise, or, of e4m3 pages,
+// up to 24, and of 64 columns up to 48, else of 128, or of 256. In tiles of 16 and of 128 rows, us: single tokens 11.1
+// and 15.1 (1 x 2048), 153 and 145 (64 x 4096), 158 and 294 (4 x 131072 in e4m3), 18.7 and 30 (16 x 5 of 2500); of 8
+// rows for each of 8 key heads in bf16 58 and 52 (64 x 1000), 47 and 42 (16 x 3000), and of 24 rows 70 and 52, 62 and
+// 43; in e4m3 of 24 rows 52 and 49, 44 and 55, of 32 rows 58 and 50, 48 and 57; of 64 columns in e4m3 of 32 rows 33 and
+// 39, 31 and 43, of 48 rows 46 and 40, 38 and 46, of 64 rows 47 and 40, 44 and 48: where the rule ends the one is as
+// often the sooner as the other. It goes by the average of a call, so a chunk among many single tokens is cut into
+// small tiles, and single tokens beside a large chunk have a large tile each (1 of 1000 over 5000 and 3 of 1 over
+// 131072: 2770 us in one call, 119 and 300 in two).
 //
 // Positions are divided until there are some workgroups for every CU, but not into parts that are mostly beginnings and
 // ends: 256 positions, or, where that leaves CUs idle, 128 (16 x 5 of 2500 in tiles of 10 heads, when it took longer in

@@ -65,8 +65,8 @@ struct Sequences {
   }
 };
 
-// The arguments that append and attention have in common; false where they are refused. Arrays of no pages, and tables of
-// no columns, are nowhere.
+// The arguments that append and attention have in common; false where they are refused. Arrays of no pages, and tables
+// of no columns, are nowhere.
 inline bool cache_arguments(int cache_type, const void *keys, const void *values, const float *key_scales,
                             const float *value_scales, const int *tables, const int *lengths, const int *starts,
                             int sequences, int rows, int pages, int max_pages) {

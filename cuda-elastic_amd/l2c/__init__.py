@@ -557,15 +557,15 @@ def cache_attention_workspace_bytes(sequences, rows, heads, kv_heads, width, pag
 
 
 def cache_attention(out, q, keys, values, tables, lengths, heads, kv_heads, width, page_size, pages, max_pages,
-                    sequences, workspace=None, rows=None, starts=None, key_scales=None, value_scales=None, window=0, scale=None,
-                    q_stride=None, out_stride=None, stream=None):
+                    sequences, workspace=None, rows=None, starts=None, key_scales=None, value_scales=None, window=0,
+                    scale=None, q_stride=None, out_stride=None, stream=None):
     """scale is 1 / sqrt(width) unless given; rows of q and out follow each other unless their strides say
     otherwise."""
     cache_type = _cache_type("cache_attention", keys, values, key_scales, value_scales, tables, lengths, starts, q, out)
     code = _c_cache_attention(out, heads * width if out_stride is None else out_stride, q,
                               heads * width if q_stride is None else q_stride, keys, values, key_scales, value_scales,
-                              cache_type, tables, lengths, starts, sequences, sequences if rows is None else rows, heads,
-                              kv_heads, width, page_size, pages, max_pages, window,
+                              cache_type, tables, lengths, starts, sequences, sequences if rows is None else rows,
+                              heads, kv_heads, width, page_size, pages, max_pages, window,
                               width ** -0.5 if scale is None else scale, workspace,
                               _workspace_bytes("cache_attention", workspace), stream)
     if code:

@@ -436,8 +436,9 @@ int l2c_decoder_logprobs(float *logprobs, float *entropies, int *top_tokens, flo
  * width: a multiple of 8, at most L2C_MAX_HEAD. page_size: any from 1 on, max_pages * page_size
  * at most 2^31 - 2^16. Strides are in values between two rows, at least the rows' own length; bf16 rows
  * hold their heads after each other. keys, values, q, k, v and out are 16-byte aligned, their
- * strides multiples of 8. keys, values and scales may be NULL if pages is 0, tables if max_pages is 0. tables, lengths and starts are read on the device: a call can be
- * captured, and replayed as they change.
+ * strides multiples of 8. keys, values and scales may be NULL if pages is 0, tables if max_pages
+ * is 0. tables, lengths and starts are read on the device: a call can be captured, and replayed
+ * as they change.
  *
  * l2c_cache_append: writes the new tokens' rows k and v (bf16, kv_heads * width values every
  *   k_stride and v_stride) into their pages. With e4m3 pages as l2c_quantize_fp8 does it: scale =
@@ -449,9 +450,10 @@ int l2c_decoder_logprobs(float *logprobs, float *entropies, int *top_tokens, flo
  *   v_j of head h / (heads / kv_heads):
  *     out[row][h] = sum_j softmax_j(scale * q[row][h] . k_j) v_j
  *   over the positions j <= p that have a page, and j > p - window unless window is 0; scale times
- *   log2(e) is finite. Whatever the other positions hold has no part in it. Where no position is left, or
- *   every score is -Inf, out is 0 (0 times a value that is not finite is NaN, though). q and out: bf16, heads * width values every q_stride and out_stride. Scores, maxima, sums
- *   and out are fp32 until out is rounded once, to nearest even. The exponentials (times the value's
+ *   log2(e) is finite. Whatever the other positions hold has no part in it. Where no position is
+ *   left, or every score is -Inf, out is 0 (0 times a value that is not finite is NaN, though). q and
+ *   out: bf16, heads * width values every q_stride and out_stride. Scores, maxima, sums and out are
+ *   fp32 until out is rounded once, to nearest even. The exponentials (times the value's
  *   scale with e4m3 pages) are held to 2^-15 of each for the product with the values where
  *   rows * (heads / kv_heads) is at most 16 * sequences (24 with e4m3 pages, 48 with those of up to 64
  *   columns), and rounded to bf16, to 2^-8 of each, in calls with more rows than that.

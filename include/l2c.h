@@ -453,10 +453,11 @@ int l2c_decoder_logprobs(float *logprobs, float *entropies, int *top_tokens, flo
  *   log2(e) is finite. Whatever the other positions hold has no part in it. Where no position is
  *   left, or every score is -Inf, out is 0 (0 times a value that is not finite is NaN, though). q and
  *   out: bf16, heads * width values every q_stride and out_stride. Scores, maxima, sums and out are
- *   fp32 until out is rounded once, to nearest even. The exponentials (times the value's
- *   scale with e4m3 pages) are held to 2^-15 of each for the product with the values where
+ *   fp32 until out is rounded once, to nearest even. The exponentials (times the value's scale with
+ *   e4m3 pages) are held to 2^-15 of each for the product with the values where
  *   rows * (heads / kv_heads) is at most 16 * sequences (24 with e4m3 pages, 48 with those of up to 64
- *   columns), and rounded to bf16, to 2^-8 of each, in calls with more rows than that.
+ *   columns), and rounded to bf16, to 2^-8 of each, in calls with more rows than that; of scales below
+ *   2^-90 less is held, since the products end at bf16's least numbers.
  *   None is above 1 before they are divided by their sum, so values below 2^128 over the number of positions
  *   that a token sees do not overflow.
  *   out overlaps none of the inputs. workspace: 16-byte aligned (may be NULL if the size below is 0),

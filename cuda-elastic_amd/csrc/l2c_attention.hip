@@ -647,7 +647,7 @@ __global__ __launch_bounds__(kThreads, kChunks > 4 ? 1 : kChunks == 2 ? 4 : 3) v
 // 8 sequences 648 us, 548 in bf16; two tiles in LDS here, too, 676: they cost registers). Of more than 128 columns a
 // tile of 64 positions needs all 512 registers and 128 KB, and is still better than one of 32 (200 over 10000
 // positions, 256 wide, 116 us and 130; 192 wide, 1000 over 4000 of 4, 139 and 157). Four waves share a tile, so that
-// two workgroups fit a CU, or eight, for which half as much is loaded (a chunk of 4096 over 16384 positions 880 to 920
+// two workgroups fit a CU, or eight, for which half as much is loaded (a chunk of 4096 over 16384 positions 880 to 940
 // us, 982 with four; three of 1000 over 5000 209 and 223), where 128 columns make that worth it and the tiles are
 // enough (four chunks of 300 over 2000 57 us with four, 64 with eight; 64 columns the same with both). Four waves of
 // more than 128 columns need the registers of eight.
